@@ -87,7 +87,12 @@ enum {
    * head (blockIdx % 8 equal) did not all run on one XCD, or an exchange between them
    * did not complete within 20 ms (the results of that call are not valid). */
   Q4D_STATUS_XCD_MAP = 4,
-  Q4D_STATUS_SYNC_TIMEOUT = 8
+  Q4D_STATUS_SYNC_TIMEOUT = 8,
+  /* Paged cache (status word of q4d_pages_t): no free page left; a sequence, count or order of
+   * the batch that cannot be; a table entry outside the pool. */
+  Q4D_STATUS_NO_PAGES = 16,
+  Q4D_STATUS_BAD_SEQUENCE = 32,
+  Q4D_STATUS_BAD_PAGE = 64
 };
 
 enum { Q4D_F16 = 0, Q4D_F32 = 1, Q4D_BF16 = 2 };
@@ -391,6 +396,116 @@ int q4d_advance(int32_t* tokens, int32_t* positions, const int32_t* next_token, 
 int q4d_advance_session(int32_t* tokens, int32_t* positions, const int32_t* next_token, const float* score,
                         int32_t* hist_tokens, float* hist_scores, int32_t* hist_count, int32_t hist_capacity,
                         int32_t* stop_state, void* stream);
+
+/* ---- paged KV cache -----------------------------------------------------------
+ * No counterpart in the reference (its cache is one contiguous tensor per sequence,
+ * common.py:186-189): the cache of many sequences as pages of one pool, so that a sequence
+ * takes the memory of the positions it holds, sequences share the pages of a common beginning,
+ * and one call serves a ragged batch: chunks of prompts beside single decode tokens.
+ *
+ * A sequence is a row of `table`: the pages of its positions 0 .. lengths[row] - 1, page_size
+ * positions each, in order (entries past those are -1).  refs[p] is the number of rows that hold
+ * page p; a page with refs 0 is free.  The q4d_pages_* calls keep these; data, table, lengths,
+ * refs and status are device memory of the caller, at the start: table -1, the others 0.
+ * A step of a model is q4d_pages_reserve once, then per layer q4d_paged_append and
+ * q4d_paged_attention on the same batch.  All are stream-ordered, read the batch on the device
+ * and can be captured into a graph.  Calls that change one cache (every q4d_pages_* call, and
+ * q4d_paged_append of one layer) must not overlap each other or the calls that read it.
+ *
+ * Values on the device are checked by the kernels: what cannot be is left out (each call says
+ * what), nothing outside the caller's buffers is read or written, and *status receives
+ * Q4D_STATUS_* bits. */
+typedef struct q4d_pages {
+  void* data;           /* [num_layers][2 (K,V)][num_pages][num_kv_heads][page_size][head_dim], 16-byte aligned */
+  int32_t dtype;        /* Q4D_F16 or Q4D_BF16 */
+  int32_t num_layers;
+  int32_t num_pages;    /* up to 2^22 */
+  int32_t num_kv_heads; /* up to 256 */
+  int32_t page_size;    /* 16, 32, 64, 128 or 256 positions */
+  int32_t head_dim;     /* 64 or 128 */
+  int32_t* table;       /* [num_seqs][max_pages] */
+  int32_t* lengths;     /* [num_seqs] */
+  int32_t* refs;        /* [num_pages] */
+  int32_t num_seqs;     /* up to 65536 */
+  int32_t max_pages;    /* max_pages * page_size up to 2^24 positions */
+  int32_t* status;      /* [1] */
+} q4d_pages_t;
+
+/* The sequences of a call and their new tokens, which are their last positions: sequence b is
+ * table row seqs[b] (NULL: row b), its new tokens are rows starts[b] .. starts[b + 1] - 1 of the
+ * token tensors.  A sequence without new tokens is passed over whatever its row is.  Token rows
+ * in no sequence (a padded batch) are not read and their outputs are left as they were. */
+typedef struct q4d_ragged {
+  const int32_t* seqs;    /* device [n] or NULL */
+  const int32_t* starts;  /* device [n + 1], not decreasing, starts[n] <= tokens */
+  int32_t n;              /* 1 .. 4096 */
+  int32_t tokens;         /* rows of the token tensors, up to 2^24 */
+  int32_t max_new;        /* no sequence has more new tokens; 1: a decode step */
+} q4d_ragged_t;
+
+/* Rotation of the first rotary_dim dims of a head by the angle tables' rows: pairs (i, i +
+ * rotary_dim / 2), or (2 i, 2 i + 1) with interleaved = 1.  Scaling for long contexts is a
+ * matter of the tables. */
+typedef struct q4d_rope {
+  const float* cos;      /* device [max_ctx][rotary_dim / 2], 16-byte aligned */
+  const float* sin;
+  int32_t max_ctx;
+  int32_t rotary_dim;    /* a multiple of 16 up to head_dim */
+  int32_t interleaved;
+} q4d_rope_t;
+
+/* Workspace of the q4d_pages_* calls (0: the descriptor is not valid); needs no initialising. */
+size_t q4d_pages_workspace_bytes(const q4d_pages_t* pages);
+/* Every sequence of the batch grows by its new tokens (lengths, table, refs).  New pages are the
+ * free ones of the lowest numbers, in the order of the batch.  Where the last page is partly
+ * filled and other rows hold it too, its rows are copied to a page of the sequence's own first,
+ * in every layer (but where the batch's sequences are all that hold it, the last of them keeps
+ * it).  All or nothing: if pages run out, a sequence would pass max_pages or occurs twice, or a
+ * row, count or page cannot be, nothing changes but the status word. */
+int q4d_pages_reserve(const q4d_pages_t* pages, const q4d_ragged_t* batch, void* ws, size_t ws_bytes, void* stream);
+/* Row dst[i] becomes a copy of row src[i] that shares its pages; src, dst: device int32 [n].
+ * dst[i] must be empty (length 0), in no src, and the first of its number in dst; a pair that
+ * cannot be is left out (Q4D_STATUS_BAD_SEQUENCE, Q4D_STATUS_BAD_PAGE).  n up to 65536. */
+int q4d_pages_fork(const q4d_pages_t* pages, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
+/* Row seqs[i] keeps its first lengths[i] positions (device int32 [n]; lengths NULL: none, which
+ * frees it); pages past them are let go.  An entry whose row is out of range or occurs earlier in
+ * seqs, or whose length is not in [0, the row's], is left out (Q4D_STATUS_BAD_SEQUENCE). */
+int q4d_pages_truncate(const q4d_pages_t* pages, const int32_t* seqs, const int32_t* lengths, int32_t n, void* stream);
+/* The held pages move to the lowest numbers, so that pages *used and up are free (used: device
+ * int32 [1], optional): the k-th held page at or past the number of held pages goes to the k-th
+ * free one below it, with its rows in every layer, its refs and the table entries that name it. */
+int q4d_pages_compact(const q4d_pages_t* pages, int32_t* used, void* ws, size_t ws_bytes, void* stream);
+/* q, k and v rows of the batch's tokens: optional per-head RMSNorm of q and k (q_gamma, k_gamma:
+ * fp32 [head_dim] or NULL, as q4d_qk_norm_rope), optional rotation at the token's position (rope
+ * NULL: none), then k and v to the sequences' pages of `layer` and q to q_out [tokens][q_heads]
+ * [head_dim] in the cache's type, for q4d_paged_attention.  q, k, v: x_dtype (Q4D_F32, Q4D_F16,
+ * Q4D_BF16) rows of heads x head_dim, row t at t * stride elements (so they may lie side by side
+ * in one projection); rows 16-byte aligned.  q and q_out may both be NULL (q_heads 0).  fp32
+ * arithmetic, rounded once.  A token past rope's max_ctx (Q4D_STATUS_BAD_POSITION) or of a
+ * sequence that cannot be is left out; into a page that cannot be nothing is written
+ * (Q4D_STATUS_BAD_PAGE).  The pages must be the sequence's own (q4d_pages_reserve sees to that). */
+int q4d_paged_append(const q4d_pages_t* pages, int32_t layer, const q4d_ragged_t* batch, const void* q, int64_t q_stride,
+                     int32_t q_heads, const void* k, int64_t k_stride, const void* v, int64_t v_stride, int32_t x_dtype,
+                     const float* q_gamma, const float* k_gamma, float eps, const q4d_rope_t* rope, void* q_out,
+                     void* stream);
+/* Workspace of q4d_paged_attention for batches of up to n sequences, `tokens` token rows and
+ * max_new new tokens a sequence; initialised once.  Two calls that may overlap need one each. */
+size_t q4d_paged_attention_workspace_bytes(const q4d_pages_t* pages, int32_t q_heads, int32_t n, int32_t tokens,
+                                           int32_t max_new);
+int q4d_paged_attention_workspace_init(void* ws, size_t ws_bytes, void* stream);
+/* Attention of the batch's new tokens over their sequences' cached positions in `layer`: token i
+ * of a sequence of T positions and a new tokens sees positions 0 .. T - a + i.
+ * out = softmax(q k^T scaling) v, q head h with kv head h / (q_heads / num_kv_heads).  q and out:
+ * rows of q_heads x head_dim in the cache's type, row t at t * stride elements, 16-byte aligned;
+ * out may be q itself.  q_heads is a multiple of num_kv_heads, up to 16 times.  Scores, softmax
+ * and sums are fp32; the probabilities enter the product with v in the cache's type.  A position
+ * whose page cannot be counts as not there (Q4D_STATUS_BAD_PAGE); a token that sees no position
+ * gives zeros.  Values a token does not see, Inf and NaN among them, never reach its output.
+ * Deterministic; a token's last bits may depend on the batch's shape and lengths, though not on
+ * the other sequences' values. */
+int q4d_paged_attention(const q4d_pages_t* pages, int32_t layer, const q4d_ragged_t* batch, const void* q,
+                        int64_t q_stride, int32_t q_heads, float scaling, void* out, int64_t out_stride, void* ws,
+                        size_t ws_bytes, void* stream);
 
 /* ---- fixed-point (RTL-exact) decode ------------------------------------------
  * The integer arithmetic of the reference's FPGA datapath, bit for bit

@@ -20,8 +20,12 @@ STATUS_BAD_TOKEN = 1
 STATUS_BAD_POSITION = 2
 STATUS_XCD_MAP = 4
 STATUS_SYNC_TIMEOUT = 8
+STATUS_NO_PAGES = 16
+STATUS_BAD_SEQUENCE = 32
+STATUS_BAD_PAGE = 64
 STATUS_NAMES = {STATUS_BAD_TOKEN: "BAD_TOKEN", STATUS_BAD_POSITION: "BAD_POSITION", STATUS_XCD_MAP: "XCD_MAP",
-                STATUS_SYNC_TIMEOUT: "SYNC_TIMEOUT"}
+                STATUS_SYNC_TIMEOUT: "SYNC_TIMEOUT", STATUS_NO_PAGES: "NO_PAGES",
+                STATUS_BAD_SEQUENCE: "BAD_SEQUENCE", STATUS_BAD_PAGE: "BAD_PAGE"}
 DECODE_XCD = 0
 DECODE_STAGED = 1
 
@@ -67,6 +71,22 @@ class Q4dModel(ctypes.Structure):
 class Q4dKVCache(ctypes.Structure):
     _fields_ = [("data", c_void_p), ("num_layers", c_int32), ("batch", c_int32), ("num_kv_heads", c_int32),
                 ("max_ctx", c_int32), ("head_dim", c_int32)]
+
+
+class Q4dPages(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("dtype", c_int32), ("num_layers", c_int32), ("num_pages", c_int32),
+                ("num_kv_heads", c_int32), ("page_size", c_int32), ("head_dim", c_int32), ("table", c_void_p),
+                ("lengths", c_void_p), ("refs", c_void_p), ("num_seqs", c_int32), ("max_pages", c_int32),
+                ("status", c_void_p)]
+
+
+class Q4dRagged(ctypes.Structure):
+    _fields_ = [("seqs", c_void_p), ("starts", c_void_p), ("n", c_int32), ("tokens", c_int32), ("max_new", c_int32)]
+
+
+class Q4dRope(ctypes.Structure):
+    _fields_ = [("cos", c_void_p), ("sin", c_void_p), ("max_ctx", c_int32), ("rotary_dim", c_int32),
+                ("interleaved", c_int32)]
 
 
 class Q4dFixedLayer(ctypes.Structure):
@@ -125,6 +145,8 @@ FX_COUNT_NAMES = ["status", "input_norm", "qkv", "qk_norm", "rope", "attention",
 _P = c_void_p
 _FM = POINTER(Q4dFixedModel)
 _FKV = POINTER(Q4dFixedKV)
+_PG = POINTER(Q4dPages)
+_RB = POINTER(Q4dRagged)
 SIGNATURES = {
     "q4d_version": ([], c_int32),
     "q4d_status_string": ([c_int32], ctypes.c_char_p),
@@ -172,6 +194,17 @@ SIGNATURES = {
     "q4d_prefill_workspace_bytes": ([POINTER(Q4dModel), c_int32], c_size_t),
     "q4d_prefill": ([POINTER(Q4dModel), _P, c_int32, c_int32, c_int32, POINTER(Q4dKVCache), _P, _P, _P, _P,
                      c_size_t, _P], c_int32),
+    "q4d_pages_workspace_bytes": ([_PG], c_size_t),
+    "q4d_pages_reserve": ([_PG, _RB, _P, c_size_t, _P], c_int32),
+    "q4d_pages_fork": ([_PG, _P, _P, c_int32, _P], c_int32),
+    "q4d_pages_truncate": ([_PG, _P, _P, c_int32, _P], c_int32),
+    "q4d_pages_compact": ([_PG, _P, _P, c_size_t, _P], c_int32),
+    "q4d_paged_append": ([_PG, c_int32, _RB, _P, ctypes.c_int64, c_int32, _P, ctypes.c_int64, _P, ctypes.c_int64,
+                          c_int32, _P, _P, c_float, POINTER(Q4dRope), _P, _P], c_int32),
+    "q4d_paged_attention_workspace_bytes": ([_PG, c_int32, c_int32, c_int32, c_int32], c_size_t),
+    "q4d_paged_attention_workspace_init": ([_P, c_size_t, _P], c_int32),
+    "q4d_paged_attention": ([_PG, c_int32, _RB, _P, ctypes.c_int64, c_int32, c_float, _P, ctypes.c_int64, _P, c_size_t,
+                             _P], c_int32),
     "q4d_fixed_tables": ([_P, c_int32, _P, c_int32], c_int32),
     "q4d_fixed_workspace_bytes": ([_FM], c_size_t),
     "q4d_fixed_workspace_init": ([_P, c_size_t, _FM, _P], c_int32),
@@ -230,7 +263,7 @@ def check(rc: int, what: str) -> None:
 
 def status_names(status: int) -> list[str]:
     """Names of the Q4D_STATUS_* bits set in a device status word."""
-    return [n for bit, n in STATUS_NAMES.items() if status & bit] + (["UNKNOWN"] if status & ~0xF else [])
+    return [n for bit, n in STATUS_NAMES.items() if status & bit] + (["UNKNOWN"] if status & ~sum(STATUS_NAMES) else [])
 
 
 def check_status(status: int, what: str) -> None:

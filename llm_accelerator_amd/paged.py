@@ -1,0 +1,356 @@
+"""Paged KV cache: many sequences in pages of one pool, and ragged batches over them.
+
+No counterpart in the reference, whose cache is one tensor per sequence
+(``Qwen3-0.6B-Base/python_each_module/common.py:186-189``); the operators stand beside
+``append_cache`` and ``manual_cached_attention`` of :mod:`.common`:
+
+* :class:`PagedKVCache` -- the pool, table, lengths and page counts on the device, with
+  :meth:`~PagedKVCache.reserve`, :meth:`~PagedKVCache.fork`, :meth:`~PagedKVCache.truncate` /
+  :meth:`~PagedKVCache.free` and :meth:`~PagedKVCache.compact` for the pages, and per layer
+  :meth:`~PagedKVCache.append` and :meth:`~PagedKVCache.attention`;
+* :class:`RaggedBatch` -- the sequences of a call and their new tokens: chunks of prompts and
+  single decode tokens side by side;
+* :class:`RopeTable` -- rotation angles: halves or neighbouring pairs, all or part of a head,
+  scaled for long contexts.
+
+Every call is launched on torch's current stream of the cache's device, allocates nothing that
+outlives it, does not synchronise, and can be captured into a graph.  Arguments that the host can
+see are checked (``ValueError`` / :class:`~llm_accelerator_amd._lib.Q4DecError`); what only the
+device knows is checked there, left out where it cannot be, and reported by
+:meth:`~PagedKVCache.status` (``Q4D_STATUS_*`` bits).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from ._lib import Q4D_BF16, Q4D_F16, Q4D_F32, Q4dPages, Q4dRagged, Q4dRope, check
+
+_DTYPES = {torch.float16: Q4D_F16, torch.bfloat16: Q4D_BF16, torch.float32: Q4D_F32}
+
+
+def _ints(t: torch.Tensor, name: str, device, n: int | None = None) -> torch.Tensor:
+    if t.dtype != torch.int32 or t.device != device or not t.is_contiguous() or (n is not None and t.numel() != n):
+        raise ValueError(f"{name} must be a contiguous int32 tensor{'' if n is None else f' of {n} elements'} on {device}")
+    return t
+
+
+class RaggedBatch:
+    """New tokens of several sequences: sequence ``b`` is table row ``seqs[b]`` (``None``: row b), its
+    new tokens, its last positions, are rows ``starts[b]`` .. ``starts[b + 1] - 1`` of the token
+    tensors.  ``seqs`` [n] and ``starts`` [n + 1] are device int32 and may change between calls (a
+    captured step is replayed on other sequences); ``tokens`` is the number of token rows and
+    ``max_new`` a bound on a sequence's new tokens (1: a decode step)."""
+
+    def __init__(self, seqs: torch.Tensor | None, starts: torch.Tensor, tokens: int, max_new: int):
+        if not starts.is_cuda:
+            raise ValueError("starts must be a GPU tensor (libq4dec has no CPU path)")
+        n = starts.numel() - 1
+        self.starts = _ints(starts, "starts", starts.device)
+        self.seqs = None if seqs is None else _ints(seqs, "seqs", starts.device, n)
+        if not 1 <= n <= 4096 or not 1 <= int(tokens) <= 1 << 24 or int(max_new) < 1:
+            raise ValueError("a batch has 1 .. 4096 sequences, 1 .. 2^24 token rows and max_new >= 1")
+        self.n, self.tokens, self.max_new = n, int(tokens), int(max_new)
+        self._desc = Q4dRagged(None if seqs is None else seqs.data_ptr(), starts.data_ptr(), n, self.tokens,
+                               min(self.max_new, self.tokens))
+        self._ref = ctypes.byref(self._desc)
+
+    @classmethod
+    def of(cls, seqs, counts, device="cuda", tokens: int | None = None) -> "RaggedBatch":
+        """From host lists: table rows and the new tokens of each; ``tokens`` rows may hold padding."""
+        if len(seqs) != len(counts) or not counts or min(counts) < 0:
+            raise ValueError("one count of new tokens, zero or more, per sequence")
+        starts = [0]
+        for c in counts:
+            starts.append(starts[-1] + int(c))
+        both = torch.tensor([int(s) for s in seqs] + starts, dtype=torch.int32).to(device)
+        return cls(both[:len(seqs)], both[len(seqs):], max(1, starts[-1]) if tokens is None else tokens,
+                   max(1, max(counts)))
+
+
+def _inv_freq(rotary_dim: int, theta: float, scaling: dict | None) -> tuple[torch.Tensor, float]:
+    """(frequencies in 64 bits, factor of cos and sin)."""
+    r = rotary_dim
+    freq = torch.arange(0, r, 2, dtype=torch.float64) / r
+    inv = theta ** -freq
+    if scaling is None:
+        return inv, 1.0
+    kind, factor = scaling["type"], float(scaling["factor"])
+    if factor < 1:
+        raise ValueError("scaling factor must be at least 1")
+    if kind == "linear":     # positions / factor
+        return inv / factor, 1.0
+    if kind == "ntk":        # a larger base: the lowest frequency is divided by factor, the highest kept
+        return (theta * factor ** (r / (r - 2))) ** -freq if r > 2 else inv / factor, 1.0
+    if kind == "yarn":       # by wavelength: long ones divided by factor, short ones kept, a ramp between
+        old = float(scaling["original_max_ctx"])
+        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+
+        def dim_of(turns):   # the pair that turns `turns` times over the old context
+            return r * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        lo, hi = max(math.floor(dim_of(fast)), 0), min(math.ceil(dim_of(slow)), r - 1)
+        ramp = ((torch.arange(r // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        return inv * (1 - ramp) + inv / factor * ramp, float(scaling.get("attention_factor", 0.1 * math.log(factor) + 1.0))
+    raise ValueError(f"unknown rotary scaling {kind!r}: linear, ntk or yarn")
+
+
+class RopeTable:
+    """cos and sin of position x frequency, fp32 [max_ctx, rotary_dim / 2]; dims past ``rotary_dim``
+    stay as they are.  Pairs are (i, i + rotary_dim / 2) (``manual_rotate_half``, common.py:148-152)
+    or, ``interleaved``, (2 i, 2 i + 1)."""
+
+    def __init__(self, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool = False):
+        if (cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32
+                or not cos.is_contiguous() or not sin.is_contiguous() or cos.device != sin.device or not cos.is_cuda):
+            raise ValueError("cos and sin must be contiguous fp32 GPU tensors [max_ctx, rotary_dim / 2]")
+        self.cos, self.sin, self.interleaved = cos, sin, bool(interleaved)
+        self.max_ctx, self.rotary_dim = cos.shape[0], 2 * cos.shape[1]
+        self._desc = Q4dRope(cos.data_ptr(), sin.data_ptr(), self.max_ctx, self.rotary_dim, int(self.interleaved))
+        self._ref = ctypes.byref(self._desc)
+
+    @classmethod
+    def build(cls, rotary_dim: int, max_ctx: int, theta: float = 1_000_000.0, scaling: dict | None = None,
+              interleaved: bool = False, device="cuda") -> "RopeTable":
+        """Angles made in 64 bits (far positions lose nothing) and rounded once.  ``scaling``: ``None``,
+        ``{"type": "linear" | "ntk", "factor": f}`` or ``{"type": "yarn", "factor": f,
+        "original_max_ctx": n}`` (optional ``beta_fast`` 32, ``beta_slow`` 1, ``attention_factor``)."""
+        cos, sin = rope_angles(rotary_dim, max_ctx, theta, scaling)
+        return cls(cos.to(device), sin.to(device), interleaved)
+
+
+def rope_angles(rotary_dim: int, max_ctx: int, theta: float, scaling: dict | None = None):
+    """(cos, sin) on the host, fp32 [max_ctx, rotary_dim / 2]."""
+    if rotary_dim <= 0 or rotary_dim % 16 or max_ctx <= 0 or theta <= 1:
+        raise ValueError("rotary_dim must be a multiple of 16, max_ctx positive, theta above 1")
+    inv, factor = _inv_freq(rotary_dim, float(theta), scaling)
+    angle = torch.arange(max_ctx, dtype=torch.float64)[:, None] * inv
+    return (angle.cos() * factor).float().contiguous(), (angle.sin() * factor).float().contiguous()
+
+
+class PagedWorkspace:
+    """Scratch of :meth:`PagedKVCache.attention`.  Calls that may overlap (two streams, two captured
+    graphs replayed side by side) need one each."""
+
+    def __init__(self, cache: "PagedKVCache", q_heads: int, n: int, tokens: int, max_new: int):
+        self.nbytes = int(_lib.load().q4d_paged_attention_workspace_bytes(cache._ref, q_heads, n, tokens,
+                                                                          min(max_new, tokens)))
+        if self.nbytes == 0:
+            raise _lib.Q4DecError(-11, "q4d_paged_attention_workspace_bytes")
+        self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=cache.device)
+        self.ptr = self.buf.data_ptr()
+        with cache._on() as stream:
+            check(_lib.load().q4d_paged_attention_workspace_init(self.ptr, self.nbytes, stream),
+                  "q4d_paged_attention_workspace_init")
+
+
+class _On:
+    """The cache's device as the current one; gives its current stream."""
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self) -> int:
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc) -> bool:
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
+class PagedKVCache:
+    """Pool [layers][K, V][pages][kv heads][page size][head dim] (fp16 or bf16), ``table`` [rows, max
+    pages], ``lengths`` [rows] and ``refs`` [pages] (int32, on the device).  Calls that change a cache
+    must not overlap each other or calls that read it."""
+
+    def __init__(self, num_layers: int, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
+                 num_seqs: int, max_ctx: int, dtype=torch.float16, device="cuda"):
+        kw = dict(dtype=torch.int32, device=device)
+        self._setup(torch.zeros((num_layers, 2, num_pages, num_kv_heads, page_size, head_dim), dtype=dtype, device=device),
+                    torch.full((num_seqs, -(-max_ctx // page_size)), -1, **kw), torch.zeros(num_seqs, **kw),
+                    torch.zeros(num_pages, **kw))
+
+    @classmethod
+    def over(cls, data: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor) -> "PagedKVCache":
+        """A cache over tensors that the caller holds."""
+        cache = cls.__new__(cls)
+        cache._setup(data, table, lengths, refs)
+        return cache
+
+    def _setup(self, data, table, lengths, refs) -> None:
+        if data.dim() != 6 or data.shape[1] != 2 or not data.is_contiguous() or table.dim() != 2:
+            raise ValueError("data must be contiguous [layers, 2, pages, kv heads, page size, head dim], table [rows, max pages]")
+        if not data.is_cuda:
+            raise ValueError("data must be a GPU tensor (libq4dec has no CPU path)")
+        if data.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("the cache is fp16 or bf16")
+        self.device, self.dtype = data.device, data.dtype
+        self.data, self.table = data, _ints(table, "table", data.device)
+        self.num_layers, _, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = data.shape
+        self.num_seqs, self.max_pages = table.shape
+        self.lengths = _ints(lengths, "lengths", data.device, self.num_seqs)
+        self.refs = _ints(refs, "refs", data.device, self.num_pages)
+        self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._desc = Q4dPages(data.data_ptr(), _DTYPES[data.dtype], self.num_layers, self.num_pages, self.num_kv_heads,
+                              self.page_size, self.head_dim, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(),
+                              self.num_seqs, self.max_pages, self._status.data_ptr())
+        self._ref = ctypes.byref(self._desc)
+        self._lib = _lib.load()
+        self._ws_bytes = int(self._lib.q4d_pages_workspace_bytes(self._ref))
+        if self._ws_bytes == 0:
+            raise _lib.Q4DecError(-11, "q4d_pages_workspace_bytes")
+        self._ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device)
+        self._wsp = self._ws.data_ptr()
+        self._index = self.device.index if self.device.index is not None else torch.cuda.current_device()
+
+    def _on(self) -> _On:
+        return _On(self._index)
+
+    def _check_batch(self, batch: RaggedBatch) -> None:
+        if batch.starts.device != self.device:
+            raise ValueError(f"the batch is on {batch.starts.device}, the cache on {self.device}")
+        if batch.seqs is None and batch.n > self.num_seqs:
+            raise ValueError(f"a batch of {batch.n} sequences without seqs, the cache has {self.num_seqs} rows")
+
+    # -- pages -------------------------------------------------------------------------
+    def reserve(self, batch: RaggedBatch) -> None:
+        """Every sequence grows by its new tokens: lengths, pages, and a copy of a partly filled last
+        page that others hold too.  All or nothing (q4d_pages_reserve)."""
+        self._check_batch(batch)
+        with self._on() as stream:
+            check(self._lib.q4d_pages_reserve(self._ref, batch._ref, self._wsp, self._ws_bytes, stream),
+                  "q4d_pages_reserve")
+
+    def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Row ``dst[i]``, which is empty, becomes a copy of row ``src[i]`` that shares its pages."""
+        n = _ints(src, "src", self.device).numel()
+        _ints(dst, "dst", self.device, n)
+        if n:
+            with self._on() as stream:
+                check(self._lib.q4d_pages_fork(self._ref, src.data_ptr(), dst.data_ptr(), n, stream), "q4d_pages_fork")
+
+    def truncate(self, seqs: torch.Tensor, lengths: torch.Tensor | None = None) -> None:
+        """Row ``seqs[i]`` keeps its first ``lengths[i]`` positions (``None``: none)."""
+        n = _ints(seqs, "seqs", self.device).numel()
+        if lengths is not None:
+            _ints(lengths, "lengths", self.device, n)
+        if n:
+            with self._on() as stream:
+                check(self._lib.q4d_pages_truncate(self._ref, seqs.data_ptr(),
+                                                   None if lengths is None else lengths.data_ptr(), n, stream),
+                      "q4d_pages_truncate")
+
+    def free(self, seqs: torch.Tensor) -> None:
+        """Rows ``seqs`` let go of all their pages."""
+        self.truncate(seqs)
+
+    def compact(self) -> torch.Tensor:
+        """Held pages move to the lowest numbers; returns how many there are (device int32 [1])."""
+        used = torch.empty(1, dtype=torch.int32, device=self.device)
+        with self._on() as stream:
+            check(self._lib.q4d_pages_compact(self._ref, used.data_ptr(), self._wsp, self._ws_bytes, stream),
+                  "q4d_pages_compact")
+        return used
+
+    # -- a layer -----------------------------------------------------------------------
+    def _token_rows(self, x: torch.Tensor, name: str, batch: RaggedBatch, heads: int | None) -> torch.Tensor:
+        """x [tokens, heads, head_dim], heads side by side; copied only if its rows cannot be read."""
+        if x.dim() != 3 or x.shape[0] != batch.tokens or x.shape[2] != self.head_dim or (heads is not None and x.shape[1] != heads):
+            raise ValueError(f"{name} must be [{batch.tokens}, {'heads' if heads is None else heads}, {self.head_dim}], got {tuple(x.shape)}")
+        if x.device != self.device:
+            raise ValueError(f"{name} is on {x.device}, the cache on {self.device}")
+        size, stride = x.element_size(), x.stride()
+        if (stride[2] != 1 or (x.shape[1] > 1 and stride[1] != self.head_dim) or stride[0] < x.shape[1] * self.head_dim
+                or stride[0] * size % 16 or x.data_ptr() % 16):
+            return x.contiguous() if not x.is_contiguous() else x.clone()
+        return x
+
+    def append(self, layer: int, batch: RaggedBatch, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+               rope: RopeTable | None = None, q_gamma: torch.Tensor | None = None, k_gamma: torch.Tensor | None = None,
+               eps: float = 1e-6, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+        """k and v [tokens, kv_heads, head_dim] of the batch's tokens into their sequences' pages, with
+        the head norm (fp32 gammas, optional) and rotation (optional) of q and k; returns the ready q
+        rows [tokens, q_heads, head_dim] in the cache's type (``None`` without q).  The inputs may be
+        slices of one projection."""
+        self._check_batch(batch)
+        kvh = self.num_kv_heads
+        k, v = self._token_rows(k, "k", batch, kvh), self._token_rows(v, "v", batch, kvh)
+        if k.dtype not in _DTYPES or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+            raise ValueError("q, k and v must be of one type: fp32, fp16 or bf16")
+        qp, qs, qh, op = None, 0, 0, None
+        if q is not None:
+            q = self._token_rows(q, "q", batch, None)
+            qp, qs, qh = q.data_ptr(), q.stride(0), q.shape[1]
+            if q_out is None:
+                q_out = torch.empty((batch.tokens, qh, self.head_dim), dtype=self.dtype, device=self.device)
+            elif (q_out.shape != q.shape or q_out.dtype != self.dtype or not q_out.is_contiguous()
+                  or q_out.device != self.device):
+                raise ValueError(f"q_out must be contiguous {self.dtype} {tuple(q.shape)} on {self.device}")
+            op = q_out.data_ptr()
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        for g, name in ((q_gamma, "q_gamma"), (k_gamma, "k_gamma")):
+            if g is not None and (g.dtype != torch.float32 or g.numel() != self.head_dim or not g.is_contiguous()
+                                  or g.device != self.device):
+                raise ValueError(f"{name} must be contiguous fp32 [{self.head_dim}] on {self.device}")
+        if rope is not None and (rope.cos.device != self.device or rope.rotary_dim > self.head_dim):
+            raise ValueError(f"the rotation must be on {self.device} and at most {self.head_dim} dims wide")
+        with self._on() as stream:
+            check(self._lib.q4d_paged_append(
+                self._ref, layer, batch._ref, qp, qs, qh, k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0),
+                _DTYPES[k.dtype], None if q_gamma is None else q_gamma.data_ptr(),
+                None if k_gamma is None else k_gamma.data_ptr(), eps, None if rope is None else rope._ref, op, stream),
+                "q4d_paged_append")
+        return q_out
+
+    def workspace(self, q_heads: int, batch: RaggedBatch) -> PagedWorkspace:
+        """Scratch for :meth:`attention` on this batch and smaller ones."""
+        return PagedWorkspace(self, q_heads, batch.n, batch.tokens, batch.max_new)
+
+    def attention(self, layer: int, batch: RaggedBatch, q: torch.Tensor, scaling: float | None = None,
+                  out: torch.Tensor | None = None, ws: PagedWorkspace | None = None) -> torch.Tensor:
+        """softmax(q k^T scaling) v of the batch's tokens over their sequences' cached positions up to
+        their own; q and the result [tokens, q_heads, head_dim] in the cache's type (``scaling``
+        ``None``: head_dim ** -0.5).  ``ws``: scratch kept by the caller (:meth:`workspace`); without
+        one the call makes its own.  Rows in no sequence are left as they were."""
+        self._check_batch(batch)
+        if q.dtype != self.dtype:
+            raise ValueError(f"q must be {self.dtype}, as the cache")
+        q = self._token_rows(q, "q", batch, None)
+        if out is None:
+            out = torch.zeros((batch.tokens, q.shape[1], self.head_dim), dtype=self.dtype, device=self.device)
+        elif (out.shape != q.shape or out.dtype != self.dtype or out.device != self.device
+              or self._token_rows(out, "out", batch, None) is not out):
+            raise ValueError(f"out must be {self.dtype} {tuple(q.shape)} on {self.device}, heads side by side, rows 16-byte aligned")
+        if ws is None:
+            ws = self.workspace(q.shape[1], batch)
+        elif ws.buf.device != self.device:
+            raise ValueError(f"the workspace is on {ws.buf.device}, the cache on {self.device}")
+        with self._on() as stream:
+            check(self._lib.q4d_paged_attention(
+                self._ref, layer, batch._ref, q.data_ptr(), q.stride(0), q.shape[1],
+                self.head_dim ** -0.5 if scaling is None else scaling, out.data_ptr(), out.stride(0), ws.ptr, ws.nbytes,
+                stream), "q4d_paged_attention")
+        return out
+
+    # -- state -------------------------------------------------------------------------
+    def status(self) -> int:
+        """The device status word (Q4D_STATUS_* bits; synchronises)."""
+        return int(self._status.item())
+
+    def raise_for_status(self, what: str) -> None:
+        """Raise Q4DecError(Q4D_ERR_STATUS) if a call left something out; the word is cleared."""
+        st = self.status()
+        if st:
+            self._status.zero_()
+            _lib.check_status(st, what)
+
+
+__all__ = ["PagedKVCache", "PagedWorkspace", "RaggedBatch", "RopeTable", "rope_angles"]
