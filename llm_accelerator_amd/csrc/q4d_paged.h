@@ -74,8 +74,19 @@ struct PagedAttnArgs {
   float scale;  // scaling * log2(e)
   int qh, bf16;
   void* ws;
+  // set by launch_paged_attention
+  int* counters;  // parts that have arrived, by join level and block
+  float* pml;     // [slots][rows][2]
+  float* pacc;    // [slots][rows][d]
+  int blocks;     // per kv head
+  // of chunk_kernel
+  int* ccounters;
+  float* cml;     // [parts][kvh][4 waves][m, l of 32 rows]
+  float* cacc;    // [parts][kvh][4 waves][32 x d]
+  int slots, max_splits;  // per kv head: blocks that parts are to fill, parts at most
 };
 size_t paged_attention_ws_bytes(int kvh, int d, int qh, int n, int tokens, int max_new);
+size_t paged_attention_ws_counters();  // bytes at the workspace's start that are zero between calls
 int launch_paged_attention(const PagedAttnArgs& a, hipStream_t st);
 
 }  // namespace q4d

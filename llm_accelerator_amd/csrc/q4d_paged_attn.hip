@@ -1,7 +1,9 @@
 // Attention of a ragged batch's new tokens over a paged KV cache (gfx950, wave64).
 //
-// One wave per (token, q head): the lanes hold D / 64 dims each and walk the positions with an
-// online softmax (running maximum and sum).
+// A kv head's query rows of a sequence are its new tokens times the G = q heads / kv heads that
+// share the kv head: row r is token r / G, head r % G.  Sequences of up to 16 rows (decode steps,
+// a few proposed tokens) are bound by reading K and V once: rows_kernel.  More rows share what is
+// read: chunk_kernel.
 #include <math.h>
 
 #include "q4d_device.h"
@@ -11,71 +13,939 @@ namespace q4d {
 
 namespace {
 
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kRows = 16;   // query rows of rows_kernel
+constexpr int kJoin = 8;         // parts joined at a time
+constexpr int kLevels = 4;       // of joins: up to 8^4 parts
+constexpr int kCounters = 1024;  // counters of a level, one per block
+constexpr int kChunkCounters = 2048;  // the same of chunk_kernel, one per part
+constexpr int kMinSplit = 4;          // steps of a part there at least
+constexpr int kStep = 128;  // positions of a block's step there: 32 a wave
+
 template <bool BF>
 __device__ __forceinline__ float to_f32(uint16_t u) {
   if constexpr (BF) return __builtin_bit_cast(float, (uint32_t)u << 16);
   else return (float)__builtin_bit_cast(_Float16, u);
 }
+template <bool BF>
+__device__ __forceinline__ uint16_t from_f32(float x) {
+  if constexpr (BF) return __builtin_bit_cast(uint16_t, (__bf16)x);
+  else return __builtin_bit_cast(uint16_t, (_Float16)x);
+}
+template <bool BF>
+__device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
+  if constexpr (BF) {
+    bf16x8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (__bf16)x[e];
+    return __builtin_bit_cast(u32x4, y);
+  } else {
+    f16x8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (_Float16)x[e];
+    return __builtin_bit_cast(u32x4, y);
+  }
+}
+template <bool BF>
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// Whether a pair of 16-bit floats holds an Inf or NaN: the exponent is all ones.
+template <bool BF>
+__device__ __forceinline__ bool pair_not_finite(uint32_t u) {
+  constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
+  return (u & e) == e || (u & (e << 16)) == e << 16;
+}
+
+// Max / sum over the four 16-lane rows of a wave, in every lane (as in q4d_attention.hip).
+template <bool SUM>
+__device__ __forceinline__ float rows4(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  const float x0 = __builtin_bit_cast(float, a0), x1 = __builtin_bit_cast(float, a1);
+  const float s = SUM ? x0 + x1 : fmaxf(x0, x1);
+  const uint32_t w = __builtin_bit_cast(uint32_t, s);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  const float y0 = __builtin_bit_cast(float, b0), y1 = __builtin_bit_cast(float, b1);
+  return SUM ? y0 + y1 : fmaxf(y0, y1);
+}
+
+__device__ __forceinline__ void store_dev(float* p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float load_dev(const float* p) {
+  return __hip_atomic_load(const_cast<float*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// 4 keys of one dim out of row-major rows in LDS: lane i of each 16 addresses 4 dims (8 bytes) of
+// key i / 4 and receives dim i of the four keys.
+__device__ __forceinline__ u32x2 read_tr4(const char* p) {
+  return __builtin_bit_cast(
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p)));
+}
+
+// `bytes` from p on as a buffer: loads past them give zeros and read nothing.
+// (p and bytes are the same in every lane, which the compiler does not always see.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* p, int bytes) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)u);
+  const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(lo | hi << 32), (short)0,
+                                           __builtin_amdgcn_readfirstlane(bytes), 0x00027000);
+}
+__device__ __forceinline__ u32x4 rows_load(__amdgpu_buffer_rsrc_t r, int offset) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 2));
+}
+
+// The running max moves only when a score exceeds it by more than this (log2 units): P = 2^(s - m)
+// stays below 2^8, far inside fp16's range, and the rescaling of the output is rare.
+constexpr float kRescale = 8.0f;
+
+// ---- up to 16 query rows a sequence --------------------------------------------------------
+// The work of a kv head is a line of steps of 128 positions, the sequences one after the other;
+// `blocks` blocks take S = ceil(steps / blocks) consecutive steps each, so every block streams as
+// many bytes whatever the lengths are (at least kMinSteps, so that a cut pays for its merge).  A
+// cut within `slack` steps of a sequence's end moves there.  A block's first and last sequences may
+// be parts: their softmax states go to the workspace (slot 1: the sequence begins in this block;
+// slot 0: it began in an earlier one), where they are joined.
+
+
+struct Cut {
+  int S, slack;
+};
+// A sequence's steps [lo, hi) of the line: the cuts inside are those of blocks first .. last.
+__device__ __forceinline__ int cut_first(const Cut& c, int lo) { return (lo + c.slack + c.S) / c.S; }
+__device__ __forceinline__ int cut_last(const Cut& c, int hi) { return (hi - c.slack - 1 + c.S) / c.S - 1; }
 
 template <int D, bool BF>
-__global__ __launch_bounds__(256) void paged_attn_simple(const PagedAttnArgs a) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int b = blockIdx.x;
-  const SeqSpan s = seq_span(a.p, a.r, b);
-  if (s.count <= 0) {
-    if (s.count < 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0)
-      atomicOr(a.p.status, Q4D_STATUS_BAD_SEQUENCE);
-    return;
-  }
-  const int h = blockIdx.y, j = h / (a.qh / a.p.kvh);
-  const int32_t* tab = a.p.table + (size_t)s.row * a.p.max_pages;
-  for (int i = blockIdx.z * 4 + w; i < s.count; i += 4 * gridDim.z) {
-    const size_t tok = s.first + i;
-    float q[E], o[E], m = -INFINITY, l = 0.f;
-    for (int e = 0; e < E; ++e) {
-      q[e] = to_f32<BF>(a.q[tok * a.q_stride + h * D + lane * E + e]) * a.scale;
-      o[e] = 0.f;
+__global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
+  constexpr int KS = D / 32, DT = D / 16, NV = D / 16, LR = D / 8;  // LR lanes of 16 bytes a row
+  constexpr int kRowBytes = 2 * D, kWaveBytes = 32 * kRowBytes;     // also 16 rows of D floats
+  __shared__ __attribute__((aligned(16))) char lds[4 * kWaveBytes];
+  __shared__ float sml[4][kRows][2];
+  __shared__ int s_sum[4], s_last;
+  extern __shared__ int s_end[];  // [n] steps of the sequences up to and with b, then [n] each of:
+  int* s_len = s_end + a.r.n;     // positions
+  int* s_first = s_len + a.r.n;   // first token row
+  int* s_row = s_first + a.r.n;   // table row and new tokens << 16
+  const int t = threadIdx.x, lane = t & 63;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kvh = a.p.kvh, G = a.qh / kvh;
+  const int k = blockIdx.x / kvh, j = blockIdx.x - k * kvh;
+
+  // ---- the cut -----------------------------------------------------------------------------
+  int W = 0;
+  bool bad = false;
+  for (int g = 0; g < a.r.n; g += 256) {
+    const int b = g + t;
+    int steps = 0;
+    if (b < a.r.n) {
+      const SeqSpan s = seq_span(a.p, a.r, b);
+      bad |= s.count < 0;
+      steps = s.count > 0 && s.count * G <= kRows ? (s.len + kStep - 1) / kStep : 0;
+      s_len[b] = s.len;
+      s_first[b] = s.first;
+      s_row[b] = s.row | s.count << 16;
     }
-    const int end = s.len - s.count + i + 1;
-    for (int pos = 0; pos < end; ++pos) {
-      const int page = tab[pos >> a.p.page_shift];
-      if (!in_range(page, a.p.num_pages)) {
-        if (lane == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_PAGE);
-        continue;
+    int x = steps;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int y = __shfl_up(x, m);
+      if (lane >= m) x += y;
+    }
+    if (g) block_sync_lds();  // the last round's sums have been read
+    if (lane == 63) s_sum[w] = x;
+    block_sync_lds();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      before += i < w ? s_sum[i] : 0;
+      all += s_sum[i];
+    }
+    if (b < a.r.n) s_end[b] = W + before + x;
+    W += all;
+  }
+  if (bad && blockIdx.x == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_SEQUENCE);
+  block_sync_lds();
+  W = __builtin_amdgcn_readfirstlane(W);
+  Cut c;
+  c.S = (W + a.blocks - 1) / a.blocks;
+  c.slack = min(c.S / 4, 2);
+  if (k * c.S >= W) return;
+  // the sequence whose steps hold step x < W
+  const auto lds_at = [&](const int* p) { return __builtin_amdgcn_readfirstlane(*p); };  // the same in every lane
+  const auto find = [&](int x) {
+    int lo = 0, hi = a.r.n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (lds_at(s_end + mid) > x) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+  };
+  const auto snap = [&](int x, int lo, int hi) {
+    if (x - lo <= c.slack && x - lo <= hi - x) return lo;
+    return hi - x <= c.slack ? hi : x;
+  };
+  int b = find(k * c.S);
+  const int from = snap(k * c.S, b ? lds_at(s_end + b - 1) : 0, lds_at(s_end + b));
+  int to = W;
+  if ((k + 1) * c.S < W) {
+    const int e = find((k + 1) * c.S);
+    to = snap((k + 1) * c.S, e ? lds_at(s_end + e - 1) : 0, lds_at(s_end + e));
+  }
+
+  const int r = lane & 15, g = lane >> 4;
+  char* vl = lds + w * kWaveBytes;
+  for (; b < a.r.n; ++b) {
+    const int lo = b ? lds_at(s_end + b - 1) : 0, hi = lds_at(s_end + b);
+    if (lo >= to) break;
+    const int x0 = max(lo, from), x1 = min(hi, to);
+    if (x0 >= x1) continue;
+    const int row_count = lds_at(s_row + b);
+    const SeqSpan s = {row_count & 0xFFFF, lds_at(s_first + b), row_count >> 16, lds_at(s_len + b)};
+    const int rows = s.count * G;
+    const int32_t* tab = a.p.table + (size_t)s.row * a.p.max_pages;
+    const int shift = a.p.page_shift, inpage = (1 << shift) - 1;
+    // this lane's query row, its last visible position, and the operand Q^T: dims 32 i + 8 g .. + 7
+    const int rr = min(r, rows - 1), tok = rr / G;
+    const int qpos = s.len - s.count + tok;
+    u32x4 q[KS];
+    {
+      const uint16_t* qp = a.q + (s.first + tok) * a.q_stride + (j * G + rr - tok * G) * D + 8 * g;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const u32x4*>(qp + 32 * i);
+    }
+    const int first_hidden = s.len - s.count + 1;  // positions from here on are hidden from some row
+
+    const int s0 = x0 - lo, s1 = x1 - lo;
+    struct Stage {
+      u32x4 k[2][KS], v[NV];
+      bool ok0, ok1;  // the first and second 16 positions' pages are there
+    } d;
+    // The page of lanes 0-31's and of lanes 32-63's 16 positions of step `it`.
+    const auto page_of = [&](int it) {
+      const int e = (it * kStep + 32 * w + ((lane & 32) >> 1)) >> shift;
+      return tab[min(e, a.p.max_pages - 1)];
+    };
+    int page = page_of(s0);
+    bool bad_page = false;
+    // Loads of step `it`, without a branch, so that the next steps' loads stay in flight while this
+    // one's are waited for: through descriptors that end with the sequence's last row (rows past it,
+    // of a page that is not there or of a step past the part's end are zeros and cost nothing).  K in
+    // operand order (score tile h row r is position 16 h + r), V row by row.
+    const auto issue = [&](int it) {
+      const int base = it * kStep + 32 * w;
+      const int p0 = __builtin_amdgcn_readlane(page, 0), p1 = __builtin_amdgcn_readlane(page, 32);
+      page = page_of(it + 1);
+      const int end = it < s1 ? s.len : 0;
+      const int n0 = min(max(end - base, 0), 16), n1 = min(max(end - base - 16, 0), 16);
+      d.ok0 = in_range(p0, a.p.num_pages);
+      d.ok1 = in_range(p1, a.p.num_pages);
+      bad_page |= (n0 && !d.ok0) || (n1 && !d.ok1);
+      const size_t o0 = page_elem(a.p, d.ok0 ? p0 : 0, j) + (size_t)(base & inpage) * D;
+      const size_t o1 = page_elem(a.p, d.ok1 ? p1 : 0, j) + (size_t)((base + 16) & inpage) * D;
+      const int b0 = d.ok0 ? n0 * kRowBytes : 0, b1 = d.ok1 ? n1 * kRowBytes : 0;
+      const auto k0 = rows_rsrc(a.kplane + o0, b0), k1 = rows_rsrc(a.kplane + o1, b1);
+      const auto v0 = rows_rsrc(a.vplane + o0, b0), v1 = rows_rsrc(a.vplane + o1, b1);
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        d.k[0][i] = rows_load(k0, r * kRowBytes + 16 * g + 64 * i);
+        d.k[1][i] = rows_load(k1, r * kRowBytes + 16 * g + 64 * i);
       }
-      const size_t at = page_elem(a.p, page, j) + (size_t)(pos & ((1 << a.p.page_shift) - 1)) * D + lane * E;
-      float x = 0.f;
-      for (int e = 0; e < E; ++e) x = fmaf(q[e], to_f32<BF>(a.kplane[at + e]), x);
-      x = wave_sum(x);
-      const float mn = fmaxf(m, x), f = m == -INFINITY ? 0.f : exp2f(m - mn), pr = exp2f(x - mn);
-      l = fmaf(l, f, pr);
-      for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], f, pr * to_f32<BF>(a.vplane[at + e]));
-      m = mn;
+#pragma unroll
+      for (int i = 0; i < NV / 2; ++i) {
+        d.v[i] = rows_load(v0, 16 * lane + 1024 * i);
+        d.v[NV / 2 + i] = rows_load(v1, 16 * lane + 1024 * i);
+      }
+    };
+
+    f32x4 o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;  // of query row r; l of this lane's positions only
+    const auto consume = [&](int it) {
+      const int base = it * kStep + 32 * w;
+      const bool ok0 = d.ok0, ok1 = d.ok1;
+      // an Inf or NaN in a V row that some query row does not see: position by position below
+      bool odd = false;
+      const bool hides = base + 32 > first_hidden;
+      if (hides && s.count > 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd |= pair_not_finite<BF>(d.v[i][e]);
+        odd = __ballot(odd) != 0;
+      }
+      // V into this wave's LDS rows: 32-byte chunk c of row x at c ^ f(x), f chosen so that the 16
+      // rows of a transposing read fall on all banks
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int row = i * (64 / LR) + lane / LR, slot = lane % LR;
+        const int f = D == 128 ? row & 7 : (row >> 1) & 3;
+        *reinterpret_cast<u32x4*>(vl + row * kRowBytes + ((slot ^ (f << 1)) << 4)) = d.v[i];
+      }
+      f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        st[0] = mfma16<BF>(d.k[0][i], q[i], st[0]);
+        st[1] = mfma16<BF>(d.k[1][i], q[i], st[1]);
+      }
+      issue(it + 1);
+      // this lane's positions: 4 g .. + 3 of either 16
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = st[e >> 2][e & 3] * a.scale;
+      if (hides || !ok0 || !ok1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (base + 16 * (e >> 2) + 4 * g + (e & 3) > qpos || !(e < 4 ? ok0 : ok1)) y[e] = -INFINITY;
+      }
+      float mx = y[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, y[e]);
+      mx = rows4<false>(mx);
+      const bool move = mx > m + kRescale || (m == -INFINITY && mx > m);
+      if (__ballot(move)) {
+        const float mn = move ? mx : m;
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][e] *= f;
+      }
+      const float ms = m == -INFINITY ? 0.f : m;
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(y[e] - ms);
+        l += p[e];
+      }
+      const u32x4 pp = pack8<BF>(p);
+      // V^T operand: dim 16 i + r, the same eight positions
+      const auto vt = [&](int i) {
+        u32x4 v;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = 16 * h + 4 * g + (r >> 2);
+          const int f = D == 128 ? row & 7 : (row >> 1) & 3;
+          const u32x2 x = read_tr4(vl + row * kRowBytes + ((i ^ f) << 5) + 8 * (r & 3));
+          v[2 * h] = x[0];
+          v[2 * h + 1] = x[1];
+        }
+        return v;
+      };
+      if (!odd) {
+#pragma unroll
+        for (int i = 0; i < DT; ++i) o[i] = mfma16<BF>(vt(i), pp, o[i]);
+      } else {
+        // 0 x Inf is NaN: each position by itself, added only where the row sees it
+        for (int x = 0; x < 32 && base + x < s.len; ++x) {
+          u32x4 keep;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            keep[e] = g == ((x & 15) >> 2) && e == 2 * (x >> 4) + ((x & 3) >> 1) ? (x & 1 ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
+#pragma unroll
+          for (int i = 0; i < DT; ++i) {
+            const f32x4 add = mfma16<BF>(vt(i) & keep, pp & keep, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[i][e] = base + x <= qpos ? o[i][e] + add[e] : o[i][e];
+          }
+        }
+      }
+    };
+    issue(s0);
+    for (int it = s0; it < s1; ++it) consume(it);
+    if (bad_page && lane == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_PAGE);
+
+    // ---- the four waves' states ----------------------------------------------------------------
+    l = rows4<true>(l);
+    if (g == 0) {
+      sml[w][r][0] = m;
+      sml[w][r][1] = l;
     }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    for (int e = 0; e < E; ++e) {
-      const float y = o[e] * inv;
-      a.out[tok * a.out_stride + h * D + lane * E + e] =
-          BF ? __builtin_bit_cast(uint16_t, (__bf16)y) : __builtin_bit_cast(uint16_t, (_Float16)y);
+    // lane holds O^T[dim 16 i + 4 g + e][row r]: 16-byte slot 4 i + g of row r at slot ^ r
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+      *reinterpret_cast<f32x4*>(vl + r * (4 * D) + (((4 * i + g) ^ r) << 4)) = o[i];
+    block_sync_lds();
+    const int row = t >> 4, sl = t & 15;  // D / 64 slots of 4 dims each: sl, sl + 16
+    constexpr int NS = D / 64;
+    float M = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) M = fmaxf(M, sml[i][row][0]);
+    float L = 0.f;
+    f32x4 acc[NS];
+#pragma unroll
+    for (int n = 0; n < NS; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float mi = sml[i][row][0], f = mi == -INFINITY ? 0.f : exp2f(mi - M);
+      L = fmaf(sml[i][row][1], f, L);
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(lds + i * kWaveBytes + row * (4 * D) + (((sl + 16 * n) ^ row) << 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][e] = mi == -INFINITY ? acc[n][e] : fmaf(x[e], f, acc[n][e]);
+      }
+    }
+    // The parts' states are joined eight at a time: of each eight the block that counts in last adds
+    // them in order and goes on with the sum as one of the next level's parts.
+    const int kf = cut_first(c, lo);
+    int count = max(0, cut_last(c, hi) - kf + 1) + 1, part = x0 == lo ? 0 : k - kf + 1;
+    // part 0 lies in block kf - 1's slot 1, part i in block kf - 1 + i's slot 0; a sum lies where its
+    // first part did, and its counter is that block's
+    for (int level = 0, step = 1; count > 1; ++level, step *= kJoin) {
+      const auto place = [&](int i) {
+        return (((size_t)(kf - 1 + i * step) * 2 + (i == 0)) * kvh + j) * kRows + row;
+      };
+      const int first = part / kJoin * kJoin, size = min(kJoin, count - first);
+      if (size > 1) {
+        if (row < rows) {
+          const size_t at = place(part);
+#pragma unroll
+          for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store_dev(a.pacc + at * D + 64 * n + 4 * sl + e, acc[n][e]);
+          if (sl == 0) {
+            store_dev(a.pml + at * 2, M);
+            store_dev(a.pml + at * 2 + 1, L);
+          }
+        }
+        __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are performed
+        __syncthreads();                // ... and every other thread's
+        int* counter = a.counters + level * kCounters + (kf - 1 + first * step) * kvh + j;
+        if (t == 0) s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == size - 1;
+        __syncthreads();
+        if (!s_last) break;
+        if (t == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // next call
+        if (row < rows) {
+          float mi[kJoin], li[kJoin];
+          f32x4 ai[kJoin][NS];
+#pragma unroll
+          for (int i = 0; i < kJoin; ++i) {
+            const size_t at = place(first + min(i, size - 1));
+            mi[i] = load_dev(a.pml + at * 2);
+            li[i] = load_dev(a.pml + at * 2 + 1);
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) ai[i][n][e] = load_dev(a.pacc + at * D + 64 * n + 4 * sl + e);
+          }
+          M = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kJoin; ++i) M = fmaxf(M, mi[i]);
+          L = 0.f;
+#pragma unroll
+          for (int n = 0; n < NS; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < kJoin; ++i) {
+            if (i >= size) continue;
+            const float f = mi[i] == -INFINITY ? 0.f : exp2f(mi[i] - M);
+            L = fmaf(li[i], f, L);
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[n][e] = mi[i] == -INFINITY ? acc[n][e] : fmaf(ai[i][n][e], f, acc[n][e]);
+          }
+        }
+      }
+      part = first / kJoin;
+      count = (count + kJoin - 1) / kJoin;
+    }
+    if (count == 1 && row < rows) {
+      const int otok = row / G;
+      uint16_t* op = a.out + (s.first + otok) * a.out_stride + (j * G + row - otok * G) * D + 4 * sl;
+      const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        const uint32_t u0 = from_f32<BF>(acc[n][0] * inv), u1 = from_f32<BF>(acc[n][1] * inv);
+        const uint32_t u2 = from_f32<BF>(acc[n][2] * inv), u3 = from_f32<BF>(acc[n][3] * inv);
+        *reinterpret_cast<u32x2*>(op + 64 * n) = u32x2{u0 | u1 << 16, u2 | u3 << 16};
+      }
+    }
+    block_sync_lds();  // the next sequence's V rows go where the states were
+  }
+}
+
+// ---- more rows ------------------------------------------------------------------------------
+// A block takes 128 query rows of a sequence for one kv head, a wave 32 of them, over a part of the
+// positions that they see, 64 at a time:
+//   S^T = K . Q^T (32x32x16 MFMA; K rows from LDS, Q^T in registers); online softmax per row; O^T +=
+//   V^T . P^T, where the S^T accumulators already are the operand layout of P^T (a lane holds 4 + 4
+//   keys of each 16 for one row) and V^T comes out of the row-major tile with the transposing read.
+// K and V tiles go from the pages to LDS by DMA one tile ahead, 16 rows a wave (one page at most).
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kTile = 128;  // query rows of a block
+constexpr int kKeys = 64;   // positions of a step
+
+template <bool BF>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Max / sum of lanes l and l ^ 32, in both.
+template <bool SUM>
+__device__ __forceinline__ float halves(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  const float x0 = __builtin_bit_cast(float, a0), x1 = __builtin_bit_cast(float, a1);
+  return SUM ? x0 + x1 : fmaxf(x0, x1);
+}
+
+// Lane i writes the 16 bytes at base + offset to LDS address lds + 16 i (lds, base wave-uniform).
+// Ordered by the kernel's own wait and barrier.
+__device__ __forceinline__ void dma16(const uint16_t* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base)
+               : "memory");
+}
+
+// The parts of a sequence's tiles: about as many steps each as fill the device's blocks once.
+struct Split {
+  int S;  // steps a part
+};
+__device__ __forceinline__ int split_parts(int steps, int S) { return max(1, (2 * steps + S) / (2 * S)); }
+
+template <int D, bool BF>
+__global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
+  constexpr int KS = D / 16, DT = D / 32, LR = D / 8;  // LR slots of 16 bytes a row
+  constexpr int kRowBytes = 2 * D, kPlane = kKeys * kRowBytes, kStage = 2 * kPlane;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
+  __shared__ int s_sum[2][4], s_last, s_odd[2][4];
+  extern __shared__ int s_end[];      // [n] items of the sequences up to and with b
+  int* s_split = s_end + a.r.n;       // [n] the same of sequences in parts
+  const int t = threadIdx.x, lane = t & 63;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int kvh = a.p.kvh, G = a.qh / kvh;
+  const int idx = blockIdx.x / kvh, j = blockIdx.x - idx * kvh;
+
+  // ---- which item ----------------------------------------------------------------------------
+  const auto tiles_of = [&](const SeqSpan& s) { return s.count * G > kRows ? (s.count * G + kTile - 1) / kTile : 0; };
+  const auto steps_of = [&](int len) { return (len + kKeys - 1) / kKeys; };
+  const auto block_scan = [&](int x, int y, int* ex, int* ey, int* allx, int* ally) {
+    int u = x, v = y;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int p = __shfl_up(u, m), q = __shfl_up(v, m);
+      if (lane >= m) {
+        u += p;
+        v += q;
+      }
+    }
+    block_sync_lds();  // the last round's sums have been read
+    if (lane == 63) {
+      s_sum[0][w] = u;
+      s_sum[1][w] = v;
+    }
+    block_sync_lds();
+    *ex = u; *ey = v; *allx = *ally = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *ex += i < w ? s_sum[0][i] : 0;
+      *ey += i < w ? s_sum[1][i] : 0;
+      *allx += s_sum[0][i];
+      *ally += s_sum[1][i];
+    }
+  };
+  int W = 0;
+  SeqSpan mine = {0, 0, 0, 0};
+  for (int g = 0; g < a.r.n; g += 256) {
+    const int b = g + t;
+    SeqSpan s = {0, 0, 0, 0};
+    if (b < a.r.n) s = seq_span(a.p, a.r, b);
+    const int n = tiles_of(s);
+    int ex, ey, aw, at;
+    block_scan((int)min((long long)n * steps_of(s.len), 1LL << 18), 0, &ex, &ey, &aw, &at);
+    W += aw;
+    if (g == 0) mine = s;
+  }
+  int S = max(kMinSplit, (W + a.slots - 1) / a.slots), items, splits;
+  for (;; S *= 2) {
+    items = splits = 0;
+    for (int g = 0; g < a.r.n; g += 256) {
+      const int b = g + t;
+      SeqSpan s = mine;
+      if (g && b < a.r.n) s = seq_span(a.p, a.r, b);
+      if (b >= a.r.n) s.count = 0;
+      const int parts = split_parts(steps_of(s.len), S), n = tiles_of(s) * parts;
+      int ex, ey, ax, ay;
+      block_scan(n, parts > 1 ? n : 0, &ex, &ey, &ax, &ay);
+      if (b < a.r.n) {
+        s_end[b] = items + ex;
+        s_split[b] = splits + ey;
+      }
+      items += ax;
+      splits += ay;
+    }
+    if (splits <= a.max_splits) break;  // (always, but for steps beyond what W counts)
+  }
+  block_sync_lds();
+  if (idx >= items) return;
+  const auto lds_at = [&](const int* p) { return __builtin_amdgcn_readfirstlane(*p); };
+  int b = 0;
+  for (int hi = a.r.n - 1; b < hi;) {
+    const int mid = (b + hi) >> 1;
+    if (lds_at(s_end + mid) > idx) hi = mid; else b = mid + 1;
+  }
+  SeqSpan s = seq_span(a.p, a.r, b);
+  s.row = __builtin_amdgcn_readfirstlane(s.row);
+  s.first = __builtin_amdgcn_readfirstlane(s.first);
+  s.count = __builtin_amdgcn_readfirstlane(s.count);
+  s.len = __builtin_amdgcn_readfirstlane(s.len);
+  const int parts = split_parts(steps_of(s.len), S), nt = tiles_of(s);
+  const int in = idx - (lds_at(s_end + b) - nt * parts);
+  // the last tiles, which see the most, first
+  const int tile = nt - 1 - in / parts, part = in % parts;
+  const int rows = s.count * G, row0 = tile * kTile + 32 * w;  // this wave's first row
+  const int old = s.len - s.count;
+  const int kend = old + (min(rows, (tile + 1) * kTile) - 1) / G + 1;
+  const int steps = steps_of(kend), st0 = part * steps / parts, st1 = (part + 1) * steps / parts;
+  const bool active = row0 < rows;  // the wave has rows
+
+  // Q^T operand: lane (row l % 32, half l / 32) holds dims 16 i + 8 half .. + 7
+  const int qc = lane & 31, hf = lane >> 5;
+  const int row = min(row0 + qc, rows - 1), tok = row / G, head = j * G + row - tok * G;
+  const int qpos = old + tok;
+  const int first_hidden = old + min(row0, rows - 1) / G + 1;  // hidden from some row of the wave
+  u32x4 q[KS];
+  {
+    const uint16_t* qp = a.q + (s.first + tok) * a.q_stride + head * D + 8 * hf;
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      q[i] = *reinterpret_cast<const u32x4*>(qp + 16 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[i][e] ^= flip;
     }
   }
+  // (a scale of 0 keeps masked scores at -Inf)
+  const float scale = fmaxf(fabsf(a.scale), 1e-30f);
+
+  // ---- K / V tiles ---------------------------------------------------------------------------
+  const int32_t* tab = a.p.table + (size_t)s.row * a.p.max_pages;
+  const int shift = a.p.page_shift, inpage = (1 << shift) - 1;
+  const auto pages_at = [&](int st) {  // lanes 16 i ..: the page of the step's 16 i .. + 15
+    const int pos = st * kKeys + 16 * (lane >> 4);
+    return tab[min(pos >> shift, a.p.max_pages - 1)];
+  };
+  constexpr int RI = 64 / LR;  // rows a DMA instruction
+  const int drow = lane / LR, dslot = lane % LR;
+  const auto kswz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
+  const auto vswz = [](int r) { return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  int pages = pages_at(st0);
+  uint64_t gone = 0;  // 16-row groups of the tile last issued whose page is not there (bits 16 i)
+  bool bad_page = false;
+  const auto issue = [&](int st, int sg) {
+    const int pos = st * kKeys + 16 * w;
+    const int page = __builtin_amdgcn_readlane(pages, 16 * w);
+    gone = __ballot(!in_range(pages, a.p.num_pages) && st * kKeys + 16 * (lane >> 4) < kend);
+    char* to = lds + sg * kStage + 16 * w * kRowBytes;
+    if (pos >= kend || !in_range(page, a.p.num_pages)) {  // nothing there: zeros
+      bad_page |= pos < kend;
+#pragma unroll
+      for (int i = 0; i < 16 / RI; ++i) {
+        *reinterpret_cast<u32x4*>(to + i * 1024 + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+        *reinterpret_cast<u32x4*>(to + kPlane + i * 1024 + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+      }
+    } else {
+      const size_t at = page_elem(a.p, page, j) + (size_t)(pos & inpage) * D;
+      const uint16_t* kp = a.kplane + at;
+      const uint16_t* vp = a.vplane + at;
+      const uint32_t l0 = __builtin_amdgcn_readfirstlane(lds0 + sg * kStage + 16 * w * kRowBytes);
+      const int last = kend - 1 - pos;  // rows past the last position repeat it (masked)
+#pragma unroll
+      for (int i = 0; i < 16 / RI; ++i) {
+        const int r = i * RI + drow, from = min(r, last) * kRowBytes;
+        dma16(kp, from + ((dslot ^ kswz(r)) << 4), l0 + i * 1024);
+        dma16(vp, from + ((dslot ^ vswz(r)) << 4), l0 + kPlane + i * 1024);
+      }
+    }
+  };
+  uint32_t ko[KS], vo[DT];  // K: row l % 32, slot 2 i + half; V: 4 dims of key 4 half + l % 16 / 4
+#pragma unroll
+  for (int i = 0; i < KS; ++i) ko[i] = qc * kRowBytes + (((2 * i + hf) ^ kswz(qc)) << 4);
+  {
+    const int i = lane & 15, key = 4 * hf + (i >> 2), db = (lane >> 4) & 1;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      vo[dt] = kPlane + key * kRowBytes + (((4 * dt + 2 * db + ((i >> 1) & 1)) ^ vswz(key)) << 4) + 8 * (i & 1);
+  }
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+  float m = -INFINITY, l = 0.f;  // l of this lane's keys only
+
+  if (st0 < st1) issue(st0, 0);
+  pages = pages_at(st0 + 1);
+  for (int st = st0; st < st1; ++st) {
+    const int sg = (st - st0) & 1, key0 = st * kKeys;
+    const uint64_t none = gone;
+    const bool edge = key0 + kKeys > old + tile * kTile / G + 1;  // hidden from some row of the block
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) expcnt(7) lgkmcnt(0): this wave's rows are there
+    if (edge) {  // an Inf or NaN among these V rows?
+      uint32_t top = 0;
+      typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+      us2 mx = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 16 / RI; ++i) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(lds + sg * kStage + kPlane + 16 * w * kRowBytes + i * 1024 + 16 * lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = __builtin_elementwise_max(mx, __builtin_bit_cast(us2, v[e] & 0x7FFF7FFFu));
+      }
+      top = max(mx.x, mx.y);
+      const bool odd = __ballot(top >= (BF ? 0x7F80u : 0x7C00u)) != 0;
+      if (lane == 0) s_odd[sg][w] = odd;
+      __builtin_amdgcn_s_waitcnt(0xc07f);
+    }
+    __builtin_amdgcn_s_barrier();  // everybody's rows are there, and the other stage is read
+    asm volatile("" ::: "memory");
+    if (st + 1 < st1) {
+      issue(st + 1, sg ^ 1);
+      pages = pages_at(st + 2);
+    }
+    if (!active || key0 > old + min(row0 + 31, rows - 1) / G) continue;  // nothing the wave's rows see
+    const char* stage = lds + sg * kStage;
+
+    f32x16 x[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[h][r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        x[h] = mfma32<BF>(*reinterpret_cast<const u32x4*>(stage + ko[i] + 32 * h * kRowBytes), q[i], x[h]);
+    // lane holds keys 32 h + 8 (r / 4) + 4 half + r % 4
+    if (key0 + kKeys > first_hidden || none) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = 32 * h + 8 * (r >> 2) + 4 * hf + (r & 3);
+          if (key0 + key > qpos || (none >> (16 * (2 * h + (r >> 3))) & 1)) x[h][r] = -INFINITY;
+        }
+    }
+    float mx = x[0][0];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[h][r]);
+    mx = halves<false>(mx) * scale;
+    const bool move = mx > m + kRescale || (m == -INFINITY && mx > m);
+    if (__ballot(move)) {
+      const float mn = move ? mx : m;
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+    }
+    const float ms = m == -INFINITY ? 0.f : m;
+    u32x4 p[4];
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float e[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        e[k] = __builtin_amdgcn_exp2f(fmaf(x[i >> 1][8 * (i & 1) + k], scale, -ms));
+        sum += e[k];
+      }
+      p[i] = pack8<BF>(e);
+    }
+    l += sum;
+    // V^T operand: dim 32 dt + l % 32, the lane's eight keys of 16 i ..
+    const auto vt = [&](int i, int dt) {
+      const u32x2 v0 = read_tr4(stage + vo[dt] + 16 * i * kRowBytes);
+      const u32x2 v1 = read_tr4(stage + vo[dt] + (16 * i + 8) * kRowBytes);
+      return u32x4{v0[0], v0[1], v1[0], v1[1]};
+    };
+    const bool odd = edge && (s_odd[sg][0] | s_odd[sg][1] | s_odd[sg][2] | s_odd[sg][3]);
+    if (!odd) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32<BF>(vt(i, dt), p[i], o[dt]);
+    } else {
+      // 0 x Inf is NaN: each position by itself, added only where the row sees it
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        for (int k = 0; k < 16 && key0 + 16 * i + k < kend; ++k) {
+          u32x4 keep;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            keep[e] = hf == ((k >> 2) & 1) && e == 2 * (k >> 3) + ((k & 3) >> 1) ? (k & 1 ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            f32x16 add;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) add[r] = 0.f;
+            add = mfma32<BF>(vt(i, dt) & keep, p[i] & keep, add);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[dt][r] = key0 + 16 * i + k <= qpos ? o[dt][r] + add[r] : o[dt][r];
+          }
+        }
+      }
+    }
+  }
+  if (bad_page && lane == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_PAGE);
+  l = halves<true>(l);
+
+  // ---- parts, joined as in rows_kernel; a lane's values lie 64 floats apart ---------------------
+  int count = parts, at_part = part;
+  const int slot0 = parts > 1 ? (lds_at(s_split + b) - nt * parts) + (in - part) : 0;
+  for (int level = 0, step = 1; count > 1; ++level, step *= kJoin) {
+    const int first = at_part / kJoin * kJoin, size = min(kJoin, count - first);
+    const auto place = [&](int i) { return ((size_t)(slot0 + i * step) * kvh + j) * 4 + w; };
+    if (size > 1) {
+      if (active) {
+        float* acc = a.cacc + place(at_part) * (32 * D) + lane;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) store_dev(acc + 64 * (16 * dt + r), o[dt][r]);
+        store_dev(a.cml + place(at_part) * 64 + lane, hf ? l : m);
+      }
+      __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are performed
+      __syncthreads();                // ... and every other thread's
+      int* counter = a.ccounters + level * kChunkCounters + (slot0 + first * step) * kvh + j;
+      if (t == 0) s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == size - 1;
+      __syncthreads();
+      if (!s_last) return;
+      if (t == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // next call
+      if (active) {
+        const auto ml = [&](int i) { return a.cml + place(first + i) * 64 + qc; };
+        float M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kJoin; ++i) M = fmaxf(M, load_dev(ml(min(i, size - 1))));
+        l = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+        for (int i = 0; i < size; ++i) {
+          const float mv = load_dev(ml(i)), f = mv == -INFINITY ? 0.f : exp2f(mv - M);
+          l = fmaf(load_dev(ml(i) + 32), f, l);
+          const float* acc = a.cacc + place(first + i) * (32 * D) + lane;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float v = load_dev(acc + 64 * (16 * dt + r));
+              o[dt][r] = mv == -INFINITY ? o[dt][r] : fmaf(v, f, o[dt][r]);
+            }
+        }
+        m = M;
+      }
+      __syncthreads();  // s_last has been read
+    }
+    at_part = first / kJoin;
+    count = (count + kJoin - 1) / kJoin;
+  }
+
+  // ---- rows out, through LDS -------------------------------------------------------------------
+  __syncthreads();  // everybody is done with the tiles
+  if (!active) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  char* T0 = lds + w * (32 * kRowBytes);  // 32 rows of D values, slot s of row r at s ^ (r & (LR - 1))
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u0 = from_f32<BF>(o[dt][4 * i] * inv), u1 = from_f32<BF>(o[dt][4 * i + 1] * inv);
+      const uint32_t u2 = from_f32<BF>(o[dt][4 * i + 2] * inv), u3 = from_f32<BF>(o[dt][4 * i + 3] * inv);
+      *reinterpret_cast<u32x2*>(T0 + qc * kRowBytes + (((4 * dt + i) ^ (qc & (LR - 1))) << 4) + 8 * hf) =
+          u32x2{u0 | u1 << 16, u2 | u3 << 16};
+    }
+#pragma unroll
+  for (int i = 0; i < 32 / RI; ++i) {
+    const int r = i * RI + drow, rr = row0 + r;
+    if (rr >= rows) continue;
+    const int tk = rr / G;
+    *reinterpret_cast<u32x4*>(a.out + (s.first + tk) * a.out_stride + (j * G + rr - tk * G) * D + 8 * dslot) =
+        *reinterpret_cast<const u32x4*>(T0 + r * kRowBytes + ((dslot ^ (r & (LR - 1))) << 4));
+  }
+}
+
+// Blocks per kv head of rows_kernel.
+int rows_blocks(int kvh) { return max(1, min(device_cus(), kCounters) / kvh); }
+// Blocks per kv head that chunk_kernel's parts are to fill: two a CU.  Sequences in parts have 4/3
+// of that many at most: P = round(steps / S) parts of a tile are at most steps / S + 1/2, and P >= 2
+// says that steps / S >= 3/2.
+int chunk_slots(int kvh) { return max(1, 2 * min(device_cus(), kChunkCounters / 4) / kvh); }
+int chunk_splits(int kvh) { return chunk_slots(kvh) * 4 / 3 + 1; }
+
+// The counters lie at the same place for every shape, since calls of several may share a workspace.
+struct Layout {
+  size_t pml, pacc, cml, cacc, total;
+};
+Layout layout(int kvh, int d, bool chunks) {
+  Layout l;
+  const size_t slots = 2 * (size_t)rows_blocks(kvh) * kvh, items = chunks ? (size_t)chunk_splits(kvh) * kvh : 0;
+  l.pml = paged_attention_ws_counters();
+  l.pacc = l.pml + align_up(slots * kRows * 2 * 4, 256);
+  l.cml = l.pacc + align_up(slots * kRows * d * 4, 256);
+  l.cacc = l.cml + align_up(items * kTile * 2 * 4, 256);
+  l.total = l.cacc + items * kTile * d * 4;
+  return l;
+}
+bool has_chunks(int qh, int kvh, int max_new) { return (long long)max_new * (qh / kvh) > kRows; }
+
+template <int D, bool BF>
+int launch(const PagedAttnArgs& a, hipStream_t st) {
+  const int kvh = a.p.kvh, G = a.qh / kvh;
+  hipLaunchKernelGGL((rows_kernel<D, BF>), dim3(a.blocks * kvh), dim3(256), a.r.n * 16, st, a);
+  int rc = check_launch();
+  if (rc || !has_chunks(a.qh, kvh, a.r.max_new)) return rc;
+  // items: a sequence's tiles are at most its rows / 128, rounded up; those in parts at most chunk_splits
+  const long long items = (long long)a.r.tokens * G / kTile + a.r.n + chunk_splits(kvh);
+  if (items * kvh > INT32_MAX) return Q4D_ERR_SHAPE;
+  hipLaunchKernelGGL((chunk_kernel<D, BF>), dim3((unsigned)(items * kvh)), dim3(256), a.r.n * 8, st, a);
+  return check_launch();
 }
 
 }  // namespace
 
-size_t paged_attention_ws_bytes(int, int, int, int, int, int) { return 256; }
+size_t paged_attention_ws_counters() { return (kLevels * kCounters + kLevels * kChunkCounters) * 4; }
+size_t paged_attention_ws_bytes(int kvh, int d, int qh, int, int, int max_new) {
+  return layout(kvh, d, has_chunks(qh, kvh, max_new)).total;
+}
 
-int launch_paged_attention(const PagedAttnArgs& a, hipStream_t st) {
-  const dim3 grid(a.r.n, a.qh, (unsigned)min((a.r.max_new + 3) / 4, 1024));
-  if (a.p.d == 128) {
-    if (a.bf16) hipLaunchKernelGGL((paged_attn_simple<128, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((paged_attn_simple<128, false>), grid, dim3(256), 0, st, a);
-  } else {
-    if (a.bf16) hipLaunchKernelGGL((paged_attn_simple<64, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((paged_attn_simple<64, false>), grid, dim3(256), 0, st, a);
-  }
-  return check_launch();
+int launch_paged_attention(const PagedAttnArgs& args, hipStream_t st) {
+  PagedAttnArgs a = args;
+  const Layout l = layout(a.p.kvh, a.p.d, has_chunks(a.qh, a.p.kvh, a.r.max_new));
+  a.counters = ws_ptr<int>(a.ws, 0);
+  a.ccounters = a.counters + kLevels * kCounters;
+  a.pml = ws_ptr<float>(a.ws, l.pml);
+  a.pacc = ws_ptr<float>(a.ws, l.pacc);
+  a.cml = ws_ptr<float>(a.ws, l.cml);
+  a.cacc = ws_ptr<float>(a.ws, l.cacc);
+  a.blocks = rows_blocks(a.p.kvh);
+  a.slots = chunk_slots(a.p.kvh);
+  a.max_splits = chunk_splits(a.p.kvh);
+  if (a.p.d == 128) return a.bf16 ? launch<128, true>(a, st) : launch<128, false>(a, st);
+  return a.bf16 ? launch<64, true>(a, st) : launch<64, false>(a, st);
 }
 
 }  // namespace q4d

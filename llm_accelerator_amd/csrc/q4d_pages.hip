@@ -698,7 +698,9 @@ size_t q4d_paged_attention_workspace_bytes(const q4d_pages_t* pages, int32_t q_h
 int q4d_paged_attention_workspace_init(void* ws, size_t ws_bytes, void* stream) {
   if (!ws) return Q4D_ERR_NULL;
   if (!aligned(ws, 256)) return Q4D_ERR_BAD_ADDR;
-  return launch_fill_i32(static_cast<int32_t*>(ws), 0, ws_bytes / 4, reinterpret_cast<hipStream_t>(stream));
+  const size_t n = paged_attention_ws_counters();
+  if (ws_bytes < n) return Q4D_ERR_CAPACITY;
+  return launch_fill_i32(static_cast<int32_t*>(ws), 0, n / 4, reinterpret_cast<hipStream_t>(stream));
 }
 
 int q4d_paged_attention(const q4d_pages_t* pages, int32_t layer, const q4d_ragged_t* batch, const void* q,
@@ -709,7 +711,7 @@ int q4d_paged_attention(const q4d_pages_t* pages, int32_t layer, const q4d_ragge
   if (!q || !out || !ws) return Q4D_ERR_NULL;
   if (layer < 0 || layer >= pages->num_layers) return Q4D_ERR_BAD_LAYER;
   const int kvh = pages->num_kv_heads, d = pages->head_dim;
-  if (q_heads <= 0 || q_heads % kvh || q_heads / kvh > 16) return Q4D_ERR_SHAPE;
+  if (q_heads <= 0 || q_heads % kvh || q_heads / kvh > 16 || !__builtin_isfinite(scaling)) return Q4D_ERR_SHAPE;
   if (q_stride < (int64_t)q_heads * d || out_stride < (int64_t)q_heads * d || q_stride > INT64_C(1) << 32 ||
       out_stride > INT64_C(1) << 32)
     return Q4D_ERR_SHAPE;

@@ -7,7 +7,7 @@ import torch
 
 import paged_ref
 from llm_accelerator_amd import _lib
-from llm_accelerator_amd.paged import PagedKVCache, RaggedBatch
+from llm_accelerator_amd.paged import PagedKVCache, PagedWorkspace, RaggedBatch
 
 pytestmark = pytest.mark.gpu
 F, B = torch.float16, torch.bfloat16
@@ -248,6 +248,11 @@ def test_python_refusals(dev):
         with pytest.raises(_lib.Q4DecError) as e:
             cache.attention(**{"layer": 0, "batch": batch, "q": q, **kw})
         assert e.value.code == err
+    small = PagedWorkspace(cache, 4, 1, 1, 1)          # of decode steps: too small for a chunk
+    chunk = RaggedBatch.of([0], [20], dev)
+    with pytest.raises(_lib.Q4DecError) as e:
+        cache.attention(0, chunk, torch.zeros(20, 4, 64, dtype=F, device=dev), ws=small)
+    assert e.value.code == -9
     with pytest.raises(ValueError):
         cache.attention(0, RaggedBatch(None, i32([0, 1, 2, 3], dev), 3, 1), q)   # three sequences, two rows
     with pytest.raises(ValueError):
@@ -340,3 +345,32 @@ def test_offsets_past_32_bits(dev):
         at = torch.arange(500 - new, 500, device=dev)
         assert torch.equal(data[0, 1, table[1, at // ps].long(), :, at % ps], -kv)
         compare(cache, batch, q, cache.attention(0, batch, q), d ** -0.5)
+
+
+@pytest.mark.parametrize("scaling", [0.0, -0.2, 3.0])
+def test_any_finite_scaling(dev, scaling):
+    cache = filled(dev, [90, 200], 2, 64, 16, F)
+    for counts in ([1, 1], [40, 3]):
+        batch = RaggedBatch.of([0, 1], counts, dev)
+        q = torch.randn(batch.tokens, 6, 64, device=dev, generator=torch.Generator(device=dev).manual_seed(5)).half()
+        compare(cache, batch, q, cache.attention(0, batch, q, scaling), scaling)
+
+
+def test_one_workspace_for_calls_of_every_shape(dev):
+    """The counters that a call finds are those the one before left, whatever its shape was."""
+    caches = [filled(dev, [3000, 700, 90], 2, 128, 16, F), filled(dev, [2000, 50, 1200, 800], 5, 64, 32, F),
+              filled(dev, [1500], 1, 128, 64, B)]
+    ws = PagedWorkspace(caches[0], 32, 4, 400, 400)
+    for cache in caches:
+        big = PagedWorkspace(cache, 16 * cache.num_kv_heads, 4, 400, 400)
+        ws = big if big.nbytes > ws.nbytes else ws
+    jobs = []
+    for i, (counts, qh) in enumerate([([1, 1, 1], 4), ([1] * 4, 15), ([1], 16), ([5, 60, 1], 8), ([100, 2, 1, 33], 5), ([300], 3),
+                                      ([8, 8, 8], 4), ([3, 3, 3, 3], 80)]):
+        cache = caches[2 if len(counts) == 1 else len(counts) - 3]
+        batch = RaggedBatch.of(list(range(len(counts))), counts, dev)
+        q = torch.randn(batch.tokens, qh, cache.head_dim, device=dev).to(cache.dtype)
+        jobs.append((cache, batch, q, cache.attention(0, batch, q)))
+    for order in (jobs, jobs[::-1], jobs[1:] + jobs[:1]):
+        for cache, batch, q, want in order:
+            assert torch.equal(cache.attention(0, batch, q, ws=ws), want)

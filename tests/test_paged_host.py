@@ -103,7 +103,8 @@ def test_append_refuses_rotations(change, code):
 @pytest.mark.parametrize("arg,value,code", [
     (1, 2, LAYER), (1, -1, LAYER), (3, None, NULL), (7, None, NULL), (9, None, NULL), (5, 12, SHAPE), (5, 0, SHAPE),
     (5, 136, SHAPE), (4, 2040, SHAPE), (8, 2040, SHAPE), (8, 1 << 33, SHAPE), (4, 2052, ADDR), (8, 2049, ADDR),
-    (3, FAKE + 8, ADDR), (7, FAKE + 2, ADDR), (9, FAKE + 128, ADDR), (10, 16, CAPACITY)])
+    (3, FAKE + 8, ADDR), (7, FAKE + 2, ADDR), (9, FAKE + 128, ADDR), (10, 16, CAPACITY), (6, float("nan"), SHAPE),
+    (6, float("inf"), SHAPE)])
 def test_attention_refuses(arg, value, code):
     args = [ctypes.byref(pages()), 0, ctypes.byref(ragged()), FAKE, 2048, 16, 0.1, FAKE, 2048, FAKE, 1 << 40, None]
     args[arg] = value
