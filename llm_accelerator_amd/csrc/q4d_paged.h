@@ -48,6 +48,19 @@ __host__ __device__ inline SeqSpan seq_span(const PagedView& p, const RaggedView
   return s;
 }
 
+#ifdef __HIPCC__
+// Inclusive sum over the lanes of a wave (DPP row shifts, then the row totals).
+__device__ __forceinline__ int wave_incl(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast 15 into rows 1, 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast 31 into rows 2, 3
+  return x;
+}
+#endif
+
 // Elements of one (layer, K or V) plane, and the first element of a page's rows of kv head j.
 __host__ __device__ inline size_t plane_elems(const PagedView& p) {
   return ((size_t)p.num_pages * p.kvh * p.d) << p.page_shift;
