@@ -647,6 +647,13 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
   const auto kswz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
   const auto vswz = [](int r) { return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+  uint32_t kfrom[16 / RI], vfrom[16 / RI];  // slot s of row r is column group s ^ swz(r)
+#pragma unroll
+  for (int i = 0; i < 16 / RI; ++i) {
+    const int r = i * RI + drow;
+    kfrom[i] = r * kRowBytes + ((dslot ^ kswz(r)) << 4);
+    vfrom[i] = r * kRowBytes + ((dslot ^ vswz(r)) << 4);
+  }
   int pages = pages_at(st0);
   uint64_t gone = 0;  // 16-row groups of the tile last issued whose page is not there (bits 16 i)
   bool bad_page = false;
@@ -667,12 +674,20 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
       const uint16_t* kp = a.kplane + at;
       const uint16_t* vp = a.vplane + at;
       const uint32_t l0 = __builtin_amdgcn_readfirstlane(lds0 + sg * kStage + 16 * w * kRowBytes);
-      const int last = kend - 1 - pos;  // rows past the last position repeat it (masked)
+      const int last = kend - 1 - pos;
+      if (last >= 15) {
 #pragma unroll
-      for (int i = 0; i < 16 / RI; ++i) {
-        const int r = i * RI + drow, from = min(r, last) * kRowBytes;
-        dma16(kp, from + ((dslot ^ kswz(r)) << 4), l0 + i * 1024);
-        dma16(vp, from + ((dslot ^ vswz(r)) << 4), l0 + kPlane + i * 1024);
+        for (int i = 0; i < 16 / RI; ++i) {
+          dma16(kp, kfrom[i], l0 + i * 1024);
+          dma16(vp, vfrom[i], l0 + kPlane + i * 1024);
+        }
+      } else {  // rows past the last position repeat it (masked)
+#pragma unroll
+        for (int i = 0; i < 16 / RI; ++i) {
+          const uint32_t up = max(i * RI + drow - last, 0) * kRowBytes;
+          dma16(kp, kfrom[i] - up, l0 + i * 1024);
+          dma16(vp, vfrom[i] - up, l0 + kPlane + i * 1024);
+        }
       }
     }
   };
@@ -788,24 +803,29 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32<BF>(vt(i, dt), p[i], o[dt]);
     } else {
-      // 0 x Inf is NaN: each position by itself, added only where the row sees it
+      // 0 x Inf is NaN: position by position, added only where the row sees it (plain arithmetic: it
+      // needs no registers beside the loop's)
+      for (int k = 0; k < kKeys && key0 + k < kend; ++k) {
+        const int word = 4 * (k >> 4) + 2 * ((k >> 3) & 1) + ((k >> 1) & 1);
+        uint32_t u = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        for (int k = 0; k < 16 && key0 + 16 * i + k < kend; ++k) {
-          u32x4 keep;
+        for (int i = 0; i < 16; ++i) u = i == word ? p[i >> 2][i & 3] : u;
+        const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const uint32_t u0 = both[0], u1 = both[1];
+        u = (k >> 2) & 1 ? u1 : u0;  // the half of the wave that holds the position
+        const float pk = to_f32<BF>((uint16_t)(k & 1 ? u >> 16 : u));
+        const bool sees = key0 + k <= qpos;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            keep[e] = hf == ((k >> 2) & 1) && e == 2 * (k >> 3) + ((k & 3) >> 1) ? (k & 1 ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            f32x16 add;
+          for (int i = 0; i < 4; ++i) {
+            const u32x2 v = *reinterpret_cast<const u32x2*>(stage + kPlane + k * kRowBytes + (((4 * dt + i) ^ vswz(k)) << 4) + 8 * hf);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) add[r] = 0.f;
-            add = mfma32<BF>(vt(i, dt) & keep, p[i] & keep, add);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[dt][r] = key0 + 16 * i + k <= qpos ? o[dt][r] + add[r] : o[dt][r];
+            for (int e = 0; e < 4; ++e) {
+              const float ve = to_f32<BF>((uint16_t)(e & 1 ? v[e >> 1] >> 16 : v[e >> 1]));
+              o[dt][4 * i + e] = sees ? fmaf(pk, ve, o[dt][4 * i + e]) : o[dt][4 * i + e];
+            }
           }
-        }
       }
     }
   }
