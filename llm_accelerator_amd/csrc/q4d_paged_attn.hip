@@ -6,6 +6,8 @@
 // read: chunk_kernel.
 #include <math.h>
 
+#include <type_traits>
+
 #include "q4d_device.h"
 #include "q4d_paged.h"
 
@@ -56,12 +58,21 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-// Whether a pair of 16-bit floats holds an Inf or NaN: the exponent is all ones.
+// Inf and NaN (the exponent is all ones) among eight 16-bit floats become 0; whether there were any.
+// A row that does not see such a value gives it the weight 0, and 0 x Inf is NaN.
 template <bool BF>
-__device__ __forceinline__ bool pair_not_finite(uint32_t u) {
+__device__ __forceinline__ bool drop_odd(u32x4& v) {
   constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
-  return (u & e) == e || (u & (e << 16)) == e << 16;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool lo = (v[i] & e) == e, hi = (v[i] & e << 16) == e << 16;
+    v[i] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+    odd |= lo || hi;
+  }
+  return odd;
 }
+__device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
 
 // Max / sum over the four 16-lane rows of a wave, in every lane (as in q4d_attention.hip).
 template <bool SUM>
@@ -236,7 +247,7 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
       return tab[min(e, a.p.max_pages - 1)];
     };
     int page = page_of(s0);
-    bool bad_page = false;
+    bool bad_page = false, odd = false;
     // Loads of step `it`, without a branch, so that the next steps' loads stay in flight while this
     // one's are waited for: through descriptors that end with the sequence's last row (rows past it,
     // of a page that is not there or of a step past the part's end are zeros and cost nothing).  K in
@@ -274,15 +285,10 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
     const auto consume = [&](int it) {
       const int base = it * kStep + 32 * w;
       const bool ok0 = d.ok0, ok1 = d.ok1;
-      // an Inf or NaN in a V row that some query row does not see: position by position below
-      bool odd = false;
       const bool hides = base + 32 > first_hidden;
-      if (hides && s.count > 1) {
+      if (hides && s.count > 1) {  // Inf and NaN become zeros; they are added after the loop
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) odd |= pair_not_finite<BF>(d.v[i][e]);
-        odd = __ballot(odd) != 0;
+        for (int i = 0; i < NV; ++i) odd |= drop_odd<BF>(d.v[i]);
       }
       // V into this wave's LDS rows: 32-byte chunk c of row x at c ^ f(x), f chosen so that the 16
       // rows of a transposing read fall on all banks
@@ -344,27 +350,31 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
         }
         return v;
       };
-      if (!odd) {
 #pragma unroll
-        for (int i = 0; i < DT; ++i) o[i] = mfma16<BF>(vt(i), pp, o[i]);
-      } else {
-        // 0 x Inf is NaN: each position by itself, added only where the row sees it
-        for (int x = 0; x < 32 && base + x < s.len; ++x) {
-          u32x4 keep;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            keep[e] = g == ((x & 15) >> 2) && e == 2 * (x >> 4) + ((x & 3) >> 1) ? (x & 1 ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
-#pragma unroll
-          for (int i = 0; i < DT; ++i) {
-            const f32x4 add = mfma16<BF>(vt(i) & keep, pp & keep, f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][e] = base + x <= qpos ? o[i][e] + add[e] : o[i][e];
-          }
-        }
-      }
+      for (int i = 0; i < DT; ++i) o[i] = mfma16<BF>(vt(i), pp, o[i]);
     };
     issue(s0);
     for (int it = s0; it < s1; ++it) consume(it);
+    if (__ballot(odd)) {
+      // this wave's positions that some row does not see (weight 1 does as well as the probability: what
+      // is added is Inf or NaN)
+      for (int it = max(s0, first_hidden / kStep); it < s1; ++it) {
+        const int base = it * kStep + 32 * w;
+        if (base + 32 <= first_hidden) continue;
+        for (int pos = base; pos < min(s.len, base + 32); ++pos) {
+          const int pg = tab[min(pos >> shift, a.p.max_pages - 1)];
+          if (!in_range(pg, a.p.num_pages)) continue;
+          const uint16_t* v = a.vplane + page_elem(a.p, pg, j) + (size_t)(pos & inpage) * D + 4 * g;
+#pragma unroll
+          for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = to_f32<BF>(v[16 * i + e]);
+              if (pos <= qpos && not_finite(x)) o[i][e] += x;
+            }
+        }
+      }
+    }
     if (bad_page && lane == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_PAGE);
 
     // ---- the four waves' states ----------------------------------------------------------------
@@ -525,7 +535,7 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
   constexpr int KS = D / 16, DT = D / 32, LR = D / 8;  // LR slots of 16 bytes a row
   constexpr int kRowBytes = 2 * D, kPlane = kKeys * kRowBytes, kStage = 2 * kPlane;
   __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
-  __shared__ int s_sum[2][4], s_last, s_odd[2][4];
+  __shared__ int s_sum[2][4], s_last, s_odd;
   extern __shared__ int s_end[];      // [n] items of the sequences up to and with b
   int* s_split = s_end + a.r.n;       // [n] the same of sequences in parts
   const int t = threadIdx.x, lane = t & 63;
@@ -561,6 +571,7 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
       *ally += s_sum[1][i];
     }
   };
+  if (t == 0) s_odd = 0;
   int W = 0;
   SeqSpan mine = {0, 0, 0, 0};
   for (int g = 0; g < a.r.n; g += 256) {
@@ -615,6 +626,7 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
   const int kend = old + (min(rows, (tile + 1) * kTile) - 1) / G + 1;
   const int steps = steps_of(kend), st0 = part * steps / parts, st1 = (part + 1) * steps / parts;
   const bool active = row0 < rows;  // the wave has rows
+  const int hidden0 = old + tile * kTile / G + 1;  // positions from here on are hidden from some row
 
   // Q^T operand: lane (row l % 32, half l / 32) holds dims 16 i + 8 half .. + 7
   const int qc = lane & 31, hf = lane >> 5;
@@ -708,47 +720,44 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
   float m = -INFINITY, l = 0.f;  // l of this lane's keys only
 
-  if (st0 < st1) issue(st0, 0);
-  pages = pages_at(st0 + 1);
-  for (int st = st0; st < st1; ++st) {
-    const int sg = (st - st0) & 1, key0 = st * kKeys;
+  // Step `st`, in LDS stage SG (the loop takes two at a time, so that operand addresses are immediates).
+  const auto take = [&](int st, auto stage_no) {
+    constexpr int SG = decltype(stage_no)::value;
+    const char* stage = lds + SG * kStage;
+    const int key0 = st * kKeys;
     const uint64_t none = gone;
-    const bool edge = key0 + kKeys > old + tile * kTile / G + 1;  // hidden from some row of the block
+    const bool edge = key0 + kKeys > hidden0;
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) expcnt(7) lgkmcnt(0): this wave's rows are there
-    if (edge) {  // an Inf or NaN among these V rows?
-      uint32_t top = 0;
-      typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-      us2 mx = {0, 0};
+    if (edge) {  // Inf and NaN among these V rows become zeros; they are added after the loop
+      bool odd = false;
 #pragma unroll
       for (int i = 0; i < 16 / RI; ++i) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(lds + sg * kStage + kPlane + 16 * w * kRowBytes + i * 1024 + 16 * lane);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx = __builtin_elementwise_max(mx, __builtin_bit_cast(us2, v[e] & 0x7FFF7FFFu));
+        u32x4* at = reinterpret_cast<u32x4*>(lds + SG * kStage + kPlane + 16 * w * kRowBytes + i * 1024 + 16 * lane);
+        u32x4 v = *at;
+        if (drop_odd<BF>(v)) {
+          *at = v;
+          odd = true;
+        }
       }
-      top = max(mx.x, mx.y);
-      const bool odd = __ballot(top >= (BF ? 0x7F80u : 0x7C00u)) != 0;
-      if (lane == 0) s_odd[sg][w] = odd;
+      if (odd) s_odd = 1;
       __builtin_amdgcn_s_waitcnt(0xc07f);
     }
     __builtin_amdgcn_s_barrier();  // everybody's rows are there, and the other stage is read
     asm volatile("" ::: "memory");
     if (st + 1 < st1) {
-      issue(st + 1, sg ^ 1);
+      issue(st + 1, SG ^ 1);
       pages = pages_at(st + 2);
     }
-    if (!active || key0 > old + min(row0 + 31, rows - 1) / G) continue;  // nothing the wave's rows see
-    const char* stage = lds + sg * kStage;
-
+    if (!active || key0 > old + min(row0 + 31, rows - 1) / G) return;  // nothing the wave's rows see
     f32x16 x[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[h][r] = 0.f;
 #pragma unroll
     for (int i = 0; i < KS; ++i)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        x[h] = mfma32<BF>(*reinterpret_cast<const u32x4*>(stage + ko[i] + 32 * h * kRowBytes), q[i], x[h]);
+      for (int h = 0; h < 2; ++h) {
+        const u32x4 kop = *reinterpret_cast<const u32x4*>(stage + ko[i] + 32 * h * kRowBytes);
+        const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        x[h] = mfma32<BF>(kop, q[i], i ? x[h] : zero);
+      }
     // lane holds keys 32 h + 8 (r / 4) + 4 half + r % 4
     if (key0 + kKeys > first_hidden || none) {
 #pragma unroll
@@ -777,56 +786,44 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
         for (int r = 0; r < 16; ++r) o[dt][r] *= f;
     }
     const float ms = m == -INFINITY ? 0.f : m;
-    u32x4 p[4];
-    float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float e[8];
+      float e[8], sum = 0.f;  // probabilities of the lane's eight keys of 16 i ..; l sums them unrounded
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         e[k] = __builtin_amdgcn_exp2f(fmaf(x[i >> 1][8 * (i & 1) + k], scale, -ms));
         sum += e[k];
       }
-      p[i] = pack8<BF>(e);
-    }
-    l += sum;
-    // V^T operand: dim 32 dt + l % 32, the lane's eight keys of 16 i ..
-    const auto vt = [&](int i, int dt) {
-      const u32x2 v0 = read_tr4(stage + vo[dt] + 16 * i * kRowBytes);
-      const u32x2 v1 = read_tr4(stage + vo[dt] + (16 * i + 8) * kRowBytes);
-      return u32x4{v0[0], v0[1], v1[0], v1[1]};
-    };
-    const bool odd = edge && (s_odd[sg][0] | s_odd[sg][1] | s_odd[sg][2] | s_odd[sg][3]);
-    if (!odd) {
+      l += sum;
+      const u32x4 p = pack8<BF>(e);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32<BF>(vt(i, dt), p[i], o[dt]);
-    } else {
-      // 0 x Inf is NaN: position by position, added only where the row sees it (plain arithmetic: it
-      // needs no registers beside the loop's)
-      for (int k = 0; k < kKeys && key0 + k < kend; ++k) {
-        const int word = 4 * (k >> 4) + 2 * ((k >> 3) & 1) + ((k >> 1) & 1);
-        uint32_t u = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) u = i == word ? p[i >> 2][i & 3] : u;
-        const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-        const uint32_t u0 = both[0], u1 = both[1];
-        u = (k >> 2) & 1 ? u1 : u0;  // the half of the wave that holds the position
-        const float pk = to_f32<BF>((uint16_t)(k & 1 ? u >> 16 : u));
-        const bool sees = key0 + k <= qpos;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const u32x2 v = *reinterpret_cast<const u32x2*>(stage + kPlane + k * kRowBytes + (((4 * dt + i) ^ vswz(k)) << 4) + 8 * hf);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float ve = to_f32<BF>((uint16_t)(e & 1 ? v[e >> 1] >> 16 : v[e >> 1]));
-              o[dt][4 * i + e] = sees ? fmaf(pk, ve, o[dt][4 * i + e]) : o[dt][4 * i + e];
-            }
-          }
+      for (int dt = 0; dt < DT; ++dt) {  // V^T operand: dim 32 dt + l % 32, the same keys
+        const u32x2 v0 = read_tr4(stage + vo[dt] + 16 * i * kRowBytes);
+        const u32x2 v1 = read_tr4(stage + vo[dt] + (16 * i + 8) * kRowBytes);
+        o[dt] = mfma32<BF>(u32x4{v0[0], v0[1], v1[0], v1[1]}, p, o[dt]);
       }
+    }
+  };
+  if (st0 < st1) issue(st0, 0);
+  pages = pages_at(st0 + 1);
+  for (int st = st0; st < st1; st += 2) {
+    take(st, std::integral_constant<int, 0>());
+    if (st + 1 < st1) take(st + 1, std::integral_constant<int, 1>());
+  }
+  __syncthreads();
+  if (s_odd && active) {
+    // (weight 1 does as well as the probability: what is added is Inf or NaN)
+    for (int key = max(st0 * kKeys, hidden0 / kKeys * kKeys); key < min(st1 * kKeys, kend); ++key) {
+      const int page = tab[min(key >> shift, a.p.max_pages - 1)];
+      if (!in_range(page, a.p.num_pages)) continue;
+      const uint16_t* v = a.vplane + page_elem(a.p, page, j) + (size_t)(key & inpage) * D + 4 * hf;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float x = to_f32<BF>(v[32 * dt + 8 * (r >> 2) + (r & 3)]);
+          if (key <= qpos && not_finite(x)) o[dt][r] += x;
+        }
     }
   }
   if (bad_page && lane == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_PAGE);
