@@ -2,8 +2,8 @@
 //
 // A kv head's query rows of a sequence are its new tokens times the G = q heads / kv heads that
 // share the kv head: row r is token r / G, head r % G.  Sequences of up to 16 rows (decode steps,
-// a few proposed tokens) are bound by reading K and V once: rows_kernel.  More rows share what is
-// read: chunk_kernel.
+// a few proposed tokens) are bound by reading K and V once: rows_part.  More rows share what is
+// read: chunk_part.  A call is one launch.
 #include <math.h>
 
 #include <type_traits>
@@ -19,11 +19,11 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kRows = 16;   // query rows of rows_kernel
+constexpr int kRows = 16;   // query rows of rows_part
 constexpr int kJoin = 8;         // parts joined at a time
 constexpr int kLevels = 4;       // of joins: up to 8^4 parts
 constexpr int kCounters = 1024;  // counters of a level, one per block
-constexpr int kChunkCounters = 2048;  // the same of chunk_kernel, one per part
+constexpr int kChunkCounters = 2048;  // the same of chunk_part, one per part
 constexpr int kMinSplit = 4;          // steps of a part there at least
 constexpr int kStep = 128;  // positions of a block's step there: 32 a wave
 
@@ -136,64 +136,90 @@ struct Cut {
 __device__ __forceinline__ int cut_first(const Cut& c, int lo) { return (lo + c.slack + c.S) / c.S; }
 __device__ __forceinline__ int cut_last(const Cut& c, int hi) { return (hi - c.slack - 1 + c.S) / c.S - 1; }
 
+// Shared memory of a block: V rows or tiles, a little more, and per-sequence arrays past 64 sequences
+// (up to 64 every wave holds one a lane).
+template <int D>
+struct Shared {
+  static constexpr int kRowsV = 4 * 32 * 2 * D;      // rows: 32 rows of V a wave, also 16 rows of floats
+  static constexpr int kChunkV = 2 * 2 * 64 * 2 * D;  // chunk: two stages of 64 rows of K and V
+  static constexpr int kMore = 4 * kRows * 2 * 4 + 64;
+};
+constexpr int kLanes = 64;
+
+// The steps (or items) of up to 64 sequences as one line, a sequence a lane: the lane whose part of
+// the line, which ends at `end`, holds x.
+__device__ __forceinline__ int lane_of(int end, int x) { return __builtin_ctzll(__ballot(end > x) | 1ULL << 63); }
+
 template <int D, bool BF>
-__global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
+__device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int* seqs, int block) {
   constexpr int KS = D / 32, DT = D / 16, NV = D / 16, LR = D / 8;  // LR lanes of 16 bytes a row
-  constexpr int kRowBytes = 2 * D, kWaveBytes = 32 * kRowBytes;     // also 16 rows of D floats
-  __shared__ __attribute__((aligned(16))) char lds[4 * kWaveBytes];
-  __shared__ float sml[4][kRows][2];
-  __shared__ int s_sum[4], s_last;
-  extern __shared__ int s_end[];  // [n] steps of the sequences up to and with b, then [n] each of:
-  int* s_len = s_end + a.r.n;     // positions
-  int* s_first = s_len + a.r.n;   // first token row
-  int* s_row = s_first + a.r.n;   // table row and new tokens << 16
+  constexpr int kRowBytes = 2 * D, kWaveBytes = 32 * kRowBytes;
+  float* sml = reinterpret_cast<float*>(lds + Shared<D>::kRowsV);  // [4 waves][16 rows] of (m, l)
+  int* s_sum = reinterpret_cast<int*>(sml + 4 * kRows * 2);        // [4]
+  int* s_last = s_sum + 4;
+  int* s_end = seqs;               // [n] steps of the sequences up to and with b
+  int* s_len = s_end + a.r.n;      // positions
+  int* s_first = s_len + a.r.n;    // first token row
+  int* s_row = s_first + a.r.n;    // table row and new tokens << 16
   const int t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kvh = a.p.kvh, G = a.qh / kvh;
-  const int k = blockIdx.x / kvh, j = blockIdx.x - k * kvh;
+  const int k = block / kvh, j = block - k * kvh;
 
   // ---- the cut -----------------------------------------------------------------------------
-  int W = 0;
+  const bool few = a.r.n <= kLanes;
+  int W = 0, l_end = 0, l_row = 0;
+  SeqSpan l_span = {0, 0, 0, 0};
   bool bad = false;
-  for (int g = 0; g < a.r.n; g += 256) {
-    const int b = g + t;
-    int steps = 0;
-    if (b < a.r.n) {
-      const SeqSpan s = seq_span(a.p, a.r, b);
-      bad |= s.count < 0;
-      steps = s.count > 0 && s.count * G <= kRows ? (s.len + kStep - 1) / kStep : 0;
-      s_len[b] = s.len;
-      s_first[b] = s.first;
-      s_row[b] = s.row | s.count << 16;
-    }
-    int x = steps;
+  const auto steps_of = [&](const SeqSpan& s) {
+    return s.count > 0 && s.count * G <= kRows ? (s.len + kStep - 1) / kStep : 0;
+  };
+  if (few) {
+    if (lane < a.r.n) l_span = seq_span(a.p, a.r, lane);
+    bad = l_span.count < 0;
+    l_row = l_span.row | l_span.count << 16;
+    l_end = wave_incl(steps_of(l_span));
+    W = __builtin_amdgcn_readlane(l_end, 63);
+  } else {
+    for (int g = 0; g < a.r.n; g += 256) {
+      const int b = g + t;
+      int steps = 0;
+      if (b < a.r.n) {
+        const SeqSpan s = seq_span(a.p, a.r, b);
+        bad |= s.count < 0;
+        steps = steps_of(s);
+        s_len[b] = s.len;
+        s_first[b] = s.first;
+        s_row[b] = s.row | s.count << 16;
+      }
+      const int x = wave_incl(steps);
+      if (g) block_sync_lds();  // the last round's sums have been read
+      if (lane == 63) s_sum[w] = x;
+      block_sync_lds();
+      int before = 0, all = 0;
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int y = __shfl_up(x, m);
-      if (lane >= m) x += y;
+      for (int i = 0; i < 4; ++i) {
+        before += i < w ? s_sum[i] : 0;
+        all += s_sum[i];
+      }
+      if (b < a.r.n) s_end[b] = W + before + x;
+      W += all;
     }
-    if (g) block_sync_lds();  // the last round's sums have been read
-    if (lane == 63) s_sum[w] = x;
     block_sync_lds();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      before += i < w ? s_sum[i] : 0;
-      all += s_sum[i];
-    }
-    if (b < a.r.n) s_end[b] = W + before + x;
-    W += all;
+    W = __builtin_amdgcn_readfirstlane(W);
   }
-  if (bad && blockIdx.x == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_SEQUENCE);
-  block_sync_lds();
-  W = __builtin_amdgcn_readfirstlane(W);
+  if (bad && block == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_SEQUENCE);
   Cut c;
   c.S = (W + a.blocks - 1) / a.blocks;
   c.slack = min(c.S / 4, 2);
   if (k * c.S >= W) return;
-  // the sequence whose steps hold step x < W
   const auto lds_at = [&](const int* p) { return __builtin_amdgcn_readfirstlane(*p); };  // the same in every lane
-  const auto find = [&](int x) {
+  const auto end_of = [&](int b) {  // steps up to and with sequence b (-1: none)
+    if (b < 0) return 0;
+    return few ? __builtin_amdgcn_readlane(l_end, b) : lds_at(s_end + b);
+  };
+  const auto find = [&](int x) {  // the sequence whose steps hold step x < W
+    if (few) return lane_of(l_end, x);
     int lo = 0, hi = a.r.n - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -206,22 +232,23 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
     return hi - x <= c.slack ? hi : x;
   };
   int b = find(k * c.S);
-  const int from = snap(k * c.S, b ? lds_at(s_end + b - 1) : 0, lds_at(s_end + b));
+  const int from = snap(k * c.S, end_of(b - 1), end_of(b));
   int to = W;
   if ((k + 1) * c.S < W) {
     const int e = find((k + 1) * c.S);
-    to = snap((k + 1) * c.S, e ? lds_at(s_end + e - 1) : 0, lds_at(s_end + e));
+    to = snap((k + 1) * c.S, end_of(e - 1), end_of(e));
   }
 
   const int r = lane & 15, g = lane >> 4;
   char* vl = lds + w * kWaveBytes;
   for (; b < a.r.n; ++b) {
-    const int lo = b ? lds_at(s_end + b - 1) : 0, hi = lds_at(s_end + b);
+    const int lo = end_of(b - 1), hi = end_of(b);
     if (lo >= to) break;
     const int x0 = max(lo, from), x1 = min(hi, to);
     if (x0 >= x1) continue;
-    const int row_count = lds_at(s_row + b);
-    const SeqSpan s = {row_count & 0xFFFF, lds_at(s_first + b), row_count >> 16, lds_at(s_len + b)};
+    const int row_count = few ? __builtin_amdgcn_readlane(l_row, b) : lds_at(s_row + b);
+    const SeqSpan s = {row_count & 0xFFFF, few ? __builtin_amdgcn_readlane(l_span.first, b) : lds_at(s_first + b),
+                       row_count >> 16, few ? __builtin_amdgcn_readlane(l_span.len, b) : lds_at(s_len + b)};
     const int rows = s.count * G;
     const int32_t* tab = a.p.table + (size_t)s.row * a.p.max_pages;
     const int shift = a.p.page_shift, inpage = (1 << shift) - 1;
@@ -380,8 +407,8 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
     // ---- the four waves' states ----------------------------------------------------------------
     l = rows4<true>(l);
     if (g == 0) {
-      sml[w][r][0] = m;
-      sml[w][r][1] = l;
+      sml[(w * kRows + r) * 2] = m;
+      sml[(w * kRows + r) * 2 + 1] = l;
     }
     // lane holds O^T[dim 16 i + 4 g + e][row r]: 16-byte slot 4 i + g of row r at slot ^ r
 #pragma unroll
@@ -392,15 +419,15 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
     constexpr int NS = D / 64;
     float M = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) M = fmaxf(M, sml[i][row][0]);
+    for (int i = 0; i < 4; ++i) M = fmaxf(M, sml[(i * kRows + row) * 2]);
     float L = 0.f;
     f32x4 acc[NS];
 #pragma unroll
     for (int n = 0; n < NS; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float mi = sml[i][row][0], f = mi == -INFINITY ? 0.f : exp2f(mi - M);
-      L = fmaf(sml[i][row][1], f, L);
+      const float mi = sml[(i * kRows + row) * 2], f = mi == -INFINITY ? 0.f : exp2f(mi - M);
+      L = fmaf(sml[(i * kRows + row) * 2 + 1], f, L);
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
         const f32x4 x = *reinterpret_cast<const f32x4*>(lds + i * kWaveBytes + row * (4 * D) + (((sl + 16 * n) ^ row) << 4));
@@ -434,9 +461,9 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
         __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are performed
         __syncthreads();                // ... and every other thread's
         int* counter = a.counters + level * kCounters + (kf - 1 + first * step) * kvh + j;
-        if (t == 0) s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == size - 1;
+        if (t == 0) *s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == size - 1;
         __syncthreads();
-        if (!s_last) break;
+        if (!*s_last) break;
         if (t == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // next call
         if (row < rows) {
           float mi[kJoin], li[kJoin];
@@ -531,96 +558,134 @@ struct Split {
 __device__ __forceinline__ int split_parts(int steps, int S) { return max(1, (2 * steps + S) / (2 * S)); }
 
 template <int D, bool BF>
-__global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
+__device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, int* seqs, int block) {
   constexpr int KS = D / 16, DT = D / 32, LR = D / 8;  // LR slots of 16 bytes a row
   constexpr int kRowBytes = 2 * D, kPlane = kKeys * kRowBytes, kStage = 2 * kPlane;
-  __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
-  __shared__ int s_sum[2][4], s_last, s_odd;
-  extern __shared__ int s_end[];      // [n] items of the sequences up to and with b
-  int* s_split = s_end + a.r.n;       // [n] the same of sequences in parts
+  int* s_sum = reinterpret_cast<int*>(lds + 2 * kStage);  // [2][4]
+  int* s_last = s_sum + 8;
+  int* s_odd = s_last + 1;
+  int* s_end = seqs;               // [n] items of the sequences up to and with b
+  int* s_split = s_end + a.r.n;    // [n] the same of sequences in parts
   const int t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kvh = a.p.kvh, G = a.qh / kvh;
-  const int idx = blockIdx.x / kvh, j = blockIdx.x - idx * kvh;
+  const int idx = block / kvh, j = block - idx * kvh;
+  if (t == 0) *s_odd = 0;
 
   // ---- which item ----------------------------------------------------------------------------
   const auto tiles_of = [&](const SeqSpan& s) { return s.count * G > kRows ? (s.count * G + kTile - 1) / kTile : 0; };
   const auto steps_of = [&](int len) { return (len + kKeys - 1) / kKeys; };
-  const auto block_scan = [&](int x, int y, int* ex, int* ey, int* allx, int* ally) {
-    int u = x, v = y;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int p = __shfl_up(u, m), q = __shfl_up(v, m);
-      if (lane >= m) {
-        u += p;
-        v += q;
-      }
-    }
-    block_sync_lds();  // the last round's sums have been read
-    if (lane == 63) {
-      s_sum[0][w] = u;
-      s_sum[1][w] = v;
-    }
-    block_sync_lds();
-    *ex = u; *ey = v; *allx = *ally = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      *ex += i < w ? s_sum[0][i] : 0;
-      *ey += i < w ? s_sum[1][i] : 0;
-      *allx += s_sum[0][i];
-      *ally += s_sum[1][i];
-    }
+  const auto work_of = [&](const SeqSpan& s) {
+    return (int)min((long long)tiles_of(s) * steps_of(s.len), 1LL << 18);
   };
-  if (t == 0) s_odd = 0;
-  int W = 0;
-  SeqSpan mine = {0, 0, 0, 0};
-  for (int g = 0; g < a.r.n; g += 256) {
-    const int b = g + t;
-    SeqSpan s = {0, 0, 0, 0};
-    if (b < a.r.n) s = seq_span(a.p, a.r, b);
-    const int n = tiles_of(s);
-    int ex, ey, aw, at;
-    block_scan((int)min((long long)n * steps_of(s.len), 1LL << 18), 0, &ex, &ey, &aw, &at);
-    W += aw;
-    if (g == 0) mine = s;
-  }
-  int S = max(kMinSplit, (W + a.slots - 1) / a.slots), items, splits;
-  for (;; S *= 2) {
-    items = splits = 0;
+  const auto share = [&](int W) { return max(kMinSplit, (W + a.slots - 1) / a.slots); };
+  SeqSpan s = {0, 0, 0, 0};
+  int parts, nt, tile, part, slot0;  // slot0: of the tile's parts in the workspace
+  if (a.r.n <= kLanes) {
+    // A sequence a lane.  Items in the order of their steps, the most first, whatever their sequence
+    // (a tile that sees much and starts last keeps a few CUs busy alone): v is the largest number of
+    // steps that more than idx items have.
+    SeqSpan l = {0, 0, 0, 0};
+    if (lane < a.r.n) l = seq_span(a.p, a.r, lane);
+    const int l_nt = tiles_of(l), l_steps = l_nt ? steps_of(l.len) : 0, rows = l.count * G, old = l.len - l.count;
+    const auto sum = [&](int x) { return __builtin_amdgcn_readlane(wave_incl(x), 63); };
+    int S = share(sum(work_of(l))), l_parts, l_split;
+    for (;; S *= 2) {
+      l_parts = split_parts(l_steps, S);
+      l_split = wave_incl(l_parts > 1 ? l_nt * l_parts : 0);
+      if (__builtin_amdgcn_readlane(l_split, 63) <= a.max_splits) break;  // (always, but for steps beyond what W counts)
+    }
+    const auto at_least = [&](int v) {  // tiles of the lane's sequence that have v steps and more
+      const long long x = ((long long)kKeys * (v - 1) - old) * G;  // that many rows before the tile's last
+      if (x <= 0) return l_nt;
+      return x < rows ? l_nt - (int)(x / kTile) : 0;
+    };
+    int lo = 1, hi = l_steps;
+#pragma unroll
+    for (int m = 32; m; m >>= 1) hi = max(hi, __shfl_xor(hi, m));
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    if (idx >= sum(l_nt * l_parts)) return;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (sum(at_least(mid) * l_parts) > idx) lo = mid; else hi = mid - 1;
+    }
+    const int more = at_least(lo + 1), here = (at_least(lo) - more) * l_parts;
+    const int end = wave_incl(here), at = idx - sum(more * l_parts);
+    const int b = lane_of(end, at);
+    const int in = at - (__builtin_amdgcn_readlane(end, b) - __builtin_amdgcn_readlane(here, b));
+    s = {__builtin_amdgcn_readlane(l.row, b), __builtin_amdgcn_readlane(l.first, b),
+         __builtin_amdgcn_readlane(l.count, b), __builtin_amdgcn_readlane(l.len, b)};
+    parts = __builtin_amdgcn_readlane(l_parts, b);
+    nt = __builtin_amdgcn_readlane(l_nt, b);
+    tile = nt - 1 - __builtin_amdgcn_readlane(more, b) - in / parts;
+    part = in % parts;
+    slot0 = __builtin_amdgcn_readlane(l_split, b) - (tile + 1) * parts;
+  } else {
+    const auto block_scan = [&](int x, int y, int* ex, int* ey, int* allx, int* ally) {
+      const int u = wave_incl(x), v = wave_incl(y);
+      block_sync_lds();  // the last round's sums have been read
+      if (lane == 63) {
+        s_sum[w] = u;
+        s_sum[4 + w] = v;
+      }
+      block_sync_lds();
+      *ex = u; *ey = v; *allx = *ally = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        *ex += i < w ? s_sum[i] : 0;
+        *ey += i < w ? s_sum[4 + i] : 0;
+        *allx += s_sum[i];
+        *ally += s_sum[4 + i];
+      }
+    };
+    int W = 0;
     for (int g = 0; g < a.r.n; g += 256) {
       const int b = g + t;
-      SeqSpan s = mine;
-      if (g && b < a.r.n) s = seq_span(a.p, a.r, b);
-      if (b >= a.r.n) s.count = 0;
-      const int parts = split_parts(steps_of(s.len), S), n = tiles_of(s) * parts;
-      int ex, ey, ax, ay;
-      block_scan(n, parts > 1 ? n : 0, &ex, &ey, &ax, &ay);
-      if (b < a.r.n) {
-        s_end[b] = items + ex;
-        s_split[b] = splits + ey;
-      }
-      items += ax;
-      splits += ay;
+      SeqSpan l = {0, 0, 0, 0};
+      if (b < a.r.n) l = seq_span(a.p, a.r, b);
+      int ex, ey, aw, at;
+      block_scan(work_of(l), 0, &ex, &ey, &aw, &at);
+      W += aw;
     }
-    if (splits <= a.max_splits) break;  // (always, but for steps beyond what W counts)
+    int S = share(W), items, splits;
+    for (;; S *= 2) {
+      items = splits = 0;
+      for (int g = 0; g < a.r.n; g += 256) {
+        const int b = g + t;
+        SeqSpan l = {0, 0, 0, 0};
+        if (b < a.r.n) l = seq_span(a.p, a.r, b);
+        const int np = split_parts(steps_of(l.len), S), n = tiles_of(l) * np;
+        int ex, ey, ax, ay;
+        block_scan(n, np > 1 ? n : 0, &ex, &ey, &ax, &ay);
+        if (b < a.r.n) {
+          s_end[b] = items + ex;
+          s_split[b] = splits + ey;
+        }
+        items += ax;
+        splits += ay;
+      }
+      if (splits <= a.max_splits) break;
+    }
+    block_sync_lds();
+    if (idx >= items) return;
+    const auto lds_at = [&](const int* p) { return __builtin_amdgcn_readfirstlane(*p); };
+    int b = 0;
+    for (int hi = a.r.n - 1; b < hi;) {
+      const int mid = (b + hi) >> 1;
+      if (lds_at(s_end + mid) > idx) hi = mid; else b = mid + 1;
+    }
+    s = seq_span(a.p, a.r, b);
+    s.row = __builtin_amdgcn_readfirstlane(s.row);
+    s.first = __builtin_amdgcn_readfirstlane(s.first);
+    s.count = __builtin_amdgcn_readfirstlane(s.count);
+    s.len = __builtin_amdgcn_readfirstlane(s.len);
+    parts = split_parts(steps_of(s.len), S);
+    nt = tiles_of(s);
+    const int in = idx - (lds_at(s_end + b) - nt * parts);
+    tile = nt - 1 - in / parts;  // a sequence's last tiles, which see the most, first
+    part = in % parts;
+    slot0 = lds_at(s_split + b) - (tile + 1) * parts;
   }
-  block_sync_lds();
-  if (idx >= items) return;
-  const auto lds_at = [&](const int* p) { return __builtin_amdgcn_readfirstlane(*p); };
-  int b = 0;
-  for (int hi = a.r.n - 1; b < hi;) {
-    const int mid = (b + hi) >> 1;
-    if (lds_at(s_end + mid) > idx) hi = mid; else b = mid + 1;
-  }
-  SeqSpan s = seq_span(a.p, a.r, b);
-  s.row = __builtin_amdgcn_readfirstlane(s.row);
-  s.first = __builtin_amdgcn_readfirstlane(s.first);
-  s.count = __builtin_amdgcn_readfirstlane(s.count);
-  s.len = __builtin_amdgcn_readfirstlane(s.len);
-  const int parts = split_parts(steps_of(s.len), S), nt = tiles_of(s);
-  const int in = idx - (lds_at(s_end + b) - nt * parts);
-  // the last tiles, which see the most, first
-  const int tile = nt - 1 - in / parts, part = in % parts;
   const int rows = s.count * G, row0 = tile * kTile + 32 * w;  // this wave's first row
   const int old = s.len - s.count;
   const int kend = old + (min(rows, (tile + 1) * kTile) - 1) / G + 1;
@@ -739,7 +804,7 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
           odd = true;
         }
       }
-      if (odd) s_odd = 1;
+      if (odd) *s_odd = 1;
       __builtin_amdgcn_s_waitcnt(0xc07f);
     }
     __builtin_amdgcn_s_barrier();  // everybody's rows are there, and the other stage is read
@@ -804,6 +869,7 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
       }
     }
   };
+  block_sync_lds();  // s_odd is 0 before anybody sets it
   if (st0 < st1) issue(st0, 0);
   pages = pages_at(st0 + 1);
   for (int st = st0; st < st1; st += 2) {
@@ -811,7 +877,7 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
     if (st + 1 < st1) take(st + 1, std::integral_constant<int, 1>());
   }
   __syncthreads();
-  if (s_odd && active) {
+  if (*s_odd && active) {
     // (weight 1 does as well as the probability: what is added is Inf or NaN)
     for (int key = max(st0 * kKeys, hidden0 / kKeys * kKeys); key < min(st1 * kKeys, kend); ++key) {
       const int page = tab[min(key >> shift, a.p.max_pages - 1)];
@@ -829,9 +895,8 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
   if (bad_page && lane == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_PAGE);
   l = halves<true>(l);
 
-  // ---- parts, joined as in rows_kernel; a lane's values lie 64 floats apart ---------------------
+  // ---- parts, joined as in rows_part; a lane's values lie 64 floats apart ---------------------
   int count = parts, at_part = part;
-  const int slot0 = parts > 1 ? (lds_at(s_split + b) - nt * parts) + (in - part) : 0;
   for (int level = 0, step = 1; count > 1; ++level, step *= kJoin) {
     const int first = at_part / kJoin * kJoin, size = min(kJoin, count - first);
     const auto place = [&](int i) { return ((size_t)(slot0 + i * step) * kvh + j) * 4 + w; };
@@ -847,9 +912,9 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
       __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are performed
       __syncthreads();                // ... and every other thread's
       int* counter = a.ccounters + level * kChunkCounters + (slot0 + first * step) * kvh + j;
-      if (t == 0) s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == size - 1;
+      if (t == 0) *s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == size - 1;
       __syncthreads();
-      if (!s_last) return;
+      if (!*s_last) return;
       if (t == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // next call
       if (active) {
         const auto ml = [&](int i) { return a.cml + place(first + i) * 64 + qc; };
@@ -905,9 +970,27 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
   }
 }
 
-// Blocks per kv head of rows_kernel.
+template <int D, bool BF>
+__global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[Shared<D>::kRowsV + Shared<D>::kMore];
+  extern __shared__ int seqs[];
+  rows_part<D, BF>(a, lds, seqs, blockIdx.x);
+}
+
+// Both: the first blocks * kvh blocks take the sequences of few rows, which stream K and V, and run
+// beside the others, which compute.
+template <int D, bool BF>
+__global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[Shared<D>::kChunkV + Shared<D>::kMore];
+  extern __shared__ int seqs[];
+  const int rows = a.blocks * a.p.kvh;
+  if ((int)blockIdx.x < rows) rows_part<D, BF>(a, lds, seqs, blockIdx.x);
+  else chunk_part<D, BF>(a, lds, seqs, blockIdx.x - rows);
+}
+
+// Blocks per kv head of rows_part.
 int rows_blocks(int kvh) { return max(1, min(device_cus(), kCounters) / kvh); }
-// Blocks per kv head that chunk_kernel's parts are to fill: two a CU.  Sequences in parts have 4/3
+// Blocks per kv head that chunk_part's parts are to fill: two a CU.  Sequences in parts have 4/3
 // of that many at most: P = round(steps / S) parts of a tile are at most steps / S + 1/2, and P >= 2
 // says that steps / S >= 3/2.
 int chunk_slots(int kvh) { return max(1, 2 * min(device_cus(), kChunkCounters / 4) / kvh); }
@@ -932,13 +1015,16 @@ bool has_chunks(int qh, int kvh, int max_new) { return (long long)max_new * (qh 
 template <int D, bool BF>
 int launch(const PagedAttnArgs& a, hipStream_t st) {
   const int kvh = a.p.kvh, G = a.qh / kvh;
-  hipLaunchKernelGGL((rows_kernel<D, BF>), dim3(a.blocks * kvh), dim3(256), a.r.n * 16, st, a);
-  int rc = check_launch();
-  if (rc || !has_chunks(a.qh, kvh, a.r.max_new)) return rc;
+  const size_t seqs = a.r.n > kLanes ? (size_t)a.r.n * 16 : 0;
+  const long long rows = (long long)a.blocks * kvh;
+  if (!has_chunks(a.qh, kvh, a.r.max_new)) {
+    hipLaunchKernelGGL((rows_kernel<D, BF>), dim3((unsigned)rows), dim3(256), seqs, st, a);
+    return check_launch();
+  }
   // items: a sequence's tiles are at most its rows / 128, rounded up; those in parts at most chunk_splits
   const long long items = (long long)a.r.tokens * G / kTile + a.r.n + chunk_splits(kvh);
-  if (items * kvh > INT32_MAX) return Q4D_ERR_SHAPE;
-  hipLaunchKernelGGL((chunk_kernel<D, BF>), dim3((unsigned)(items * kvh)), dim3(256), a.r.n * 8, st, a);
+  if (rows + items * kvh > INT32_MAX) return Q4D_ERR_SHAPE;
+  hipLaunchKernelGGL((chunk_kernel<D, BF>), dim3((unsigned)(rows + items * kvh)), dim3(256), seqs, st, a);
   return check_launch();
 }
 

@@ -374,3 +374,33 @@ def test_one_workspace_for_calls_of_every_shape(dev):
     for order in (jobs, jobs[::-1], jobs[1:] + jobs[:1]):
         for cache, batch, q, want in order:
             assert torch.equal(cache.attention(0, batch, q, ws=ws), want)
+
+
+@pytest.mark.parametrize("n", [64, 65, 300, 4096])
+def test_many_sequences(dev, n):
+    """As many sequences as lanes, one more, more than threads, and the most: decode steps, chunks and
+    sequences without new tokens mixed."""
+    lengths = [1 + (29 * i) % 90 for i in range(n)]
+    counts = [min(lengths[i], (0, 1, 1, 3, 40)[(7 * i) % 5]) for i in range(n)]
+    cache = filled(dev, lengths, 1, 64, 16, F)
+    for most in (3, 40):
+        few = [c if c <= most else 2 for c in counts]
+        batch = RaggedBatch.of(list(range(n)), few, dev)
+        q = torch.randn(batch.tokens, 3, 64, device=dev, generator=torch.Generator(device=dev).manual_seed(n)).half()
+        out = cache.attention(0, batch, q)
+        assert cache.status() == 0
+        some = sorted({0, 1, n // 2, n - 2, n - 1} | set(range(0, n, max(1, n // 60))))
+        at = batch.starts.tolist()
+        rows = torch.cat([torch.arange(at[b], at[b + 1]) for b in some])
+        one = RaggedBatch.of(some, [few[b] for b in some], dev)
+        compare(cache, one, q[rows], out[rows], 64 ** -0.5)
+
+
+def test_prompts_of_many_lengths_finish_in_any_order(dev):
+    """Tiles of several sequences in the order of their steps: lengths on both sides of a tile and a step."""
+    seqs = [(700, 700), (64, 64), (65, 65), (1300, 130), (127, 127), (128, 128), (129, 129), (900, 17), (33, 1), (2000, 511)]
+    cache = filled(dev, [n for n, _ in seqs], 2, 128, 16, B)
+    for qh in (2, 6, 14):
+        batch = RaggedBatch.of(list(range(len(seqs))), [a for _, a in seqs], dev)
+        q = torch.randn(batch.tokens, qh, 128, device=dev, generator=torch.Generator(device=dev).manual_seed(qh)).to(B)
+        compare(cache, batch, q, cache.attention(0, batch, q), 128 ** -0.5)
