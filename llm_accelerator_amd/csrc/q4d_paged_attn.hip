@@ -551,11 +551,11 @@ __device__ __forceinline__ void dma16(const uint16_t* base, uint32_t offset, uin
                : "memory");
 }
 
-// The parts of a sequence's tiles: about as many steps each as fill the device's blocks once.
-struct Split {
-  int S;  // steps a part
-};
+// A tile of n steps is cut into round(n / S) parts, S the steps that fill the device's blocks once (two
+// a CU; at least kMinSplit, so that a part pays for its join).  With more than half a step too few
+// or too many a part's steps lie within 3/4 S .. 3/2 S.
 __device__ __forceinline__ int split_parts(int steps, int S) { return max(1, (2 * steps + S) / (2 * S)); }
+constexpr int kMaxParts = 64;
 
 template <int D, bool BF>
 __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, int* seqs, int block) {
@@ -575,51 +575,86 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   // ---- which item ----------------------------------------------------------------------------
   const auto tiles_of = [&](const SeqSpan& s) { return s.count * G > kRows ? (s.count * G + kTile - 1) / kTile : 0; };
   const auto steps_of = [&](int len) { return (len + kKeys - 1) / kKeys; };
-  const auto work_of = [&](const SeqSpan& s) {
-    return (int)min((long long)tiles_of(s) * steps_of(s.len), 1LL << 18);
+  // steps of a sequence's tile, and of all its tiles (they grow evenly from the first to the last)
+  const auto tile_steps = [&](const SeqSpan& s, int tile) {
+    return steps_of(s.len - s.count + (min(s.count * G, (tile + 1) * kTile) - 1) / G + 1);
   };
-  const auto share = [&](int W) { return max(kMinSplit, (W + a.slots - 1) / a.slots); };
+  const auto work_of = [&](const SeqSpan& s) {
+    const int n = tiles_of(s);
+    return n ? (int)min((long long)n * (tile_steps(s, 0) + steps_of(s.len)) / 2, 1LL << 18) : 0;
+  };
+  const auto share = [&](int W, int most) {
+    return max(max(kMinSplit, (W + a.slots - 1) / a.slots), (most + kMaxParts - 2) / (kMaxParts - 1));
+  };
   SeqSpan s = {0, 0, 0, 0};
-  int parts, nt, tile, part, slot0;  // slot0: of the tile's parts in the workspace
+  int parts, tile, part, slots;  // slots: lane i's is the workspace slot of the tile's part i
   if (a.r.n <= kLanes) {
-    // A sequence a lane.  Items in the order of their steps, the most first, whatever their sequence
-    // (a tile that sees much and starts last keeps a few CUs busy alone): v is the largest number of
-    // steps that more than idx items have.
+    // A sequence a lane.
     SeqSpan l = {0, 0, 0, 0};
     if (lane < a.r.n) l = seq_span(a.p, a.r, lane);
-    const int l_nt = tiles_of(l), l_steps = l_nt ? steps_of(l.len) : 0, rows = l.count * G, old = l.len - l.count;
+    const int l_nt = tiles_of(l), l_rows = l_nt ? l.count * G : 0, l_old = l.len - l.count;
     const auto sum = [&](int x) { return __builtin_amdgcn_readlane(wave_incl(x), 63); };
-    int S = share(sum(work_of(l))), l_parts, l_split;
-    for (;; S *= 2) {
-      l_parts = split_parts(l_steps, S);
-      l_split = wave_incl(l_parts > 1 ? l_nt * l_parts : 0);
-      if (__builtin_amdgcn_readlane(l_split, 63) <= a.max_splits) break;  // (always, but for steps beyond what W counts)
-    }
-    const auto at_least = [&](int v) {  // tiles of the lane's sequence that have v steps and more
+    // tiles of v steps and more, of a sequence with `rows` rows after `old` positions: the last ones
+    const auto at_least = [&](int v, int nt, int rows, int old) {
       const long long x = ((long long)kKeys * (v - 1) - old) * G;  // that many rows before the tile's last
-      if (x <= 0) return l_nt;
-      return x < rows ? l_nt - (int)(x / kTile) : 0;
+      if (x <= 0) return nt;
+      return x < rows ? nt - (int)(x / kTile) : 0;
     };
-    int lo = 1, hi = l_steps;
+    const int tiles = sum(l_nt);
+    if (tiles == 0) return;
+    int most = l_nt ? steps_of(l.len) : 0;
 #pragma unroll
-    for (int m = 32; m; m >>= 1) hi = max(hi, __shfl_xor(hi, m));
-    hi = __builtin_amdgcn_readfirstlane(hi);
-    if (idx >= sum(l_nt * l_parts)) return;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (sum(at_least(mid) * l_parts) > idx) lo = mid; else hi = mid - 1;
+    for (int m = 32; m; m >>= 1) most = max(most, __shfl_xor(most, m));
+    most = __builtin_amdgcn_readfirstlane(most);
+    // Layer p = lane + 1: the tiles of p parts and more, which have steps >= p S - S / 2; layer 1 counts
+    // those of two and more, like layer 2.  Sizes of the layers, and of lane b's sequences' share.
+    int S = share(sum(work_of(l)), most), size = 0, end = 0;
+    const auto in_layer = [&](int b) {
+      return at_least(S * max(lane + 1, 2) - S / 2, __builtin_amdgcn_readlane(l_nt, b),
+                      __builtin_amdgcn_readlane(l_rows, b), __builtin_amdgcn_readlane(l_old, b));
+    };
+    const uint64_t mine = __ballot(l_nt > 0);
+    for (;; S += (S + 3) / 4) {
+      size = 0;
+      if (2 * most + S >= 4 * S)  // (otherwise nothing is cut)
+        for (uint64_t todo = mine; todo; todo &= todo - 1) size += in_layer(__builtin_ctzll(todo));
+      end = wave_incl(size);
+      if (__builtin_amdgcn_readlane(end, 63) <= a.max_splits) break;  // (always, but for roundings and steps past what W counts)
     }
-    const int more = at_least(lo + 1), here = (at_least(lo) - more) * l_parts;
-    const int end = wave_incl(here), at = idx - sum(more * l_parts);
-    const int b = lane_of(end, at);
-    const int in = at - (__builtin_amdgcn_readlane(end, b) - __builtin_amdgcn_readlane(here, b));
+    const int split = __builtin_amdgcn_readlane(end, 63), first = __builtin_amdgcn_readlane(end, 0);
+    int b, rank;  // the tile's, from the sequence's last
+    if (idx >= split - first + tiles) return;
+    if (idx < split - first) {
+      // second and later parts, which are about S steps each, come first
+      const int layer = lane_of(end, first + idx);
+      const int at = first + idx - (__builtin_amdgcn_readlane(end, layer) - __builtin_amdgcn_readlane(size, layer));
+      const int n = at_least(S * (layer + 1) - S / 2, l_nt, l_rows, l_old), upto = wave_incl(n);
+      b = lane_of(upto, at);
+      rank = at - (__builtin_amdgcn_readlane(upto, b) - __builtin_amdgcn_readlane(n, b));
+      part = layer;
+    } else {
+      // then the first (or only) parts, the tiles of the most steps first, whatever their sequence (one
+      // that sees much and starts last keeps a few CUs busy alone): more than `at` tiles have v steps
+      const int at = idx - (split - first);
+      int v = 1, hi = most;
+      while (v < hi) {
+        const int mid = (v + hi + 1) >> 1;
+        if (sum(at_least(mid, l_nt, l_rows, l_old)) > at) v = mid; else hi = mid - 1;
+      }
+      const int more = at_least(v + 1, l_nt, l_rows, l_old), here = at_least(v, l_nt, l_rows, l_old) - more;
+      const int upto = wave_incl(here), left = at - sum(more);
+      b = lane_of(upto, left);
+      rank = __builtin_amdgcn_readlane(more, b) + left -
+             (__builtin_amdgcn_readlane(upto, b) - __builtin_amdgcn_readlane(here, b));
+      part = 0;
+    }
     s = {__builtin_amdgcn_readlane(l.row, b), __builtin_amdgcn_readlane(l.first, b),
          __builtin_amdgcn_readlane(l.count, b), __builtin_amdgcn_readlane(l.len, b)};
-    parts = __builtin_amdgcn_readlane(l_parts, b);
-    nt = __builtin_amdgcn_readlane(l_nt, b);
-    tile = nt - 1 - __builtin_amdgcn_readlane(more, b) - in / parts;
-    part = in % parts;
-    slot0 = __builtin_amdgcn_readlane(l_split, b) - (tile + 1) * parts;
+    tile = tiles_of(s) - 1 - rank;
+    parts = split_parts(tile_steps(s, tile), S);
+    slots = end - size + rank;
+    if (parts > 1)
+      for (uint64_t todo = mine & ((1ULL << b) - 1); todo; todo &= todo - 1) slots += in_layer(__builtin_ctzll(todo));
   } else {
     const auto block_scan = [&](int x, int y, int* ex, int* ey, int* allx, int* ally) {
       const int u = wave_incl(x), v = wave_incl(y);
@@ -638,7 +673,8 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
         *ally += s_sum[4 + i];
       }
     };
-    int W = 0;
+    // every tile of a sequence in as many parts as its last
+    int S = 0, W = 0, items, splits;
     for (int g = 0; g < a.r.n; g += 256) {
       const int b = g + t;
       SeqSpan l = {0, 0, 0, 0};
@@ -647,8 +683,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
       block_scan(work_of(l), 0, &ex, &ey, &aw, &at);
       W += aw;
     }
-    int S = share(W), items, splits;
-    for (;; S *= 2) {
+    for (S = share(W, steps_of(a.p.max_pages << a.p.page_shift));; S += (S + 3) / 4) {
       items = splits = 0;
       for (int g = 0; g < a.r.n; g += 256) {
         const int b = g + t;
@@ -680,11 +715,10 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
     s.count = __builtin_amdgcn_readfirstlane(s.count);
     s.len = __builtin_amdgcn_readfirstlane(s.len);
     parts = split_parts(steps_of(s.len), S);
-    nt = tiles_of(s);
-    const int in = idx - (lds_at(s_end + b) - nt * parts);
+    const int nt = tiles_of(s), in = idx - (lds_at(s_end + b) - nt * parts);
     tile = nt - 1 - in / parts;  // a sequence's last tiles, which see the most, first
     part = in % parts;
-    slot0 = lds_at(s_split + b) - (tile + 1) * parts;
+    slots = lds_at(s_split + b) - (tile + 1) * parts + lane;
   }
   const int rows = s.count * G, row0 = tile * kTile + 32 * w;  // this wave's first row
   const int old = s.len - s.count;
@@ -899,7 +933,8 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   int count = parts, at_part = part;
   for (int level = 0, step = 1; count > 1; ++level, step *= kJoin) {
     const int first = at_part / kJoin * kJoin, size = min(kJoin, count - first);
-    const auto place = [&](int i) { return ((size_t)(slot0 + i * step) * kvh + j) * 4 + w; };
+    const auto slot = [&](int i) { return (size_t)__builtin_amdgcn_readlane(slots, i * step) * kvh + j; };
+    const auto place = [&](int i) { return slot(i) * 4 + w; };
     if (size > 1) {
       if (active) {
         float* acc = a.cacc + place(at_part) * (32 * D) + lane;
@@ -911,7 +946,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
       }
       __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are performed
       __syncthreads();                // ... and every other thread's
-      int* counter = a.ccounters + level * kChunkCounters + (slot0 + first * step) * kvh + j;
+      int* counter = a.ccounters + level * kChunkCounters + slot(first);
       if (t == 0) *s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == size - 1;
       __syncthreads();
       if (!*s_last) return;
@@ -990,9 +1025,8 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
 
 // Blocks per kv head of rows_part.
 int rows_blocks(int kvh) { return max(1, min(device_cus(), kCounters) / kvh); }
-// Blocks per kv head that chunk_part's parts are to fill: two a CU.  Sequences in parts have 4/3
-// of that many at most: P = round(steps / S) parts of a tile are at most steps / S + 1/2, and P >= 2
-// says that steps / S >= 3/2.
+// Blocks per kv head that chunk_part's parts are to fill: two a CU.  Tiles in parts have 4/3 of that
+// many parts at most: round(n / S) is at most n / S + 1/2, and two or more says n / S >= 3/2.
 int chunk_slots(int kvh) { return max(1, 2 * min(device_cus(), kChunkCounters / 4) / kvh); }
 int chunk_splits(int kvh) { return chunk_slots(kvh) * 4 / 3 + 1; }
 
@@ -1021,7 +1055,7 @@ int launch(const PagedAttnArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((rows_kernel<D, BF>), dim3((unsigned)rows), dim3(256), seqs, st, a);
     return check_launch();
   }
-  // items: a sequence's tiles are at most its rows / 128, rounded up; those in parts at most chunk_splits
+  // items: a sequence's tiles are at most its rows / 128, rounded up; more parts at most chunk_splits
   const long long items = (long long)a.r.tokens * G / kTile + a.r.n + chunk_splits(kvh);
   if (rows + items * kvh > INT32_MAX) return Q4D_ERR_SHAPE;
   hipLaunchKernelGGL((chunk_kernel<D, BF>), dim3((unsigned)(rows + items * kvh)), dim3(256), seqs, st, a);
