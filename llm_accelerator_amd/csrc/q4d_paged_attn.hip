@@ -105,7 +105,7 @@ __device__ __forceinline__ u32x2 read_tr4(const char* p) {
 
 // `bytes` from p on as a buffer: loads past them give zeros and read nothing.
 // (p and bytes are the same in every lane, which the compiler does not always see.)
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* p, int bytes) {
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int bytes) {
   const uint64_t u = reinterpret_cast<uint64_t>(p);
   const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)u);
   const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(u >> 32));
@@ -114,6 +114,17 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* p, i
 }
 __device__ __forceinline__ u32x4 rows_load(__amdgpu_buffer_rsrc_t r, int offset) {
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 2));
+}
+
+// Four floats that another XCD's block writes or reads in this launch: the same accesses as
+// store_dev / load_dev (device scope, past the caches that are not shared), 16 bytes at a time.
+constexpr int kDeviceScope = 16;  // sc1
+__device__ __forceinline__ void store_dev4(__amdgpu_buffer_rsrc_t r, int offset, f32x4 v) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, v), r, offset, 0, kDeviceScope);
+}
+__device__ __forceinline__ f32x4 load_dev4(__amdgpu_buffer_rsrc_t r, int offset) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, kDeviceScope));
 }
 
 // The running max moves only when a score exceeds it by more than this (log2 units): P = 2^(s - m)
@@ -849,14 +860,32 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
     }
     if (!active || key0 > old + min(row0 + 31, rows - 1) / G) return;  // nothing the wave's rows see
     f32x16 x[2];
+    {
+      u32x4 kop[KS][2];  // all of the tile's operands on their way before the first product waits
 #pragma unroll
-    for (int i = 0; i < KS; ++i)
+      for (int i = 0; i < KS; ++i)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const u32x4 kop = *reinterpret_cast<const u32x4*>(stage + ko[i] + 32 * h * kRowBytes);
-        const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        x[h] = mfma32<BF>(kop, q[i], i ? x[h] : zero);
+        for (int h = 0; h < 2; ++h) kop[i][h] = *reinterpret_cast<const u32x4*>(stage + ko[i] + 32 * h * kRowBytes);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          x[h] = mfma32<BF>(kop[i][h], q[i], i ? x[h] : zero);
+        }
+    }
+    // V^T operands of 16 keys: dims 32 dt + l % 32, the lane's eight keys of 16 i ..
+    const auto load_v = [&](int i, u32x4 (&v)[DT]) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const u32x2 v0 = read_tr4(stage + vo[dt] + 16 * i * kRowBytes);
+        const u32x2 v1 = read_tr4(stage + vo[dt] + (16 * i + 8) * kRowBytes);
+        v[dt] = u32x4{v0[0], v0[1], v1[0], v1[1]};
       }
+    };
+    u32x4 v[2][DT];
+    load_v(0, v[0]);
     // lane holds keys 32 h + 8 (r / 4) + 4 half + r % 4
     if (key0 + kKeys > first_hidden || none) {
 #pragma unroll
@@ -885,22 +914,23 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
         for (int r = 0; r < 16; ++r) o[dt][r] *= f;
     }
     const float ms = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float e[8], sum = 0.f;  // probabilities of the lane's eight keys of 16 i ..; l sums them unrounded
+    // the lane's eight probabilities of each 16 keys; l sums them unrounded
+    const auto probs = [&](int i) {
+      float e[8], sum = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         e[k] = __builtin_amdgcn_exp2f(fmaf(x[i >> 1][8 * (i & 1) + k], scale, -ms));
         sum += e[k];
       }
       l += sum;
-      const u32x4 p = pack8<BF>(e);
+      return pack8<BF>(e);
+    };
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {  // V^T operand: dim 32 dt + l % 32, the same keys
-        const u32x2 v0 = read_tr4(stage + vo[dt] + 16 * i * kRowBytes);
-        const u32x2 v1 = read_tr4(stage + vo[dt] + (16 * i + 8) * kRowBytes);
-        o[dt] = mfma32<BF>(u32x4{v0[0], v0[1], v1[0], v1[1]}, p, o[dt]);
-      }
+    for (int i = 0; i < 4; ++i) {
+      if (i < 3) load_v(i + 1, v[(i + 1) & 1]);
+      const u32x4 p = probs(i);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32<BF>(v[i & 1][dt], p, o[dt]);
     }
   };
   block_sync_lds();  // s_odd is 0 before anybody sets it
@@ -929,7 +959,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   if (bad_page && lane == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_PAGE);
   l = halves<true>(l);
 
-  // ---- parts, joined as in rows_part; a lane's values lie 64 floats apart ---------------------
+  // ---- parts, joined as in rows_part; a lane's values lie together by fours ---------------------
   int count = parts, at_part = part;
   for (int level = 0, step = 1; count > 1; ++level, step *= kJoin) {
     const int first = at_part / kJoin * kJoin, size = min(kJoin, count - first);
@@ -937,11 +967,12 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
     const auto place = [&](int i) { return slot(i) * 4 + w; };
     if (size > 1) {
       if (active) {
-        float* acc = a.cacc + place(at_part) * (32 * D) + lane;
+        const auto acc = rows_rsrc(a.cacc + place(at_part) * (32 * D), 32 * D * 4);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) store_dev(acc + 64 * (16 * dt + r), o[dt][r]);
+          for (int r = 0; r < 16; r += 4)
+            store_dev4(acc, (16 * dt + r) * 256 + 16 * lane, f32x4{o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]});
         store_dev(a.cml + place(at_part) * 64 + lane, hf ? l : m);
       }
       __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are performed
@@ -961,17 +992,32 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
-        for (int i = 0; i < size; ++i) {
-          const float mv = load_dev(ml(i)), f = mv == -INFINITY ? 0.f : exp2f(mv - M);
-          l = fmaf(load_dev(ml(i) + 32), f, l);
-          const float* acc = a.cacc + place(first + i) * (32 * D) + lane;
+        // two parts' values are in flight together
+        for (int i0 = 0; i0 < size; i0 += 2) {
+          f32x4 v[2][4 * DT];
+          float mv[2], lv[2];
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
+          for (int k = 0; k < 2; ++k) {
+            const int i = min(i0 + k, size - 1);
+            mv[k] = load_dev(ml(i));
+            lv[k] = load_dev(ml(i) + 32);
+            const auto acc = rows_rsrc(a.cacc + place(first + i) * (32 * D), 32 * D * 4);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float v = load_dev(acc + 64 * (16 * dt + r));
-              o[dt][r] = mv == -INFINITY ? o[dt][r] : fmaf(v, f, o[dt][r]);
-            }
+            for (int n = 0; n < 4 * DT; ++n) v[k][n] = load_dev4(acc, n * 1024 + 16 * lane);
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (i0 + k >= size) break;
+            const float f = mv[k] == -INFINITY ? 0.f : exp2f(mv[k] - M);
+            l = fmaf(lv[k], f, l);
+#pragma unroll
+            for (int n = 0; n < 4 * DT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float y = o[n >> 2][4 * (n & 3) + e];
+                o[n >> 2][4 * (n & 3) + e] = mv[k] == -INFINITY ? y : fmaf(v[k][n][e], f, y);
+              }
+          }
         }
         m = M;
       }
