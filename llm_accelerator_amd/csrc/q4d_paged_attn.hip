@@ -147,6 +147,16 @@ struct Cut {
 __device__ __forceinline__ int cut_first(const Cut& c, int lo) { return (lo + c.slack + c.S) / c.S; }
 __device__ __forceinline__ int cut_last(const Cut& c, int hi) { return (hi - c.slack - 1 + c.S) / c.S - 1; }
 
+// The kernels' argument block as the hardware passes it (both have it as their only argument).  Read
+// through this at the end of a sequence, its fields are not kept in scalar registers through the loops
+// (kept, they pushed the loop's own scalars out: 60 v_readlane of 150 vector instructions a step).
+typedef const __attribute__((address_space(4))) PagedAttnArgs* KernelArgs;
+__device__ __forceinline__ KernelArgs late_args() {
+  KernelArgs p = (KernelArgs)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return p;
+}
+
 // Shared memory of a block: V rows or tiles, a little more, and per-sequence arrays past 64 sequences
 // (up to 64 every wave holds one a lane).
 template <int D>
@@ -268,7 +278,8 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
     const int qpos = s.len - s.count + tok;
     u32x4 q[KS];
     {
-      const uint16_t* qp = a.q + (s.first + tok) * a.q_stride + (j * G + rr - tok * G) * D + 8 * g;
+      const KernelArgs late = late_args();
+      const uint16_t* qp = late->q + (s.first + tok) * late->q_stride + (j * G + rr - tok * G) * D + 8 * g;
 #pragma unroll
       for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const u32x4*>(qp + 32 * i);
     }
@@ -394,6 +405,7 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
     issue(s0);
     for (int it = s0; it < s1; ++it) consume(it);
     if (__ballot(odd)) {
+      const uint16_t* vplane = late_args()->vplane;
       // this wave's positions that some row does not see (weight 1 does as well as the probability: what
       // is added is Inf or NaN)
       for (int it = max(s0, first_hidden / kStep); it < s1; ++it) {
@@ -402,7 +414,7 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
         for (int pos = base; pos < min(s.len, base + 32); ++pos) {
           const int pg = tab[min(pos >> shift, a.p.max_pages - 1)];
           if (!in_range(pg, a.p.num_pages)) continue;
-          const uint16_t* v = a.vplane + page_elem(a.p, pg, j) + (size_t)(pos & inpage) * D + 4 * g;
+          const uint16_t* v = vplane + page_elem(a.p, pg, j) + (size_t)(pos & inpage) * D + 4 * g;
 #pragma unroll
           for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -448,30 +460,31 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
     }
     // The parts' states are joined eight at a time: of each eight the block that counts in last adds
     // them in order and goes on with the sum as one of the next level's parts.
+    const KernelArgs late = late_args();
+    const auto pacc = rows_rsrc(late->pacc, 1 << 30);
+    float* pml = late->pml;
     const int kf = cut_first(c, lo);
     int count = max(0, cut_last(c, hi) - kf + 1) + 1, part = x0 == lo ? 0 : k - kf + 1;
     // part 0 lies in block kf - 1's slot 1, part i in block kf - 1 + i's slot 0; a sum lies where its
     // first part did, and its counter is that block's
     for (int level = 0, step = 1; count > 1; ++level, step *= kJoin) {
       const auto place = [&](int i) {
-        return (((size_t)(kf - 1 + i * step) * 2 + (i == 0)) * kvh + j) * kRows + row;
+        return (((kf - 1 + i * step) * 2 + (i == 0)) * kvh + j) * kRows + row;
       };
       const int first = part / kJoin * kJoin, size = min(kJoin, count - first);
       if (size > 1) {
         if (row < rows) {
-          const size_t at = place(part);
+          const int at = place(part);
 #pragma unroll
-          for (int n = 0; n < NS; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) store_dev(a.pacc + at * D + 64 * n + 4 * sl + e, acc[n][e]);
+          for (int n = 0; n < NS; ++n) store_dev4(pacc, (at * D + 64 * n + 4 * sl) * 4, acc[n]);
           if (sl == 0) {
-            store_dev(a.pml + at * 2, M);
-            store_dev(a.pml + at * 2 + 1, L);
+            store_dev(pml + at * 2, M);
+            store_dev(pml + at * 2 + 1, L);
           }
         }
         __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are performed
         __syncthreads();                // ... and every other thread's
-        int* counter = a.counters + level * kCounters + (kf - 1 + first * step) * kvh + j;
+        int* counter = late->counters + level * kCounters + (kf - 1 + first * step) * kvh + j;
         if (t == 0) *s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == size - 1;
         __syncthreads();
         if (!*s_last) break;
@@ -481,13 +494,11 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
           f32x4 ai[kJoin][NS];
 #pragma unroll
           for (int i = 0; i < kJoin; ++i) {
-            const size_t at = place(first + min(i, size - 1));
-            mi[i] = load_dev(a.pml + at * 2);
-            li[i] = load_dev(a.pml + at * 2 + 1);
+            const int at = place(first + min(i, size - 1));
+            mi[i] = load_dev(pml + at * 2);
+            li[i] = load_dev(pml + at * 2 + 1);
 #pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) ai[i][n][e] = load_dev(a.pacc + at * D + 64 * n + 4 * sl + e);
+            for (int n = 0; n < NS; ++n) ai[i][n] = load_dev4(pacc, (at * D + 64 * n + 4 * sl) * 4);
           }
           M = -INFINITY;
 #pragma unroll
@@ -512,7 +523,7 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
     }
     if (count == 1 && row < rows) {
       const int otok = row / G;
-      uint16_t* op = a.out + (s.first + otok) * a.out_stride + (j * G + row - otok * G) * D + 4 * sl;
+      uint16_t* op = late->out + (s.first + otok) * late->out_stride + (j * G + row - otok * G) * D + 4 * sl;
       const float inv = L == 0.f ? 0.f : 1.0f / L;
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
@@ -960,6 +971,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   l = halves<true>(l);
 
   // ---- parts, joined as in rows_part; a lane's values lie together by fours ---------------------
+  const KernelArgs late = late_args();
   int count = parts, at_part = part;
   for (int level = 0, step = 1; count > 1; ++level, step *= kJoin) {
     const int first = at_part / kJoin * kJoin, size = min(kJoin, count - first);
@@ -967,23 +979,23 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
     const auto place = [&](int i) { return slot(i) * 4 + w; };
     if (size > 1) {
       if (active) {
-        const auto acc = rows_rsrc(a.cacc + place(at_part) * (32 * D), 32 * D * 4);
+        const auto acc = rows_rsrc(late->cacc + place(at_part) * (32 * D), 32 * D * 4);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
           for (int r = 0; r < 16; r += 4)
             store_dev4(acc, (16 * dt + r) * 256 + 16 * lane, f32x4{o[dt][r], o[dt][r + 1], o[dt][r + 2], o[dt][r + 3]});
-        store_dev(a.cml + place(at_part) * 64 + lane, hf ? l : m);
+        store_dev(late->cml + place(at_part) * 64 + lane, hf ? l : m);
       }
       __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are performed
       __syncthreads();                // ... and every other thread's
-      int* counter = a.ccounters + level * kChunkCounters + slot(first);
+      int* counter = late->ccounters + level * kChunkCounters + slot(first);
       if (t == 0) *s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == size - 1;
       __syncthreads();
       if (!*s_last) return;
       if (t == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // next call
       if (active) {
-        const auto ml = [&](int i) { return a.cml + place(first + i) * 64 + qc; };
+        const auto ml = [&](int i) { return late->cml + place(first + i) * 64 + qc; };
         float M = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kJoin; ++i) M = fmaxf(M, load_dev(ml(min(i, size - 1))));
@@ -1001,7 +1013,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
             const int i = min(i0 + k, size - 1);
             mv[k] = load_dev(ml(i));
             lv[k] = load_dev(ml(i) + 32);
-            const auto acc = rows_rsrc(a.cacc + place(first + i) * (32 * D), 32 * D * 4);
+            const auto acc = rows_rsrc(late->cacc + place(first + i) * (32 * D), 32 * D * 4);
 #pragma unroll
             for (int n = 0; n < 4 * DT; ++n) v[k][n] = load_dev4(acc, n * 1024 + 16 * lane);
           }
@@ -1046,7 +1058,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
     const int r = i * RI + drow, rr = row0 + r;
     if (rr >= rows) continue;
     const int tk = rr / G;
-    *reinterpret_cast<u32x4*>(a.out + (s.first + tk) * a.out_stride + (j * G + rr - tk * G) * D + 8 * dslot) =
+    *reinterpret_cast<u32x4*>(late->out + (s.first + tk) * late->out_stride + (j * G + rr - tk * G) * D + 8 * dslot) =
         *reinterpret_cast<const u32x4*>(T0 + r * kRowBytes + ((dslot ^ (r & (LR - 1))) << 4));
   }
 }
