@@ -89,10 +89,13 @@ enum {
   Q4D_STATUS_XCD_MAP = 4,
   Q4D_STATUS_SYNC_TIMEOUT = 8,
   /* Paged cache (status word of q4d_pages_t): no free page left; a sequence, count or order of
-   * the batch that cannot be; a table entry outside the pool. */
+   * the batch that cannot be; a table entry outside the pool; q4d_pages_reserve was refused (for
+   * one of these or BAD_POSITION), and so is every later one, and q4d_paged_append writes
+   * nothing, until the word is cleared. */
   Q4D_STATUS_NO_PAGES = 16,
   Q4D_STATUS_BAD_SEQUENCE = 32,
-  Q4D_STATUS_BAD_PAGE = 64
+  Q4D_STATUS_BAD_PAGE = 64,
+  Q4D_STATUS_NOT_RESERVED = 128
 };
 
 enum { Q4D_F16 = 0, Q4D_F32 = 1, Q4D_BF16 = 2 };
@@ -461,7 +464,11 @@ size_t q4d_pages_workspace_bytes(const q4d_pages_t* pages);
  * filled and other rows hold it too, its rows are copied to a page of the sequence's own first,
  * in every layer (but where the batch's sequences are all that hold it, the last of them keeps
  * it).  All or nothing: if pages run out, a sequence would pass max_pages or occurs twice, or a
- * row, count or page cannot be, nothing changes but the status word. */
+ * row, count or page cannot be, nothing changes but the status word.  That then says
+ * Q4D_STATUS_NOT_RESERVED too, and until it is cleared every later reserve is refused and
+ * q4d_paged_append leaves all tokens out: the last positions that lengths name are older ones.
+ * So a step that finds no pages, also one of several that were launched or replayed ahead,
+ * leaves the cache as the last good step left it (what its q4d_paged_attention gives means nothing). */
 int q4d_pages_reserve(const q4d_pages_t* pages, const q4d_ragged_t* batch, void* ws, size_t ws_bytes, void* stream);
 /* Row dst[i] becomes a copy of row src[i] that shares its pages; src, dst: device int32 [n].
  * dst[i] must be empty (length 0), in no src, and the first of its number in dst; a pair that
@@ -483,7 +490,8 @@ int q4d_pages_compact(const q4d_pages_t* pages, int32_t* used, void* ws, size_t 
  * in one projection); rows 16-byte aligned.  q and q_out may both be NULL (q_heads 0).  fp32
  * arithmetic, rounded once.  A token past rope's max_ctx (Q4D_STATUS_BAD_POSITION) or of a
  * sequence that cannot be is left out; into a page that cannot be nothing is written
- * (Q4D_STATUS_BAD_PAGE).  The pages must be the sequence's own (q4d_pages_reserve sees to that). */
+ * (Q4D_STATUS_BAD_PAGE).  The pages must be the sequence's own (q4d_pages_reserve sees to that);
+ * after a refused reserve (Q4D_STATUS_NOT_RESERVED) all tokens are left out. */
 int q4d_paged_append(const q4d_pages_t* pages, int32_t layer, const q4d_ragged_t* batch, const void* q, int64_t q_stride,
                      int32_t q_heads, const void* k, int64_t k_stride, const void* v, int64_t v_stride, int32_t x_dtype,
                      const float* q_gamma, const float* k_gamma, float eps, const q4d_rope_t* rope, void* q_out,

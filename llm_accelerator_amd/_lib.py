@@ -23,9 +23,10 @@ STATUS_SYNC_TIMEOUT = 8
 STATUS_NO_PAGES = 16
 STATUS_BAD_SEQUENCE = 32
 STATUS_BAD_PAGE = 64
+STATUS_NOT_RESERVED = 128
 STATUS_NAMES = {STATUS_BAD_TOKEN: "BAD_TOKEN", STATUS_BAD_POSITION: "BAD_POSITION", STATUS_XCD_MAP: "XCD_MAP",
                 STATUS_SYNC_TIMEOUT: "SYNC_TIMEOUT", STATUS_NO_PAGES: "NO_PAGES",
-                STATUS_BAD_SEQUENCE: "BAD_SEQUENCE", STATUS_BAD_PAGE: "BAD_PAGE"}
+                STATUS_BAD_SEQUENCE: "BAD_SEQUENCE", STATUS_BAD_PAGE: "BAD_PAGE", STATUS_NOT_RESERVED: "NOT_RESERVED"}
 DECODE_XCD = 0
 DECODE_STAGED = 1
 

@@ -162,10 +162,11 @@ __global__ __launch_bounds__(1024) void reserve_kernel(const PagedView p, const 
     count[i] = b < r.n ? r.starts[b + 1] : 0;
     row[i] = b < r.n ? (r.seqs ? r.seqs[b] : b) : 0;
   }
+  const int held_back = t ? 0 : *p.status & Q4D_STATUS_NOT_RESERVED;
   for (int i = t; i < 65536 / 32; i += 1024) seen[i] = 0;
   if (t == 0) s_err = s_copies = 0;
   __syncthreads();
-  int err = 0;
+  int err = held_back;
 #pragma unroll
   for (int i = 0; i < B; ++i) {
     const int b = t + 1024 * i;
@@ -208,7 +209,7 @@ __global__ __launch_bounds__(1024) void reserve_kernel(const PagedView p, const 
   shared = __syncthreads_or(shared);
   if (s_err) {
     if (t == 0) {
-      atomicOr(p.status, s_err);
+      atomicOr(p.status, s_err | Q4D_STATUS_NOT_RESERVED);
       *w.copies = 0;
     }
     return;
@@ -283,7 +284,7 @@ __global__ __launch_bounds__(1024) void reserve_kernel(const PagedView p, const 
   }
   if (found < total) {
     if (t == 0) {
-      atomicOr(p.status, Q4D_STATUS_NO_PAGES);
+      atomicOr(p.status, Q4D_STATUS_NO_PAGES | Q4D_STATUS_NOT_RESERVED);
       *w.copies = 0;
     }
     return;
@@ -549,8 +550,9 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs a) {
   const long long wave = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int tok = (int)(wave / a.per), part = (int)(wave % a.per);
   if (tok >= a.r.tokens) return;
+  const int refused = *a.p.status & Q4D_STATUS_NOT_RESERVED;  // (nobody sets this bit meanwhile)
   const int b = entry_of(a.r, tok, lane);
-  if (b >= a.r.n) return;
+  if (b >= a.r.n || refused) return;
   const SeqSpan s = seq_span(a.p, a.r, b);
   if (s.count < 0 || tok < s.first || tok >= s.first + s.count) {
     if (lane == 0 && s.count < 0) atomicOr(a.p.status, Q4D_STATUS_BAD_SEQUENCE);

@@ -4,7 +4,7 @@ the rotation in 64 bits."""
 import numpy as np
 import torch
 
-from llm_accelerator_amd._lib import STATUS_BAD_PAGE, STATUS_BAD_POSITION, STATUS_BAD_SEQUENCE, STATUS_NO_PAGES
+from llm_accelerator_amd._lib import STATUS_BAD_PAGE, STATUS_BAD_POSITION, STATUS_BAD_SEQUENCE, STATUS_NOT_RESERVED, STATUS_NO_PAGES
 
 
 class Pages:
@@ -22,7 +22,7 @@ class Pages:
         return -(-n // self.ps)
 
     def reserve(self, seqs, counts):
-        err = 0
+        err = self.status & STATUS_NOT_RESERVED
         grow = [(s, c) for s, c in zip(seqs, counts) if c != 0]
         for i, (s, c) in enumerate(grow):
             if c < 0 or not 0 <= s < len(self.lengths) or s in [g[0] for g in grow[:i]]:
@@ -32,7 +32,7 @@ class Pages:
             elif self.lengths[s] % self.ps and not 0 <= self.table[s][self.lengths[s] // self.ps] < len(self.refs):
                 err |= STATUS_BAD_PAGE
         if err:
-            self.status |= err
+            self.status |= err | STATUS_NOT_RESERVED
             return
         last = {s: self.table[s][self.lengths[s] // self.ps] if self.lengths[s] % self.ps else None for s, _ in grow}
         shared = {}
@@ -44,7 +44,7 @@ class Pages:
         need = [(s, s in copies, self.held(self.lengths[s] + c) - self.held(self.lengths[s])) for s, c in grow]
         free = [p for p, r in enumerate(self.refs) if r == 0]
         if sum(c + k for _, c, k in need) > len(free):
-            self.status |= STATUS_NO_PAGES
+            self.status |= STATUS_NO_PAGES | STATUS_NOT_RESERVED
             return
         for s, copy, more in need:
             have = self.held(self.lengths[s])

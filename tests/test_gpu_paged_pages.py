@@ -12,6 +12,8 @@ from llm_accelerator_amd.paged import PagedKVCache, RaggedBatch
 
 pytestmark = pytest.mark.gpu
 
+HELD = _lib.STATUS_NOT_RESERVED
+
 
 def i32(v, dev):
     return torch.tensor(v, dtype=torch.int32, device=dev)
@@ -99,7 +101,7 @@ def test_reserve_is_all_or_nothing(dev):
                               ([2, 0], [1, 100], _lib.STATUS_BAD_POSITION)):
         reserve(cache, model, seqs, counts)
         same(cache, model)
-        assert model.status == bit
+        assert model.status == bit | HELD
         with pytest.raises(_lib.Q4DecError):
             cache.raise_for_status("reserve")
         model.status = 0
@@ -108,7 +110,7 @@ def test_reserve_is_all_or_nothing(dev):
     # counts that cannot be: decreasing starts, past the token rows, past max_new
     for starts, tokens, most in (([0, 5, 3], 8, 8), ([0, 4, 9], 8, 8), ([0, 6, 7], 8, 5), ([-2, 1, 2], 8, 8)):
         cache.reserve(RaggedBatch(i32([2, 3], dev), i32(starts, dev), tokens, most))
-        model.status = _lib.STATUS_BAD_SEQUENCE
+        model.status = _lib.STATUS_BAD_SEQUENCE | HELD
         same(cache, model)
         cache._status.zero_()
     # a partly filled last page whose entry is outside the pool
@@ -119,7 +121,7 @@ def test_reserve_is_all_or_nothing(dev):
         cache._status.zero_()
         reserve(cache, model, [3, 0], [1, 1])
         same(cache, model)
-        assert model.status == _lib.STATUS_BAD_PAGE
+        assert model.status == _lib.STATUS_BAD_PAGE | HELD
 
 
 def test_fork_and_truncate_leave_out_what_cannot_be(dev):
@@ -170,7 +172,7 @@ def test_empty_lists_and_full_rows(dev):
     same(cache, model)
     reserve(cache, model, [1], [1])
     same(cache, model)
-    assert model.status == _lib.STATUS_BAD_POSITION
+    assert model.status == _lib.STATUS_BAD_POSITION | HELD
     assert int(cache.compact().item()) == 4
 
 

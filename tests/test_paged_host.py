@@ -260,5 +260,5 @@ def test_python_arguments_are_checked():
 
 
 def test_status_names():
-    assert _lib.status_names(16 | 32 | 64) == ["NO_PAGES", "BAD_SEQUENCE", "BAD_PAGE"]
-    assert _lib.status_names(128) == ["UNKNOWN"]
+    assert _lib.status_names(16 | 32 | 64 | 128) == ["NO_PAGES", "BAD_SEQUENCE", "BAD_PAGE", "NOT_RESERVED"]
+    assert _lib.status_names(256) == ["UNKNOWN"]
