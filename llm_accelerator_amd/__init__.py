@@ -8,6 +8,7 @@ and for stream handles.
 * :mod:`.common`  -- drop-in mirror of the reference's ``common.py`` /
   ``run_manual_one_token`` functions
 * :mod:`.decode`  -- greedy decode driver with device-side token feedback
+* :mod:`.paged`   -- paged KV cache: ragged batches, append, attention, pages
 * :mod:`.build`   -- in-tree build of ``libq4dec.so`` for gfx950
 """
 

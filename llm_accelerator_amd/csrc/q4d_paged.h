@@ -88,12 +88,13 @@ struct PagedAttnArgs {
   int qh, bf16;
   void* ws;
   // set by launch_paged_attention
+  // of rows_part
   int* counters;  // parts that have arrived, by join level and block
-  float* pml;     // [slots][rows][2]
-  float* pacc;    // [slots][rows][d]
+  float* pml;     // [block][2 slots][kvh][16 rows][m, l]
+  float* pacc;    // [block][2 slots][kvh][16 rows][d]
   int blocks;     // per kv head
-  // of chunk_kernel
-  int* ccounters;
+  // of chunk_part
+  int* ccounters;  // by join level and part
   float* cml;     // [parts][kvh][4 waves][m, l of 32 rows]
   float* cacc;    // [parts][kvh][4 waves][32 x d]
   int slots, max_splits;  // per kv head: blocks that parts are to fill, parts at most

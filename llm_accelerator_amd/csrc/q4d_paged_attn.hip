@@ -2,8 +2,11 @@
 //
 // A kv head's query rows of a sequence are its new tokens times the G = q heads / kv heads that
 // share the kv head: row r is token r / G, head r % G.  Sequences of up to 16 rows (decode steps,
-// a few proposed tokens) are bound by reading K and V once: rows_part.  More rows share what is
-// read: chunk_part.  A call is one launch.
+// a few proposed tokens; 16 is what one MFMA takes) are bound by reading K and V once: rows_part.
+// More rows share what is read: chunk_part.  A call is one launch.
+// Both sides of the 16: decode steps on chunk_part would take 15 us instead of 8.6 (one sequence of
+// 700 positions), 154 instead of 129 (64 of 4000), 34 instead of 23 (3 of 32700); 24 sequences of 5
+// tokens and 10 rows 33 instead of 28.
 #include <math.h>
 
 #include <type_traits>
@@ -19,13 +22,12 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kRows = 16;   // query rows of rows_part
-constexpr int kJoin = 8;         // parts joined at a time
-constexpr int kLevels = 4;       // of joins: up to 8^4 parts
-constexpr int kCounters = 1024;  // counters of a level, one per block
+constexpr int kRows = 16;             // query rows of rows_part
+constexpr int kStep = 128;            // positions of a block's step there: 32 a wave
+constexpr int kJoin = 8;              // parts joined at a time
+constexpr int kLevels = 4;            // of joins: up to 8^4 parts
+constexpr int kCounters = 1024;       // counters of a level, one per block
 constexpr int kChunkCounters = 2048;  // the same of chunk_part, one per part
-constexpr int kMinSplit = 4;          // steps of a part there at least
-constexpr int kStep = 128;  // positions of a block's step there: 32 a wave
 
 template <bool BF>
 __device__ __forceinline__ float to_f32(uint16_t u) {
@@ -112,6 +114,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int b
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(lo | hi << 32), (short)0,
                                            __builtin_amdgcn_readfirstlane(bytes), 0x00027000);
 }
+// Non-temporal: every row is read once (64 sequences of 4000 positions 129 instead of 144 us; 3 of
+// 32700 with 16-position pages 23.3 instead of 22.2).
 __device__ __forceinline__ u32x4 rows_load(__amdgpu_buffer_rsrc_t r, int offset) {
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 2));
 }
@@ -128,18 +132,26 @@ __device__ __forceinline__ f32x4 load_dev4(__amdgpu_buffer_rsrc_t r, int offset)
 }
 
 // The running max moves only when a score exceeds it by more than this (log2 units): P = 2^(s - m)
-// stays below 2^8, far inside fp16's range, and the rescaling of the output is rare.
+// stays below 2^8, far inside fp16's range, and the rescaling of the output is rare (whole prompts
+// 187 instead of 193 us, nothing where K and V are streamed).
 constexpr float kRescale = 8.0f;
 
 // ---- up to 16 query rows a sequence --------------------------------------------------------
 // The work of a kv head is a line of steps of 128 positions, the sequences one after the other;
 // `blocks` blocks take S = ceil(steps / blocks) consecutive steps each, so every block streams as
-// many bytes whatever the lengths are (at least kMinSteps, so that a cut pays for its merge).  A
-// cut within `slack` steps of a sequence's end moves there.  A block's first and last sequences may
-// be parts: their softmax states go to the workspace (slot 1: the sequence begins in this block;
-// slot 0: it began in an earlier one), where they are joined.
-
-
+// many bytes whatever the lengths are.  A cut within `slack` steps of a sequence's end moves there,
+// which saves its join (24 sequences of 1500 positions and 5 tokens 28.2 instead of 28.8 us).  A
+// block's first and last sequences may be parts: their softmax states go to the workspace (slot 1:
+// the sequence begins in this block; slot 0: it began in an earlier one), where they are joined.
+// A step: S^T = K . Q^T (16x16x32 MFMA, K rows straight from memory in operand order, two tiles of 16
+// positions a wave), online softmax per row, O^T += V^T . P^T, where the S^T accumulators already are
+// the operand layout of P^T and V^T comes out of the wave's own LDS rows with the transposing read, so
+// that the waves meet only at a sequence's end.  P is rounded to the cache's type, as the product
+// wants; the sum l takes it unrounded.
+// Bound by the K and V stream: 64 sequences of 4000 positions (790 MB) 125-129 us, 6.2 TB/s, which is
+// what reads alone reach; short ones by a chain of ten dependent memory round trips (cut, page, rows,
+// join): 8.6 us for one of 700 positions, 23 us (3.2 TB/s) for 3 of 32700, 28 us (3.9 TB/s) for 24 of
+// 1500 and 5 tokens.  One block a CU: two take 133 / 26 / 31.6 us of these.
 struct Cut {
   int S, slack;
 };
@@ -543,6 +555,12 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
 //   V^T . P^T, where the S^T accumulators already are the operand layout of P^T (a lane holds 4 + 4
 //   keys of each 16 for one row) and V^T comes out of the row-major tile with the transposing read.
 // K and V tiles go from the pages to LDS by DMA one tile ahead, 16 rows a wave (one page at most).
+// Two blocks a CU, so that one's products run under the other's softmax.  4 prompts of up to 3500
+// positions, 16 / 8 heads: 173-187 us, 780-840 TFLOP/s of what rows see (a product of 8192^3 reaches
+// 1365); 512 tokens after 4097 41 us.  The matrix unit is 38 % busy, vector instructions 24 %, and DMA
+// costs 15 % of throughput.  Measured and no faster: the next step's first product interleaved with this
+// one's exponentials in a wave (180), the same with 8 waves that share tiles two and three steps ahead
+// (187), with 64 rows a wave and 512 registers (264: accumulators move between the register files).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTile = 128;  // query rows of a block
@@ -574,8 +592,10 @@ __device__ __forceinline__ void dma16(const uint16_t* base, uint32_t offset, uin
 }
 
 // A tile of n steps is cut into round(n / S) parts, S the steps that fill the device's blocks once (two
-// a CU; at least kMinSplit, so that a part pays for its join).  With more than half a step too few
-// or too many a part's steps lie within 3/4 S .. 3/2 S.
+// a CU; at least kMinSplit, so that a part pays for its join).  Parts then have 3/4 S .. 3/2 S steps.
+// kMinSplit 2 / 4 / 8: 3 sequences of 900 positions and 40 tokens 19.0 / 19.5 / 20.8 us, one of 20000 and
+// 64 tokens 49.2 / 49.7 / 47.3, 512 tokens after 4097 no difference.
+constexpr int kMinSplit = 4;
 __device__ __forceinline__ int split_parts(int steps, int S) { return max(1, (2 * steps + S) / (2 * S)); }
 constexpr int kMaxParts = 64;
 
@@ -1071,7 +1091,8 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
 }
 
 // Both: the first blocks * kvh blocks take the sequences of few rows, which stream K and V, and run
-// beside the others, which compute.
+// beside the others, which compute: 38 decode steps of 3000 positions and two chunks of 700 tokens
+// 93-96 us, two launches one after the other 103.
 template <int D, bool BF>
 __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[Shared<D>::kChunkV + Shared<D>::kMore];

@@ -334,7 +334,8 @@ class PagedKVCache:
         """softmax(q k^T scaling) v of the batch's tokens over their sequences' cached positions up to
         their own; q and the result [tokens, q_heads, head_dim] in the cache's type (``scaling``
         ``None``: head_dim ** -0.5).  ``ws``: scratch kept by the caller (:meth:`workspace`); without
-        one the call makes its own.  Rows in no sequence are left as they were."""
+        one the call makes its own.  ``out`` may be ``q`` itself.  Rows in no sequence are left as they
+        were (zeros in an ``out`` of the call's own)."""
         self._check_batch(batch)
         if q.dtype != self.dtype:
             raise ValueError(f"q must be {self.dtype}, as the cache")

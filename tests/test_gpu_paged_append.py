@@ -174,3 +174,23 @@ def test_append_on_a_stream_and_in_a_graph(dev):
         out.zero_()
         cache.append(0, batch, x, x, -x, rope, q_out=out)
         assert torch.equal(out, replayed) and torch.equal(cache.data, data) and cache.status() == 0
+
+
+@pytest.mark.parametrize("tokens,qh,kvh,d", [(2100, 14, 5, 64), (4500, 3, 2, 128), (11000, 14, 5, 64), (5000, 20, 3, 128)])
+def test_many_tokens_as_few(dev, tokens, qh, kvh, d):
+    """A wave takes one, two or four groups of head rows by how many there are: a token's values are those
+    that it has in a small batch, bit for bit."""
+    cache = setup(dev, [tokens], [tokens], kvh, d, 64, torch.float16)
+    x = torch.randn(tokens, qh + 2 * kvh, d, device=dev)
+    rope = RopeTable.build(d, tokens, device=dev)
+    gamma = 1 + 0.1 * torch.randn(d, device=dev)
+    split = lambda y: (y[:, :qh], y[:, qh:qh + kvh], y[:, qh + kvh:])  # noqa: E731
+    got = cache.append(1, RaggedBatch.of([0], [tokens], dev), *split(x), rope, gamma, gamma)
+    data = cache.data.clone()
+    cache.data.fill_(7.0)
+    out = torch.empty_like(got)
+    for at in range(0, tokens, 100):
+        n = min(100, tokens - at)
+        cache.lengths[0] = at + n
+        out[at:at + n] = cache.append(1, RaggedBatch.of([0], [n], dev), *split(x[at:at + n]), rope, gamma, gamma)
+    assert torch.equal(out, got) and torch.equal(cache.data, data) and cache.status() == 0
