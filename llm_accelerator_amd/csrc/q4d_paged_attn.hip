@@ -593,9 +593,17 @@ __device__ __forceinline__ void dma16(const uint16_t* base, uint32_t offset, uin
 
 // A tile of n steps is cut into round(n / S) parts, S the steps that fill the device's blocks once (two
 // a CU; at least kMinSplit, so that a part pays for its join).  Parts then have 3/4 S .. 3/2 S steps.
-// kMinSplit 2 / 4 / 8: 3 sequences of 900 positions and 40 tokens 19.0 / 19.5 / 20.8 us, one of 20000 and
-// 64 tokens 49.2 / 49.7 / 47.3, 512 tokens after 4097 no difference.
+// kMinSplit 2 / 4 / 6: one sequence of 1500 positions and 20 tokens 20.8 / 18.7 / 19.8 us, 2 of 200 fresh
+// ones 12.8 / 11.2 / 11.2, 3 of 900 and 40 tokens 19.1 / 19.7 / 21.1.
 constexpr int kMinSplit = 4;
+// One block a CU instead of two where that leaves two under kOneSteps steps each (the joins of twice the
+// parts cost more than the overlap gives), or where rows_part's blocks have more steps than these and
+// keep the CU busy beside.  Two / one, us: 64 tokens after 20000 (4.9 steps) 48 / 39.5, 40 sequences of 500
+// positions and 20 tokens (4) 35.5 / 22.6, 16 of 3000 with two kv heads (2.8) 33 / 30; 24 of 1500 (6.5) 37 /
+// 38.2, two chunks of 700 beside 14 decode steps (7) 58 / 65, 60 tokens after 30000 (7.3) 57 / 49.5, 512
+// after 4097 (8.7) 41.5 / 44, 2048 fresh ones (9) 39 / 46.  Chunks of 700 beside decode steps of k times
+// their steps: k 0.5: 58 / 65, 1.2: 96 / 87, 2.2: 143 / 121.
+constexpr int kOneSteps = 6;
 __device__ __forceinline__ int split_parts(int steps, int S) { return max(1, (2 * steps + S) / (2 * S)); }
 constexpr int kMaxParts = 64;
 
@@ -625,8 +633,13 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
     const int n = tiles_of(s);
     return n ? (int)min((long long)n * (tile_steps(s, 0) + steps_of(s.len)) / 2, 1LL << 18) : 0;
   };
-  const auto share = [&](int W, int most) {
-    return max(max(kMinSplit, (W + a.slots - 1) / a.slots), (most + kMaxParts - 2) / (kMaxParts - 1));
+  // steps of rows_part's sequences, which stream K and V beside these
+  const auto beside_of = [&](const SeqSpan& s) {
+    return s.count > 0 && s.count * G <= kRows ? (s.len + kStep - 1) / kStep : 0;
+  };
+  const auto share = [&](int W, int most, int beside) {
+    const int slots = W < kOneSteps * a.slots || beside > W ? (a.slots + 1) / 2 : a.slots;
+    return max(max(kMinSplit, (W + slots - 1) / slots), (most + kMaxParts - 2) / (kMaxParts - 1));
   };
   SeqSpan s = {0, 0, 0, 0};
   int parts, tile, part, slots;  // slots: lane i's is the workspace slot of the tile's part i
@@ -650,7 +663,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
     most = __builtin_amdgcn_readfirstlane(most);
     // Layer p = lane + 1: the tiles of p parts and more, which have steps >= p S - S / 2; layer 1 counts
     // those of two and more, like layer 2.  Sizes of the layers, and of lane b's sequences' share.
-    int S = share(sum(work_of(l)), most), size = 0, end = 0;
+    int S = share(sum(work_of(l)), most, sum(beside_of(l))), size = 0, end = 0;
     const auto in_layer = [&](int b) {
       return at_least(S * max(lane + 1, 2) - S / 2, __builtin_amdgcn_readlane(l_nt, b),
                       __builtin_amdgcn_readlane(l_rows, b), __builtin_amdgcn_readlane(l_old, b));
@@ -716,16 +729,17 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
       }
     };
     // every tile of a sequence in as many parts as its last
-    int S = 0, W = 0, items, splits;
+    int S = 0, W = 0, beside = 0, items, splits;
     for (int g = 0; g < a.r.n; g += 256) {
       const int b = g + t;
       SeqSpan l = {0, 0, 0, 0};
       if (b < a.r.n) l = seq_span(a.p, a.r, b);
       int ex, ey, aw, at;
-      block_scan(work_of(l), 0, &ex, &ey, &aw, &at);
+      block_scan(work_of(l), beside_of(l), &ex, &ey, &aw, &at);
       W += aw;
+      beside += at;
     }
-    for (S = share(W, steps_of(a.p.max_pages << a.p.page_shift));; S += (S + 3) / 4) {
+    for (S = share(W, steps_of(a.p.max_pages << a.p.page_shift), beside);; S += (S + 3) / 4) {
       items = splits = 0;
       for (int g = 0; g < a.r.n; g += 256) {
         const int b = g + t;
@@ -1092,7 +1106,7 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
 
 // Both: the first blocks * kvh blocks take the sequences of few rows, which stream K and V, and run
 // beside the others, which compute: 38 decode steps of 3000 positions and two chunks of 700 tokens
-// 93-96 us, two launches one after the other 103.
+// 87 us (when both were two launches, one after the other, they took 7 us more than together).
 template <int D, bool BF>
 __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[Shared<D>::kChunkV + Shared<D>::kMore];
