@@ -146,8 +146,10 @@ constexpr float kRescale = 8.0f;
 // A step: S^T = K . Q^T (16x16x32 MFMA, K rows straight from memory in operand order, two tiles of 16
 // positions a wave), online softmax per row, O^T += V^T . P^T, where the S^T accumulators already are
 // the operand layout of P^T and V^T comes out of the wave's own LDS rows with the transposing read, so
-// that the waves meet only at a sequence's end.  P is rounded to the cache's type, as the product
-// wants; the sum l takes it unrounded.
+// that the waves meet only at a sequence's end.  The product takes P as two numbers of the cache's
+// type, the rounded value and what that leaves (22 or 16 bits together; the stream hides the second
+// product: 1 % of a long batch's time, and outputs as close to 64 bits as their own rounding lets
+// them be instead of 1.4 times as far).
 // Bound by the K and V stream: 64 sequences of 4000 positions (790 MB) 125-129 us, 6.2 TB/s, which is
 // what reads alone reach; short ones by a chain of ten dependent memory round trips (cut, page, rows,
 // join): 8.6 us for one of 700 positions, 23 us (3.2 TB/s) for 3 of 32700, 28 us (3.9 TB/s) for 24 of
@@ -398,6 +400,10 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
         l += p[e];
       }
       const u32x4 pp = pack8<BF>(p);
+      float rest[8];  // what the rounding leaves
+#pragma unroll
+      for (int e = 0; e < 8; ++e) rest[e] = p[e] - to_f32<BF>((uint16_t)(e & 1 ? pp[e >> 1] >> 16 : pp[e >> 1]));
+      const u32x4 pr = pack8<BF>(rest);
       // V^T operand: dim 16 i + r, the same eight positions
       const auto vt = [&](int i) {
         u32x4 v;
@@ -412,7 +418,11 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
         return v;
       };
 #pragma unroll
-      for (int i = 0; i < DT; ++i) o[i] = mfma16<BF>(vt(i), pp, o[i]);
+      for (int i = 0; i < DT; ++i) {
+        const u32x4 v = vt(i);
+        o[i] = mfma16<BF>(v, pp, o[i]);
+        o[i] = mfma16<BF>(v, pr, o[i]);
+      }
     };
     issue(s0);
     for (int it = s0; it < s1; ++it) consume(it);
@@ -554,6 +564,8 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
 //   S^T = K . Q^T (32x32x16 MFMA; K rows from LDS, Q^T in registers); online softmax per row; O^T +=
 //   V^T . P^T, where the S^T accumulators already are the operand layout of P^T (a lane holds 4 + 4
 //   keys of each 16 for one row) and V^T comes out of the row-major tile with the transposing read.
+// P is rounded to the cache's type, which the product takes (here a second product would cost a quarter of
+// the time); the sum l takes it unrounded.
 // K and V tiles go from the pages to LDS by DMA one tile ahead, 16 rows a wave (one page at most).
 // Two blocks a CU, so that one's products run under the other's softmax.  4 prompts of up to 3500
 // positions, 16 / 8 heads: 173-187 us, 780-840 TFLOP/s of what rows see (a product of 8192^3 reaches
