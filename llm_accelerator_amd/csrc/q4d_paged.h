@@ -69,6 +69,8 @@ __host__ __device__ inline size_t page_elem(const PagedView& p, int page, int j)
   return (((size_t)page * p.kvh + j) << p.page_shift) * p.d;
 }
 
+constexpr long long kMaxBlocks = (1 << 24) - 1;  // of 256 threads: a launch has fewer than 2^32
+
 // Host: the descriptors' checks (Q4D_OK or an error code).
 int check_pages(const q4d_pages_t* p);
 int check_ragged(const q4d_ragged_t* r);

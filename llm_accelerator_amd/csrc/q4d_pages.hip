@@ -776,7 +776,7 @@ int q4d_paged_append(const q4d_pages_t* pages, int32_t layer, const q4d_ragged_t
   const int each = groups_per_wave((long long)batch->tokens * groups);
   a.per = (groups + each - 1) / each;
   const long long waves = (long long)batch->tokens * a.per;
-  if ((waves + 3) / 4 > INT32_MAX) return Q4D_ERR_SHAPE;
+  if ((waves + 3) / 4 > kMaxBlocks) return Q4D_ERR_SHAPE;
   const unsigned blocks = (unsigned)((waves + 3) / 4);
   const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const bool bf = pages->dtype == Q4D_BF16;

@@ -111,6 +111,16 @@ def test_attention_refuses(arg, value, code):
     assert _lib.load().q4d_paged_attention(*args) == code
 
 
+def test_more_blocks_than_a_launch_has_are_refused():
+    lib = _lib.load()
+    p = pages(num_kv_heads=256, head_dim=64)
+    r = ragged(tokens=1 << 24, max_new=1 << 24)
+    p, r, big, wide = ctypes.byref(p), ctypes.byref(r), 1 << 40, 4096 * 64
+    assert lib.q4d_paged_attention(p, 0, r, FAKE, wide, 4096, 0.1, FAKE, wide, FAKE, big, None) == SHAPE
+    assert lib.q4d_paged_append(p, 0, r, FAKE, wide, 4096, FAKE, wide, FAKE, wide, 0, None, None, 1e-6, None, FAKE,
+                                None) == SHAPE
+
+
 def test_page_calls_refuse():
     lib, p, r = _lib.load(), ctypes.byref(pages()), ctypes.byref(ragged())
     need = lib.q4d_pages_workspace_bytes(p)
