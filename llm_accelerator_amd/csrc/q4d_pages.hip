@@ -63,8 +63,8 @@ constexpr int kMaxBatch = 4096;
 struct PageWs {
   int32_t* copies;  // [1] number of entries of src / dst / rows
   int32_t* ids;     // [num_pages] compact: holes in order
-  int32_t* a;       // [num_pages] reserve: the batch's holders of a page; compact: movers in order
-  int32_t* b;       // [num_pages] reserve: the last of them; compact: where a page goes
+  int32_t* a;       // [num_pages] compact: movers in order
+  int32_t* b;       // [num_pages] compact: where a page goes
   int32_t *src, *dst, *rows;  // [max(num_pages, kMaxBatch)]
 };
 
@@ -119,16 +119,21 @@ __device__ __forceinline__ int pages_of(int len, int shift) { return (len + (1 <
 // One block, since every decision hangs on all of them: the batch is at most 4096 sequences (four a
 // thread, read once) and the refs a few 10,000 ints, of which a round looks at 16384 (a wave at 1024
 // in a row, four loads a lane), the first of them read ahead.  What it costs is the chain of dependent
-// reads (starts and seqs, lengths, the last page, its refs) and a round's scan: 200 sequences that grow
-// 15 us, 20 with the copy's launch.
+// reads (starts and seqs, lengths, the last page, its refs) and a round's scan: 7 us for 200 sequences that
+// grow by a token, 10 where they take 2300 of 19000 pages.
+// Shared last pages are few: they are counted in a hash table in LDS (by atomics on global memory it
+// took 5 us more), whose place the list of free pages takes over.
 constexpr int kRound = 16384;
+constexpr int kIds = 16384;        // free pages listed at a time
+constexpr int kSlots = kIds / 3;   // of the hash table, for up to kMaxBatch pages
+static_assert(kSlots > kMaxBatch, "an empty slot ends every search");
 
 __global__ __launch_bounds__(1024) void reserve_kernel(const PagedView p, const RaggedView r, const PageWs w) {
   constexpr int B = kMaxBatch / 1024;
   __shared__ uint32_t seen[65536 / 32];
   __shared__ int end[kMaxBatch];  // pages taken by sequences up to and with b
   __shared__ int row_of[kMaxBatch], have_of[kMaxBatch];  // have: pages held, bit 31: the last is copied first
-  __shared__ int ids[kRound];
+  __shared__ int ids[kIds];
   __shared__ __attribute__((aligned(16))) int sums[16];
   __shared__ int s_err, s_copies;
   const int t = threadIdx.x, lane = t & 63;
@@ -216,22 +221,26 @@ __global__ __launch_bounds__(1024) void reserve_kernel(const PagedView p, const 
     return;
   }
   // a page that several rows hold: how many of the batch, and which of them is the last
+  int slot[B];
+  int *key = ids, *holders = ids + kSlots, *last_of = ids + 2 * kSlots;
   if (shared) {
-#pragma unroll
-    for (int i = 0; i < B; ++i) {
-      if (refs[i] <= 1) continue;
-      w.a[last[i]] = 0;
-      w.b[last[i]] = -1;
+    for (int i = t; i < kSlots; i += 1024) {
+      key[i] = last_of[i] = -1;
+      holders[i] = 0;
     }
-    __threadfence();  // what other waves of the block change next is in the L2
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < B; ++i) {
       if (refs[i] <= 1) continue;
-      atomicAdd(&w.a[last[i]], 1);
-      atomicMax(&w.b[last[i]], t + 1024 * i);
+      slot[i] = (uint32_t)last[i] * 2654435761u % kSlots;
+      for (;;) {
+        const int old = atomicCAS(&key[slot[i]], -1, last[i]);
+        if (old == -1 || old == last[i]) break;
+        slot[i] = slot[i] + 1 == kSlots ? 0 : slot[i] + 1;
+      }
+      atomicAdd(&holders[slot[i]], 1);
+      atomicMax(&last_of[slot[i]], t + 1024 * i);
     }
-    __threadfence();
     __syncthreads();
   }
   int total = 0;
@@ -239,7 +248,7 @@ __global__ __launch_bounds__(1024) void reserve_kernel(const PagedView p, const 
   for (int i = 0; i < B; ++i) {
     const int b = t + 1024 * i;
     if (1024 * i >= r.n) break;
-    const bool cow = refs[i] > 1 && !(load_now(&w.a[last[i]]) == refs[i] && load_now(&w.b[last[i]]) == b);
+    const bool cow = refs[i] > 1 && !(holders[slot[i]] == refs[i] && last_of[slot[i]] == b);
     const int have = pages_of(len[i], p.page_shift);
     const int take = count[i] ? pages_of(len[i] + count[i], p.page_shift) - have + cow : 0;
     int sum;
@@ -250,10 +259,9 @@ __global__ __launch_bounds__(1024) void reserve_kernel(const PagedView p, const 
     total += sum;
   }
 
-  // The free pages of the lowest numbers, a round's at a time in LDS: first whether there are enough
-  // (no more than the first round is looked at, mostly), then the k-th to whom it goes.
-  const auto collect = [&](int p0) {
-    const Refs f = p0 ? load_round(p0) : ahead;
+  // The free pages of the lowest numbers: a round's have the numbers from `found` on, and those below
+  // base + kIds are listed in LDS.  (block_excl's barriers lie between the table's last use and this.)
+  const auto collect = [&](const Refs& f, int p0, int found, int base) {
     const uint64_t below = lane ? ~0ULL >> (64 - lane) : 0;
     int first[4], wave_total = 0;  // of this lane's load i, in the wave's order: by load, lane, element
 #pragma unroll
@@ -267,22 +275,22 @@ __global__ __launch_bounds__(1024) void reserve_kernel(const PagedView p, const 
       }
     }
     int n;
-    const int base = waves_excl(wave_total, t, sums, &n);
+    const int before = found - base + waves_excl(wave_total, t, sums, &n);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      int k = base + first[i];
+      int k = before + first[i];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (f.v[i][e] == 0) ids[k++] = p0 + (t >> 6) * 1024 + 256 * i + 4 * lane + e;
+        if (f.v[i][e] == 0) {
+          if (k < kIds) ids[k] = p0 + (t >> 6) * 1024 + 256 * i + 4 * lane + e;
+          ++k;
+        }
     }
     return n;
   };
-  int got = 0, found = 0, rounds = 0;
-  for (int p0 = 0; p0 < p.num_pages && found < total; p0 += kRound) {
-    got = collect(p0);
-    found += got;
-    ++rounds;
-  }
+  int found = 0;  // all rounds that it takes, so that it is known whether there are enough
+  for (int p0 = 0; p0 < p.num_pages && found < total; p0 += kRound)
+    found += collect(p0 ? load_round(p0) : ahead, p0, found, 0);
   if (found < total) {
     if (t == 0) {
       atomicOr(p.status, Q4D_STATUS_NO_PAGES | Q4D_STATUS_NOT_RESERVED);
@@ -290,11 +298,16 @@ __global__ __launch_bounds__(1024) void reserve_kernel(const PagedView p, const 
     }
     return;
   }
-  for (int i = 0, given = 0; i < rounds; ++i) {
-    if (rounds > 1) got = collect(i * kRound);
+  for (int base = 0; base < total; base += kIds) {
+    if (base) {  // what is given is free no more, so the next ones are the lowest
+      __syncthreads();
+      found = base;
+      for (int p0 = 0; p0 < p.num_pages && found < min(total, base + kIds); p0 += kRound)
+        found += collect(load_round(p0), p0, found, base);
+    }
     __syncthreads();  // ids (and end, row_of, have_of)
-    for (int k = given + t; k < min(total, given + got); k += 1024) {
-      const int id = ids[k - given];
+    for (int k = base + t; k < min(total, base + kIds); k += 1024) {
+      const int id = ids[k - base];
       int lo = 0, hi = r.n - 1;  // the first b with end[b] > k
       while (lo < hi) {
         const int mid = (lo + hi) >> 1;
@@ -314,8 +327,6 @@ __global__ __launch_bounds__(1024) void reserve_kernel(const PagedView p, const 
         tab[have + j - cow] = id;
       }
     }
-    given += got;
-    __syncthreads();
   }
   __syncthreads();  // the copies have read the lengths, and are counted
 #pragma unroll
@@ -668,7 +679,7 @@ int check_page_ws(const q4d_pages_t* p, const void* ws, size_t bytes) {
 
 // Blocks of a copy: a unit is 4 to 64 KB, and blocks with one or two units each keep more reads in
 // flight than few with many (48 partly filled pages of 28 layers, 1024 / 4096 / 8192 blocks: a step
-// of beams 85 / 70 / 71 us; 70 whole pages moved 211 / 213 / 205 us; nothing to copy: no difference).
+// of beams 85 / 70 / 71 us when its other kernels took 21; 70 whole pages moved 211 / 213 / 205 us; nothing to copy: no difference).
 constexpr int kCopyBlocks = 8192;
 
 }  // namespace

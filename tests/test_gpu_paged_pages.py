@@ -201,3 +201,37 @@ def test_pages_in_a_captured_graph(dev):
         model.truncate([d, c])
         same(cache, model)
     assert model.status == 0
+
+
+def test_more_pages_at_once_than_are_listed_at_a_time(dev):
+    """One call takes 20,000 pages of 45,000, between pages that are held: several lists of 16,384."""
+    cache, model = pair(dev, 45000, 16, 64, 600, layers=1, kvh=1)
+    reserve(cache, model, list(range(20)), [16 * 300 + i for i in range(20)])
+    cache.free(i32(list(range(0, 20, 3)), dev))
+    model.truncate(list(range(0, 20, 3)))
+    cache.fork(i32([1, 2], dev), i32([60, 61], dev))
+    model.fork([1, 2], [60, 61])
+    reserve(cache, model, [60] + list(range(20, 56)) + [61], [16 * 40] + [16 * 560 - i for i in range(36)] + [5])
+    same(cache, model, rows=False)
+    assert model.status == 0 and sum(r != 0 for r in model.refs) > 20000 + 3600
+    reserve(cache, model, [0, 56], [9000, 9600])
+    same(cache, model)
+
+
+@pytest.mark.parametrize("rows", [300, 1365, 2048])
+def test_many_shared_last_pages(dev, rows):
+    """Every sequence of the batch shares its last page: with one that writes too, with one that does not, or
+    with both."""
+    cache, model = pair(dev, 4 * rows, 16, 3 * rows, 3, layers=1, kvh=1)
+    first = list(range(rows))
+    reserve(cache, model, first, [1 + i % 15 for i in first])
+    second = [rows + i for i in first]
+    cache.fork(i32(first, dev), i32(second, dev))
+    model.fork(first, second)
+    third = first[::3]
+    cache.fork(i32(third, dev), i32([2 * rows + i for i in third], dev))
+    model.fork(third, [2 * rows + i for i in third])
+    both = [s for i in first for s in ((i, rows + i) if i % 2 else (rows + i, i))]
+    reserve(cache, model, both, [1] * len(both))
+    same(cache, model)
+    assert model.status == 0
