@@ -570,10 +570,11 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
 // K and V tiles go from the pages to LDS by DMA one tile ahead, 16 rows a wave (one page at most).
 // Two blocks a CU, so that one's products run under the other's softmax.  4 prompts of up to 3500
 // positions, 16 / 8 heads: 173-187 us, 780-840 TFLOP/s of what rows see (a product of 8192^3 reaches
-// 1365); 512 tokens after 4097 41 us.  The matrix unit is 38 % busy, vector instructions 24 %, and DMA
-// costs 15 % of throughput.  Measured and no faster: the next step's first product interleaved with this
-// one's exponentials in a wave (180), the same with 8 waves that share tiles two and three steps ahead
-// (187), with 64 rows a wave and 512 registers (264: accumulators move between the register files).
+// 1365), 2 prompts of 12000 970; 512 tokens after 4097 41 us.  Taken apart (prompts, 178 us): the products
+// and their operands from LDS alone 133, which is 1350 TFLOP/s and the rate of a library's product; the
+// softmax adds 25, DMA 20.  Measured and no faster: the next step's first product interleaved with this
+// one's exponentials in a wave (180), the same with 8 waves that share tiles two or three steps ahead
+// (185), with 64 rows a wave and 512 registers (264: accumulators move between the register files).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTile = 128;  // query rows of a block
