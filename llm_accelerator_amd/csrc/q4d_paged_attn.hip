@@ -602,7 +602,7 @@ __device__ __forceinline__ float halves(float v) {
 // Ordered by the kernel's own wait and barrier.
 __device__ __forceinline__ void dma16(const uint16_t* base, uint32_t offset, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base)
-               : "memory");
+               : "memory", "m0");
 }
 
 // A tile of n steps is cut into round(n / S) parts, S the steps that fill the device's blocks once (two
