@@ -506,10 +506,9 @@ int q4d_paged_attention_workspace_init(void* ws, size_t ws_bytes, void* stream);
  * out = softmax(q k^T scaling) v, q head h with kv head h / (q_heads / num_kv_heads).  q and out:
  * rows of q_heads x head_dim in the cache's type, row t at t * stride elements, 16-byte aligned;
  * out may be q itself.  q_heads is a multiple of num_kv_heads, up to 16 times.  Scores, softmax
- * and sums are fp32; the probabilities enter the product with v in the cache's type (as two of
- * them, value and remainder, where a kv head has up to 16 query rows of a sequence).  A position
- * whose page cannot be counts as not there (Q4D_STATUS_BAD_PAGE); a token that sees no position
- * gives zeros.  Values a token does not see, Inf and NaN among them, never reach its output.
+ * and sums are fp32; the probabilities enter the product with v in the cache's type (for sequences
+ * of few new tokens as two numbers of it, value and remainder).  A position whose page cannot be
+ * counts as not there (Q4D_STATUS_BAD_PAGE); a token that sees no position gives zeros.  Values a token does not see, Inf and NaN among them, never reach its output.
  * Deterministic; a token's last bits may depend on the batch's shape and lengths, though not on
  * the other sequences' values. */
 int q4d_paged_attention(const q4d_pages_t* pages, int32_t layer, const q4d_ragged_t* batch, const void* q,

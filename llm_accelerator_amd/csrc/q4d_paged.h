@@ -92,8 +92,8 @@ struct PagedAttnArgs {
   // set by launch_paged_attention
   // of rows_part
   int* counters;  // parts that have arrived, by join level and block
-  float* pml;     // [block][2 slots][kvh][16 rows][m, l]
-  float* pacc;    // [block][2 slots][kvh][16 rows][d]
+  float* pml;     // [block][2 slots][kvh][16 or 32 rows][m, l]
+  float* pacc;    // [block][2 slots][kvh][16 or 32 rows][d]
   int blocks;     // per kv head
   // of chunk_part
   int* ccounters;  // by join level and part

@@ -6,7 +6,9 @@
 // More rows share what is read: chunk_part.  A call is one launch.
 // Both sides of the 16: decode steps on chunk_part would take 15 us instead of 8.6 (one sequence of
 // 700 positions), 154 instead of 129 (64 of 4000), 34 instead of 23 (3 of 32700); 24 sequences of 5
-// tokens and 10 rows 33 instead of 28.
+// tokens and 10 rows 33 instead of 28.  Batches of up to 32 rows a sequence take rows_part too, in two
+// groups (4 tokens of 8 heads a kv head, two groups / chunk_part: one sequence of 700 positions 13.6 /
+// 15.7 us, one of 6000 with two kv heads 17.8 / 22.5, 24 of 1500 33.4 / 35.4, 64 of 4000 139 / 152).
 #include <math.h>
 
 #include <type_traits>
@@ -22,7 +24,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kRows = 16;             // query rows of rows_part
+constexpr int kRows = 16;             // query rows of a group of rows_part, which takes one or two
 constexpr int kStep = 128;            // positions of a block's step there: 32 a wave
 constexpr int kJoin = 8;              // parts joined at a time
 constexpr int kLevels = 4;            // of joins: up to 8^4 parts
@@ -185,7 +187,7 @@ constexpr int kLanes = 64;
 // the line, which ends at `end`, holds x.
 __device__ __forceinline__ int lane_of(int end, int x) { return __builtin_ctzll(__ballot(end > x) | 1ULL << 63); }
 
-template <int D, bool BF>
+template <int D, bool BF, int R>
 __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int* seqs, int block) {
   constexpr int KS = D / 32, DT = D / 16, NV = D / 16, LR = D / 8;  // LR lanes of 16 bytes a row
   constexpr int kRowBytes = 2 * D, kWaveBytes = 32 * kRowBytes;
@@ -207,7 +209,7 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
   SeqSpan l_span = {0, 0, 0, 0};
   bool bad = false;
   const auto steps_of = [&](const SeqSpan& s) {
-    return s.count > 0 && s.count * G <= kRows ? (s.len + kStep - 1) / kStep : 0;
+    return s.count > 0 && s.count * G <= R * kRows ? (s.len + kStep - 1) / kStep : 0;
   };
   if (few) {
     if (lane < a.r.n) l_span = seq_span(a.p, a.r, lane);
@@ -287,273 +289,313 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
     const int rows = s.count * G;
     const int32_t* tab = a.p.table + (size_t)s.row * a.p.max_pages;
     const int shift = a.p.page_shift, inpage = (1 << shift) - 1;
-    // this lane's query row, its last visible position, and the operand Q^T: dims 32 i + 8 g .. + 7
-    const int rr = min(r, rows - 1), tok = rr / G;
-    const int qpos = s.len - s.count + tok;
-    u32x4 q[KS];
-    {
-      const KernelArgs late = late_args();
-      const uint16_t* qp = late->q + (s.first + tok) * late->q_stride + (j * G + rr - tok * G) * D + 8 * g;
+    // of one or two groups of 16 query rows
+    const auto serve = [&](auto groups) {
+      constexpr int H = decltype(groups)::value;
+      // this lane's query row of either 16, its last visible position, and the operand Q^T: dims 32 i + 8 g .. + 7
+      int qpos[H];
+      u32x4 q[H][KS];
 #pragma unroll
-      for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const u32x4*>(qp + 32 * i);
-    }
-    const int first_hidden = s.len - s.count + 1;  // positions from here on are hidden from some row
+      for (int h = 0; h < H; ++h) {
+        const int rr = min(kRows * h + r, rows - 1), tok = rr / G;
+        qpos[h] = s.len - s.count + tok;
+        const KernelArgs late = late_args();
+        const uint16_t* qp = late->q + (s.first + tok) * late->q_stride + (j * G + rr - tok * G) * D + 8 * g;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) q[h][i] = *reinterpret_cast<const u32x4*>(qp + 32 * i);
+      }
+      const int first_hidden = s.len - s.count + 1;  // positions from here on are hidden from some row
 
-    const int s0 = x0 - lo, s1 = x1 - lo;
-    struct Stage {
-      u32x4 k[2][KS], v[NV];
-      bool ok0, ok1;  // the first and second 16 positions' pages are there
-    } d;
-    // The page of lanes 0-31's and of lanes 32-63's 16 positions of step `it`.
-    const auto page_of = [&](int it) {
-      const int e = (it * kStep + 32 * w + ((lane & 32) >> 1)) >> shift;
-      return tab[min(e, a.p.max_pages - 1)];
-    };
-    int page = page_of(s0);
-    bool bad_page = false, odd = false;
-    // Loads of step `it`, without a branch, so that the next steps' loads stay in flight while this
-    // one's are waited for: through descriptors that end with the sequence's last row (rows past it,
-    // of a page that is not there or of a step past the part's end are zeros and cost nothing).  K in
-    // operand order (score tile h row r is position 16 h + r), V row by row.
-    const auto issue = [&](int it) {
-      const int base = it * kStep + 32 * w;
-      const int p0 = __builtin_amdgcn_readlane(page, 0), p1 = __builtin_amdgcn_readlane(page, 32);
-      page = page_of(it + 1);
-      const int end = it < s1 ? s.len : 0;
-      const int n0 = min(max(end - base, 0), 16), n1 = min(max(end - base - 16, 0), 16);
-      d.ok0 = in_range(p0, a.p.num_pages);
-      d.ok1 = in_range(p1, a.p.num_pages);
-      bad_page |= (n0 && !d.ok0) || (n1 && !d.ok1);
-      const size_t o0 = page_elem(a.p, d.ok0 ? p0 : 0, j) + (size_t)(base & inpage) * D;
-      const size_t o1 = page_elem(a.p, d.ok1 ? p1 : 0, j) + (size_t)((base + 16) & inpage) * D;
-      const int b0 = d.ok0 ? n0 * kRowBytes : 0, b1 = d.ok1 ? n1 * kRowBytes : 0;
-      const auto k0 = rows_rsrc(a.kplane + o0, b0), k1 = rows_rsrc(a.kplane + o1, b1);
-      const auto v0 = rows_rsrc(a.vplane + o0, b0), v1 = rows_rsrc(a.vplane + o1, b1);
+      const int s0 = x0 - lo, s1 = x1 - lo;
+      struct Stage {
+        u32x4 k[2][KS], v[NV];
+        bool ok0, ok1;  // the first and second 16 positions' pages are there
+      } d;
+      // The page of lanes 0-31's and of lanes 32-63's 16 positions of step `it`.
+      const auto page_of = [&](int it) {
+        const int e = (it * kStep + 32 * w + ((lane & 32) >> 1)) >> shift;
+        return tab[min(e, a.p.max_pages - 1)];
+      };
+      int page = page_of(s0);
+      bool bad_page = false, odd = false;
+      // Loads of step `it`, without a branch, so that the next steps' loads stay in flight while this
+      // one's are waited for: through descriptors that end with the sequence's last row (rows past it,
+      // of a page that is not there or of a step past the part's end are zeros and cost nothing).  K in
+      // operand order (score tile h row r is position 16 h + r), V row by row.
+      const auto issue = [&](int it) {
+        const int base = it * kStep + 32 * w;
+        const int p0 = __builtin_amdgcn_readlane(page, 0), p1 = __builtin_amdgcn_readlane(page, 32);
+        page = page_of(it + 1);
+        const int end = it < s1 ? s.len : 0;
+        const int n0 = min(max(end - base, 0), 16), n1 = min(max(end - base - 16, 0), 16);
+        d.ok0 = in_range(p0, a.p.num_pages);
+        d.ok1 = in_range(p1, a.p.num_pages);
+        bad_page |= (n0 && !d.ok0) || (n1 && !d.ok1);
+        const size_t o0 = page_elem(a.p, d.ok0 ? p0 : 0, j) + (size_t)(base & inpage) * D;
+        const size_t o1 = page_elem(a.p, d.ok1 ? p1 : 0, j) + (size_t)((base + 16) & inpage) * D;
+        const int b0 = d.ok0 ? n0 * kRowBytes : 0, b1 = d.ok1 ? n1 * kRowBytes : 0;
+        const auto k0 = rows_rsrc(a.kplane + o0, b0), k1 = rows_rsrc(a.kplane + o1, b1);
+        const auto v0 = rows_rsrc(a.vplane + o0, b0), v1 = rows_rsrc(a.vplane + o1, b1);
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        d.k[0][i] = rows_load(k0, r * kRowBytes + 16 * g + 64 * i);
-        d.k[1][i] = rows_load(k1, r * kRowBytes + 16 * g + 64 * i);
-      }
+        for (int i = 0; i < KS; ++i) {
+          d.k[0][i] = rows_load(k0, r * kRowBytes + 16 * g + 64 * i);
+          d.k[1][i] = rows_load(k1, r * kRowBytes + 16 * g + 64 * i);
+        }
 #pragma unroll
-      for (int i = 0; i < NV / 2; ++i) {
-        d.v[i] = rows_load(v0, 16 * lane + 1024 * i);
-        d.v[NV / 2 + i] = rows_load(v1, 16 * lane + 1024 * i);
-      }
-    };
+        for (int i = 0; i < NV / 2; ++i) {
+          d.v[i] = rows_load(v0, 16 * lane + 1024 * i);
+          d.v[NV / 2 + i] = rows_load(v1, 16 * lane + 1024 * i);
+        }
+      };
 
-    f32x4 o[DT];
+      f32x4 o[H][DT];
+      float m[H], l[H];  // of query rows r and 16 + r; l of this lane's positions only
 #pragma unroll
-    for (int i = 0; i < DT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;  // of query row r; l of this lane's positions only
-    const auto consume = [&](int it) {
-      const int base = it * kStep + 32 * w;
-      const bool ok0 = d.ok0, ok1 = d.ok1;
-      const bool hides = base + 32 > first_hidden;
-      if (hides && s.count > 1) {  // Inf and NaN become zeros; they are added after the loop
+      for (int h = 0; h < H; ++h) {
+        m[h] = -INFINITY;
+        l[h] = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) odd |= drop_odd<BF>(d.v[i]);
+        for (int i = 0; i < DT; ++i) o[h][i] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
-      // V into this wave's LDS rows: 32-byte chunk c of row x at c ^ f(x), f chosen so that the 16
-      // rows of a transposing read fall on all banks
+      const auto consume = [&](int it) {
+        const int base = it * kStep + 32 * w;
+        const bool ok0 = d.ok0, ok1 = d.ok1;
+        const bool hides = base + 32 > first_hidden;
+        if (hides && s.count > 1) {  // Inf and NaN become zeros; they are added after the loop
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int row = i * (64 / LR) + lane / LR, slot = lane % LR;
-        const int f = D == 128 ? row & 7 : (row >> 1) & 3;
-        *reinterpret_cast<u32x4*>(vl + row * kRowBytes + ((slot ^ (f << 1)) << 4)) = d.v[i];
+          for (int i = 0; i < NV; ++i) odd |= drop_odd<BF>(d.v[i]);
+        }
+        // V into this wave's LDS rows: 32-byte chunk c of row x at c ^ f(x), f chosen so that the 16
+        // rows of a transposing read fall on all banks
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int row = i * (64 / LR) + lane / LR, slot = lane % LR;
+          const int f = D == 128 ? row & 7 : (row >> 1) & 3;
+          *reinterpret_cast<u32x4*>(vl + row * kRowBytes + ((slot ^ (f << 1)) << 4)) = d.v[i];
+        }
+        f32x4 st[H][2];
+#pragma unroll
+        for (int h = 0; h < H; ++h) st[h][0] = st[h][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            st[h][0] = mfma16<BF>(d.k[0][i], q[h][i], st[h][0]);
+            st[h][1] = mfma16<BF>(d.k[1][i], q[h][i], st[h][1]);
+          }
+        issue(it + 1);
+        u32x4 pp[H], pr[H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          // this lane's positions: 4 g .. + 3 of either 16
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = st[h][e >> 2][e & 3] * a.scale;
+          if (hides || !ok0 || !ok1) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (base + 16 * (e >> 2) + 4 * g + (e & 3) > qpos[h] || !(e < 4 ? ok0 : ok1)) y[e] = -INFINITY;
+          }
+          float mx = y[0];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) mx = fmaxf(mx, y[e]);
+          mx = rows4<false>(mx);
+          const bool move = mx > m[h] + kRescale || (m[h] == -INFINITY && mx > m[h]);
+          if (__ballot(move)) {
+            const float mn = move ? mx : m[h];
+            const float f = m[h] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[h] - mn);
+            m[h] = mn;
+            l[h] *= f;
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[h][i][e] *= f;
+          }
+          const float ms = m[h] == -INFINITY ? 0.f : m[h];
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(y[e] - ms);
+            l[h] += p[e];
+          }
+          pp[h] = pack8<BF>(p);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)  // what the rounding leaves
+            p[e] -= to_f32<BF>((uint16_t)(e & 1 ? pp[h][e >> 1] >> 16 : pp[h][e >> 1]));
+          pr[h] = pack8<BF>(p);
+        }
+        // V^T operand: dim 16 i + r, the same eight positions
+        const auto vt = [&](int i) {
+          u32x4 v;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = 16 * h + 4 * g + (r >> 2);
+            const int f = D == 128 ? row & 7 : (row >> 1) & 3;
+            const u32x2 x = read_tr4(vl + row * kRowBytes + ((i ^ f) << 5) + 8 * (r & 3));
+            v[2 * h] = x[0];
+            v[2 * h + 1] = x[1];
+          }
+          return v;
+        };
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          const u32x4 v = vt(i);
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            o[h][i] = mfma16<BF>(v, pp[h], o[h][i]);
+            o[h][i] = mfma16<BF>(v, pr[h], o[h][i]);
+          }
+        }
+      };
+      issue(s0);
+      for (int it = s0; it < s1; ++it) consume(it);
+      if (__ballot(odd)) {
+        const uint16_t* vplane = late_args()->vplane;
+        // this wave's positions that some row does not see (weight 1 does as well as the probability: what
+        // is added is Inf or NaN)
+        for (int it = max(s0, first_hidden / kStep); it < s1; ++it) {
+          const int base = it * kStep + 32 * w;
+          if (base + 32 <= first_hidden) continue;
+          for (int pos = base; pos < min(s.len, base + 32); ++pos) {
+            const int pg = tab[min(pos >> shift, a.p.max_pages - 1)];
+            if (!in_range(pg, a.p.num_pages)) continue;
+            const uint16_t* v = vplane + page_elem(a.p, pg, j) + (size_t)(pos & inpage) * D + 4 * g;
+#pragma unroll
+            for (int i = 0; i < DT; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = to_f32<BF>(v[16 * i + e]);
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+                  if (pos <= qpos[h] && not_finite(x)) o[h][i][e] += x;
+              }
+          }
+        }
       }
-      f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+      if (bad_page && lane == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_PAGE);
+
+      // ---- the four waves' states ----------------------------------------------------------------
+      // a thread takes row t / 16 of either 16 and D / 64 slots of 4 dims each: sl, sl + 16
+      const int row = t >> 4, sl = t & 15;
+      constexpr int NS = D / 64;
+      float M[H], L[H];
+      f32x4 acc[H][NS];
 #pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        st[0] = mfma16<BF>(d.k[0][i], q[i], st[0]);
-        st[1] = mfma16<BF>(d.k[1][i], q[i], st[1]);
-      }
-      issue(it + 1);
-      // this lane's positions: 4 g .. + 3 of either 16
-      float y[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = st[e >> 2][e & 3] * a.scale;
-      if (hides || !ok0 || !ok1) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (base + 16 * (e >> 2) + 4 * g + (e & 3) > qpos || !(e < 4 ? ok0 : ok1)) y[e] = -INFINITY;
-      }
-      float mx = y[0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) mx = fmaxf(mx, y[e]);
-      mx = rows4<false>(mx);
-      const bool move = mx > m + kRescale || (m == -INFINITY && mx > m);
-      if (__ballot(move)) {
-        const float mn = move ? mx : m;
-        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        l *= f;
+      for (int h = 0; h < H; ++h) {
+        if (h) block_sync_lds();  // the first rows' states have been read
+        l[h] = rows4<true>(l[h]);
+        if (g == 0) {
+          sml[(w * kRows + r) * 2] = m[h];
+          sml[(w * kRows + r) * 2 + 1] = l[h];
+        }
+        // lane holds O^T[dim 16 i + 4 g + e][row r]: 16-byte slot 4 i + g of row r at slot ^ r
 #pragma unroll
         for (int i = 0; i < DT; ++i)
+          *reinterpret_cast<f32x4*>(vl + r * (4 * D) + (((4 * i + g) ^ r) << 4)) = o[h][i];
+        block_sync_lds();
+        M[h] = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[i][e] *= f;
-      }
-      const float ms = m == -INFINITY ? 0.f : m;
-      float p[8];
+        for (int i = 0; i < 4; ++i) M[h] = fmaxf(M[h], sml[(i * kRows + row) * 2]);
+        L[h] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(y[e] - ms);
-        l += p[e];
-      }
-      const u32x4 pp = pack8<BF>(p);
-      float rest[8];  // what the rounding leaves
+        for (int n = 0; n < NS; ++n) acc[h][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) rest[e] = p[e] - to_f32<BF>((uint16_t)(e & 1 ? pp[e >> 1] >> 16 : pp[e >> 1]));
-      const u32x4 pr = pack8<BF>(rest);
-      // V^T operand: dim 16 i + r, the same eight positions
-      const auto vt = [&](int i) {
-        u32x4 v;
+        for (int i = 0; i < 4; ++i) {
+          const float mi = sml[(i * kRows + row) * 2], f = mi == -INFINITY ? 0.f : exp2f(mi - M[h]);
+          L[h] = fmaf(sml[(i * kRows + row) * 2 + 1], f, L[h]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = 16 * h + 4 * g + (r >> 2);
-          const int f = D == 128 ? row & 7 : (row >> 1) & 3;
-          const u32x2 x = read_tr4(vl + row * kRowBytes + ((i ^ f) << 5) + 8 * (r & 3));
-          v[2 * h] = x[0];
-          v[2 * h + 1] = x[1];
+          for (int n = 0; n < NS; ++n) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(lds + i * kWaveBytes + row * (4 * D) + (((sl + 16 * n) ^ row) << 4));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[h][n][e] = mi == -INFINITY ? acc[h][n][e] : fmaf(x[e], f, acc[h][n][e]);
+          }
         }
-        return v;
-      };
+      }
+      // The parts' states are joined eight at a time: of each eight the block that counts in last adds
+      // them in order and goes on with the sum as one of the next level's parts.
+      const KernelArgs late = late_args();
+      const auto pacc = rows_rsrc(late->pacc, 1 << 30);
+      float* pml = late->pml;
+      const int kf = cut_first(c, lo);
+      int count = max(0, cut_last(c, hi) - kf + 1) + 1, part = x0 == lo ? 0 : k - kf + 1;
+      // part 0 lies in block kf - 1's slot 1, part i in block kf - 1 + i's slot 0; a sum lies where its
+      // first part did, and its counter is that block's
+      for (int level = 0, step = 1; count > 1; ++level, step *= kJoin) {
+        const auto place = [&](int i, int h) {
+          return ((((kf - 1 + i * step) * 2 + (i == 0)) * kvh + j) * R + h) * kRows + row;
+        };
+        const int first = part / kJoin * kJoin, size = min(kJoin, count - first);
+        if (size > 1) {
 #pragma unroll
-      for (int i = 0; i < DT; ++i) {
-        const u32x4 v = vt(i);
-        o[i] = mfma16<BF>(v, pp, o[i]);
-        o[i] = mfma16<BF>(v, pr, o[i]);
+          for (int h = 0; h < H; ++h) {
+            if (kRows * h + row >= rows) continue;
+            const int at = place(part, h);
+#pragma unroll
+            for (int n = 0; n < NS; ++n) store_dev4(pacc, (at * D + 64 * n + 4 * sl) * 4, acc[h][n]);
+            if (sl == 0) {
+              store_dev(pml + at * 2, M[h]);
+              store_dev(pml + at * 2 + 1, L[h]);
+            }
+          }
+          __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are performed
+          __syncthreads();                // ... and every other thread's
+          int* counter = late->counters + level * kCounters + (kf - 1 + first * step) * kvh + j;
+          if (t == 0) *s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == size - 1;
+          __syncthreads();
+          if (!*s_last) break;
+          if (t == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // next call
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            if (kRows * h + row >= rows) continue;
+            float mi[kJoin], li[kJoin];
+            f32x4 ai[kJoin][NS];
+#pragma unroll
+            for (int i = 0; i < kJoin; ++i) {
+              const int at = place(first + min(i, size - 1), h);
+              mi[i] = load_dev(pml + at * 2);
+              li[i] = load_dev(pml + at * 2 + 1);
+#pragma unroll
+              for (int n = 0; n < NS; ++n) ai[i][n] = load_dev4(pacc, (at * D + 64 * n + 4 * sl) * 4);
+            }
+            M[h] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kJoin; ++i) M[h] = fmaxf(M[h], mi[i]);
+            L[h] = 0.f;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) acc[h][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < kJoin; ++i) {
+              if (i >= size) continue;
+              const float f = mi[i] == -INFINITY ? 0.f : exp2f(mi[i] - M[h]);
+              L[h] = fmaf(li[i], f, L[h]);
+#pragma unroll
+              for (int n = 0; n < NS; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  acc[h][n][e] = mi[i] == -INFINITY ? acc[h][n][e] : fmaf(ai[i][n][e], f, acc[h][n][e]);
+            }
+          }
+        }
+        part = first / kJoin;
+        count = (count + kJoin - 1) / kJoin;
+      }
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const int at = kRows * h + row;
+        if (count > 1 || at >= rows) continue;
+        const int otok = at / G;
+        uint16_t* op = late->out + (s.first + otok) * late->out_stride + (j * G + at - otok * G) * D + 4 * sl;
+        const float inv = L[h] == 0.f ? 0.f : 1.0f / L[h];
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          const uint32_t u0 = from_f32<BF>(acc[h][n][0] * inv), u1 = from_f32<BF>(acc[h][n][1] * inv);
+          const uint32_t u2 = from_f32<BF>(acc[h][n][2] * inv), u3 = from_f32<BF>(acc[h][n][3] * inv);
+          *reinterpret_cast<u32x2*>(op + 64 * n) = u32x2{u0 | u1 << 16, u2 | u3 << 16};
+        }
       }
     };
-    issue(s0);
-    for (int it = s0; it < s1; ++it) consume(it);
-    if (__ballot(odd)) {
-      const uint16_t* vplane = late_args()->vplane;
-      // this wave's positions that some row does not see (weight 1 does as well as the probability: what
-      // is added is Inf or NaN)
-      for (int it = max(s0, first_hidden / kStep); it < s1; ++it) {
-        const int base = it * kStep + 32 * w;
-        if (base + 32 <= first_hidden) continue;
-        for (int pos = base; pos < min(s.len, base + 32); ++pos) {
-          const int pg = tab[min(pos >> shift, a.p.max_pages - 1)];
-          if (!in_range(pg, a.p.num_pages)) continue;
-          const uint16_t* v = vplane + page_elem(a.p, pg, j) + (size_t)(pos & inpage) * D + 4 * g;
-#pragma unroll
-          for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = to_f32<BF>(v[16 * i + e]);
-              if (pos <= qpos && not_finite(x)) o[i][e] += x;
-            }
-        }
-      }
-    }
-    if (bad_page && lane == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_PAGE);
-
-    // ---- the four waves' states ----------------------------------------------------------------
-    l = rows4<true>(l);
-    if (g == 0) {
-      sml[(w * kRows + r) * 2] = m;
-      sml[(w * kRows + r) * 2 + 1] = l;
-    }
-    // lane holds O^T[dim 16 i + 4 g + e][row r]: 16-byte slot 4 i + g of row r at slot ^ r
-#pragma unroll
-    for (int i = 0; i < DT; ++i)
-      *reinterpret_cast<f32x4*>(vl + r * (4 * D) + (((4 * i + g) ^ r) << 4)) = o[i];
-    block_sync_lds();
-    const int row = t >> 4, sl = t & 15;  // D / 64 slots of 4 dims each: sl, sl + 16
-    constexpr int NS = D / 64;
-    float M = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) M = fmaxf(M, sml[(i * kRows + row) * 2]);
-    float L = 0.f;
-    f32x4 acc[NS];
-#pragma unroll
-    for (int n = 0; n < NS; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float mi = sml[(i * kRows + row) * 2], f = mi == -INFINITY ? 0.f : exp2f(mi - M);
-      L = fmaf(sml[(i * kRows + row) * 2 + 1], f, L);
-#pragma unroll
-      for (int n = 0; n < NS; ++n) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(lds + i * kWaveBytes + row * (4 * D) + (((sl + 16 * n) ^ row) << 4));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[n][e] = mi == -INFINITY ? acc[n][e] : fmaf(x[e], f, acc[n][e]);
-      }
-    }
-    // The parts' states are joined eight at a time: of each eight the block that counts in last adds
-    // them in order and goes on with the sum as one of the next level's parts.
-    const KernelArgs late = late_args();
-    const auto pacc = rows_rsrc(late->pacc, 1 << 30);
-    float* pml = late->pml;
-    const int kf = cut_first(c, lo);
-    int count = max(0, cut_last(c, hi) - kf + 1) + 1, part = x0 == lo ? 0 : k - kf + 1;
-    // part 0 lies in block kf - 1's slot 1, part i in block kf - 1 + i's slot 0; a sum lies where its
-    // first part did, and its counter is that block's
-    for (int level = 0, step = 1; count > 1; ++level, step *= kJoin) {
-      const auto place = [&](int i) {
-        return (((kf - 1 + i * step) * 2 + (i == 0)) * kvh + j) * kRows + row;
-      };
-      const int first = part / kJoin * kJoin, size = min(kJoin, count - first);
-      if (size > 1) {
-        if (row < rows) {
-          const int at = place(part);
-#pragma unroll
-          for (int n = 0; n < NS; ++n) store_dev4(pacc, (at * D + 64 * n + 4 * sl) * 4, acc[n]);
-          if (sl == 0) {
-            store_dev(pml + at * 2, M);
-            store_dev(pml + at * 2 + 1, L);
-          }
-        }
-        __builtin_amdgcn_s_waitcnt(0);  // this thread's stores are performed
-        __syncthreads();                // ... and every other thread's
-        int* counter = late->counters + level * kCounters + (kf - 1 + first * step) * kvh + j;
-        if (t == 0) *s_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == size - 1;
-        __syncthreads();
-        if (!*s_last) break;
-        if (t == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // next call
-        if (row < rows) {
-          float mi[kJoin], li[kJoin];
-          f32x4 ai[kJoin][NS];
-#pragma unroll
-          for (int i = 0; i < kJoin; ++i) {
-            const int at = place(first + min(i, size - 1));
-            mi[i] = load_dev(pml + at * 2);
-            li[i] = load_dev(pml + at * 2 + 1);
-#pragma unroll
-            for (int n = 0; n < NS; ++n) ai[i][n] = load_dev4(pacc, (at * D + 64 * n + 4 * sl) * 4);
-          }
-          M = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < kJoin; ++i) M = fmaxf(M, mi[i]);
-          L = 0.f;
-#pragma unroll
-          for (int n = 0; n < NS; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int i = 0; i < kJoin; ++i) {
-            if (i >= size) continue;
-            const float f = mi[i] == -INFINITY ? 0.f : exp2f(mi[i] - M);
-            L = fmaf(li[i], f, L);
-#pragma unroll
-            for (int n = 0; n < NS; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[n][e] = mi[i] == -INFINITY ? acc[n][e] : fmaf(ai[i][n][e], f, acc[n][e]);
-          }
-        }
-      }
-      part = first / kJoin;
-      count = (count + kJoin - 1) / kJoin;
-    }
-    if (count == 1 && row < rows) {
-      const int otok = row / G;
-      uint16_t* op = late->out + (s.first + otok) * late->out_stride + (j * G + row - otok * G) * D + 4 * sl;
-      const float inv = L == 0.f ? 0.f : 1.0f / L;
-#pragma unroll
-      for (int n = 0; n < NS; ++n) {
-        const uint32_t u0 = from_f32<BF>(acc[n][0] * inv), u1 = from_f32<BF>(acc[n][1] * inv);
-        const uint32_t u2 = from_f32<BF>(acc[n][2] * inv), u3 = from_f32<BF>(acc[n][3] * inv);
-        *reinterpret_cast<u32x2*>(op + 64 * n) = u32x2{u0 | u1 << 16, u2 | u3 << 16};
-      }
-    }
+    if (R > 1 && rows > kRows) serve(std::integral_constant<int, R>());
+    else serve(std::integral_constant<int, 1>());
     block_sync_lds();  // the next sequence's V rows go where the states were
   }
 }
@@ -1111,11 +1153,11 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   }
 }
 
-template <int D, bool BF>
+template <int D, bool BF, int R>
 __global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[Shared<D>::kRowsV + Shared<D>::kMore];
   extern __shared__ int seqs[];
-  rows_part<D, BF>(a, lds, seqs, blockIdx.x);
+  rows_part<D, BF, R>(a, lds, seqs, blockIdx.x);
 }
 
 // Both: the first blocks * kvh blocks take the sequences of few rows, which stream K and V, and run
@@ -1126,7 +1168,7 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[Shared<D>::kChunkV + Shared<D>::kMore];
   extern __shared__ int seqs[];
   const int rows = a.blocks * a.p.kvh;
-  if ((int)blockIdx.x < rows) rows_part<D, BF>(a, lds, seqs, blockIdx.x);
+  if ((int)blockIdx.x < rows) rows_part<D, BF, 1>(a, lds, seqs, blockIdx.x);
   else chunk_part<D, BF>(a, lds, seqs, blockIdx.x - rows);
 }
 
@@ -1145,21 +1187,29 @@ Layout layout(int kvh, int d, bool chunks) {
   Layout l;
   const size_t slots = 2 * (size_t)rows_blocks(kvh) * kvh, items = chunks ? (size_t)chunk_splits(kvh) * kvh : 0;
   l.pml = paged_attention_ws_counters();
-  l.pacc = l.pml + align_up(slots * kRows * 2 * 4, 256);
-  l.cml = l.pacc + align_up(slots * kRows * d * 4, 256);
+  l.pacc = l.pml + align_up(slots * 2 * kRows * 2 * 4, 256);
+  l.cml = l.pacc + align_up(slots * 2 * kRows * d * 4, 256);
   l.cacc = l.cml + align_up(items * kTile * 2 * 4, 256);
   l.total = l.cacc + items * kTile * d * 4;
   return l;
 }
-bool has_chunks(int qh, int kvh, int max_new) { return (long long)max_new * (qh / kvh) > kRows; }
+// Groups of 16 query rows that the batch's sequences have at most: rows_part takes all of them if that is one
+// or two, else (0) the sequences of one, and chunk_part the others.  Two groups beside chunks, or in the
+// kernel for one, cost that one 3 to 7 % (mixed 87 / 93 us, 64 decode steps 129 / 132).
+int row_groups(int qh, int kvh, int max_new) {
+  const long long rows = (long long)max_new * (qh / kvh);
+  return rows <= kRows ? 1 : rows <= 2 * kRows ? 2 : 0;
+}
+bool has_chunks(int qh, int kvh, int max_new) { return row_groups(qh, kvh, max_new) == 0; }
 
 template <int D, bool BF>
 int launch(const PagedAttnArgs& a, hipStream_t st) {
   const int kvh = a.p.kvh, G = a.qh / kvh;
   const size_t seqs = a.r.n > kLanes ? (size_t)a.r.n * 16 : 0;
   const long long rows = (long long)a.blocks * kvh;
-  if (!has_chunks(a.qh, kvh, a.r.max_new)) {
-    hipLaunchKernelGGL((rows_kernel<D, BF>), dim3((unsigned)rows), dim3(256), seqs, st, a);
+  if (const int groups = row_groups(a.qh, kvh, a.r.max_new)) {
+    if (groups == 1) hipLaunchKernelGGL((rows_kernel<D, BF, 1>), dim3((unsigned)rows), dim3(256), seqs, st, a);
+    else hipLaunchKernelGGL((rows_kernel<D, BF, 2>), dim3((unsigned)rows), dim3(256), seqs, st, a);
     return check_launch();
   }
   // items: a sequence's tiles are at most its rows / 128, rounded up; more parts at most chunk_splits

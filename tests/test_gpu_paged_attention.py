@@ -82,6 +82,10 @@ CHUNKS = [  # (length, new) of every sequence, q heads, kv heads, dim, page, typ
     ([(129, 128), (4000, 64)], 16, 16, 64, 64, F), ([(i + 3, 1 + i % 3) for i in range(70)], 6, 3, 128, 16, F),
     ([(1025, 2)] * 3 + [(40, 40)], 32, 2, 128, 64, B), ([(700, 33)] * 5, 2, 2, 128, 64, F),
     ([(333, 333), (12, 12)], 16, 1, 128, 256, B), ([(4500, 18)], 8, 8, 128, 16, F),
+    # at most 17 to 32 rows a kv head, sequences of one group of 16 among them
+    ([(700, 4)], 64, 8, 128, 64, F), ([(5000, 4), (3, 3), (129, 2), (900, 0), (64, 1)], 16, 2, 128, 16, B),
+    ([(300 + 31 * i, 1 + i % 8) for i in range(20)], 8, 2, 64, 32, F), ([(2, 2), (2000, 2)], 32, 2, 128, 256, F),
+    ([(32, 32), (33, 17), (31, 31), (1000, 16)], 3, 3, 64, 16, B), ([(40 + i, 1 + i % 5) for i in range(90)], 12, 2, 128, 64, F),
 ]
 
 
@@ -99,7 +103,7 @@ def test_chunks_vs_fp64(dev, seqs, qh, kvh, d, ps, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F, B], ids=["f16", "bf16"])
-@pytest.mark.parametrize("new,length", [(5, 40), (40, 100), (150, 150)])
+@pytest.mark.parametrize("new,length", [(5, 40), (12, 90), (16, 700), (40, 100), (150, 150)])
 def test_what_a_token_does_not_see_does_not_reach_it(dev, new, length, dtype):
     """Inf and NaN in the keys and values of later tokens of the same chunk: earlier rows are as without
     them, later ones are not finite."""
@@ -151,7 +155,7 @@ def test_extreme_scores(dev):
     assert bool(((out[0].double() - v.mean(0)).abs() <= 2.0 ** -10 * v.abs().mean(0)).all())
 
 
-@pytest.mark.parametrize("counts", [(1, 1, 1, 1), (3, 1, 2, 2), (40, 1, 17, 9)], ids=str)
+@pytest.mark.parametrize("counts", [(1, 1, 1, 1), (3, 1, 2, 2), (12, 1, 16, 9), (40, 1, 17, 9)], ids=str)
 def test_bad_pages_are_positions_that_are_not_there(dev, counts):
     lengths = [150, 90, 64, 47]
     cache = filled(dev, lengths, 2, 128, 16, F)
@@ -273,7 +277,7 @@ def test_python_refusals(dev):
         PagedKVCache(1, 4, 24, 2, 64, 2, 64, F, dev)
 
 
-@pytest.mark.parametrize("counts", [[1] * 5, [3, 1, 2, 8, 5], [90, 1, 33, 2, 1]], ids=str)
+@pytest.mark.parametrize("counts", [[1] * 5, [3, 1, 2, 8, 5], [13, 1, 16, 2, 9], [90, 1, 33, 2, 1]], ids=str)
 def test_streams_and_graphs_share_a_workspace_in_turn(dev, counts):
     """Two captured calls of one workspace, replayed in turn between eager ones, on lengths that change."""
     cache = filled(dev, [900, 600, 2000, 50, 130], 2, 128, 16, F)
