@@ -839,6 +839,15 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   const bool active = row0 < rows;  // the wave has rows
   const int hidden0 = old + tile * kTile / G + 1;  // positions from here on are hidden from some row
 
+  // the first tiles' pages, the query rows and the first tile are on their way together
+  const int32_t* tab = a.p.table + (size_t)s.row * a.p.max_pages;
+  const int shift = a.p.page_shift, inpage = (1 << shift) - 1;
+  const auto pages_at = [&](int st) {  // lanes 16 i ..: the page of the step's 16 i .. + 15
+    const int pos = st * kKeys + 16 * (lane >> 4);
+    return tab[min(pos >> shift, a.p.max_pages - 1)];
+  };
+  int pages = pages_at(st0), pages_next = pages_at(st0 + 1);
+
   // Q^T operand: lane (row l % 32, half l / 32) holds dims 16 i + 8 half .. + 7
   const int qc = lane & 31, hf = lane >> 5;
   const int row = min(row0 + qc, rows - 1), tok = row / G, head = j * G + row - tok * G;
@@ -847,24 +856,13 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   u32x4 q[KS];
   {
     const uint16_t* qp = a.q + (s.first + tok) * a.q_stride + head * D + 8 * hf;
-    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      q[i] = *reinterpret_cast<const u32x4*>(qp + 16 * i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) q[i][e] ^= flip;
-    }
+    for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const u32x4*>(qp + 16 * i);
   }
   // (a scale of 0 keeps masked scores at -Inf)
   const float scale = fmaxf(fabsf(a.scale), 1e-30f);
 
   // ---- K / V tiles ---------------------------------------------------------------------------
-  const int32_t* tab = a.p.table + (size_t)s.row * a.p.max_pages;
-  const int shift = a.p.page_shift, inpage = (1 << shift) - 1;
-  const auto pages_at = [&](int st) {  // lanes 16 i ..: the page of the step's 16 i .. + 15
-    const int pos = st * kKeys + 16 * (lane >> 4);
-    return tab[min(pos >> shift, a.p.max_pages - 1)];
-  };
   constexpr int RI = 64 / LR;  // rows a DMA instruction
   const int drow = lane / LR, dslot = lane % LR;
   const auto kswz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
@@ -877,7 +875,6 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
     kfrom[i] = r * kRowBytes + ((dslot ^ kswz(r)) << 4);
     vfrom[i] = r * kRowBytes + ((dslot ^ vswz(r)) << 4);
   }
-  int pages = pages_at(st0);
   uint64_t gone = 0;  // 16-row groups of the tile last issued whose page is not there (bits 16 i)
   bool bad_page = false;
   const auto issue = [&](int st, int sg) {
@@ -1036,7 +1033,13 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   };
   block_sync_lds();  // s_odd is 0 before anybody sets it
   if (st0 < st1) issue(st0, 0);
-  pages = pages_at(st0 + 1);
+  pages = pages_next;
+  if (a.scale < 0.f) {
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[i][e] ^= 0x80008000u;
+  }
   for (int st = st0; st < st1; st += 2) {
     take(st, std::integral_constant<int, 0>());
     if (st + 1 < st1) take(st + 1, std::integral_constant<int, 1>());
