@@ -660,6 +660,8 @@ constexpr int kMinSplit = 4;
 // after 4097 (8.7) 41.5 / 44, 2048 fresh ones (9) 39 / 46.  Chunks of 700 beside decode steps of k times
 // their steps: k 0.5: 58 / 65, 1.2: 96 / 87, 2.2: 143 / 121.
 constexpr int kOneSteps = 6;
+// A sequence's tiles are at most its rows / kTile, rounded up.
+__host__ __device__ inline long long tiles_most(int tokens, int G, int n) { return (long long)tokens * G / kTile + n; }
 __device__ __forceinline__ int split_parts(int steps, int S) { return max(1, (2 * steps + S) / (2 * S)); }
 constexpr int kMaxParts = 64;
 
@@ -697,6 +699,9 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
     const int slots = W < kOneSteps * a.slots || beside > W ? (a.slots + 1) / 2 : a.slots;
     return max(max(kMinSplit, (W + slots - 1) / slots), (most + kMaxParts - 2) / (kMaxParts - 1));
   };
+  // Starts that go back and forth (a bad batch) can ask for more tiles than the launch has blocks: then no
+  // block does anything, so that no part waits for one that never comes.
+  const long long most_tiles = tiles_most(a.r.tokens, G, a.r.n);
   SeqSpan s = {0, 0, 0, 0};
   int parts, tile, part, slots;  // slots: lane i's is the workspace slot of the tile's part i
   if (a.r.n <= kLanes) {
@@ -712,7 +717,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
       return x < rows ? nt - (int)(x / kTile) : 0;
     };
     const int tiles = sum(l_nt);
-    if (tiles == 0) return;
+    if (tiles == 0 || tiles > most_tiles) return;
     int most = l_nt ? steps_of(l.len) : 0;
 #pragma unroll
     for (int m = 32; m; m >>= 1) most = max(most, __shfl_xor(most, m));
@@ -786,6 +791,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
     };
     // every tile of a sequence in as many parts as its last
     int S = 0, W = 0, beside = 0, items, splits;
+    long long tiles = 0;
     for (int g = 0; g < a.r.n; g += 256) {
       const int b = g + t;
       SeqSpan l = {0, 0, 0, 0};
@@ -794,7 +800,10 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
       block_scan(work_of(l), beside_of(l), &ex, &ey, &aw, &at);
       W += aw;
       beside += at;
+      block_scan(tiles_of(l) & 0xFFF, tiles_of(l) >> 12, &ex, &ey, &aw, &at);
+      tiles += aw + ((long long)at << 12);
     }
+    if (tiles > most_tiles) return;
     for (S = share(W, steps_of(a.p.max_pages << a.p.page_shift), beside);; S += (S + 3) / 4) {
       items = splits = 0;
       for (int g = 0; g < a.r.n; g += 256) {
@@ -1215,8 +1224,8 @@ int launch(const PagedAttnArgs& a, hipStream_t st) {
     else hipLaunchKernelGGL((rows_kernel<D, BF, 2>), dim3((unsigned)rows), dim3(256), seqs, st, a);
     return check_launch();
   }
-  // items: a sequence's tiles are at most its rows / 128, rounded up; more parts at most chunk_splits
-  const long long items = (long long)a.r.tokens * G / kTile + a.r.n + chunk_splits(kvh);
+  // items: tiles, and more parts of them at most chunk_splits
+  const long long items = tiles_most(a.r.tokens, G, a.r.n) + chunk_splits(kvh);
   if (rows + items * kvh > kMaxBlocks) return Q4D_ERR_SHAPE;
   hipLaunchKernelGGL((chunk_kernel<D, BF>), dim3((unsigned)(rows + items * kvh)), dim3(256), seqs, st, a);
   return check_launch();

@@ -332,6 +332,25 @@ def test_two_calls_at_once_with_their_own_workspaces(dev):
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+@pytest.mark.parametrize("n", [20, 64, 130, 700])
+def test_starts_that_go_back_and_forth_leave_the_workspace_as_it_was(dev, n):
+    """More tiles than the token rows have: the bad batch is reported, the next call is as ever."""
+    cache = filled(dev, [900] * n, 1, 128, 16, F)
+    good = RaggedBatch.of(list(range(n))[:8], [60, 1, 30, 100, 1, 2, 5, 50], dev)
+    q = torch.randn(good.tokens, 16, 128, device=dev).half()
+    ws = max((cache.workspace(16, good), PagedWorkspace(cache, 16, n, 200, 200)), key=lambda w: w.nbytes)
+    want = cache.attention(0, good, q, ws=ws)
+    for low, high in ((0, 200), (150, 200), (3, 40)):
+        starts = [(low, high)[b % 2] for b in range(n + 1)]
+        bad = RaggedBatch(i32(list(range(n)), dev), i32(starts, dev), 200, 200)
+        print(f"[bad] n={n} {low} {high}", flush=True)
+        cache.attention(0, bad, torch.zeros(200, 16, 128, dtype=F, device=dev), ws=ws)
+        assert cache.status() == _lib.STATUS_BAD_SEQUENCE
+        cache._status.zero_()
+        assert torch.equal(cache.attention(0, good, q, ws=ws), want)
+    assert cache.status() == 0
+
+
 def test_offsets_past_32_bits(dev):
     """A pool of more than 2^31 elements a plane, the sequence in its last pages."""
     kvh, d, ps = 8, 128, 64
