@@ -148,27 +148,7 @@ class PagedWorkspace:
             raise _lib.Q4DecError(-11, "q4d_paged_attention_workspace_bytes")
         self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=cache.device)
         self.ptr, self._index = self.buf.data_ptr(), cache._index
-        with cache._on() as stream:
-            check(_lib.load().q4d_paged_attention_workspace_init(self.ptr, self.nbytes, stream),
-                  "q4d_paged_attention_workspace_init")
-
-
-class _On:
-    """The cache's device as the current one; gives its current stream."""
-
-    def __init__(self, index: int):
-        self.index = index
-
-    def __enter__(self) -> int:
-        self.prev = _device()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-        return _stream(self.index)
-
-    def __exit__(self, *exc) -> bool:
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
-        return False
+        cache._call("q4d_paged_attention_workspace_init", self.ptr, self.nbytes)
 
 
 class PagedKVCache:
@@ -216,8 +196,20 @@ class PagedKVCache:
         self._wsp = self._ws.data_ptr()
         self._index = data.get_device()
 
-    def _on(self) -> _On:
-        return _On(self._index)
+    def _call(self, name: str, *args) -> None:
+        """The entry point on the cache's device and its current stream."""
+        call = getattr(self._lib, name)
+        here = _device()
+        if here == self._index:
+            rc = call(*args, _stream(here))
+        else:
+            torch.cuda.set_device(self._index)
+            try:
+                rc = call(*args, _stream(self._index))
+            finally:
+                torch.cuda.set_device(here)
+        if rc:
+            check(rc, name)
 
     def _check_batch(self, batch: RaggedBatch) -> None:
         if batch._index != self._index:
@@ -231,17 +223,14 @@ class PagedKVCache:
         page that others hold too.  All or nothing; a refused one also holds back later calls and
         :meth:`append` until :meth:`raise_for_status` clears the word (q4d_pages_reserve)."""
         self._check_batch(batch)
-        with self._on() as stream:
-            check(self._lib.q4d_pages_reserve(self._ref, batch._ref, self._wsp, self._ws_bytes, stream),
-                  "q4d_pages_reserve")
+        self._call("q4d_pages_reserve", self._ref, batch._ref, self._wsp, self._ws_bytes)
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Row ``dst[i]``, which is empty, becomes a copy of row ``src[i]`` that shares its pages."""
         n = _ints(src, "src", self.device).numel()
         _ints(dst, "dst", self.device, n)
         if n:
-            with self._on() as stream:
-                check(self._lib.q4d_pages_fork(self._ref, src.data_ptr(), dst.data_ptr(), n, stream), "q4d_pages_fork")
+            self._call("q4d_pages_fork", self._ref, src.data_ptr(), dst.data_ptr(), n)
 
     def truncate(self, seqs: torch.Tensor, lengths: torch.Tensor | None = None) -> None:
         """Row ``seqs[i]`` keeps its first ``lengths[i]`` positions (``None``: none)."""
@@ -249,10 +238,7 @@ class PagedKVCache:
         if lengths is not None:
             _ints(lengths, "lengths", self.device, n)
         if n:
-            with self._on() as stream:
-                check(self._lib.q4d_pages_truncate(self._ref, seqs.data_ptr(),
-                                                   None if lengths is None else lengths.data_ptr(), n, stream),
-                      "q4d_pages_truncate")
+            self._call("q4d_pages_truncate", self._ref, seqs.data_ptr(), None if lengths is None else lengths.data_ptr(), n)
 
     def free(self, seqs: torch.Tensor) -> None:
         """Rows ``seqs`` let go of all their pages."""
@@ -261,9 +247,7 @@ class PagedKVCache:
     def compact(self) -> torch.Tensor:
         """Held pages move to the lowest numbers; returns how many there are (device int32 [1])."""
         used = torch.empty(1, dtype=torch.int32, device=self.device)
-        with self._on() as stream:
-            check(self._lib.q4d_pages_compact(self._ref, used.data_ptr(), self._wsp, self._ws_bytes, stream),
-                  "q4d_pages_compact")
+        self._call("q4d_pages_compact", self._ref, used.data_ptr(), self._wsp, self._ws_bytes)
         return used
 
     # -- a layer -----------------------------------------------------------------------
@@ -318,11 +302,9 @@ class PagedKVCache:
                 raise ValueError(f"{name} must be contiguous fp32 [{self.head_dim}] on {self.device}")
         if rope is not None and (rope._index != self._index or rope.rotary_dim > self.head_dim):
             raise ValueError(f"the rotation must be on {self.device} and at most {self.head_dim} dims wide")
-        with self._on() as stream:
-            check(self._lib.q4d_paged_append(
-                self._ref, layer, batch._ref, qp, qs, qh, kp, ks, vp, vs, _DTYPES[kind], None if q_gamma is None else q_gamma.data_ptr(),
-                None if k_gamma is None else k_gamma.data_ptr(), eps, None if rope is None else rope._ref, op, stream),
-                "q4d_paged_append")
+        self._call("q4d_paged_append", self._ref, layer, batch._ref, qp, qs, qh, kp, ks, vp, vs, _DTYPES[kind],
+                   None if q_gamma is None else q_gamma.data_ptr(), None if k_gamma is None else k_gamma.data_ptr(), eps,
+                   None if rope is None else rope._ref, op)
         return q_out
 
     def workspace(self, q_heads: int, batch: RaggedBatch) -> PagedWorkspace:
@@ -349,10 +331,8 @@ class PagedKVCache:
             ws = self.workspace(qh, batch)
         elif ws._index != self._index:
             raise ValueError(f"the workspace is on {ws.buf.device}, the cache on {self.device}")
-        with self._on() as stream:
-            check(self._lib.q4d_paged_attention(
-                self._ref, layer, batch._ref, qp, qs, qh, self.head_dim ** -0.5 if scaling is None else scaling, op, os,
-                ws.ptr, ws.nbytes, stream), "q4d_paged_attention")
+        self._call("q4d_paged_attention", self._ref, layer, batch._ref, qp, qs, qh,
+                   self.head_dim ** -0.5 if scaling is None else scaling, op, os, ws.ptr, ws.nbytes)
         return out
 
     # -- state -------------------------------------------------------------------------
