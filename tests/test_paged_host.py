@@ -272,3 +272,32 @@ def test_python_arguments_are_checked():
 def test_status_names():
     assert _lib.status_names(16 | 32 | 64 | 128) == ["NO_PAGES", "BAD_SEQUENCE", "BAD_PAGE", "NOT_RESERVED"]
     assert _lib.status_names(256) == ["UNKNOWN"]
+
+
+def test_calls_run_on_the_cache_s_device(monkeypatch):
+    """On another current device: the cache's is made current for the call, with its own stream, and the
+    caller's again afterwards, whether the call succeeds, fails or raises."""
+    cache = paged.PagedKVCache.__new__(paged.PagedKVCache)
+    cache._index = 3
+    now, log = [0], []
+    monkeypatch.setattr(paged, "_device", lambda: now[0])
+    monkeypatch.setattr(paged, "_stream", lambda i: 100 + i)
+    monkeypatch.setattr(torch.cuda, "set_device", lambda i: now.__setitem__(0, i))
+
+    class Lib:
+        def q4d_some_call(self, *args):
+            log.append((now[0], args))
+            if args[0] == "raise":
+                raise TypeError
+            return args[0]
+    cache._lib = Lib()
+    for here in (0, 3):
+        now[0] = here
+        cache._call("q4d_some_call", 0, "x")
+        assert log[-1] == (3, (0, "x", 103)) and now[0] == here
+        with pytest.raises(_lib.Q4DecError):
+            cache._call("q4d_some_call", SHAPE)
+        assert now[0] == here
+        with pytest.raises(TypeError):
+            cache._call("q4d_some_call", "raise")
+        assert now[0] == here
