@@ -509,7 +509,8 @@ int q4d_paged_attention_workspace_init(void* ws, size_t ws_bytes, void* stream);
  * and sums are fp32; the probabilities enter the product with v in the cache's type (for sequences
  * of few new tokens as two numbers of it, value and remainder).  A position whose page cannot be
  * counts as not there (Q4D_STATUS_BAD_PAGE); a token that sees no position gives zeros.  Values
- * a token does not see, Inf and NaN among them, never reach its output.  Deterministic; a token's
+ * a token does not see, Inf and NaN among them, never reach its output; Inf and NaN of v that it
+ * sees make that dim of it Inf or NaN, however small their weights are.  Deterministic; a token's
  * last bits may depend on the batch's shape and lengths, though not on the other sequences'
  * values. */
 int q4d_paged_attention(const q4d_pages_t* pages, int32_t layer, const q4d_ragged_t* batch, const void* q,

@@ -9,6 +9,7 @@
 // tokens and 10 rows 33 instead of 28.  Batches of up to 32 rows a sequence take rows_part too, in two
 // groups (4 tokens of 8 heads a kv head, two groups / chunk_part: one sequence of 700 positions 13.6 /
 // 15.7 us, one of 6000 with two kv heads 17.8 / 22.5, 24 of 1500 33.4 / 35.4, 64 of 4000 139 / 152).
+#include <float.h>
 #include <math.h>
 
 #include <type_traits>
@@ -62,8 +63,15 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
+// Inf and NaN of V.  A row that does not see such a value gives it the weight 0, and so does the product's
+// 16-bit type to a small weight or to what the rounding of one leaves: 0 x Inf is NaN.  So the products are
+// taken as if there were none, which a part's sums show at its end: 0 x Inf and a weight x Inf stay Inf or
+// NaN through every later sum and rescaling.  Only then the part is done again with those values set to
+// zero, and they are added after the loop for the rows that see them (with the weight 1, which does as well:
+// what is added is Inf or NaN).  Which 64ths of the part's steps have some is kept as bits.  The sum l of such
+// a row's weights is stored with a minus sign: see join_factor.
+
 // Inf and NaN (the exponent is all ones) among eight 16-bit floats become 0; whether there were any.
-// A row that does not see such a value gives it the weight 0, and 0 x Inf is NaN.
 template <bool BF>
 __device__ __forceinline__ bool drop_odd(u32x4& v) {
   constexpr uint32_t e = BF ? 0x7F80u : 0x7C00u;
@@ -77,6 +85,17 @@ __device__ __forceinline__ bool drop_odd(u32x4& v) {
   return odd;
 }
 __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
+__device__ __forceinline__ uint32_t sign_of(float x) { return __builtin_bit_cast(uint32_t, x) & 0x80000000u; }
+__device__ __forceinline__ float with_sign(float x, uint32_t sign) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) | sign);
+}
+
+// What a part's sums (maximum m, sum of weights l) are multiplied with when they are joined to others with the
+// maximum M; never 0 where l says that there is Inf or NaN among them, which have to stay what they are.
+__device__ __forceinline__ float join_factor(float m, float l, float M) {
+  const float f = m == -INFINITY ? 0.f : exp2f(m - M);
+  return sign_of(l) ? fmaxf(f, 0x1p-149f) : f;
+}
 
 // Max / sum over the four 16-lane rows of a wave, in every lane (as in q4d_attention.hip).
 template <bool SUM>
@@ -317,7 +336,9 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
         return tab[min(e, a.p.max_pages - 1)];
       };
       int page = page_of(s0);
-      bool bad_page = false, odd = false;
+      bool bad_page = false;
+      uint64_t odd = 0;  // 64ths of the steps where Inf and NaN of V were set to zero
+      const int per = (s1 - s0 + 63) / 64;
       // Loads of step `it`, without a branch, so that the next steps' loads stay in flight while this
       // one's are waited for: through descriptors that end with the sequence's last row (rows past it,
       // of a page that is not there or of a step past the part's end are zeros and cost nothing).  K in
@@ -350,20 +371,15 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
 
       f32x4 o[H][DT];
       float m[H], l[H];  // of query rows r and 16 + r; l of this lane's positions only
-#pragma unroll
-      for (int h = 0; h < H; ++h) {
-        m[h] = -INFINITY;
-        l[h] = 0.f;
-#pragma unroll
-        for (int i = 0; i < DT; ++i) o[h][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      }
-      const auto consume = [&](int it) {
+      const auto consume = [&](int it, auto again) {
         const int base = it * kStep + 32 * w;
         const bool ok0 = d.ok0, ok1 = d.ok1;
         const bool hides = base + 32 > first_hidden;
-        if (hides && s.count > 1) {  // Inf and NaN become zeros; they are added after the loop
+        if constexpr (again) {
+          bool any = false;
 #pragma unroll
-          for (int i = 0; i < NV; ++i) odd |= drop_odd<BF>(d.v[i]);
+          for (int i = 0; i < NV; ++i) any |= drop_odd<BF>(d.v[i]);
+          if (__ballot(any)) odd |= 1ULL << ((it - s0) / per);
         }
         // V into this wave's LDS rows: 32-byte chunk c of row x at c ^ f(x), f chosen so that the 16
         // rows of a transposing read fall on all banks
@@ -447,30 +463,55 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
           }
         }
       };
-      issue(s0);
-      for (int it = s0; it < s1; ++it) consume(it);
-      if (__ballot(odd)) {
-        const uint16_t* vplane = late_args()->vplane;
-        // this wave's positions that some row does not see (weight 1 does as well as the probability: what
-        // is added is Inf or NaN)
-        for (int it = max(s0, first_hidden / kStep); it < s1; ++it) {
-          const int base = it * kStep + 32 * w;
-          if (base + 32 <= first_hidden) continue;
-          for (int pos = base; pos < min(s.len, base + 32); ++pos) {
-            const int pg = tab[min(pos >> shift, a.p.max_pages - 1)];
-            if (!in_range(pg, a.p.num_pages)) continue;
-            const uint16_t* v = vplane + page_elem(a.p, pg, j) + (size_t)(pos & inpage) * D + 4 * g;
+      const auto pass = [&](auto again) {
 #pragma unroll
-            for (int i = 0; i < DT; ++i)
+        for (int h = 0; h < H; ++h) {
+          m[h] = -INFINITY;
+          l[h] = 0.f;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float x = to_f32<BF>(v[16 * i + e]);
-#pragma unroll
-                for (int h = 0; h < H; ++h)
-                  if (pos <= qpos[h] && not_finite(x)) o[h][i][e] += x;
-              }
-          }
+          for (int i = 0; i < DT; ++i) o[h][i] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
+        issue(s0);
+        for (int it = s0; it < s1; ++it) consume(it, again);
+#pragma unroll
+        for (int h = 0; h < H; ++h) l[h] = rows4<true>(l[h]);
+      };
+      pass(std::false_type());
+      float zero = 0.f;  // NaN if a sum is Inf or NaN
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) zero = fmaf(o[h][i][e], 0.f, zero);
+      if (__builtin_expect(__ballot(zero != 0.f) != 0, 0)) {
+        page = page_of(s0);
+        pass(std::true_type());
+        const uint16_t* vplane = late_args()->vplane;
+        for (; odd; odd &= odd - 1)
+          for (int i = 0, it = s0 + __builtin_ctzll(odd) * per; i < per && it < s1; ++i, ++it) {
+            const int base = it * kStep + 32 * w;  // this wave's positions
+            for (int pos = base; pos < min(s.len, base + 32); ++pos) {
+              const int pg = tab[min(pos >> shift, a.p.max_pages - 1)];
+              if (!in_range(pg, a.p.num_pages)) continue;
+#pragma unroll
+              for (int h = 0; h < H; ++h)
+                if (pos <= qpos[h]) {
+                  m[h] = fmaxf(m[h], -FLT_MAX);  // (joined whatever the scores are)
+                  l[h] = with_sign(l[h], 0x80000000u);
+                }
+              const uint16_t* v = vplane + page_elem(a.p, pg, j) + (size_t)(pos & inpage) * D + 4 * g;
+#pragma unroll
+              for (int i = 0; i < DT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float x = to_f32<BF>(v[16 * i + e]);
+#pragma unroll
+                  for (int h = 0; h < H; ++h)
+                    if (pos <= qpos[h] && not_finite(x)) o[h][i][e] += x;
+                }
+            }
+          }
       }
       if (bad_page && lane == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_PAGE);
 
@@ -483,7 +524,6 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         if (h) block_sync_lds();  // the first rows' states have been read
-        l[h] = rows4<true>(l[h]);
         if (g == 0) {
           sml[(w * kRows + r) * 2] = m[h];
           sml[(w * kRows + r) * 2 + 1] = l[h];
@@ -497,19 +537,22 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
 #pragma unroll
         for (int i = 0; i < 4; ++i) M[h] = fmaxf(M[h], sml[(i * kRows + row) * 2]);
         L[h] = 0.f;
+        uint32_t sign = 0;
 #pragma unroll
         for (int n = 0; n < NS; ++n) acc[h][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float mi = sml[(i * kRows + row) * 2], f = mi == -INFINITY ? 0.f : exp2f(mi - M[h]);
-          L[h] = fmaf(sml[(i * kRows + row) * 2 + 1], f, L[h]);
+          const float li = sml[(i * kRows + row) * 2 + 1], f = join_factor(sml[(i * kRows + row) * 2], li, M[h]);
+          L[h] = fmaf(fabsf(li), f, L[h]);
+          sign |= sign_of(li);
 #pragma unroll
           for (int n = 0; n < NS; ++n) {
             const f32x4 x = *reinterpret_cast<const f32x4*>(lds + i * kWaveBytes + row * (4 * D) + (((sl + 16 * n) ^ row) << 4));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[h][n][e] = mi == -INFINITY ? acc[h][n][e] : fmaf(x[e], f, acc[h][n][e]);
+            for (int e = 0; e < 4; ++e) acc[h][n][e] = fmaf(x[e], f, acc[h][n][e]);
           }
         }
+        L[h] = with_sign(L[h], sign);
       }
       // The parts' states are joined eight at a time: of each eight the block that counts in last adds
       // them in order and goes on with the sum as one of the next level's parts.
@@ -561,19 +604,21 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
 #pragma unroll
             for (int i = 0; i < kJoin; ++i) M[h] = fmaxf(M[h], mi[i]);
             L[h] = 0.f;
+            uint32_t sign = 0;
 #pragma unroll
             for (int n = 0; n < NS; ++n) acc[h][n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < kJoin; ++i) {
               if (i >= size) continue;
-              const float f = mi[i] == -INFINITY ? 0.f : exp2f(mi[i] - M[h]);
-              L[h] = fmaf(li[i], f, L[h]);
+              const float f = join_factor(mi[i], li[i], M[h]);
+              L[h] = fmaf(fabsf(li[i]), f, L[h]);
+              sign |= sign_of(li[i]);
 #pragma unroll
               for (int n = 0; n < NS; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  acc[h][n][e] = mi[i] == -INFINITY ? acc[h][n][e] : fmaf(ai[i][n][e], f, acc[h][n][e]);
+                for (int e = 0; e < 4; ++e) acc[h][n][e] = fmaf(ai[i][n][e], f, acc[h][n][e]);
             }
+            L[h] = with_sign(L[h], sign);
           }
         }
         part = first / kJoin;
@@ -585,7 +630,7 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
         if (count > 1 || at >= rows) continue;
         const int otok = at / G;
         uint16_t* op = late->out + (s.first + otok) * late->out_stride + (j * G + at - otok * G) * D + 4 * sl;
-        const float inv = L[h] == 0.f ? 0.f : 1.0f / L[h];
+        const float inv = L[h] == 0.f ? 0.f : 1.0f / fabsf(L[h]);
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
           const uint32_t u0 = from_f32<BF>(acc[h][n][0] * inv), u1 = from_f32<BF>(acc[h][n][1] * inv);
@@ -670,15 +715,15 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   constexpr int KS = D / 16, DT = D / 32, LR = D / 8;  // LR slots of 16 bytes a row
   constexpr int kRowBytes = 2 * D, kPlane = kKeys * kRowBytes, kStage = 2 * kPlane;
   int* s_sum = reinterpret_cast<int*>(lds + 2 * kStage);  // [2][4]
-  int* s_last = s_sum + 8;
-  int* s_odd = s_last + 1;
+  int* s_again = s_sum + 8;  // [4]
+  unsigned long long* s_odd = reinterpret_cast<unsigned long long*>(s_again + 4);
+  int* s_last = s_again + 6;
   int* s_end = seqs;               // [n] items of the sequences up to and with b
   int* s_split = s_end + a.r.n;    // [n] the same of sequences in parts
   const int t = threadIdx.x, lane = t & 63;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kvh = a.p.kvh, G = a.qh / kvh;
   const int idx = block / kvh, j = block - idx * kvh;
-  if (t == 0) *s_odd = 0;
 
   // ---- which item ----------------------------------------------------------------------------
   const auto tiles_of = [&](const SeqSpan& s) { return s.count * G > kRows ? (s.count * G + kTile - 1) / kTile : 0; };
@@ -846,7 +891,6 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   const int kend = old + (min(rows, (tile + 1) * kTile) - 1) / G + 1;
   const int steps = steps_of(kend), st0 = part * steps / parts, st1 = (part + 1) * steps / parts;
   const bool active = row0 < rows;  // the wave has rows
-  const int hidden0 = old + tile * kTile / G + 1;  // positions from here on are hidden from some row
 
   // the first tiles' pages, the query rows and the first tile are on their way together
   const int32_t* tab = a.p.table + (size_t)s.row * a.p.max_pages;
@@ -931,21 +975,17 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   }
 
   f32x16 o[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
-  float m = -INFINITY, l = 0.f;  // l of this lane's keys only
+  float m, l;  // l of this lane's keys only
+  const int per = (st1 - st0 + 63) / 64;
 
   // Step `st`, in LDS stage SG (the loop takes two at a time, so that operand addresses are immediates).
-  const auto take = [&](int st, auto stage_no) {
+  const auto take = [&](int st, auto stage_no, auto again) {
     constexpr int SG = decltype(stage_no)::value;
     const char* stage = lds + SG * kStage;
     const int key0 = st * kKeys;
     const uint64_t none = gone;
-    const bool edge = key0 + kKeys > hidden0;
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) expcnt(7) lgkmcnt(0): this wave's rows are there
-    if (edge) {  // Inf and NaN among these V rows become zeros; they are added after the loop
+    if constexpr (again) {
       bool odd = false;
 #pragma unroll
       for (int i = 0; i < 16 / RI; ++i) {
@@ -956,7 +996,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
           odd = true;
         }
       }
-      if (odd) *s_odd = 1;
+      if (odd) atomicOr(s_odd, 1ULL << ((st - st0) / per));
       __builtin_amdgcn_s_waitcnt(0xc07f);
     }
     __builtin_amdgcn_s_barrier();  // everybody's rows are there, and the other stage is read
@@ -1040,7 +1080,19 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
       for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32<BF>(v[i & 1][dt], p, o[dt]);
     }
   };
-  block_sync_lds();  // s_odd is 0 before anybody sets it
+  const auto pass = [&](auto again) {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+    for (int st = st0; st < st1; st += 2) {
+      take(st, std::integral_constant<int, 0>(), again);
+      if (st + 1 < st1) take(st + 1, std::integral_constant<int, 1>(), again);
+    }
+    l = halves<true>(l);
+  };
   if (st0 < st1) issue(st0, 0);
   pages = pages_next;
   if (a.scale < 0.f) {
@@ -1049,28 +1101,41 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
 #pragma unroll
       for (int e = 0; e < 4; ++e) q[i][e] ^= 0x80008000u;
   }
-  for (int st = st0; st < st1; st += 2) {
-    take(st, std::integral_constant<int, 0>());
-    if (st + 1 < st1) take(st + 1, std::integral_constant<int, 1>());
-  }
+  pass(std::false_type());
+  float zero = 0.f;  // NaN if a sum is Inf or NaN
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) zero = fmaf(o[dt][r], 0.f, zero);
+  s_again[w] = __ballot(zero != 0.f) != 0;
+  if (t == 0) *s_odd = 0;
   __syncthreads();
-  if (*s_odd && active) {
-    // (weight 1 does as well as the probability: what is added is Inf or NaN)
-    for (int key = max(st0 * kKeys, hidden0 / kKeys * kKeys); key < min(st1 * kKeys, kend); ++key) {
-      const int page = tab[min(key >> shift, a.p.max_pages - 1)];
-      if (!in_range(page, a.p.num_pages)) continue;
-      const uint16_t* v = a.vplane + page_elem(a.p, page, j) + (size_t)(key & inpage) * D + 4 * hf;
+  if (__builtin_expect(s_again[0] | s_again[1] | s_again[2] | s_again[3], 0)) {  // (then the part has steps)
+    pages = pages_at(st0);
+    issue(st0, 0);
+    pages = pages_at(st0 + 1);
+    pass(std::true_type());
+    __syncthreads();
+    if (active)
+      for (uint64_t odd = *s_odd; odd; odd &= odd - 1) {
+        const int key0 = (st0 + __builtin_ctzll(odd) * per) * kKeys;
+        for (int key = key0; key < min(min(st1 * kKeys, key0 + per * kKeys), kend); ++key) {
+          const int page = tab[min(key >> shift, a.p.max_pages - 1)];
+          if (key > qpos || !in_range(page, a.p.num_pages)) continue;
+          m = fmaxf(m, -FLT_MAX);  // (joined whatever the scores are)
+          l = with_sign(l, 0x80000000u);
+          const uint16_t* v = a.vplane + page_elem(a.p, page, j) + (size_t)(key & inpage) * D + 4 * hf;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+          for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float x = to_f32<BF>(v[32 * dt + 8 * (r >> 2) + (r & 3)]);
-          if (key <= qpos && not_finite(x)) o[dt][r] += x;
+            for (int r = 0; r < 16; ++r) {
+              const float x = to_f32<BF>(v[32 * dt + 8 * (r >> 2) + (r & 3)]);
+              if (not_finite(x)) o[dt][r] += x;
+            }
         }
-    }
+      }
   }
   if (bad_page && lane == 0) atomicOr(a.p.status, Q4D_STATUS_BAD_PAGE);
-  l = halves<true>(l);
 
   // ---- parts, joined as in rows_part; a lane's values lie together by fours ---------------------
   const KernelArgs late = late_args();
@@ -1099,6 +1164,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
       if (active) {
         const auto ml = [&](int i) { return late->cml + place(first + i) * 64 + qc; };
         float M = -INFINITY;
+        uint32_t sign = 0;
 #pragma unroll
         for (int i = 0; i < kJoin; ++i) M = fmaxf(M, load_dev(ml(min(i, size - 1))));
         l = 0.f;
@@ -1122,17 +1188,19 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             if (i0 + k >= size) break;
-            const float f = mv[k] == -INFINITY ? 0.f : exp2f(mv[k] - M);
-            l = fmaf(lv[k], f, l);
+            const float f = join_factor(mv[k], lv[k], M);
+            l = fmaf(fabsf(lv[k]), f, l);
+            sign |= sign_of(lv[k]);
 #pragma unroll
             for (int n = 0; n < 4 * DT; ++n)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float y = o[n >> 2][4 * (n & 3) + e];
-                o[n >> 2][4 * (n & 3) + e] = mv[k] == -INFINITY ? y : fmaf(v[k][n][e], f, y);
+                o[n >> 2][4 * (n & 3) + e] = fmaf(v[k][n][e], f, y);
               }
           }
         }
+        l = with_sign(l, sign);
         m = M;
       }
       __syncthreads();  // s_last has been read
@@ -1144,7 +1212,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   // ---- rows out, through LDS -------------------------------------------------------------------
   __syncthreads();  // everybody is done with the tiles
   if (!active) return;
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const float inv = l == 0.f ? 0.f : 1.0f / fabsf(l);
   char* T0 = lds + w * (32 * kRowBytes);  // 32 rows of D values, slot s of row r at s ^ (r & (LR - 1))
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)

@@ -1,0 +1,114 @@
+"""Attention over pages where the values are hard: Inf and NaN that a token sees, by kind; scores that are
+-Inf or of any scale; sums beyond the cache type's largest number; probabilities that must not be rounded
+to 16 bits."""
+
+import math
+
+import pytest
+import torch
+
+import paged_ref
+from llm_accelerator_amd.paged import PagedKVCache, RaggedBatch
+from test_gpu_paged_attention import filled, i32
+
+pytestmark = pytest.mark.gpu
+F, B = torch.float16, torch.bfloat16
+INF, NAN = float("inf"), float("nan")
+
+
+def queries(dev, batch, qh, d, dtype, seed=1):
+    return torch.randn(batch.tokens, qh, d, device=dev, generator=torch.Generator(device=dev).manual_seed(seed)).to(dtype)
+
+
+def at(cache, row, pos):
+    return int(cache.table[row, pos // cache.page_size]), pos % cache.page_size
+
+
+def check_kinds(cache, batch, q, out, scaling):
+    """Every output is NaN, Inf or -Inf where the 64-bit one is, and within the bound elsewhere."""
+    ref, size, tiny = paged_ref.attend(cache, 0, batch, q, scaling)
+    assert torch.equal(out.isnan(), ref.isnan())
+    assert torch.equal(out.isposinf(), ref.isposinf()) and torch.equal(out.isneginf(), ref.isneginf())
+    ok = ref.isfinite()
+    bound = paged_ref.attend_bound(ref, size, tiny, q.dtype)
+    assert bool(((out.double() - ref).abs() <= bound)[ok].all())
+    return ok
+
+
+# (positions, new tokens) of every sequence, q heads, kv heads, dim, page, and places (sequence, position)
+SEEN = [
+    ([(1, 1)], 16, 8, 128, 64, [(0, 0)]),
+    ([(700, 1)], 16, 8, 128, 64, [(0, 0), (0, 351), (0, 699)]),
+    ([(300, 1), (37, 1), (2500, 1)], 4, 1, 64, 16, [(0, 5), (1, 36), (2, 1200)]),
+    ([(9000, 1)], 8, 1, 128, 32, [(0, 40), (0, 8990)]),          # many parts
+    ([(300, 5)], 16, 8, 128, 64, [(0, 100), (0, 296), (0, 299)]),
+    ([(700, 4)], 16, 2, 64, 16, [(0, 100), (0, 698)]),           # two groups of rows
+    ([(900, 60)], 4, 2, 128, 64, [(0, 40), (0, 838), (0, 870)]),  # a chunk: before its edge and in it
+    ([(6000, 40)], 8, 1, 64, 16, [(0, 17), (0, 3001), (0, 5990)]),
+    ([(300, 300)], 2, 2, 128, 128, [(0, 0), (0, 128), (0, 290)]),
+    ([(500, 1), (400, 70), (90, 2)], 4, 2, 128, 16, [(0, 77), (1, 50), (1, 380), (2, 89)]),
+]
+
+
+@pytest.mark.parametrize("dtype", [F, B], ids=["f16", "bf16"])
+@pytest.mark.parametrize("seqs,qh,kvh,d,ps,places", SEEN, ids=lambda v: "x".join(f"{a}:{b}" for a, b in v) if isinstance(v, list) else str(v))
+def test_inf_and_nan_that_a_token_sees(dev, seqs, qh, kvh, d, ps, places, dtype):
+    """Inf gives Inf, -Inf gives -Inf, NaN and both signs give NaN, in that dim alone."""
+    cache = filled(dev, [n for n, _ in seqs], kvh, d, ps, dtype)
+    batch = RaggedBatch.of(list(range(len(seqs))), [a for _, a in seqs], dev)
+    q = queries(dev, batch, qh, d, dtype)
+    ws = cache.workspace(qh, batch)
+    for s, pos in places:
+        page, off = at(cache, s, pos)
+        saved = cache.data[0, 1, page, :, off].clone()
+        for dim, value in ((3, INF), (d - 1, -INF), (17, NAN)):
+            cache.data[0, 1, page, :, off, dim] = value
+        other = max(0, pos - 1)                       # (the same position in the first case)
+        page2, off2 = at(cache, s, other)
+        saved2 = cache.data[0, 1, page2, :, off2, 40].clone()
+        cache.data[0, 1, page2, :, off2, 40] = INF
+        if other != pos:
+            cache.data[0, 1, page, :, off, 40] = -INF
+        print(f"[seen] {s} {pos}", flush=True)
+        ok = check_kinds(cache, batch, q, cache.attention(0, batch, q, ws=ws), d ** -0.5)
+        assert not bool(ok.all()) and cache.status() == 0
+        cache.data[0, 1, page2, :, off2, 40] = saved2
+        cache.data[0, 1, page, :, off] = saved
+    assert bool(check_kinds(cache, batch, q, cache.attention(0, batch, q, ws=ws), d ** -0.5).all())
+
+
+@pytest.mark.parametrize("dtype", [F, B], ids=["f16", "bf16"])
+@pytest.mark.parametrize("length,new,qh,kvh", [(700, 1, 4, 2), (9000, 1, 8, 1), (300, 5, 4, 2), (900, 60, 4, 2), (6000, 40, 8, 1)])
+def test_an_inf_of_the_smallest_weight_counts(dev, length, new, qh, kvh, dtype):
+    """The first half's probabilities are e^-424 and less: nothing in 32 bits, and still Inf where V is Inf."""
+    cache = filled(dev, [length], kvh, 128, 16, dtype)
+    batch = RaggedBatch.of([0], [new], dev)
+    q = queries(dev, batch, qh, 128, dtype)
+    q[..., 0] = 8.0
+    for pos in range(0, length // 2, 16):
+        page, _ = at(cache, 0, pos)
+        cache.data[0, 0, page, :, :min(16, length // 2 - pos), 0] = -600.0
+    for pos in (5, length // 2 - 1):
+        page, off = at(cache, 0, pos)
+        cache.data[0, 1, page, :, off, 9] = INF
+        cache.data[0, 1, page, :, off, 10] = -INF
+        cache.data[0, 1, page, :, off, 11] = NAN
+        out = cache.attention(0, batch, q)
+        check_kinds(cache, batch, q, out, 128 ** -0.5)
+        assert bool(out[..., 9].isposinf().all()) and bool(out[..., 10].isneginf().all())
+        cache.data[0, 1, page, :, off, 9:12] = 0
+
+
+def test_a_value_past_fp16_is_inf_from_the_append_on(dev):
+    """v = 1e5 becomes Inf in an fp16 cache, and so do the outputs of the tokens that see it, however many they are."""
+    cache = PagedKVCache(1, 40, 16, 2, 64, 2, 512, F, dev)
+    for counts in ([1, 90], [1, 1], [5, 2], [20, 1]):
+        batch = RaggedBatch.of([0, 1], counts, dev)
+        cache.reserve(batch)
+        x = torch.randn(batch.tokens, 8, 64, device=dev)
+        x[:, 6:, 7] = 1e5
+        x[:, 6:, 8] = -1e5
+        out = cache.attention(0, batch, cache.append(0, batch, x[:, :4], x[:, 4:6], x[:, 6:]))
+        assert bool(out[..., 7].isposinf().all()) and bool(out[..., 8].isneginf().all())
+        out[..., 7:9] = 0
+        assert bool(out.isfinite().all()) and cache.status() == 0
