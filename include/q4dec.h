@@ -506,8 +506,8 @@ int q4d_paged_attention_workspace_init(void* ws, size_t ws_bytes, void* stream);
  * out = softmax(q k^T scaling) v, q head h with kv head h / (q_heads / num_kv_heads).  q and out:
  * rows of q_heads x head_dim in the cache's type, row t at t * stride elements, 16-byte aligned;
  * out may be q itself.  q_heads is a multiple of num_kv_heads, up to 16 times.  Scores, softmax
- * and sums are fp32; the probabilities enter the product with v in the cache's type (for sequences
- * of few new tokens as two numbers of it, value and remainder).  A position whose page cannot be
+ * and sums are fp32; the probabilities enter the product with v as two numbers of the cache's type,
+ * value and remainder (22 bits together in fp16, 16 in bf16).  A position whose page cannot be
  * counts as not there (Q4D_STATUS_BAD_PAGE); a token that sees no position gives zeros.  Values
  * a token does not see, Inf and NaN among them, never reach its output; Inf and NaN of v that it
  * sees make that dim of it Inf or NaN, however small their weights are.  Deterministic; a token's

@@ -56,6 +56,26 @@ __device__ __forceinline__ u32x4 pack8(const float (&x)[8]) {
     return __builtin_bit_cast(u32x4, y);
   }
 }
+// x as value and remainder: v = x in 16 bits, rest = x - v (exact in fp32) in 16 bits.
+template <bool BF>
+__device__ __forceinline__ void pack8_rest(float (&x)[8], u32x4& v, u32x4& rest) {
+  v = pack8<BF>(x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF) {
+      x[2 * i] -= to_f32<BF>((uint16_t)v[i]);
+      x[2 * i + 1] -= to_f32<BF>((uint16_t)(v[i] >> 16));
+    } else {  // one mixed multiply-add each out of the pair (seen through, the compiler would round every x once more)
+      uint32_t u = v[i];
+      float minus = -1.f;
+      asm("" : "+v"(u));
+      asm("" : "+s"(minus));
+      x[2 * i] = fmaf(to_f32<BF>((uint16_t)u), minus, x[2 * i]);
+      x[2 * i + 1] = fmaf(to_f32<BF>((uint16_t)(u >> 16)), minus, x[2 * i + 1]);
+    }
+  }
+  rest = pack8<BF>(x);
+}
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   if constexpr (BF)
@@ -434,11 +454,7 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
             p[e] = __builtin_amdgcn_exp2f(y[e] - ms);
             l[h] += p[e];
           }
-          pp[h] = pack8<BF>(p);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)  // what the rounding leaves
-            p[e] -= to_f32<BF>((uint16_t)(e & 1 ? pp[h][e >> 1] >> 16 : pp[h][e >> 1]));
-          pr[h] = pack8<BF>(p);
+          pack8_rest<BF>(p, pp[h], pr[h]);
         }
         // V^T operand: dim 16 i + r, the same eight positions
         const auto vt = [&](int i) {
@@ -651,17 +667,17 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
 //   S^T = K . Q^T (32x32x16 MFMA; K rows from LDS, Q^T in registers); online softmax per row; O^T +=
 //   V^T . P^T, where the S^T accumulators already are the operand layout of P^T (a lane holds 4 + 4
 //   keys of each 16 for one row) and V^T comes out of the row-major tile with the transposing read.
-// P is rounded to the cache's type, which the product takes (a second product of the remainder as in
-// rows_part would cost prompts 215 instead of 173 us, 512 tokens after 4097 48.5 instead of 42); the sum l
-// takes it unrounded.
+// The product takes P as two numbers of the cache's type, as in rows_part: rounded once it was as far again
+// from 64 bits as the output's own rounding (2.9e-4 instead of 2.1e-4 in fp16, 2.1e-3 instead of 1.6e-3 in
+// bf16), and a token's precision went by how many came with it.  The second product costs prompts 212 instead of
+// 165 us, 512 tokens after 4097 44 instead of 39.
 // K and V tiles go from the pages to LDS by DMA one tile ahead, 16 rows a wave (one page at most).
 // Two blocks a CU, so that one's products run under the other's softmax.  4 prompts of up to 3500
-// positions, 16 / 8 heads: 173-187 us, 780-840 TFLOP/s of what rows see (a product of 8192^3 reaches
-// 1365), 2 prompts of 12000 970; 512 tokens after 4097 41 us.  Taken apart (prompts, 178 us): the products
-// and their operands from LDS alone 133, which is 1350 TFLOP/s and the rate of a library's product; the
-// softmax adds 25, DMA 20.  Measured and no faster: the next step's first product interleaved with this
-// one's exponentials in a wave (180), the same with 8 waves that share tiles two or three steps ahead
-// (185), with 64 rows a wave and 512 registers (264: accumulators move between the register files).
+// positions, 16 / 8 heads: 212 us, 690 TFLOP/s of what rows see and, with the remainder's product, 1030 of
+// what the matrix units do (a product of 8192^3 reaches 1365); 512 tokens after 4097 44 us.  Measured with one
+// product and no faster than this order's 178 us: the next step's first product interleaved with this one's
+// exponentials in a wave (180), the same with 8 waves that share tiles two or three steps ahead (185), with 64
+// rows a wave and 512 registers (264: accumulators move between the register files).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTile = 128;  // query rows of a block
@@ -1061,8 +1077,8 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
         for (int r = 0; r < 16; ++r) o[dt][r] *= f;
     }
     const float ms = m == -INFINITY ? 0.f : m;
-    // the lane's eight probabilities of each 16 keys; l sums them unrounded
-    const auto probs = [&](int i) {
+    // the lane's eight probabilities of each 16 keys, as value and remainder; l sums them unrounded
+    const auto probs = [&](int i, u32x4& p, u32x4& rest) {
       float e[8], sum = 0.f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -1070,14 +1086,17 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
         sum += e[k];
       }
       l += sum;
-      return pack8<BF>(e);
+      pack8_rest<BF>(e, p, rest);
     };
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (i < 3) load_v(i + 1, v[(i + 1) & 1]);
-      const u32x4 p = probs(i);
+      u32x4 p, rest;
+      probs(i, p, rest);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32<BF>(v[i & 1][dt], p, o[dt]);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32<BF>(v[i & 1][dt], rest, o[dt]);
     }
   };
   const auto pass = [&](auto again) {

@@ -112,3 +112,43 @@ def test_a_value_past_fp16_is_inf_from_the_append_on(dev):
         assert bool(out[..., 7].isposinf().all()) and bool(out[..., 8].isneginf().all())
         out[..., 7:9] = 0
         assert bool(out.isfinite().all()) and cache.status() == 0
+
+
+def two_groups(dev, length, new, kvh, d, ps, dtype):
+    """A cache and a query of exact scores: the even positions' are 0, the odd ones' -scaling.  With a scaling
+    of -log(1 / 2 + eps / 4) an odd position's weight is half-way between two numbers of the cache's type,
+    and V, 1 and -(2 - eps), cancels: 16-bit weights move the output by a third of eps, which nothing hides."""
+    cache = filled(dev, [length], kvh, d, ps, dtype, garbage=False)
+    pos = torch.arange(length, device=dev)
+    page, off = cache.table[0, pos // ps].long(), pos % ps
+    odd = (pos % 2 == 1).to(dtype)
+    k = torch.zeros(length, kvh, d, device=dev, dtype=dtype)
+    k[:, :, 0] = odd[:, None]
+    v = torch.where(pos % 2 == 1, torch.finfo(dtype).eps - 2.0, 1.0).to(dtype).view(-1, 1, 1).expand(length, kvh, d)
+    cache.data[0, 0, page, :, off] = k
+    cache.data[0, 1, page, :, off] = v
+    q = torch.zeros(new, 4 * kvh, d, device=dev, dtype=dtype)
+    q[..., 0] = -1.0
+    return cache, q
+
+
+@pytest.mark.parametrize("dtype", [F, B], ids=["f16", "bf16"])
+@pytest.mark.parametrize("length,new,d", [(64, 1, 64), (600, 1, 128), (3000, 4, 64), (600, 3, 128), (600, 8, 64), (640, 120, 128),
+                                          (4000, 30, 64), (256, 256, 128)])
+def test_probabilities_keep_more_than_16_bits(dev, length, new, d, dtype):
+    """Scores are exact (a product of two numbers, scaled in fp32), so a weight is off by 2^-20 (exponent of up to
+    2 in base 2, its factors and the exponential: 2^-23 each, and the maximum's), the weights' remainders by 2^-22
+    (fp16) or 2^-16 (bf16), or 2^-25 of the largest, which may be taken 2^8 low only where scores differ by more;
+    sums of up to `length` fp32 terms of one size by 2^-24 of length / 4 (a wave's or half wave's share, joined in
+    few more steps), and the output by its own half step."""
+    step = torch.finfo(dtype).eps
+    scaling = -math.log(0.5 + 0.25 * step)
+    cache, q = two_groups(dev, length, new, 1, d, 16, dtype)
+    batch = RaggedBatch.of([0], [new], dev)
+    out = cache.attention(0, batch, q, scaling)
+    ref, size, _ = paged_ref.attend(cache, 0, batch, q, scaling)
+    rest = 2.0 ** -22 if dtype == F else 2.0 ** -16
+    bound = step / 2 * ref.abs() + (2.0 ** -20 + rest + 2.0 ** -24 * (length / 4 + 64)) * size
+    worst = float(((out.double() - ref).abs() / bound).max())
+    print(f"[precision] {worst:.3f} of the bound", flush=True)
+    assert worst <= 1
