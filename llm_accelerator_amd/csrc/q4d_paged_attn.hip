@@ -176,6 +176,15 @@ __device__ __forceinline__ f32x4 load_dev4(__amdgpu_buffer_rsrc_t r, int offset)
 // stays below 2^8, far inside fp16's range, and the rescaling of the output is rare (whole prompts
 // 187 instead of 193 us, nothing where K and V are streamed).
 constexpr float kRescale = 8.0f;
+// bf16 values reach 3e38, and their sums pass fp32 where their mean does not.  A part whose sums came out
+// Inf (see drop_odd) is done again with weights of 2^(8 - 32) at most, so that 2^24 positions have room, and
+// every join of up to eight parts leaves room for four bits.  Powers of two change no result but those that
+// fp32 would hold as subnormals.
+constexpr float kHeadroom = 32.0f;
+template <bool BF>
+__device__ __forceinline__ float join_max(float M) {
+  return BF ? M + 4.0f : M;
+}
 
 // ---- up to 16 query rows a sequence --------------------------------------------------------
 // The work of a kv head is a line of steps of 128 positions, the sequences one after the other;
@@ -436,6 +445,7 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
 #pragma unroll
           for (int e = 1; e < 8; ++e) mx = fmaxf(mx, y[e]);
           mx = rows4<false>(mx);
+          if constexpr (BF && again) mx += kHeadroom;
           const bool move = mx > m[h] + kRescale || (m[h] == -INFINITY && mx > m[h]);
           if (__ballot(move)) {
             const float mn = move ? mx : m[h];
@@ -552,6 +562,7 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
         M[h] = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4; ++i) M[h] = fmaxf(M[h], sml[(i * kRows + row) * 2]);
+        M[h] = join_max<BF>(M[h]);
         L[h] = 0.f;
         uint32_t sign = 0;
 #pragma unroll
@@ -619,6 +630,7 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
             M[h] = -INFINITY;
 #pragma unroll
             for (int i = 0; i < kJoin; ++i) M[h] = fmaxf(M[h], mi[i]);
+            M[h] = join_max<BF>(M[h]);
             L[h] = 0.f;
             uint32_t sign = 0;
 #pragma unroll
@@ -1065,6 +1077,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[h][r]);
     mx = halves<false>(mx) * scale;
+    if constexpr (BF && again) mx += kHeadroom;
     const bool move = mx > m + kRescale || (m == -INFINITY && mx > m);
     if (__ballot(move)) {
       const float mn = move ? mx : m;
@@ -1186,6 +1199,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
         uint32_t sign = 0;
 #pragma unroll
         for (int i = 0; i < kJoin; ++i) M = fmaxf(M, load_dev(ml(min(i, size - 1))));
+        M = join_max<BF>(M);
         l = 0.f;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)

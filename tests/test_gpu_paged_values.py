@@ -152,3 +152,44 @@ def test_probabilities_keep_more_than_16_bits(dev, length, new, d, dtype):
     worst = float(((out.double() - ref).abs() / bound).max())
     print(f"[precision] {worst:.3f} of the bound", flush=True)
     assert worst <= 1
+
+
+@pytest.mark.parametrize("length,new,qh,kvh", [(2, 1, 2, 1), (700, 1, 4, 2), (9000, 1, 8, 1), (700, 4, 8, 1), (300, 60, 4, 2),
+                                              (6000, 40, 8, 1), (256, 256, 2, 2)])
+def test_means_of_the_largest_bf16_values_are_finite(dev, length, new, qh, kvh):
+    """A weighted mean of values up to 3.2e38 is no larger than they are, though their sum passes fp32: equal
+    scores, scores that rise by 6 (in base 2) from one 64 positions to the next, and random ones."""
+    cache = filled(dev, [length], kvh, 128, 16, B, garbage=False)
+    batch = RaggedBatch.of([0], [new], dev)
+    pos = torch.arange(length, device=dev)
+    page, off = cache.table[0, pos // 16].long(), pos % 16
+    v = torch.linspace(2.0e38, 3.2e38, 128, device=dev).to(B)
+    cache.data[0, 1, page, :, off] = v.expand(length, kvh, 128).contiguous()
+    q = torch.zeros(new, qh, 128, dtype=B, device=dev)
+    q[..., 0] = 1.0
+    for kind in ("equal", "rising", "random"):
+        k = torch.zeros(length, kvh, 128, device=dev)
+        if kind == "rising":
+            k[..., 0] = ((pos // 64) * 4.0).clamp(max=200)[:, None]
+        elif kind == "random":
+            k[..., 0] = 3 * torch.randn(length, kvh, device=dev, generator=torch.Generator(device=dev).manual_seed(2))
+        cache.data[0, 0, page, :, off] = k.to(B)
+        out = cache.attention(0, batch, q, 1.0)
+        assert bool(out.isfinite().all()), kind
+        # the mean of one value is that value; weights and sums as in test_probabilities_keep_more_than_16_bits
+        bound = (2.0 ** -8 + 2.0 ** -16 + 2.0 ** -14) * v.double()
+        assert bool(((out.double() - v.double()).abs() <= bound).all()), kind
+
+
+def test_large_and_small_dims_side_by_side(dev):
+    """Dims of 3e38 beside dims of 1e-25: the large ones' sums are taken with room above, the small ones keep theirs."""
+    for new, length in ((1, 500), (50, 500)):
+        cache = filled(dev, [length], 1, 64, 16, B, garbage=False)
+        batch = RaggedBatch.of([0], [new], dev)
+        cache.data[0, 1, :, :, :, :32] *= 1e38
+        cache.data[0, 1, :, :, :, :32] = cache.data[0, 1, :, :, :, :32].clamp(-3.3e38, 3.3e38)
+        cache.data[0, 1, :, :, :, 32:] *= 1e-25
+        cache.data[0, 1, :, :, :, 0] = 3.2e38
+        q = queries(dev, batch, 2, 64, B)
+        out = cache.attention(0, batch, q, 0.02)
+        assert bool(check_kinds(cache, batch, q, out, 0.02).all())
