@@ -117,6 +117,15 @@ __device__ __forceinline__ float join_factor(float m, float l, float M) {
   return sign_of(l) ? fmaxf(f, 0x1p-149f) : f;
 }
 
+// 1 / the sum of a row's weights.  That is 0 where the row sees no position (its output is then zeros), and
+// where every score that it sees is -Inf, for which the softmax is NaN: the pages up to position `last` tell.
+__device__ __forceinline__ float inverse_sum(float l, const PagedView& p, const int32_t* tab, int last) {
+  if (l != 0.f) return 1.0f / fabsf(l);
+  for (int i = 0; i <= last >> p.page_shift; ++i)
+    if (in_range(tab[i], p.num_pages)) return NAN;
+  return 0.f;
+}
+
 // Max / sum over the four 16-lane rows of a wave, in every lane (as in q4d_attention.hip).
 template <bool SUM>
 __device__ __forceinline__ float rows4(float v) {
@@ -658,7 +667,7 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
         if (count > 1 || at >= rows) continue;
         const int otok = at / G;
         uint16_t* op = late->out + (s.first + otok) * late->out_stride + (j * G + at - otok * G) * D + 4 * sl;
-        const float inv = L[h] == 0.f ? 0.f : 1.0f / fabsf(L[h]);
+        const float inv = inverse_sum(L[h], a.p, tab, s.len - s.count + otok);
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
           const uint32_t u0 = from_f32<BF>(acc[h][n][0] * inv), u1 = from_f32<BF>(acc[h][n][1] * inv);
@@ -1245,7 +1254,7 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
   // ---- rows out, through LDS -------------------------------------------------------------------
   __syncthreads();  // everybody is done with the tiles
   if (!active) return;
-  const float inv = l == 0.f ? 0.f : 1.0f / fabsf(l);
+  const float inv = inverse_sum(l, a.p, tab, qpos);
   char* T0 = lds + w * (32 * kRowBytes);  // 32 rows of D values, slot s of row r at s ^ (r & (LR - 1))
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)

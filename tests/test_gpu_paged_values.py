@@ -193,3 +193,26 @@ def test_large_and_small_dims_side_by_side(dev):
         q = queries(dev, batch, 2, 64, B)
         out = cache.attention(0, batch, q, 0.02)
         assert bool(check_kinds(cache, batch, q, out, 0.02).all())
+
+
+@pytest.mark.parametrize("dtype", [F, B], ids=["f16", "bf16"])
+@pytest.mark.parametrize("length,new,qh,kvh", [(1, 1, 2, 1), (700, 1, 4, 2), (9000, 1, 8, 1), (300, 5, 4, 2), (900, 60, 4, 2),
+                                              (6000, 40, 8, 1), (200, 200, 2, 2)])
+def test_scores_that_are_all_minus_inf(dev, length, new, qh, kvh, dtype):
+    """exp(-Inf - -Inf) is NaN, as in the definition; zeros are for tokens that see no position.  One finite
+    score is enough for finite outputs."""
+    cache = filled(dev, [length, length], kvh, 64, 16, dtype, garbage=False)
+    batch = RaggedBatch.of([0, 1], [new, new], dev)
+    q = queries(dev, batch, qh, 64, dtype)
+    q[..., 0] = 1.0
+    cache.data[0, 0, :, :, :, 0] = -INF
+    out = cache.attention(0, batch, q)
+    assert bool(out.isnan().all()) and cache.status() == 0
+    page, off = at(cache, 1, length - new)
+    cache.data[0, 0, page, :, off, 0] = 0.5
+    ok = check_kinds(cache, batch, q, cache.attention(0, batch, q), 64 ** -0.5)
+    assert bool(ok[new:].all()) and not bool(ok[:new].any())
+    # no page of the first sequence is there: zeros, and the second is as before
+    cache.table[0] = -1
+    out = cache.attention(0, batch, q)
+    assert bool((out[:new] == 0).all()) and bool(out[new:].isfinite().all())
