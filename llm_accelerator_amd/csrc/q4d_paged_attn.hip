@@ -949,8 +949,9 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
 #pragma unroll
     for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const u32x4*>(qp + 16 * i);
   }
-  // (a scale of 0 keeps masked scores at -Inf)
-  const float scale = fmaxf(fabsf(a.scale), 1e-30f);
+  // Scores are scaled as they enter the exponential, hidden ones at -Inf by then: the scale is positive, its
+  // sign and a scale of 0 go to the query.
+  const float scale = a.scale == 0.f ? 1.f : fabsf(a.scale);
 
   // ---- K / V tiles ---------------------------------------------------------------------------
   constexpr int RI = 64 / LR;  // rows a DMA instruction
@@ -1141,6 +1142,14 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
     for (int i = 0; i < KS; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) q[i][e] ^= 0x80008000u;
+  } else if (a.scale == 0.f) {  // (Inf x 0 is NaN)
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = 0.f * to_f32<BF>((uint16_t)(e & 1 ? q[i][e >> 1] >> 16 : q[i][e >> 1]));
+      q[i] = pack8<BF>(y);
+    }
   }
   pass(std::false_type());
   float zero = 0.f;  // NaN if a sum is Inf or NaN

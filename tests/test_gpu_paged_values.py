@@ -216,3 +216,22 @@ def test_scores_that_are_all_minus_inf(dev, length, new, qh, kvh, dtype):
     cache.table[0] = -1
     out = cache.attention(0, batch, q)
     assert bool((out[:new] == 0).all()) and bool(out[new:].isfinite().all())
+
+
+@pytest.mark.parametrize("counts", [[1, 1], [40, 3]], ids=str)
+def test_scalings_near_zero(dev, counts):
+    """Scores are scaled by the value that is given, however small; by 0 they are all equal, but Inf x 0 is NaN."""
+    cache = filled(dev, [90, 200], 2, 64, 16, B)
+    batch = RaggedBatch.of([0, 1], counts, dev)
+    q = queries(dev, batch, 6, 64, B, 5)
+    for scaling, size in ((1e-33, 1e16), (-1e-33, 1e16), (3e-36, 1e18), (0.0, 1.0), (-0.0, 1e18)):
+        rows = torch.arange(90, device=dev)
+        page, off = cache.table[0, rows // 16].long(), rows % 16
+        saved = cache.data[0, 0, page, :, off].clone()
+        cache.data[0, 0, page, :, off] = saved * size
+        big = (q.float() * size).to(B)
+        check_kinds(cache, batch, big, cache.attention(0, batch, big, scaling), scaling)
+        cache.data[0, 0, page[7], :, off[7], 3] = INF
+        out = cache.attention(0, batch, q, 0.0)
+        assert bool(out[:counts[0]].isnan().all()) and bool(out[counts[0]:].isfinite().all())
+        cache.data[0, 0, page, :, off] = saved
