@@ -235,3 +235,39 @@ def test_scalings_near_zero(dev, counts):
         out = cache.attention(0, batch, q, 0.0)
         assert bool(out[:counts[0]].isnan().all()) and bool(out[counts[0]:].isfinite().all())
         cache.data[0, 0, page, :, off] = saved
+
+
+def wider(cache, max_pages):
+    """The same cache with room for more pages a row."""
+    table = torch.full((cache.num_seqs, max_pages), -1, dtype=torch.int32, device=cache.device)
+    table[:, :cache.max_pages] = cache.table
+    return PagedKVCache.over(cache.data, table, cache.lengths, cache.refs)
+
+
+MANY = [  # the chunks (positions, new tokens) among decode steps, sequences in all, q heads, kv heads, dim, page, type
+    ([(6000, 20)], 65, 16, 1, 64, 16, F),                        # some 20 parts: joined in two levels
+    ([(600, 600)], 66, 16, 1, 128, 32, B),                       # first tiles of fewer steps than the last's parts
+    ([(4000, 300), (2000, 20), (2500, 77)], 70, 4, 2, 128, 64, F),
+    ([(3000, 600), (5000, 50), (129, 128)], 130, 6, 3, 64, 16, B),
+    ([(2000, 120), (1000, 1000)], 300, 2, 2, 128, 16, F),
+    ([(2600, 33)] * 5, 69, 8, 1, 64, 64, F),
+]
+
+
+@pytest.mark.parametrize("chunks,n,qh,kvh,d,ps,dtype", MANY, ids=lambda v: f"{len(v)}x{max(v)}" if isinstance(v, list) else str(v))
+def test_more_sequences_than_lanes_with_chunks_in_parts(dev, chunks, n, qh, kvh, d, ps, dtype):
+    """Against 64 bits, repeated on one workspace, and bit for bit the same whatever the table has room for."""
+    seqs = [(1 + (29 * i) % 90, i % 4 != 0) for i in range(n - len(chunks))]
+    for i, c in enumerate(chunks):
+        seqs.insert((37 * i + 11) % n, c)
+    cache = filled(dev, [t for t, _ in seqs], kvh, d, ps, dtype, seed=n)
+    batch = RaggedBatch.of(list(range(n)), [int(a) for _, a in seqs], dev)
+    q = queries(dev, batch, qh, d, dtype, n)
+    ws = cache.workspace(qh, batch)
+    out = cache.attention(0, batch, q, ws=ws)
+    check_kinds(cache, batch, q, out, d ** -0.5)
+    assert cache.status() == 0
+    assert torch.equal(cache.attention(0, batch, q, ws=ws), out)
+    for room in (2 * cache.max_pages, (1 << 20) // ps):
+        assert torch.equal(wider(cache, room).attention(0, batch, q, ws=ws), out), room
+    assert torch.equal(cache.attention(0, batch, q, ws=ws), out)
