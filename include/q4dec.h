@@ -432,6 +432,8 @@ typedef struct q4d_pages {
   int32_t num_seqs;     /* up to 65536 */
   int32_t max_pages;    /* max_pages * page_size up to 2^24 positions */
   int32_t* status;      /* [1] */
+  int32_t max_ctx;      /* positions that a row may grow to, up to max_pages * page_size; 0: that many.  A rotation
+                         * has to cover them: q4d_pages_reserve refuses a step before any of it is written */
 } q4d_pages_t;
 
 /* The sequences of a call and their new tokens, which are their last positions: sequence b is
@@ -463,7 +465,7 @@ size_t q4d_pages_workspace_bytes(const q4d_pages_t* pages);
  * free ones of the lowest numbers, in the order of the batch.  Where the last page is partly
  * filled and other rows hold it too, its rows are copied to a page of the sequence's own first,
  * in every layer (but where the batch's sequences are all that hold it, the last of them keeps
- * it).  All or nothing: if pages run out, a sequence would pass max_pages or occurs twice, or a
+ * it).  All or nothing: if pages run out, a sequence would pass max_ctx or occurs twice, or a
  * row, count or page cannot be, nothing changes but the status word.  That then says
  * Q4D_STATUS_NOT_RESERVED too, and until it is cleared every later reserve is refused and
  * q4d_paged_append leaves all tokens out: the last positions that lengths name are older ones.

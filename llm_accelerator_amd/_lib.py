@@ -78,7 +78,7 @@ class Q4dPages(ctypes.Structure):
     _fields_ = [("data", c_void_p), ("dtype", c_int32), ("num_layers", c_int32), ("num_pages", c_int32),
                 ("num_kv_heads", c_int32), ("page_size", c_int32), ("head_dim", c_int32), ("table", c_void_p),
                 ("lengths", c_void_p), ("refs", c_void_p), ("num_seqs", c_int32), ("max_pages", c_int32),
-                ("status", c_void_p)]
+                ("status", c_void_p), ("max_ctx", c_int32)]
 
 
 class Q4dRagged(ctypes.Structure):

@@ -14,6 +14,7 @@ struct PagedView {
   int32_t* refs;
   int32_t* status;
   int num_layers, num_pages, kvh, page_shift, d, num_seqs, max_pages;
+  int max_ctx;  // positions that a row may grow to
 };
 
 struct RaggedView {

@@ -21,7 +21,7 @@ int check_pages(const q4d_pages_t* p) {
   if (p->head_dim != 64 && p->head_dim != 128) return Q4D_ERR_SHAPE;
   if (p->num_layers <= 0 || p->num_pages <= 0 || p->num_pages > 1 << 22 || p->num_kv_heads <= 0 ||
       p->num_kv_heads > 256 || p->num_seqs <= 0 || p->num_seqs > 65536 || p->max_pages <= 0 ||
-      (long long)p->max_pages * ps > 1 << 24)
+      (long long)p->max_pages * ps > 1 << 24 || p->max_ctx < 0 || p->max_ctx > p->max_pages * ps)
     return Q4D_ERR_SHAPE;
   if (!aligned(p->data, 16) || !aligned(p->table, 4) || !aligned(p->lengths, 4) || !aligned(p->refs, 4) ||
       !aligned(p->status, 4))
@@ -50,6 +50,7 @@ PagedView paged_view(const q4d_pages_t* p) {
   v.d = p->head_dim;
   v.num_seqs = p->num_seqs;
   v.max_pages = p->max_pages;
+  v.max_ctx = p->max_ctx ? p->max_ctx : p->max_pages * p->page_size;
   return v;
 }
 
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(1024) void reserve_kernel(const PagedView p, const 
     if (!count[i]) continue;
     if (len[i] < 0 || len[i] > most) {
       err |= Q4D_STATUS_BAD_SEQUENCE;
-    } else if (len[i] + (long long)count[i] > most) {
+    } else if (len[i] + (long long)count[i] > p.max_ctx) {
       err |= Q4D_STATUS_BAD_POSITION;
     } else if (len[i] & (ps - 1)) {
       last[i] = p.table[(size_t)row[i] * p.max_pages + (len[i] >> p.page_shift)];

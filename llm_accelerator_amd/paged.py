@@ -153,7 +153,8 @@ class PagedWorkspace:
 
 class PagedKVCache:
     """Pool [layers][K, V][pages][kv heads][page size][head dim] (fp16 or bf16), ``table`` [rows, max
-    pages], ``lengths`` [rows] and ``refs`` [pages] (int32, on the device).  Calls that change a cache
+    pages], ``lengths`` [rows] and ``refs`` [pages] (int32, on the device).  A sequence grows to
+    ``max_ctx`` positions at most (a table of angles should have as many).  Calls that change a cache
     must not overlap each other or calls that read it."""
 
     def __init__(self, num_layers: int, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
@@ -161,16 +162,17 @@ class PagedKVCache:
         kw = dict(dtype=torch.int32, device=device)
         self._setup(torch.zeros((num_layers, 2, num_pages, num_kv_heads, page_size, head_dim), dtype=dtype, device=device),
                     torch.full((num_seqs, -(-max_ctx // page_size)), -1, **kw), torch.zeros(num_seqs, **kw),
-                    torch.zeros(num_pages, **kw))
+                    torch.zeros(num_pages, **kw), max_ctx)
 
     @classmethod
-    def over(cls, data: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor) -> "PagedKVCache":
-        """A cache over tensors that the caller holds."""
+    def over(cls, data: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
+             max_ctx: int | None = None) -> "PagedKVCache":
+        """A cache over tensors that the caller holds (``max_ctx`` ``None``: what a table row has room for)."""
         cache = cls.__new__(cls)
-        cache._setup(data, table, lengths, refs)
+        cache._setup(data, table, lengths, refs, max_ctx)
         return cache
 
-    def _setup(self, data, table, lengths, refs) -> None:
+    def _setup(self, data, table, lengths, refs, max_ctx) -> None:
         if data.dim() != 6 or data.shape[1] != 2 or not data.is_contiguous() or table.dim() != 2:
             raise ValueError("data must be contiguous [layers, 2, pages, kv heads, page size, head dim], table [rows, max pages]")
         if not data.is_cuda:
@@ -181,12 +183,16 @@ class PagedKVCache:
         self.data, self.table = data, _ints(table, "table", data.device)
         self.num_layers, _, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = data.shape
         self.num_seqs, self.max_pages = table.shape
+        room = self.max_pages * self.page_size
+        self.max_ctx = room if max_ctx is None else int(max_ctx)
+        if not 1 <= self.max_ctx <= room:
+            raise ValueError(f"max_ctx must be 1 .. {room}, what a table row has room for")
         self.lengths = _ints(lengths, "lengths", data.device, self.num_seqs)
         self.refs = _ints(refs, "refs", data.device, self.num_pages)
         self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._desc = Q4dPages(data.data_ptr(), _DTYPES[data.dtype], self.num_layers, self.num_pages, self.num_kv_heads,
                               self.page_size, self.head_dim, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(),
-                              self.num_seqs, self.max_pages, self._status.data_ptr())
+                              self.num_seqs, self.max_pages, self._status.data_ptr(), self.max_ctx)
         self._ref = ctypes.byref(self._desc)
         self._lib = _lib.load()
         self._ws_bytes = int(self._lib.q4d_pages_workspace_bytes(self._ref))
