@@ -469,8 +469,11 @@ size_t q4d_pages_workspace_bytes(const q4d_pages_t* pages);
  * row, count or page cannot be, nothing changes but the status word.  That then says
  * Q4D_STATUS_NOT_RESERVED too, and until it is cleared every later reserve is refused and
  * q4d_paged_append leaves all tokens out: the last positions that lengths name are older ones.
- * So a step that finds no pages, also one of several that were launched or replayed ahead,
- * leaves the cache as the last good step left it (what its q4d_paged_attention gives means nothing). */
+ * So a step of reserve, append and attention that finds no pages, also one of several that were launched
+ * or replayed ahead, leaves the cache as the last good step left it (what its q4d_paged_attention
+ * gives means nothing).  fork, truncate and compact are carried out all the same, since letting go of pages
+ * is what makes room: a step that forks or frees is launched when the status of the one before is known, or
+ * its forks and frees stand after a refusal. */
 int q4d_pages_reserve(const q4d_pages_t* pages, const q4d_ragged_t* batch, void* ws, size_t ws_bytes, void* stream);
 /* Row dst[i] becomes a copy of row src[i] that shares its pages; src, dst: device int32 [n].
  * dst[i] must be empty (length 0), in no src, and the first of its number in dst; a pair that

@@ -227,7 +227,8 @@ class PagedKVCache:
     def reserve(self, batch: RaggedBatch) -> None:
         """Every sequence grows by its new tokens: lengths, pages, and a copy of a partly filled last
         page that others hold too.  All or nothing; a refused one also holds back later calls and
-        :meth:`append` until :meth:`raise_for_status` clears the word (q4d_pages_reserve)."""
+        :meth:`append` until :meth:`raise_for_status` clears the word; the other page calls are carried
+        out all the same (q4d_pages_reserve)."""
         self._check_batch(batch)
         self._call("q4d_pages_reserve", self._ref, batch._ref, self._wsp, self._ws_bytes)
 

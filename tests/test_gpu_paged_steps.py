@@ -51,3 +51,42 @@ def test_rows_end_at_max_ctx(dev, max_ctx, ps):
     for bad in (0, -1, room.max_ctx + 1):
         with pytest.raises(ValueError):
             PagedKVCache.over(made.data, made.table, made.lengths, made.refs, bad)
+
+
+def test_page_calls_run_on_after_a_refused_reserve(dev):
+    """A captured step of fork, reserve, append and free, launched ahead: after the refusal nothing is written
+    into a page and no length grows, but forks and frees are carried out, since freeing is what makes room."""
+    cache = PagedKVCache(1, 5, 16, 2, 64, 6, 64, F, dev)
+    first = RaggedBatch.of([0, 1], [17, 20], dev)          # two pages each, one is free
+    cache.reserve(first)
+    src, dst, gone = i32([0], dev), i32([2], dev), i32([5], dev)
+    batch = RaggedBatch.of([2], [1], dev)
+    x = torch.randn(1, 4, 64, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(g, stream=side):
+        cache.fork(src, dst)
+        cache.reserve(batch)
+        cache.append(0, batch, None, x[:, :2], x[:, 2:])
+        cache.free(gone)
+    torch.cuda.current_stream().wait_stream(side)
+    g.replay()                                             # takes the last page for the fork's own copy
+    assert cache.status() == 0 and cache.lengths.tolist() == [17, 20, 18, 0, 0, 0]
+    data = cache.data.clone()
+    for s, d, r in ((1, 3, 5), (2, 4, 1)):                 # no page for the fork of 1; then all is held back
+        src.copy_(i32([s], dev))
+        dst.copy_(i32([d], dev))
+        gone.copy_(i32([r], dev))
+        batch.seqs.copy_(i32([d], dev))
+        g.replay()
+    assert cache.status() == _lib.STATUS_NO_PAGES | _lib.STATUS_NOT_RESERVED
+    assert torch.equal(cache.data, data)
+    assert cache.lengths.tolist() == [17, 0, 18, 20, 18, 0]   # 3 and 4 are forks that have not grown, 1 is gone
+    assert cache.refs.sum().item() == 2 + 2 + 2 + 2
+    with pytest.raises(_lib.Q4DecError):
+        cache.raise_for_status("step")
+    cache.free(i32([0, 2], dev))
+    batch.seqs.copy_(i32([3], dev))
+    cache.reserve(batch)
+    assert cache.status() == 0 and cache.lengths.tolist() == [0, 0, 0, 21, 18, 0]
