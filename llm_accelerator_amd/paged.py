@@ -73,6 +73,8 @@ class RaggedBatch:
         starts = [0]
         for c in counts:
             starts.append(starts[-1] + int(c))
+        if tokens is not None and tokens < starts[-1]:
+            raise ValueError(f"{tokens} token rows for {starts[-1]} new tokens")
         both = torch.tensor([int(s) for s in seqs] + starts, dtype=torch.int32).to(device)
         return cls(both[:len(seqs)], both[len(seqs):], max(1, starts[-1]) if tokens is None else tokens,
                    max(1, max(counts)))
