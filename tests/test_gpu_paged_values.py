@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import paged_ref
+from llm_accelerator_amd import _lib
 from llm_accelerator_amd.paged import PagedKVCache, RaggedBatch
 from test_gpu_paged_attention import filled, i32
 
@@ -271,3 +272,58 @@ def test_more_sequences_than_lanes_with_chunks_in_parts(dev, chunks, n, qh, kvh,
     for room in (2 * cache.max_pages, (1 << 20) // ps):
         assert torch.equal(wider(cache, room).attention(0, batch, q, ws=ws), out), room
     assert torch.equal(cache.attention(0, batch, q, ws=ws), out)
+
+
+@pytest.mark.parametrize("dtype", [F, B], ids=["f16", "bf16"])
+@pytest.mark.parametrize("length,new", [(1, 1), (300, 1), (5000, 1), (90, 12), (700, 40), (4000, 25), (150, 150)])
+def test_inf_and_nan_in_keys(dev, length, new, dtype):
+    """A score of Inf or NaN makes the tokens that see it NaN, one of -Inf is a weight of 0, for each head by the
+    signs of its query; tokens that do not see it are as without it."""
+    cache = filled(dev, [length], 2, 128, 16, dtype)
+    batch = RaggedBatch.of([0], [new], dev)
+    q = queries(dev, batch, 8, 128, dtype)
+    clean = cache.attention(0, batch, q)
+    kinds = set()
+    for pos in sorted({0, length // 2, max(0, length - new + new // 2), length - 1}):
+        page, off = at(cache, 0, pos)
+        saved = cache.data[0, 0, page, :, off].clone()
+        for value, dims in ((INF, slice(5, 6)), (-INF, slice(5, 6)), (INF, slice(5, 7)), (NAN, slice(9, 10))):
+            cache.data[0, 0, page, :, off, dims] = value
+            out = cache.attention(0, batch, q)
+            ok = check_kinds(cache, batch, q, out, 128 ** -0.5)
+            kinds |= {bool(x) for x in ok.flatten().unique()}
+            before = max(0, pos - (length - new))           # the tokens that do not see it
+            err = (out[:before].double() - clean[:before].double()).abs()
+            assert bool((err <= torch.finfo(dtype).eps * clean[:before].double().abs() + 2.0 ** -14).all())
+            cache.data[0, 0, page, :, off] = saved
+    assert kinds == {False, True} or length == 1
+    assert torch.equal(cache.attention(0, batch, q), clean)
+
+
+@pytest.mark.parametrize("counts", [(2, 1, 3, 1), (5, 4, 6, 2), (30, 64, 20, 9), (3, 40, 50, 1)], ids=str)
+def test_entries_beside_a_bad_one(dev, counts):
+    """starts go back by one: the entry that decreases is left out, and so is nothing else.  All rows but the
+    one that two entries claim are compared."""
+    cache = filled(dev, [150, 90, 64, 47], 2, 128, 32, F)
+    starts = [0]
+    for c in counts:
+        starts.append(starts[-1] + c)
+    starts[2] = starts[1] - 1                      # entry 1 is bad, entry 2 begins on entry 0's last row
+    counts = [b - a for a, b in zip(starts, starts[1:])]
+    lengths = [150, 90, max(64, counts[2]), 47]
+    if counts[2] > 64:
+        cache = filled(dev, lengths, 2, 128, 32, F)
+    batch = RaggedBatch(i32([0, 1, 2, 3], dev), i32(starts, dev), starts[4], max(counts))
+    q = queries(dev, batch, 4, 128, F)
+    out = torch.full_like(q, 3.0)
+    cache.attention(0, batch, q, out=out)
+    for b, contested in ((0, counts[0] - 1), (2, 0), (3, None)):
+        rows = q[starts[b]:starts[b + 1]]
+        one = RaggedBatch.of([b], [counts[b]], dev)
+        ref, size, tiny = paged_ref.attend(cache, 0, one, rows, 128 ** -0.5)
+        bad = (out[starts[b]:starts[b + 1]].double() - ref).abs() > paged_ref.attend_bound(ref, size, tiny, F)
+        bad = bad.flatten(1).any(1)
+        if contested is not None:
+            bad[contested] = False
+        assert not bool(bad.any()), b
+    assert cache.status() == _lib.STATUS_BAD_SEQUENCE
