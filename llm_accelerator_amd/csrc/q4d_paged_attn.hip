@@ -4,11 +4,11 @@
 // share the kv head: row r is token r / G, head r % G.  Sequences of up to 16 rows (decode steps,
 // a few proposed tokens; 16 is what one MFMA takes) are bound by reading K and V once: rows_part.
 // More rows share what is read: chunk_part.  A call is one launch.
-// Both sides of the 16: decode steps on chunk_part would take 15 us instead of 8.6 (one sequence of
-// 700 positions), 154 instead of 129 (64 of 4000), 34 instead of 23 (3 of 32700); 24 sequences of 5
-// tokens and 10 rows 33 instead of 28.  Batches of up to 32 rows a sequence take rows_part too, in two
-// groups (4 tokens of 8 heads a kv head, two groups / chunk_part: one sequence of 700 positions 13.6 /
-// 15.7 us, one of 6000 with two kv heads 17.8 / 22.5, 24 of 1500 33.4 / 35.4, 64 of 4000 139 / 152).
+// Both sides of the 16: decode steps on chunk_part would take 15 us instead of 8.0 (one sequence of
+// 700 positions), 151 instead of 122 (64 of up to 4000), 31 instead of 22 (3 of up to 32700); 24 sequences of
+// 5 tokens and 10 rows 34 instead of 26.  Batches of up to 32 rows a sequence take rows_part too, in two
+// groups (4 tokens of 8 heads a kv head, two groups / chunk_part: one sequence of 700 positions 13.0 /
+// 15.7 us, one of 6000 with two kv heads 17.4 / 21.0, 24 of up to 1500 21.8 / 22.4, 64 of up to 4000 144 / 154).
 #include <float.h>
 #include <math.h>
 
@@ -164,8 +164,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int b
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(lo | hi << 32), (short)0,
                                            __builtin_amdgcn_readfirstlane(bytes), 0x00027000);
 }
-// Non-temporal: every row is read once (64 sequences of 4000 positions 129 instead of 144 us; 3 of
-// 32700 with 16-position pages 23.3 instead of 22.2).
+// Non-temporal: every row is read once (64 sequences of up to 4000 positions 122 instead of 138 us; 3 of
+// up to 32700 with 16-position pages 22.0 instead of 20.9).
 __device__ __forceinline__ u32x4 rows_load(__amdgpu_buffer_rsrc_t r, int offset) {
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 0, 2));
 }
@@ -183,7 +183,7 @@ __device__ __forceinline__ f32x4 load_dev4(__amdgpu_buffer_rsrc_t r, int offset)
 
 // The running max moves only when a score exceeds it by more than this (log2 units): P = 2^(s - m)
 // stays below 2^8, far inside fp16's range, and the rescaling of the output is rare (whole prompts
-// 187 instead of 193 us, nothing where K and V are streamed).
+// 182 instead of 187 us, nothing where K and V are streamed).
 constexpr float kRescale = 8.0f;
 // bf16 values reach 3e38, and their sums pass fp32 where their mean does not.  A part whose sums came out
 // Inf (see drop_odd) is done again with weights of 2^(8 - 32) at most, so that 2^24 positions have room, and
@@ -199,7 +199,7 @@ __device__ __forceinline__ float join_max(float M) {
 // The work of a kv head is a line of steps of 128 positions, the sequences one after the other;
 // `blocks` blocks take S = ceil(steps / blocks) consecutive steps each, so every block streams as
 // many bytes whatever the lengths are.  A cut within `slack` steps of a sequence's end moves there,
-// which saves its join (24 sequences of 1500 positions and 5 tokens 28.2 instead of 28.8 us).  A
+// which saves its join (24 sequences of up to 1500 positions and 5 tokens 26.3 instead of 26.8 us).  A
 // block's first and last sequences may be parts: their softmax states go to the workspace (slot 1:
 // the sequence begins in this block; slot 0: it began in an earlier one), where they are joined.
 // A step: S^T = K . Q^T (16x16x32 MFMA, K rows straight from memory in operand order, two tiles of 16
@@ -209,10 +209,10 @@ __device__ __forceinline__ float join_max(float M) {
 // type, the rounded value and what that leaves (22 or 16 bits together; the stream hides the second
 // product: 1 % of a long batch's time, and outputs as close to 64 bits as their own rounding lets
 // them be instead of 1.4 times as far).
-// Bound by the K and V stream: 64 sequences of 4000 positions (790 MB) 125-129 us, 6.2 TB/s, which is
+// Bound by the K and V stream: 64 sequences of up to 4000 positions (790 MB) 120-123 us, 6.4 TB/s, which is
 // what reads alone reach; short ones by a chain of ten dependent memory round trips (cut, page, rows,
-// join): 8.6 us for one of 700 positions, 23 us (3.2 TB/s) for 3 of 32700, 28 us (3.9 TB/s) for 24 of
-// 1500 and 5 tokens.  One block a CU: two take 133 / 26 / 31.6 us of these.
+// join): 7.9 us for one of 700 positions, 21-22 us (3.4 TB/s) for 3 of up to 32700, 26 us (4.2 TB/s) for 24
+// of up to 1500 and 5 tokens.  One block a CU: two take 126 / 8.1 / 25.5 / 29.2 us.
 struct Cut {
   int S, slack;
 };
@@ -694,11 +694,12 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
 // 165 us, 512 tokens after 4097 44 instead of 39.
 // K and V tiles go from the pages to LDS by DMA one tile ahead, 16 rows a wave (one page at most).
 // Two blocks a CU, so that one's products run under the other's softmax.  4 prompts of up to 3500
-// positions, 16 / 8 heads: 212 us, 690 TFLOP/s of what rows see and, with the remainder's product, 1030 of
-// what the matrix units do (a product of 8192^3 reaches 1365); 512 tokens after 4097 44 us.  Measured with one
-// product and no faster than this order's 178 us: the next step's first product interleaved with this one's
-// exponentials in a wave (180), the same with 8 waves that share tiles two or three steps ahead (185), with 64
-// rows a wave and 512 registers (264: accumulators move between the register files).
+// positions, 16 / 8 heads: 212-220 us, 660-690 TFLOP/s of what rows see and, with the remainder's product,
+// 990-1030 of what the matrix units do, which are busy 54 % of the time (a product of 8192^3 reaches 1365);
+// 512 tokens after 4097 44 us.  Measured with one product and no faster than this order's 178 us: the next
+// step's first product interleaved with this one's exponentials in a wave (180), the same with 8 waves that
+// share tiles two or three steps ahead (185), with 64 rows a wave and 512 registers (264: accumulators move
+// between the register files).
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTile = 128;  // query rows of a block
@@ -731,16 +732,18 @@ __device__ __forceinline__ void dma16(const uint16_t* base, uint32_t offset, uin
 
 // A tile of n steps is cut into round(n / S) parts, S the steps that fill the device's blocks once (two
 // a CU; at least kMinSplit, so that a part pays for its join).  Parts then have 3/4 S .. 3/2 S steps.
-// kMinSplit 2 / 4 / 6: one sequence of 1500 positions and 20 tokens 20.8 / 18.7 / 19.8 us, 2 of 200 fresh
-// ones 12.8 / 11.2 / 11.2, 3 of 900 and 40 tokens 19.1 / 19.7 / 21.1.
+// kMinSplit 2 / 4 / 6: one sequence of 1500 positions and 20 tokens 19.2 / 17.8 / 19.7 us, 2 of 200 fresh
+// ones 14.8 / 12.7 / 12.6, 3 of 900 and 40 tokens 18.9 / 19.4 / 20.2.
 constexpr int kMinSplit = 4;
 // One block a CU instead of two where that leaves two under kOneSteps steps each (the joins of twice the
 // parts cost more than the overlap gives), or where rows_part's blocks have more steps than these and
-// keep the CU busy beside.  Two / one, us: 64 tokens after 20000 (4.9 steps) 48 / 39.5, 40 sequences of 500
-// positions and 20 tokens (4) 35.5 / 22.6, 16 of 3000 with two kv heads (2.8) 33 / 30; 24 of 1500 (6.5) 37 /
-// 38.2, two chunks of 700 beside 14 decode steps (7) 58 / 65, 60 tokens after 30000 (7.3) 57 / 49.5, 512
-// after 4097 (8.7) 41.5 / 44, 2048 fresh ones (9) 39 / 46.  Chunks of 700 beside decode steps of k times
-// their steps: k 0.5: 58 / 65, 1.2: 96 / 87, 2.2: 143 / 121.
+// keep the CU busy beside.  Two / one, us: 64 tokens after 20000 (4.9 steps) 48 / 40, 40 sequences of 500
+// positions and 20 tokens (5) 43 / 29, 16 of 3000 with two kv heads (2.9) 36.2 / 34.7; two chunks of 700
+// after 1500 beside 9 decode steps (7) 64 / 70, 60 tokens after 30000 (7.3) 56 / 50, 2048 fresh ones (8.3) 42 /
+// 47, 512 after 4097 (8.7) 43.4 / 42.9, 24 of 1500 and 20 tokens (9) 57 / 45: past the line it goes by how full
+// the tiles are, too, which the rule does not look at.  Those two chunks beside 17 / 31 / 60 decode steps of 3000
+// positions (0.9 / 1.6 / 3.1 of their steps): 79 / 82, 101 / 104, 163 / 147; two of up to 700 of 3000 beside 38
+// (3.2) 100 / 93.
 constexpr int kOneSteps = 6;
 // A sequence's tiles are at most its rows / kTile, rounded up.
 __host__ __device__ inline long long tiles_most(int tokens, int G, int n) { return (long long)tokens * G / kTile + n; }
@@ -1301,8 +1304,8 @@ __global__ __launch_bounds__(256, 2) void rows_kernel(const PagedAttnArgs a) {
 }
 
 // Both: the first blocks * kvh blocks take the sequences of few rows, which stream K and V, and run
-// beside the others, which compute: 38 decode steps of 3000 positions and two chunks of 700 tokens
-// 87 us (when both were two launches, one after the other, they took 7 us more than together).
+// beside the others, which compute: 38 decode steps of up to 3000 positions and two chunks of up to 700 tokens
+// 86 us (as two launches, one after the other, they took 7 us more than together).
 template <int D, bool BF>
 __global__ __launch_bounds__(256, 2) void chunk_kernel(const PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[Shared<D>::kChunkV + Shared<D>::kMore];
@@ -1335,7 +1338,7 @@ Layout layout(int kvh, int d, bool chunks) {
 }
 // Groups of 16 query rows that the batch's sequences have at most: rows_part takes all of them if that is one
 // or two, else (0) the sequences of one, and chunk_part the others.  Two groups beside chunks, or in the
-// kernel for one, cost that one 3 to 7 % (mixed 87 / 93 us, 64 decode steps 129 / 132).
+// kernel for one, cost that one 3 to 12 % (mixed 94.6 / 97, 64 decode steps 128.3 / 133.3, one 8.7 / 9.8 us).
 int row_groups(int qh, int kvh, int max_new) {
   const long long rows = (long long)max_new * (qh / kvh);
   return rows <= kRows ? 1 : rows <= 2 * kRows ? 2 : 0;

@@ -287,7 +287,8 @@ class PagedKVCache:
         """k and v [tokens, kv_heads, head_dim] of the batch's tokens into their sequences' pages, with
         the head norm (fp32 gammas, optional) and rotation (optional) of q and k; returns the ready q
         rows [tokens, q_heads, head_dim] in the cache's type (``None`` without q).  The inputs may be
-        slices of one projection."""
+        slices of one projection.  Rows in no sequence are left as they were (they hold anything in a
+        ``q_out`` of the call's own)."""
         self._check_batch(batch)
         tokens, kind = batch.tokens, k.dtype
         if kind not in _DTYPES or v.dtype != kind or (q is not None and q.dtype != kind):
