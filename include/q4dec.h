@@ -493,7 +493,8 @@ int q4d_pages_compact(const q4d_pages_t* pages, int32_t* used, void* ws, size_t 
  * [head_dim] in the cache's type, for q4d_paged_attention.  q, k, v: x_dtype (Q4D_F32, Q4D_F16,
  * Q4D_BF16) rows of heads x head_dim, row t at t * stride elements (so they may lie side by side
  * in one projection); rows 16-byte aligned.  q and q_out may both be NULL (q_heads 0).  fp32
- * arithmetic, rounded once.  A token past rope's max_ctx (Q4D_STATUS_BAD_POSITION) or of a
+ * arithmetic, rounded once (past the largest number of the cache's type to Inf, which q4d_paged_attention
+ * takes as it is).  A token past rope's max_ctx (Q4D_STATUS_BAD_POSITION) or of a
  * sequence that cannot be is left out; into a page that cannot be nothing is written
  * (Q4D_STATUS_BAD_PAGE).  The pages must be the sequence's own (q4d_pages_reserve sees to that);
  * after a refused reserve (Q4D_STATUS_NOT_RESERVED) all tokens are left out. */

@@ -327,3 +327,46 @@ def test_entries_beside_a_bad_one(dev, counts):
             bad[contested] = False
         assert not bool(bad.any()), b
     assert cache.status() == _lib.STATUS_BAD_SEQUENCE
+
+
+@pytest.mark.parametrize("counts", [[1, 1, 1], [5, 1, 3], [70, 1, 20]], ids=str)
+def test_values_that_come_and_go_between_replays(dev, counts):
+    """A captured call: Inf, NaN and the largest bf16 values appear in V and are
+    gone again, and every replay is as the eager call and as 64 bits."""
+    cache = filled(dev, [3000, 500, 900], 2, 128, 16, B)
+    batch = RaggedBatch.of([0, 1, 2], counts, dev)
+    q = queries(dev, batch, 4, 128, B)
+    ws, out = cache.workspace(4, batch), torch.zeros_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(g, stream=side):
+        cache.attention(0, batch, q, out=out, ws=ws)
+    torch.cuda.current_stream().wait_stream(side)
+    clean = cache.data.clone()
+    want = cache.attention(0, batch, q)
+    for value in (INF, None, NAN, 3.3e38, None, -INF):
+        cache.data.copy_(clean)
+        if value is not None:
+            for s, pos in ((0, 1500), (1, 3), (2, 899)):
+                page, off = at(cache, s, pos)
+                cache.data[0, 1, page, :, off, 20:24] = value
+        g.replay()
+        check_kinds(cache, batch, q, out, 128 ** -0.5)
+        got = out.clone()
+        again = cache.attention(0, batch, q, ws=ws)
+        assert torch.equal(got.isnan(), again.isnan()) and torch.equal(got.nan_to_num(1.0), again.nan_to_num(1.0))
+        if value is None:
+            assert torch.equal(got, want)
+    assert cache.status() == 0
+
+
+@pytest.mark.parametrize("length,new", [(9000, 1), (2000, 300)])
+def test_every_value_nan_or_inf(dev, length, new):
+    cache = filled(dev, [length], 1, 64, 64, F)
+    batch = RaggedBatch.of([0], [new], dev)
+    q = queries(dev, batch, 4, 64, F)
+    cache.data[0, 1, ..., :32] = NAN
+    cache.data[0, 1, ..., 32:] = -INF
+    out = cache.attention(0, batch, q)
+    assert bool(out[..., :32].isnan().all()) and bool(out[..., 32:].isneginf().all())
