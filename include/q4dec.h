@@ -515,11 +515,10 @@ int q4d_paged_attention_workspace_init(void* ws, size_t ws_bytes, void* stream);
  * and sums are fp32; the probabilities enter the product with v as two numbers of the cache's type,
  * value and remainder (22 bits together in fp16, 16 in bf16).  A position whose page cannot be
  * counts as not there (Q4D_STATUS_BAD_PAGE); a token that sees no position gives zeros
- * (one whose scores are all -Inf NaN, as the softmax is).  Values
- * a token does not see, Inf and NaN among them, never reach its output; Inf and NaN of v that it
- * sees make that dim of it Inf or NaN, however small their weights are.  Deterministic; a token's
- * last bits may depend on the batch's shape and lengths, though not on the other sequences'
- * values. */
+ * (one whose scores are all -Inf NaN, as the softmax is).  Values a token does not see, Inf and NaN
+ * among them, never reach its output; Inf and NaN of v that it sees make that dim of it Inf or NaN,
+ * however small their weights are (NaN if 0, of a score of -Inf).  Deterministic; a token's last bits
+ * may depend on the batch's shape and lengths, though not on the other sequences' values. */
 int q4d_paged_attention(const q4d_pages_t* pages, int32_t layer, const q4d_ragged_t* batch, const void* q,
                         int64_t q_stride, int32_t q_heads, float scaling, void* out, int64_t out_stride, void* ws,
                         size_t ws_bytes, void* stream);

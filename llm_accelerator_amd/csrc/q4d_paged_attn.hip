@@ -88,7 +88,7 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 // taken as if there were none, which a part's sums show at its end: 0 x Inf and a weight x Inf stay Inf or
 // NaN through every later sum and rescaling.  Only then the part is done again with those values set to
 // zero, and they are added after the loop for the rows that see them (with the weight 1, which does as well:
-// what is added is Inf or NaN).  Which 64ths of the part's steps have some is kept as bits.  The sum l of such
+// what is added is Inf or NaN; as NaN where the score is -Inf and the weight 0).  Which 64ths of the part's steps have some is kept as bits.  The sum l of such
 // a row's weights is stored with a minus sign: see join_factor.
 
 // Inf and NaN (the exponent is all ones) among eight 16-bit floats become 0; whether there were any.
@@ -103,6 +103,17 @@ __device__ __forceinline__ bool drop_odd(u32x4& v) {
     odd |= lo || hi;
   }
   return odd;
+}
+// Eight products of 16-bit floats, summed.
+template <bool BF>
+__device__ __forceinline__ float dot8(u32x4 a, u32x4 b) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s = fmaf(to_f32<BF>((uint16_t)a[i]), to_f32<BF>((uint16_t)b[i]), s);
+    s = fmaf(to_f32<BF>((uint16_t)(a[i] >> 16)), to_f32<BF>((uint16_t)(b[i] >> 16)), s);
+  }
+  return s;
 }
 __device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) < INFINITY); }
 __device__ __forceinline__ uint32_t sign_of(float x) { return __builtin_bit_cast(uint32_t, x) & 0x80000000u; }
@@ -522,20 +533,28 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
       if (__builtin_expect(__ballot(zero != 0.f) != 0, 0)) {
         page = page_of(s0);
         pass(std::true_type());
-        const uint16_t* vplane = late_args()->vplane;
+        const KernelArgs late = late_args();
         for (; odd; odd &= odd - 1)
           for (int i = 0, it = s0 + __builtin_ctzll(odd) * per; i < per && it < s1; ++i, ++it) {
             const int base = it * kStep + 32 * w;  // this wave's positions
             for (int pos = base; pos < min(s.len, base + 32); ++pos) {
               const int pg = tab[min(pos >> shift, a.p.max_pages - 1)];
               if (!in_range(pg, a.p.num_pages)) continue;
+              const size_t at = page_elem(a.p, pg, j) + (size_t)(pos & inpage) * D;
+              bool none[H];  // the weight is 0
 #pragma unroll
-              for (int h = 0; h < H; ++h)
+              for (int h = 0; h < H; ++h) {
+                float score = 0.f;
+#pragma unroll
+                for (int i = 0; i < KS; ++i)
+                  score += dot8<BF>(q[h][i], *reinterpret_cast<const u32x4*>(late->kplane + at + 32 * i + 8 * g));
+                none[h] = rows4<true>(score) * late->scale == -INFINITY;
                 if (pos <= qpos[h]) {
                   m[h] = fmaxf(m[h], -FLT_MAX);  // (joined whatever the scores are)
                   l[h] = with_sign(l[h], 0x80000000u);
                 }
-              const uint16_t* v = vplane + page_elem(a.p, pg, j) + (size_t)(pos & inpage) * D + 4 * g;
+              }
+              const uint16_t* v = late->vplane + at + 4 * g;
 #pragma unroll
               for (int i = 0; i < DT; ++i)
 #pragma unroll
@@ -543,7 +562,7 @@ __device__ __forceinline__ void rows_part(const PagedAttnArgs& a, char* lds, int
                   const float x = to_f32<BF>(v[16 * i + e]);
 #pragma unroll
                   for (int h = 0; h < H; ++h)
-                    if (pos <= qpos[h] && not_finite(x)) o[h][i][e] += x;
+                    if (pos <= qpos[h] && not_finite(x)) o[h][i][e] += none[h] ? NAN : x;
                 }
             }
           }
@@ -1183,16 +1202,23 @@ __device__ __forceinline__ void chunk_part(const PagedAttnArgs& a, char* lds, in
         const int key0 = (st0 + __builtin_ctzll(odd) * per) * kKeys;
         for (int key = key0; key < min(min(st1 * kKeys, key0 + per * kKeys), kend); ++key) {
           const int page = tab[min(key >> shift, a.p.max_pages - 1)];
-          if (key > qpos || !in_range(page, a.p.num_pages)) continue;
+          if (!in_range(page, a.p.num_pages)) continue;
+          const size_t at = page_elem(a.p, page, j) + (size_t)(key & inpage) * D;
+          float score = 0.f;
+#pragma unroll
+          for (int i = 0; i < KS; ++i)
+            score += dot8<BF>(q[i], *reinterpret_cast<const u32x4*>(a.kplane + at + 16 * i + 8 * hf));
+          const bool none = halves<true>(score) * scale == -INFINITY;  // the weight is 0
+          if (key > qpos) continue;
           m = fmaxf(m, -FLT_MAX);  // (joined whatever the scores are)
           l = with_sign(l, 0x80000000u);
-          const uint16_t* v = a.vplane + page_elem(a.p, page, j) + (size_t)(key & inpage) * D + 4 * hf;
+          const uint16_t* v = a.vplane + at + 4 * hf;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const float x = to_f32<BF>(v[32 * dt + 8 * (r >> 2) + (r & 3)]);
-              if (not_finite(x)) o[dt][r] += x;
+              if (not_finite(x)) o[dt][r] += none ? NAN : x;
             }
         }
       }

@@ -370,3 +370,23 @@ def test_every_value_nan_or_inf(dev, length, new):
     cache.data[0, 1, ..., 32:] = -INF
     out = cache.attention(0, batch, q)
     assert bool(out[..., :32].isnan().all()) and bool(out[..., 32:].isneginf().all())
+
+
+@pytest.mark.parametrize("dtype", [F, B], ids=["f16", "bf16"])
+@pytest.mark.parametrize("length,new,qh,kvh", [(1, 1, 2, 1), (700, 1, 4, 2), (9000, 1, 8, 1), (700, 4, 8, 1), (900, 60, 4, 2),
+                                              (6000, 40, 8, 1)])
+def test_an_inf_of_weight_zero_is_nan(dev, length, new, qh, kvh, dtype):
+    """The score -Inf has the weight 0, and 0 x Inf is NaN; the other dims are as without the position."""
+    cache = filled(dev, [length], kvh, 128, 16, dtype)
+    batch = RaggedBatch.of([0], [new], dev)
+    q = queries(dev, batch, qh, 128, dtype)
+    q[..., 0] = 1.0
+    for pos in {0, length // 3, length - 1}:
+        page, off = at(cache, 0, pos)
+        saved = cache.data[0, :, page, :, off].clone()
+        cache.data[0, 0, page, :, off, 0] = -INF
+        cache.data[0, 1, page, :, off, 30] = INF
+        out = cache.attention(0, batch, q)
+        check_kinds(cache, batch, q, out, 128 ** -0.5)
+        assert bool(out[-1, :, 30].isnan().all()) and (length == 1 or bool(out[:, :, 31].isfinite().all()))
+        cache.data[0, :, page, :, off] = saved
