@@ -523,6 +523,59 @@ int q4d_paged_attention(const q4d_pages_t* pages, int32_t layer, const q4d_ragge
                         int64_t q_stride, int32_t q_heads, float scaling, void* out, int64_t out_stride, void* ws,
                         size_t ws_bytes, void* stream);
 
+/* ---- microscaled 4-bit floats, log probabilities --------------------------------
+ * No counterpart in the reference (its weights are the integers of q4d_matrix_t, and its only
+ * answer is the argmax, 10_validate_full_run_one_token.py:52-56): weights and activations in the
+ * 4-bit format that the matrix units read as it is, products with them, and how likely tokens are.
+ *
+ * A row of cols values (a multiple of 32) is cols / 32 blocks of 32 codes and a scale: value =
+ * code 2^(scale - 127), scale 255: NaN.  A code is a sign (bit 3) and one of 0, 0.5, 1, 1.5, 2, 3,
+ * 4, 6 (bits 2..0); the even column is in the low nibble (as in q4d_matrix_t). */
+typedef struct q4d_mx {
+  const uint8_t* w;  /* [rows, cols/2], 16-byte aligned */
+  const uint8_t* s;  /* [rows, cols/32] */
+  int32_t rows;
+  int32_t cols;
+} q4d_mx_t;
+
+enum { Q4D_MX_FLOOR = 0, Q4D_MX_CEIL = 1 };
+/* Rows of x (fp32, fp16 or bf16, ld elements apart, 16-byte aligned) as codes and scales.  A block's
+ * exponent is floor(log2(largest magnitude)) - 2 (Q4D_MX_FLOOR: magnitudes past 6 become 6) or the
+ * smallest with which none passes 6 (Q4D_MX_CEIL), within -127 .. 127; values go to the nearest code,
+ * ties to the even one.  A block with Inf or NaN is NaN (codes 0). */
+int q4d_mx_quantize(const void* x, int32_t dtype, int64_t ld, int32_t rows, int32_t cols, int32_t rule, uint8_t* packed,
+                    uint8_t* scale, void* stream);
+/* y [rows, cols] = the values, in y_dtype (16-byte aligned): exact in fp32 and bf16 but for what lies past
+ * their largest number (Inf), rounded once in fp16. */
+int q4d_mx_dequantize(const q4d_mx_t* t, void* y, int32_t y_dtype, void* stream);
+/* y[m, :] = W x[m, :], m < M: x fp16 or bf16, row m at m * x_stride elements, 16-byte aligned rows;
+ * y [M, rows] in any of the three types, 16-byte aligned.  The weights enter as numbers of x's type
+ * (as q4d_mx_dequantize makes them); fp32 sums, rounded once.  A row's last bits may depend on M,
+ * though not on the other rows' values. */
+int q4d_mx_linear(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M, void* y, int32_t y_dtype,
+                  void* stream);
+/* The same with x [M, cols] in 4 bits too: products and scales are exact, sums fp32. */
+int q4d_mx_matmul(const q4d_mx_t* w, const q4d_mx_t* x, void* y, int32_t y_dtype, void* stream);
+/* How likely token targets[m] is under the output head w ([vocab, hidden]) at hidden row x[m] (as in
+ * q4d_mx_linear), with z = W x[m] in fp32 and never in memory: logprob[m] = z[target] - log sum e^z
+ * (a target outside the vocabulary, a padded row's: NaN), entropy[m] of the distribution, best[m] =
+ * the largest log probability.  A row whose z hold NaN or +Inf gives NaN.  ws: 256-byte aligned,
+ * q4d_mx_score_workspace_bytes(w->rows, M) bytes, holds nothing between calls. */
+size_t q4d_mx_score_workspace_bytes(int32_t rows, int32_t M);
+int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M, const int32_t* targets,
+                 float* logprob, float* entropy, float* best, void* ws, size_t ws_bytes, void* stream);
+/* Of logits (fp32, fp16 or bf16, row i at i * stride elements, vocab up to 2^20): the entropy [rows]; with
+ * targets (device int32 [rows] or NULL) logprob[i] of token targets[i] and its rank[i], the number of
+ * tokens before it; and the `top` (0 .. 32, at most vocab) most likely tokens, top_ids and top_logprobs
+ * [rows, top], in order.  Tokens are ordered by logit, equal ones by index, the lowest first; NaN comes
+ * last.  A target outside the vocabulary: logprob NaN, rank -1.  -Inf (a masked token) has the
+ * probability 0; a row with nothing else, or with NaN or +Inf, has NaN for its log probabilities and
+ * entropy.  fp32 arithmetic.  ws: 256-byte aligned, holds nothing between calls. */
+size_t q4d_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top);
+int q4d_token_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_t rows, int32_t vocab, const int32_t* targets,
+                       int32_t top, float* logprob, int32_t* rank, float* entropy, float* top_logprobs, int32_t* top_ids,
+                       void* ws, size_t ws_bytes, void* stream);
+
 /* ---- fixed-point (RTL-exact) decode ------------------------------------------
  * The integer arithmetic of the reference's FPGA datapath, bit for bit
  * (Qwen3-0.6B-Base/python_each_module/56_export_persistent_multitoken_layer_golden.py:468-561

@@ -90,6 +90,10 @@ class Q4dRope(ctypes.Structure):
                 ("interleaved", c_int32)]
 
 
+class Q4dMX(ctypes.Structure):
+    _fields_ = [("w", c_void_p), ("s", c_void_p), ("rows", c_int32), ("cols", c_int32)]
+
+
 class Q4dFixedLayer(ctypes.Structure):
     _fields_ = [("input_gamma", c_void_p), ("post_gamma", c_void_p), ("q_gamma", c_void_p), ("k_gamma", c_void_p)]
 
@@ -148,6 +152,7 @@ _FM = POINTER(Q4dFixedModel)
 _FKV = POINTER(Q4dFixedKV)
 _PG = POINTER(Q4dPages)
 _RB = POINTER(Q4dRagged)
+_MX = POINTER(Q4dMX)
 SIGNATURES = {
     "q4d_version": ([], c_int32),
     "q4d_status_string": ([c_int32], ctypes.c_char_p),
@@ -206,6 +211,15 @@ SIGNATURES = {
     "q4d_paged_attention_workspace_init": ([_P, c_size_t, _P], c_int32),
     "q4d_paged_attention": ([_PG, c_int32, _RB, _P, ctypes.c_int64, c_int32, c_float, _P, ctypes.c_int64, _P, c_size_t,
                              _P], c_int32),
+    "q4d_mx_quantize": ([_P, c_int32, ctypes.c_int64, c_int32, c_int32, c_int32, _P, _P, _P], c_int32),
+    "q4d_mx_dequantize": ([_MX, _P, c_int32, _P], c_int32),
+    "q4d_mx_linear": ([_MX, _P, c_int32, ctypes.c_int64, c_int32, _P, c_int32, _P], c_int32),
+    "q4d_mx_matmul": ([_MX, _MX, _P, c_int32, _P], c_int32),
+    "q4d_mx_score_workspace_bytes": ([c_int32, c_int32], c_size_t),
+    "q4d_mx_score": ([_MX, _P, c_int32, ctypes.c_int64, c_int32, _P, _P, _P, _P, _P, c_size_t, _P], c_int32),
+    "q4d_token_logprobs_workspace_bytes": ([c_int32, c_int32, c_int32], c_size_t),
+    "q4d_token_logprobs": ([_P, c_int32, ctypes.c_int64, c_int32, c_int32, _P, c_int32, _P, _P, _P, _P, _P, _P, c_size_t,
+                            _P], c_int32),
     "q4d_fixed_tables": ([_P, c_int32, _P, c_int32], c_int32),
     "q4d_fixed_workspace_bytes": ([_FM], c_size_t),
     "q4d_fixed_workspace_init": ([_P, c_size_t, _FM, _P], c_int32),

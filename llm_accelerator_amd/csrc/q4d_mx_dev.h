@@ -1,0 +1,89 @@
+// Microscaled 4-bit floats (gfx950): a row of K values is K / 32 blocks; a block is 32 codes of
+// sign, 2 exponent bits and 1 mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6) and one scale byte s that
+// stands for 2^(s - 127), 255 for NaN.  Codes lie two a byte, the even column in the low nibble;
+// 16 bytes are one block.
+#pragma once
+
+#include <math.h>
+
+#include "q4d_device.h"
+#include "q4d_mx.h"
+
+namespace q4d {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// A scale byte as the conversions take it: they read the exponent field alone, 0 as 2^-127 and 255 as NaN.
+__device__ __forceinline__ float mx_scale(uint32_t s) { return __builtin_bit_cast(float, s << 23); }
+
+// Two codes (byte SEL of w) as fp32, and as a pair of 16-bit floats: one instruction each, exact but where
+// the type cannot hold the value (fp16: blocks of scales outside 2^-23 .. 2^13, rounded or Inf).
+template <int SEL, bool BF>
+__device__ __forceinline__ uint32_t mx_pair(uint32_t w, float scale) {
+  if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, SEL));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, SEL));
+}
+// Eight codes (columns 8 j .. + 7 of a block are its word j) as 16-bit floats.
+template <bool BF>
+__device__ __forceinline__ u32x4 mx_dequant8(uint32_t w, float scale) {
+  return u32x4{mx_pair<0, BF>(w, scale), mx_pair<1, BF>(w, scale), mx_pair<2, BF>(w, scale), mx_pair<3, BF>(w, scale)};
+}
+
+// A softmax's sums over some logits z: the maximum m, l = sum e^(z - m) and t = sum (z - m) e^(z - m), from
+// which log(sum e^z) = m + log l and the entropy log l - t / l.  fp32; a NaN among the logits makes l NaN,
+// and where all are -Inf l is 0 (and the joined l NaN at the end, as the softmax is).
+struct SoftSum {
+  float m, l, t;
+};
+// The sums of N logits given their maximum.
+template <int N, class F>
+__device__ __forceinline__ SoftSum soft_sum(float m, F z) {
+  const float ms = m == -INFINITY ? 0.f : m;
+  SoftSum s = {m, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = z(i) - ms, e = __expf(d);
+    s.l += e;
+    s.t = e > 0.f ? fmaf(d, e, s.t) : s.t;  // (-Inf x 0 counts as 0)
+  }
+  return s;
+}
+__device__ __forceinline__ SoftSum soft_join(SoftSum a, SoftSum b) {
+  const float m = fmaxf(a.m, b.m), ms = m == -INFINITY ? 0.f : m;
+  const float da = a.m - ms, db = b.m - ms, fa = __expf(da), fb = __expf(db);
+  return {m, fmaf(a.l, fa, b.l * fb),
+          (fa > 0.f ? fa * fmaf(da, a.l, a.t) : 0.f) + (fb > 0.f ? fb * fmaf(db, b.l, b.t) : 0.f)};
+}
+
+// Outputs n .. n + 3 of row m, those below N, rounded once to the output's type.
+__device__ __forceinline__ void store_out4(const MxProduct& a, int m, int n, f32x4 v) {
+  const size_t at = (size_t)m * a.N + n;
+  if (a.y_dtype == Q4D_F32) {
+    float* y = static_cast<float*>(a.y) + at;
+    if (n + 4 <= a.N && a.N % 4 == 0) {
+      *reinterpret_cast<f32x4*>(y) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < a.N) y[e] = v[e];
+    }
+    return;
+  }
+  uint32_t u[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    u[e] = a.y_dtype == Q4D_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)v[e]) : __builtin_bit_cast(uint16_t, (_Float16)v[e]);
+  uint16_t* y = static_cast<uint16_t*>(a.y) + at;
+  if (n + 4 <= a.N && a.N % 4 == 0) {
+    *reinterpret_cast<u32x2*>(y) = u32x2{u[0] | u[1] << 16, u[2] | u[3] << 16};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (n + e < a.N) y[e] = (uint16_t)u[e];
+  }
+}
+
+}  // namespace q4d

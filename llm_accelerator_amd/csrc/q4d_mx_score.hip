@@ -1,0 +1,138 @@
+// Entry points of the products with microscaled 4-bit weights, and the last step of a score: the sums
+// that the product's blocks left of each row are joined.
+#include <math.h>
+
+#include "q4d_mx.h"
+#include "q4d_mx_dev.h"
+
+namespace q4d {
+namespace {
+
+struct JoinArgs {
+  const float* stats;  // [parts][M][3]
+  const float* hit;    // [M]
+  const int32_t* targets;
+  int parts, M, N;
+  float *logprob, *entropy, *best;
+};
+
+// 16 rows a block, 16 threads a row; a thread's parts in order, then the threads', so that a row's sums
+// do not depend on the other rows.
+__global__ __launch_bounds__(256) void mx_score_join_kernel(const JoinArgs a) {
+  __shared__ float s_stat[256][3];
+  const int t = threadIdx.x, m = blockIdx.x * 16 + (t & 15);
+  SoftSum s = {-INFINITY, 0.f, 0.f};
+  if (m < a.M)
+    for (int p = t >> 4; p < a.parts; p += 16) {
+      const float* at = a.stats + ((size_t)p * a.M + m) * 3;
+      s = soft_join(s, SoftSum{at[0], at[1], at[2]});
+    }
+  s_stat[t][0] = s.m;
+  s_stat[t][1] = s.l;
+  s_stat[t][2] = s.t;
+  __syncthreads();
+  if (t >= 16 || m >= a.M) return;
+  for (int i = 1; i < 16; ++i) {
+    const float* at = s_stat[16 * i + t];
+    s = soft_join(s, SoftSum{at[0], at[1], at[2]});
+  }
+  const float ll = s.m == -INFINITY ? NAN : logf(s.l);
+  const int target = a.targets[m];
+  a.logprob[m] = target >= 0 && target < a.N ? (a.hit[m] - s.m) - ll : NAN;
+  a.entropy[m] = ll - s.t / s.l;
+  a.best[m] = -ll;
+}
+
+// Batches of up to this many rows take the kernel of few rows.
+constexpr int kFewRows = 64;
+
+int check_x(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M) {
+  if (const int rc = check_mx(w)) return rc;
+  if (!x) return Q4D_ERR_NULL;
+  if (x_dtype != Q4D_F16 && x_dtype != Q4D_BF16) return Q4D_ERR_DTYPE;
+  if (M <= 0 || (M > 1 && x_stride < w->cols)) return Q4D_ERR_SHAPE;
+  return aligned(x, 16) && (M == 1 || x_stride % 8 == 0) ? Q4D_OK : Q4D_ERR_BAD_ADDR;
+}
+int check_y(const void* y, int32_t y_dtype) {
+  if (!y) return Q4D_ERR_NULL;
+  if (y_dtype != Q4D_F16 && y_dtype != Q4D_BF16 && y_dtype != Q4D_F32) return Q4D_ERR_DTYPE;
+  return aligned(y, 16) ? Q4D_OK : Q4D_ERR_BAD_ADDR;
+}
+int product(const MxProduct& p, MxKind kind, hipStream_t st) {
+  return p.M <= kFewRows ? launch_mx_rows(p, kind, st) : launch_mx_gemm(p, kind, st);
+}
+MxKind kind_of(int32_t x_dtype) { return x_dtype == Q4D_BF16 ? MX_BF16 : MX_F16; }
+
+size_t hit_bytes(int M) { return align_up((size_t)M * 4, 256); }
+
+}  // namespace
+}  // namespace q4d
+
+using namespace q4d;
+
+extern "C" int q4d_mx_linear(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M, void* y,
+                             int32_t y_dtype, void* stream) {
+  int rc = check_x(w, x, x_dtype, x_stride, M);
+  if (rc || (rc = check_y(y, y_dtype))) return rc;
+  MxProduct p = {};
+  p.w = w->w;
+  p.ws = w->s;
+  p.x = x;
+  p.x_stride = M == 1 ? w->cols : x_stride;
+  p.M = M;
+  p.N = w->rows;
+  p.K = w->cols;
+  p.y = y;
+  p.y_dtype = y_dtype;
+  return product(p, kind_of(x_dtype), reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" int q4d_mx_matmul(const q4d_mx_t* w, const q4d_mx_t* x, void* y, int32_t y_dtype, void* stream) {
+  int rc = check_mx(w);
+  if (rc || (rc = check_mx(x)) || (rc = check_y(y, y_dtype))) return rc;
+  if (x->cols != w->cols) return Q4D_ERR_SHAPE;
+  MxProduct p = {};
+  p.w = w->w;
+  p.ws = w->s;
+  p.x = x->w;
+  p.xs = x->s;
+  p.M = x->rows;
+  p.N = w->rows;
+  p.K = w->cols;
+  p.y = y;
+  p.y_dtype = y_dtype;
+  return product(p, MX_X4, reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t q4d_mx_score_workspace_bytes(int32_t rows, int32_t M) {
+  if (rows <= 0 || M <= 0) return 0;
+  return hit_bytes(M) + (size_t)mx_gemm_parts(rows) * M * 12;
+}
+
+extern "C" int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M,
+                            const int32_t* targets, float* logprob, float* entropy, float* best, void* ws, size_t ws_bytes,
+                            void* stream) {
+  int rc = check_x(w, x, x_dtype, x_stride, M);
+  if (rc) return rc;
+  if (!targets || !logprob || !entropy || !best || !ws) return Q4D_ERR_NULL;
+  if (!aligned(targets, 4) || !aligned(logprob, 4) || !aligned(entropy, 4) || !aligned(best, 4) || !aligned(ws, 256))
+    return Q4D_ERR_BAD_ADDR;
+  if (ws_bytes < q4d_mx_score_workspace_bytes(w->rows, M)) return Q4D_ERR_CAPACITY;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  MxProduct p = {};
+  p.w = w->w;
+  p.ws = w->s;
+  p.x = x;
+  p.x_stride = M == 1 ? w->cols : x_stride;
+  p.M = M;
+  p.N = w->rows;
+  p.K = w->cols;
+  p.targets = targets;
+  p.hit = ws_ptr<float>(ws, 0);
+  p.stats = ws_ptr<float>(ws, hit_bytes(M));
+  const int parts = mx_gemm_parts(p.N);
+  if ((rc = launch_mx_gemm_score(p, kind_of(x_dtype), st))) return rc;
+  const JoinArgs j = {p.stats, p.hit, targets, parts, M, p.N, logprob, entropy, best};
+  hipLaunchKernelGGL(mx_score_join_kernel, dim3((unsigned)((M + 15) / 16)), dim3(256), 0, st, j);
+  return check_launch();
+}

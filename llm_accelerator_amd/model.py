@@ -343,6 +343,22 @@ def current_stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def call_on(index: int, name: str, *args) -> None:
+    """Entry point ``name`` on device ``index`` and that device's current stream; raises on an error code."""
+    call = getattr(_lib.load(), name)
+    here = torch._C._cuda_getDevice()
+    if here == index:
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(here))
+    else:
+        torch.cuda.set_device(index)
+        try:
+            rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+        finally:
+            torch.cuda.set_device(here)
+    if rc:
+        _lib.check(rc, name)
+
+
 def algorithmic_bytes_layer(cfg: Qwen3Config, ctx: int) -> int:
     """HBM bytes one decode step of one layer must move at context ``ctx``
     (positions attended = ctx + 1 after the append): Q4 weights + scales, the
@@ -421,4 +437,4 @@ def ceil_div(a: int, b: int) -> int:
 __all__ = ["Qwen3Config", "Q4Tensor", "Q4ForCausalLM", "Q4DecoderLayer", "Q4Backbone", "RotaryEmbedding",
            "KVCache", "Workspace", "random_q4", "random_gamma", "random_host_weights", "build_model",
            "algorithmic_bytes_layer", "fixed_layer_bytes", "with_context", "stage_bytes_layer", "prefill_flops", "batched_step_bytes", "gemv_bytes",
-           "current_stream", "ceil_div"]
+           "current_stream", "call_on", "ceil_div"]

@@ -1,0 +1,205 @@
+"""Microscaled 4-bit floats: the 4-bit format that the MI355X's matrix units read as it is.
+
+No counterpart in the reference, whose 4-bit weights are integers with a scale per 64 columns
+(``Source/Q4_FORMAT.md:75-140``, :class:`~llm_accelerator_amd.model.Q4Tensor`); the operators stand
+beside ``quantize_weight_q4``, ``manual_linear_from_weight`` and the LM head's argmax:
+
+* :func:`mx_quantize` -- a matrix as an :class:`MXTensor` (blocks of 32 codes and a power of two);
+  :meth:`MXTensor.dequantize` -- the values back;
+* :func:`mx_linear` -- ``x @ W.T`` with such weights, x in 16 bits or an :class:`MXTensor` itself;
+* :func:`mx_score` -- how likely given tokens are under an output head of such weights, without the
+  logits in memory.
+
+Every call is launched on torch's current stream of its tensors' device, does not synchronise, keeps
+nothing between calls and can be captured into a graph.  Arguments are checked (``ValueError`` /
+:class:`~llm_accelerator_amd._lib.Q4DecError`).
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import Q4D_BF16, Q4D_F16, Q4D_F32, Q4dMX
+from .model import call_on
+
+BLOCK = 32
+_DTYPES = {torch.float16: Q4D_F16, torch.bfloat16: Q4D_BF16, torch.float32: Q4D_F32}
+_RULES = {"floor": 0, "ceil": 1}
+
+
+class MXTensor:
+    """A matrix of microscaled 4-bit floats: ``packed`` uint8 [rows, cols/2] (the even column in the low
+    nibble) and ``scale`` uint8 [rows, cols/32] (2^(scale - 127); 255: NaN)."""
+
+    def __init__(self, packed: torch.Tensor, scale: torch.Tensor):
+        if packed.dtype != torch.uint8 or scale.dtype != torch.uint8:
+            raise TypeError("MXTensor needs uint8 packed codes and uint8 scales")
+        if packed.dim() != 2 or packed.shape[0] == 0 or packed.shape[1] == 0 or packed.shape[1] % (BLOCK // 2):
+            raise ValueError(f"packed must be [rows, cols/2] with cols a multiple of {BLOCK}, got {tuple(packed.shape)}")
+        rows, half = packed.shape
+        if scale.shape != (rows, 2 * half // BLOCK):
+            raise ValueError(f"scale shape {tuple(scale.shape)} does not match packed {tuple(packed.shape)}")
+        if packed.device != scale.device:
+            raise ValueError(f"packed is on {packed.device}, scale on {scale.device}")
+        packed, scale = packed.contiguous(), scale.contiguous()
+        self.packed = packed.clone() if packed.data_ptr() % 16 else packed  # the kernels read 16-byte aligned rows
+        self.scale = scale
+        self.shape = (rows, 2 * half)
+        self._desc = Q4dMX(self.packed.data_ptr(), scale.data_ptr(), rows, 2 * half)
+        self._ref = ctypes.byref(self._desc)
+        self._index = packed.get_device()
+
+    @property
+    def device(self) -> torch.device:
+        return self.packed.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.packed.numel() + self.scale.numel()
+
+    def to(self, device) -> "MXTensor":
+        return MXTensor(self.packed.to(device), self.scale.to(device))
+
+    def numpy(self) -> tuple[np.ndarray, np.ndarray]:
+        return self.packed.cpu().numpy(), self.scale.cpu().numpy()
+
+    @classmethod
+    def from_numpy(cls, packed: np.ndarray, scale: np.ndarray, device="cpu") -> "MXTensor":
+        return cls(torch.from_numpy(np.ascontiguousarray(packed, dtype=np.uint8)).to(device),
+                   torch.from_numpy(np.ascontiguousarray(scale, dtype=np.uint8)).to(device))
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values [rows, cols]: exact in fp32 and bf16 (Inf past their largest number), rounded once
+        in fp16."""
+        if dtype not in _DTYPES:
+            raise ValueError(f"dtype must be fp32, fp16 or bf16, got {dtype}")
+        _on_gpu(self)
+        y = torch.empty(self.shape, dtype=dtype, device=self.device)
+        call_on(self._index, "q4d_mx_dequantize", self._ref, y.data_ptr(), _DTYPES[dtype])
+        return y
+
+
+def _on_gpu(t) -> None:
+    if t._index < 0:
+        raise ValueError("the MXTensor must be on a GPU (libq4dec has no CPU path)")
+
+
+def _rows(x: torch.Tensor, name: str, cols: int | None = None):
+    """(x, its rows, elements from row to row) of x [..., cols], copied only if its rows cannot be read in place."""
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor (libq4dec has no CPU path)")
+    if x.dim() == 0 or (cols is not None and x.shape[-1] != cols):
+        raise ValueError(f"{name} must be [..., {'cols' if cols is None else cols}], got {tuple(x.shape)}")
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    step = x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    if x.data_ptr() % 16 or (x.shape[1] > 1 and x.stride(1) != 1) or step < x.shape[1] or step * x.element_size() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        step = x.shape[1]
+    return x, x.shape[0], step
+
+
+def mx_quantize(x: torch.Tensor, rule: str = "floor") -> MXTensor:
+    """x [rows, cols] (or [..., cols], whose leading dims become rows; fp32, fp16 or bf16) as an
+    :class:`MXTensor`.  A block's power of two is 2^e, e = floor(log2(largest magnitude)) - 2
+    (``"floor"``, the format's own rule: magnitudes past 6 x 2^e become that) or the smallest e with which
+    none passes 6 x 2^e (``"ceil"``); values go to the nearest code, ties to the even one.  A block with
+    Inf or NaN is NaN."""
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"x must be fp32, fp16 or bf16, got {x.dtype}")
+    if rule not in _RULES:
+        raise ValueError(f"unknown rule {rule!r}: floor or ceil")
+    if x.dim() and (x.shape[-1] == 0 or x.shape[-1] % BLOCK):
+        raise ValueError(f"the last dim must be a multiple of {BLOCK}, got {x.shape[-1]}")
+    x, rows, step = _rows(x, "x")
+    if rows == 0:
+        raise ValueError("expected at least one row")
+    cols = x.shape[1]
+    packed = torch.empty((rows, cols // 2), dtype=torch.uint8, device=x.device)
+    scale = torch.empty((rows, cols // BLOCK), dtype=torch.uint8, device=x.device)
+    call_on(x.get_device(), "q4d_mx_quantize", x.data_ptr(), _DTYPES[x.dtype], step, rows, cols, _RULES[rule],
+            packed.data_ptr(), scale.data_ptr())
+    return MXTensor(packed, scale)
+
+
+def mx_linear(x: torch.Tensor | MXTensor, weight: MXTensor, out_dtype: torch.dtype | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x @ weight.T``: x [..., cols] in fp16 or bf16, where the weights enter as numbers of that type
+    (``weight.dequantize(x.dtype)``), or an :class:`MXTensor` [rows, cols], where both enter as they are.
+    fp32 sums, rounded once to ``out_dtype`` (fp32, fp16 or bf16; ``None``: x's type, bf16 for an
+    MXTensor).  ``out``: a contiguous result of the caller's."""
+    if not isinstance(weight, MXTensor):
+        raise TypeError("weight must be an MXTensor")
+    _on_gpu(weight)
+    n, cols = weight.shape
+    codes = isinstance(x, MXTensor)
+    if codes:
+        _on_gpu(x)
+        if x.shape[1] != cols:
+            raise ValueError(f"x has {x.shape[1]} columns, the weights {cols}")
+        index, lead, kind, m = x._index, (x.shape[0],), torch.bfloat16, x.shape[0]
+    else:
+        if x.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"x must be fp16, bf16 or an MXTensor, got {x.dtype}")
+        lead, kind = x.shape[:-1], x.dtype
+        x, m, step = _rows(x, "x", cols)
+        index = x.get_device()
+    if index != weight._index:
+        raise ValueError(f"x is on {x.device}, the weights on {weight.device}")
+    if out is None:
+        kind = kind if out_dtype is None else out_dtype
+        if kind not in _DTYPES:
+            raise ValueError(f"out_dtype must be fp32, fp16 or bf16, got {kind}")
+        out = torch.empty((*lead, n), dtype=kind, device=weight.device)
+    elif (out.dtype not in _DTYPES or out_dtype not in (None, out.dtype) or out.shape != (*lead, n) or not out.is_contiguous()
+          or out.get_device() != index or out.data_ptr() % 16):
+        raise ValueError(f"out must be contiguous {tuple((*lead, n))} in fp32, fp16 or bf16 (out_dtype) on {weight.device}, 16-byte aligned")
+    if m == 0:
+        return out
+    if codes:
+        call_on(index, "q4d_mx_matmul", weight._ref, x._ref, out.data_ptr(), _DTYPES[out.dtype])
+    else:
+        call_on(index, "q4d_mx_linear", weight._ref, x.data_ptr(), _DTYPES[x.dtype], step, m, out.data_ptr(), _DTYPES[out.dtype])
+    return out
+
+
+class MXScores(NamedTuple):
+    logprob: torch.Tensor   # of the given tokens
+    entropy: torch.Tensor   # of the distributions
+    best: torch.Tensor      # the largest log probability
+
+
+def mx_score(hidden: torch.Tensor, weight: MXTensor, targets: torch.Tensor) -> MXScores:
+    """How likely ``targets`` [...] (int32) are under the output head ``weight`` [vocab, cols] at the rows
+    ``hidden`` [..., cols] (fp16 or bf16): the log softmax of ``mx_linear(hidden, weight)`` in fp32 at the
+    targets, its entropy and its maximum, fp32 [...] each, without the products in memory.  A target
+    outside the vocabulary (a padded row's) gives NaN."""
+    if not isinstance(weight, MXTensor):
+        raise TypeError("weight must be an MXTensor")
+    _on_gpu(weight)
+    if hidden.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"hidden must be fp16 or bf16, got {hidden.dtype}")
+    lead = hidden.shape[:-1]
+    x, m, step = _rows(hidden, "hidden", weight.shape[1])
+    index = x.get_device()
+    if index != weight._index:
+        raise ValueError(f"hidden is on {x.device}, the weights on {weight.device}")
+    if targets.dtype != torch.int32 or targets.shape != lead or targets.get_device() != index:
+        raise ValueError(f"targets must be int32 {tuple(lead)} on {x.device}")
+    targets = targets.contiguous()
+    got = torch.empty((3, *lead), dtype=torch.float32, device=x.device)
+    if m:
+        nbytes = int(_lib.load().q4d_mx_score_workspace_bytes(weight.shape[0], m))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        base, row = got.data_ptr(), 4 * m
+        call_on(index, "q4d_mx_score", weight._ref, x.data_ptr(), _DTYPES[x.dtype], step, m, targets.data_ptr(), base,
+                base + row, base + 2 * row, ws.data_ptr(), nbytes)
+    return MXScores(*got.unbind(0))
+
+
+__all__ = ["MXTensor", "MXScores", "mx_quantize", "mx_linear", "mx_score"]

@@ -1,0 +1,197 @@
+"""token_logprobs against the log softmax in 64 bits; ranks and alternatives equal, ties to the lowest index.
+
+Tolerance: the logits are given, so only the softmax's sums count: see test_gpu_mx_score (64 additions in a
+thread there 32, the same joins): log sum e^z is off by (H + 434) 2^-23, the entropy by that and twice that
+of H + log l + 1.
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from llm_accelerator_amd.logprobs import MAX_VOCAB, token_logprobs
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def reference(x: torch.Tensor, targets, top: int):
+    """On the CPU in 64 bits; order by value then index by a stable sort."""
+    x = x.double().cpu()
+    key = torch.where(x.isnan(), torch.full_like(x, -math.inf), x)
+    order = torch.sort(key, dim=-1, descending=True, stable=True).indices
+    if x.isnan().any():  # NaN after -Inf
+        order = torch.stack([torch.cat([o[~r[o].isnan()], o[r[o].isnan()]]) for o, r in zip(order, x)])
+    lp = torch.log_softmax(x, -1)
+    h = -torch.where(lp.exp() > 0, lp.exp() * lp, torch.zeros_like(lp)).sum(-1)
+    h = torch.where(lp.isnan().any(-1), torch.nan, h)
+    got = {"entropy": h, "top_ids": order[:, :top].int(), "top_logprobs": lp.gather(1, order[:, :top])}
+    if targets is not None:
+        t = targets.cpu().long()
+        ok = (t >= 0) & (t < x.shape[1])
+        tc = t.clamp(0, x.shape[1] - 1)
+        where = (order == tc[:, None]).int().argmax(-1)
+        got["rank"] = torch.where(ok, where, -1).int()
+        got["logprob"] = torch.where(ok, lp.gather(1, tc[:, None])[:, 0], torch.nan)
+    return got
+
+
+def check(x, targets, top):
+    got = token_logprobs(x, targets, top)
+    want = reference(x, targets, top)
+    h = torch.nan_to_num(want["entropy"])
+    lse = (h + 434) * 2.0 ** -23
+    logl = -torch.nan_to_num(torch.log_softmax(x.double().cpu(), -1).amax(-1))
+    assert torch.equal(got.top_ids.cpu(), want["top_ids"])
+    if targets is None:
+        assert got.logprob is None and got.rank is None
+    else:
+        assert torch.equal(got.rank.cpu(), want["rank"])
+        close(got.logprob, want["logprob"], lse)
+    close(got.top_logprobs, want["top_logprobs"], lse[:, None])
+    close(got.entropy, want["entropy"], lse + 2 * lse * (h + logl + 1))
+    return got
+
+
+def close(a, b, tol):
+    a = a.double().cpu()
+    assert a.shape == b.shape and torch.equal(a.isnan(), b.isnan()) and torch.equal(a.isinf(), b.isinf())
+    fine = b.isfinite()
+    err = torch.where(fine, a - b, 0).abs()
+    bound = tol + 2.0 ** -22 * (torch.where(fine, b, 0).abs() + 1)
+    assert (err <= bound).all(), f"{(err / bound).max().item():.2f} of the bound"
+
+
+def logits(rows, vocab, dtype, dev, seed=0, scale=3.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return (scale * torch.randn(rows, vocab, generator=g, device=dev)).to(dtype)
+
+
+def targets(rows, vocab, dev, seed=0):
+    t = torch.from_numpy(np.random.default_rng(seed).integers(0, vocab, rows)).to(dev).int()
+    t[0], t[-1] = 0, vocab - 1
+    return t
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (1, 1, 0), (3, 2, 2), (2, 7, 7), (5, 31, 31), (4, 33, 32), (1, 255, 5), (3, 256, 1),
+                                            (2, 257, 32), (7, 4097, 20), (3, 16383, 8), (2, 16384, 32), (2, 16385, 32), (3, 32769, 1),
+                                            (1, 151936, 5), (9, 151669, 20), (70, 1000, 3), (2, 262144, 32)])
+def test_shapes(dev, rows, vocab, top, dtype):
+    check(logits(rows, vocab, dtype, dev, seed=vocab), targets(rows, vocab, dev, seed=rows), top)
+
+
+def test_largest_vocabulary(dev):
+    check(logits(2, MAX_VOCAB, torch.float32, dev), targets(2, MAX_VOCAB, dev), 32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [5, 300, 16390, 40000])
+def test_ties(dev, vocab, dtype):
+    """All equal; two values; runs of equal values; -0 beside 0: the lowest index first."""
+    top = min(32, vocab)
+    x = torch.zeros(6, vocab, device=dev)
+    x[1] = torch.arange(vocab, device=dev) % 2
+    x[2] = -(torch.arange(vocab, device=dev) // 7).float() % 13
+    x[3, ::2] = -0.0
+    x[4] = torch.arange(vocab, device=dev).float().div(vocab).round(decimals=2)  # ascending
+    x[5] = -x[4]
+    check(x.to(dtype), torch.tensor([0, 1, vocab - 1, vocab - 2, vocab // 2, 2], device=dev, dtype=torch.int32), top)
+
+
+@pytest.mark.parametrize("vocab", [300, 16385, 70000])
+def test_orders_that_crowd_one_thread(dev, vocab):
+    """The best logits of a row all in one thread's or wave's reach, ascending and descending rows."""
+    x = logits(5, vocab, torch.float32, dev)
+    at = torch.arange(vocab, device=dev)
+    x[0] = torch.where(at % 256 == 17, x[0].abs() + 100 + at / vocab, x[0])
+    x[1] = torch.where(at % 256 < 4, x[1].abs() + 50, x[1])
+    x[2] = at / 7.0
+    x[3] = -at / 7.0
+    x[4] = torch.where(at % 1024 // 8 == 3, 9.0, x[4])
+    check(x, targets(5, vocab, dev), 32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [40, 16385, 50000])
+def test_masked_rows(dev, vocab, dtype):
+    x = logits(7, vocab, dtype, dev)
+    low = torch.finfo(dtype).min
+    x[0] = -math.inf                    # nothing left
+    x[1, 1:] = -math.inf                # one token left
+    x[2, : vocab // 2] = -math.inf
+    x[3, vocab // 2:] = low             # masked with the type's lowest value
+    x[4] = low                          # nothing but it: all equally likely
+    x[5, 3:] = -math.inf                # fewer left than alternatives asked for
+    x[6, : vocab - 1] = -math.inf
+    t = torch.tensor([0, 0, 1, vocab - 1, vocab - 1, 5, vocab - 1], device=dev, dtype=torch.int32)
+    got = check(x, t, min(vocab, 20))
+    assert got.logprob[0].isnan() and got.entropy[0].isnan()
+    assert got.logprob[1].item() == 0 and got.entropy[1].item() == 0
+    assert got.logprob[2].item() == -math.inf and got.logprob[5].item() == -math.inf
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [40, 20000])
+def test_inf_and_nan(dev, vocab, dtype):
+    x = logits(6, vocab, dtype, dev)
+    clean = token_logprobs(x, targets(6, vocab, dev), top=4)
+    x[0, 5] = math.inf
+    x[1, 7] = math.nan
+    x[2, 3:9] = math.nan
+    x[2, 9:] = -math.inf
+    x[3] = math.nan
+    t = targets(6, vocab, dev)
+    t[1] = 7
+    got = check(x, t, 20)
+    assert got.logprob[:4].isnan().all() and got.entropy[:4].isnan().all() and got.top_logprobs[:4].isnan().all()
+    assert got.rank[1].item() == vocab - 1 and got.top_ids[0, 0].item() == 5
+    assert torch.equal(got.top_ids[4:, :4], clean.top_ids[4:]) and torch.equal(got.logprob[4:], clean.logprob[4:])
+
+
+def test_targets_outside(dev):
+    x = logits(5, 1000, torch.float32, dev)
+    t = torch.tensor([-1, 1000, 999, 2 ** 31 - 1, -2 ** 31], device=dev, dtype=torch.int32)
+    got = check(x, t, 3)
+    assert got.rank.tolist()[:2] == [-1, -1] and got.rank[2].item() >= 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_and_leading_dims(dev, dtype):
+    wide = logits(12, 5003, dtype, dev)
+    base = check(wide[:, 1:4999].contiguous(), targets(12, 4998, dev), 9)
+    t = targets(12, 4998, dev)
+    for v in (wide[:, 1:4999], torch.cat([wide, wide], 1)[:, 1:4999], wide.t().contiguous().t()[:, 1:4999]):
+        got = token_logprobs(v, t, top=9)
+        assert all(torch.equal(a, b) for a, b in zip(got, base))
+    got = token_logprobs(wide[:, 1:4999].reshape(3, 4, 4998), t.view(3, 4), top=9)
+    assert got.top_ids.shape == (3, 4, 9) and torch.equal(got.top_ids.view(12, 9), base.top_ids) and torch.equal(got.rank.view(12), base.rank)
+    one = token_logprobs(wide[3, 1:4999], t[3], top=9)
+    assert one.entropy.shape == () and torch.equal(one.top_logprobs, base.top_logprobs[3])
+    every = token_logprobs(wide[0:1, 1:4999].expand(4, 4998), None, top=2)
+    assert (every.top_ids == base.top_ids[0, :2]).all()
+
+
+def test_long_rows_past_32_bits(dev):
+    """A row that begins past 2^32 bytes."""
+    big = torch.zeros(4, 1 << 30, device=dev, dtype=torch.float16)
+    x = big[:, 5:3000 + 5]
+    x.copy_(logits(4, 3000, torch.float16, dev))
+    want = token_logprobs(x.contiguous(), targets(4, 3000, dev), top=5)
+    got = token_logprobs(x, targets(4, 3000, dev), top=5)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_no_rows_and_refusals(dev):
+    x = logits(3, 100, torch.float32, dev)
+    t = targets(3, 100, dev)
+    got = token_logprobs(x[:0], t[:0], top=4)
+    assert got.entropy.shape == (0,) and got.top_ids.shape == (0, 4)
+    for bad in (lambda: token_logprobs(x.double(), t), lambda: token_logprobs(x, t.long()), lambda: token_logprobs(x, t[:2]),
+                lambda: token_logprobs(x, t, top=33), lambda: token_logprobs(x, t, top=-1), lambda: token_logprobs(x[:, :4], t, top=5),
+                lambda: token_logprobs(x.cpu(), t), lambda: token_logprobs(x, t.cpu()), lambda: token_logprobs(x[0, 0], t[0]),
+                lambda: token_logprobs(torch.empty(1, MAX_VOCAB + 1, device=dev, dtype=torch.float16))):
+        with pytest.raises(ValueError):
+            bad()

@@ -1,0 +1,174 @@
+"""mx_linear (16-bit activations and 4-bit ones) against products in 64 bits.
+
+Tolerance: the products of the numbers that enter are exact in fp32 (at most 8 + 11 bits), and a sum of K
+of them in any order is off by at most one fp32 step (2^-23) of sum |x w| an addition, K of them; then the
+output's rounding, eps / 2 of its type.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+import mx_ref
+from llm_accelerator_amd.mx import MXTensor, mx_linear, mx_quantize
+
+pytestmark = pytest.mark.gpu
+HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}  # steps of subnormals
+
+
+def make(rng, n, k, dev, lo=119, hi=125):
+    p, s = mx_ref.random_mx(rng, n, k, lo, hi)
+    return MXTensor.from_numpy(p, s, device=dev), torch.from_numpy(mx_ref.values(p, s)).to(dev)
+
+
+def compare(y, x, w):
+    """y against x w^T, both float64 on the device."""
+    want, size = x @ w.T, x.abs() @ w.abs().T
+    k = x.shape[1]
+    tol = k * 2.0 ** -23 * size + HALF[y.dtype] * (want.abs() + k * 2.0 ** -23 * size) + TINY[y.dtype]
+    err = (y.double() - want).abs()
+    assert (err <= tol).all(), f"{(err - tol).max().item():.3e} past the bound, {(err / tol.clamp(min=1e-300)).max().item():.2f} of it"
+
+
+SHAPES = [(1, 1, 32), (1, 16, 64), (1, 2048, 1024), (2, 17, 96), (3, 255, 160), (5, 64, 2048), (15, 33, 128), (16, 1000, 1056),
+          (17, 48, 224), (31, 129, 288), (33, 16, 512), (48, 1024, 2048), (63, 257, 320), (64, 70, 4096), (65, 256, 64),
+          (100, 3, 1024), (127, 255, 96), (128, 256, 256), (129, 257, 288), (200, 1000, 1024), (257, 513, 1056), (300, 64, 32),
+          (513, 2048, 192)]
+
+
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16, "mx"])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_shapes(dev, m, n, k, kind):
+    rng = np.random.default_rng(m + 7 * n + 13 * k)
+    w, wv = make(rng, n, k, dev)
+    if kind == "mx":
+        x, xv = make(rng, m, k, dev, 122, 130)
+    else:
+        x = torch.from_numpy(rng.standard_normal((m, k))).to(dev).to(kind)
+        xv = x.double()
+    for out in (None, torch.float32, torch.float16, torch.bfloat16):
+        y = mx_linear(x, w, out_dtype=out)
+        assert y.shape == (m, n) and y.dtype == (out or (torch.bfloat16 if kind == "mx" else kind))
+        compare(y, xv, wv)
+
+
+@pytest.mark.parametrize("m", [1, 40, 150])
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
+def test_strides_leading_dims_and_out(dev, m, kind):
+    rng = np.random.default_rng(m)
+    w, wv = make(rng, 130, 160, dev)
+    wide = torch.from_numpy(rng.standard_normal((m, 400))).to(dev).to(kind)
+    views = [wide[:, 80:240], torch.cat([wide, wide[:, :1]], 1)[:, 80:240], torch.cat([wide[:, :1], wide], 1)[:, 81:241],
+             wide.t().contiguous().t()[:, 80:240]]
+    base = mx_linear(views[0].contiguous(), w)
+    compare(base, views[0].double(), wv)
+    for v in views:
+        assert torch.equal(mx_linear(v, w), base)
+    y = mx_linear(views[0].reshape(1, m, 160), w)
+    assert y.shape == (1, m, 130) and torch.equal(y[0], base)
+    same = mx_linear(views[0][0:1].expand(m, 160), w)
+    assert torch.equal(same, same[0:1].expand(m, 130))
+    # a result of the caller's; nothing beside it is written
+    room = torch.full((m + 2, 136), 7.0, device=dev, dtype=kind)
+    out = room.view(-1)[136:136 + m * 130].view(m, 130)
+    got = mx_linear(views[0], w, out=out)
+    assert got is out and torch.equal(out, base)
+    flat = room.view(-1)
+    assert (flat[:136] == 7).all() and (flat[136 + m * 130:] == 7).all()
+
+
+def test_one_vector_and_no_rows(dev):
+    rng = np.random.default_rng(3)
+    w, wv = make(rng, 64, 96, dev)
+    x = torch.from_numpy(rng.standard_normal(96)).to(dev).to(torch.bfloat16)
+    y = mx_linear(x, w, out_dtype=torch.float32)
+    assert y.shape == (64,)
+    compare(y[None], x[None].double(), wv)
+    assert mx_linear(x.new_zeros(0, 96), w).shape == (0, 64)
+
+
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16, "mx"])
+@pytest.mark.parametrize("m,k", [(3, 96), (40, 1024), (150, 96), (150, 224)])
+def test_inf_and_nan_stay_in_their_rows(dev, m, k, kind):
+    rng = np.random.default_rng(k)
+    w, wv = make(rng, 70, k, dev)
+    x = torch.from_numpy(rng.standard_normal((m, k))).to(dev).to(torch.bfloat16 if kind == "mx" else kind)
+    clean = mx_linear(mx_quantize(x) if kind == "mx" else x, w, out_dtype=torch.float32)
+    x[1, k - 1], x[2, 0] = float("inf"), float("nan")
+    y = mx_linear(mx_quantize(x) if kind == "mx" else x, w, out_dtype=torch.float32)
+    keep = torch.ones(m, dtype=torch.bool, device=dev)
+    keep[1] = keep[2] = False
+    assert torch.equal(y[keep], clean[keep])
+    assert y[2].isnan().all()
+    if kind == "mx":
+        assert y[1].isnan().all()  # a block with Inf is NaN
+    else:
+        last = wv[:, k - 1]
+        assert y[1][last == 0].isnan().all()  # Inf x 0
+        assert (y[1][last > 0] == float("inf")).all() and (y[1][last < 0] == float("-inf")).all()
+
+
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16, "mx"])
+@pytest.mark.parametrize("m,k", [(3, 96), (40, 256), (150, 288)])
+def test_nan_blocks_of_weights_reach_their_outputs_alone(dev, m, k, kind):
+    rng = np.random.default_rng(k + 1)
+    p, s = mx_ref.random_mx(rng, 70, k)
+    s[5, 0] = s[69, -1] = 255
+    w = MXTensor.from_numpy(p, s, device=dev)
+    x = torch.from_numpy(rng.standard_normal((m, k))).to(dev).to(torch.bfloat16 if kind == "mx" else kind)
+    y = mx_linear(mx_quantize(x) if kind == "mx" else x, w, out_dtype=torch.float32)
+    bad = y.isnan().all(0)
+    assert bad[5] and bad[69] and bad.sum().item() == 2 and y[:, ~bad].isfinite().all()
+
+
+@pytest.mark.parametrize("m", [3, 150])
+def test_ends_of_the_scales(dev, m):
+    """Scales 0 and 254; in fp16 the weights enter as fp16 numbers."""
+    rng = np.random.default_rng(m)
+    p, s = mx_ref.random_mx(rng, 33, 128)
+    p &= 0x33  # magnitudes up to 1.5, so that 2^127 of them is finite
+    s[:, 0], s[:, 1] = 0, 254
+    w = MXTensor.from_numpy(p, s, device=dev)
+    v = torch.from_numpy(mx_ref.values(p, s)).to(dev)
+    x = torch.from_numpy(rng.standard_normal((m, 128))).to(dev).to(torch.bfloat16)
+    x[:, 32:64] *= 2.0 ** -120
+    compare(mx_linear(x, w, out_dtype=torch.float32), x.double(), v)
+    q = mx_quantize(x)
+    compare(mx_linear(q, w, out_dtype=torch.float32), q.dequantize().double(), v)
+    h = x.half()
+    h[:, 32:64] = 1
+    got = mx_linear(h, w, out_dtype=torch.float32)
+    want = h.double() @ w.dequantize(torch.float16).double().T
+    assert torch.equal(got.isfinite(), want.isfinite())
+    fine = want.isfinite()
+    assert torch.allclose(got[fine].double(), want[fine], rtol=0, atol=128 * 2.0 ** -23 * 65504 * 4)
+
+
+def test_deterministic_and_rows_apart(dev):
+    rng = np.random.default_rng(9)
+    w, _ = make(rng, 500, 1024, dev)
+    for m in (1, 20, 64, 300):
+        x = torch.from_numpy(rng.standard_normal((m, 1024))).to(dev).to(torch.bfloat16)
+        a = mx_linear(x, w)
+        assert torch.equal(a, mx_linear(x, w))
+        y = x.clone()
+        y[m // 2:] = y[m // 2:] * 3 + 1  # other rows' values change nothing
+        assert torch.equal(mx_linear(y, w)[:m // 2], a[:m // 2])
+
+
+def test_refusals(dev):
+    rng = np.random.default_rng(1)
+    w, _ = make(rng, 16, 64, dev)
+    x = torch.zeros(3, 64, device=dev, dtype=torch.float16)
+    for bad in (lambda: mx_linear(x.float(), w), lambda: mx_linear(x[:, :32], w), lambda: mx_linear(x.cpu(), w),
+                lambda: mx_linear(x, w, out_dtype=torch.float64), lambda: mx_linear(x, w.to("cpu")),
+                lambda: mx_linear(x, w, out=torch.empty(3, 15, device=dev)), lambda: mx_linear(x, w, out=torch.empty(3, 16)),
+                lambda: mx_linear(x, w, out=torch.empty(16, 3, device=dev).t()),
+                lambda: mx_linear(x, w, out_dtype=torch.float16, out=torch.empty(3, 16, device=dev)),
+                lambda: mx_linear(mx_quantize(x[:, :32]), w), lambda: mx_linear(torch.zeros((), device=dev).half(), w),
+                lambda: mx_quantize(x[:0])):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        mx_linear(x, x)
