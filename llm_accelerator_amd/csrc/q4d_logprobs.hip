@@ -1,10 +1,14 @@
 // Log probabilities of given tokens, ranks, entropy and the most likely alternatives out of logits
 // (gfx950, wave64), in one pass over them.
 //
-// A row is cut into parts of 256 x 64 logits; a block holds a part in registers, 64 logits a thread, and
-// leaves the part's softmax sums, how many of its logits come before the target, and its K best.  The
-// K best: of each thread's best the K-th best over the block is a bound that K logits reach, and the few
-// that reach it are gathered in LDS and ordered by counting.  A second kernel joins a row's parts.
+// A row is cut into parts of 256 x HELD logits; a block holds a part in registers, HELD logits a thread, and
+// leaves the part's softmax sums, how many of its logits come before the target, and its K best.  A row
+// of one part is finished there; else a second kernel joins a row's parts, a wave a row.
+//
+// The K best: in each wave the K-th largest of the lanes' own maxima is a bound that K logits reach, found
+// bit by bit with ballots; the few logits of the part that reach the largest such bound are gathered in
+// LDS and ordered by counting.  Where they are too many (equal logits, masks) or NaN matters the bound
+// is found again among keys of value and index, which no two logits share.
 //
 // Logits are ordered by value, then by index, the lower first; NaN comes last, after -Inf.
 #include <math.h>
@@ -16,10 +20,11 @@ namespace q4d {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kHeld = 64;                     // logits of a thread
-constexpr int kPart = kThreads * kHeld;
+constexpr int kHeldMost = 64;                 // logits of a thread
+constexpr int kHeldFew = 16;                  // ... where there are few parts
 constexpr int kTop = 32;                      // alternatives at most
 constexpr int kMaxParts = 64;                 // of a row: vocabularies of up to 2^20
+constexpr int kGather = 256;                  // logits that are ordered without a second bound
 
 struct LogprobArgs {
   const void* logits;
@@ -56,43 +61,120 @@ __device__ __forceinline__ float logit(const void* p, size_t i) {
   else if constexpr (DT == Q4D_BF16) return (float)static_cast<const __bf16*>(p)[i];
   else return (float)static_cast<const _Float16*>(p)[i];
 }
+// V consecutive logits, 16 bytes at any alignment of the type.
+template <int DT, int V>
+__device__ __forceinline__ void load_logits(const void* p, size_t i, float* x) {
+  u32x4 v;
+  __builtin_memcpy(&v, static_cast<const char*>(p) + i * (16 / V), 16);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t u = v[e];
+    if constexpr (DT == Q4D_F32) {
+      x[e] = __builtin_bit_cast(float, u);
+    } else if constexpr (DT == Q4D_BF16) {
+      x[2 * e] = __builtin_bit_cast(float, u << 16);
+      x[2 * e + 1] = __builtin_bit_cast(float, u & 0xFFFF0000u);
+    } else {
+      const f16x2 h = __builtin_bit_cast(f16x2, u);
+      x[2 * e] = (float)h[0];
+      x[2 * e + 1] = (float)h[1];
+    }
+  }
+}
+template <bool SUM>
+__device__ __forceinline__ float wave_all(float v) { return SUM ? wave_sum(v) : wave_max(v); }
 
+// What a row's outputs are once its sums are whole.
 template <int DT>
+__device__ __forceinline__ void finish_row(const LogprobArgs& a, int row, const SoftSum& s, float ll, int before) {
+  a.entropy[row] = ll - s.t / s.l;
+  if (!a.targets) return;
+  const int target = a.targets[row];
+  const bool have = target >= 0 && target < a.vocab;
+  a.logprob[row] = have ? (logit<DT>(a.logits, (size_t)((long long)row * a.stride) + target) - s.m) - ll : NAN;
+  a.rank[row] = have ? before : -1;
+}
+__device__ __forceinline__ void finish_top(const LogprobArgs& a, int row, const SoftSum& s, float ll, int rank, uint64_t key) {
+  a.top_logprobs[(size_t)row * a.top + rank] = (key_value(key) - s.m) - ll;
+  a.top_ids[(size_t)row * a.top + rank] = key_index(key);
+}
+__device__ __forceinline__ float log_sum(const SoftSum& s) { return s.m == -INFINITY ? NAN : logf(s.l); }
+
+template <int DT, int HELD>
 __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const LogprobArgs a) {
+  constexpr int V = DT == Q4D_F32 ? 4 : 8, CH = HELD / V, kPart = kThreads * HELD;
+  constexpr int kCand = HELD * kTop;
+  static_assert(kCand >= kGather, "");
   __shared__ float s_stat[4][3];
   __shared__ int s_before[4];
+  __shared__ uint32_t s_wave[4];
   __shared__ uint64_t s_key[kThreads];
-  __shared__ uint64_t s_cand[kHeld * kTop];
+  __shared__ uint64_t s_cand[kCand];
   __shared__ uint64_t s_bound;
-  __shared__ int s_count;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  __shared__ int s_count, s_more;
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
   const int base = part * kPart;
   const size_t row0 = (size_t)((long long)row * a.stride);
+  const auto index = [&](int c) { return base + (c * kThreads + t) * V; };  // of a thread's chunk
 
-  float x[kHeld];
+  float x[HELD];
+  if (base + kPart <= a.vocab) {
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) {
-    const int at = base + i * kThreads + t;
-    x[i] = at < a.vocab ? logit<DT>(a.logits, row0 + at) : -INFINITY;
+    for (int c = 0; c < CH; ++c) load_logits<DT, V>(a.logits, row0 + index(c), x + c * V);
+  } else {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int at = index(c);
+      if (at + V <= a.vocab) {
+        load_logits<DT, V>(a.logits, row0 + at, x + c * V);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[c * V + e] = at + e < a.vocab ? logit<DT>(a.logits, row0 + at + e) : -INFINITY;
+      }
+    }
   }
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kHeld; ++i) top = fmaxf(top, x[i]);
-  SoftSum s = soft_sum<kHeld>(top, [&](int i) { return x[i]; });
-#pragma unroll
-  for (int m = 32; m; m >>= 1)
-    s = soft_join(s, SoftSum{__shfl_xor(s.m, m), __shfl_xor(s.l, m), __shfl_xor(s.t, m)});
-
-  int before = 0;
+  int target = -1;
+  float goal = 0.f;
   if (a.targets) {
-    const int target = a.targets[row];
-    if (target >= 0 && target < a.vocab) {
-      const uint64_t key = order_key(logit<DT>(a.logits, row0 + target), target);
+    target = a.targets[row];
+    if (target < 0 || target >= a.vocab) target = -1;
+    else goal = logit<DT>(a.logits, row0 + target);
+  }
+  if (t == 0) s_count = s_more = 0;
+
+  // ---- softmax sums --------------------------------------------------------------------------
+  float mine = x[0];
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        const int at = base + i * kThreads + t;
-        before += at < a.vocab && order_key(x[i], at) > key;
+  for (int i = 1; i < HELD; ++i) mine = fmaxf(mine, x[i]);
+  const float top = wave_all<false>(mine);
+  SoftSum s = soft_sum<HELD>(top, [&](int i) { return x[i]; });
+  s.l = wave_all<true>(s.l);
+  s.t = wave_all<true>(s.t);
+
+  // ---- logits before the target ----------------------------------------------------------------
+  int before = 0;
+  if (target >= 0) {
+    if (goal != goal) {  // NaN: all that are not, and the NaN of lower index
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) {
+        const int at = index(i / V) + i % V;
+        before += at < a.vocab && (x[i] == x[i] || at < target);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int first = base + (c * kThreads + 64 * w) * V;  // of the wave's 64 V
+        if (first + 64 * V <= target) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) before += x[c * V + e] >= goal;
+        } else if (first > target) {  // (what lies past the row's end is -Inf, above which no goal lies)
+#pragma unroll
+          for (int e = 0; e < V; ++e) before += x[c * V + e] > goal;
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) before += x[c * V + e] > goal || (x[c * V + e] == goal && index(c) + e < target);
+        }
       }
     }
 #pragma unroll
@@ -104,57 +186,111 @@ __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const LogprobArg
     s_stat[w][2] = s.t;
     s_before[w] = before;
   }
-  const size_t slot = (size_t)row * a.parts + part;
+
+  // ---- the K best ------------------------------------------------------------------------------
+  int count = 0;
   if (a.top) {
-    uint64_t mine = 0;
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const int at = base + i * kThreads + t;
-      const uint64_t k = at < a.vocab ? order_key(x[i], at) : 0;
-      mine = k > mine ? k : mine;
+    const uint32_t u = order_bits(mine);  // (of a thread without a number: of -Inf or NaN, which the keys tell apart)
+    uint32_t bound = 0;
+    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+      const int reach = __popcll(__ballot(u >= (bound | bit)));
+      if (reach >= a.top) bound |= bit;
+      if (reach == a.top) break;
     }
-    s_key[t] = mine;
-    if (t == 0) {
-      s_count = 0;
-      s_bound = 1;  // (fewer than `top` threads have any: all are candidates)
-    }
+    if (lane == 0) s_wave[w] = bound;
     __syncthreads();
-    int ahead = 0;
-    for (int i = 0; i < kThreads; ++i) ahead += s_key[i] > mine;
-    if (mine && ahead == a.top - 1) s_bound = mine;
-    __syncthreads();
-    const uint64_t bound = s_bound;
-    if (mine >= bound) {
+    bound = max(max(s_wave[0], s_wave[1]), max(s_wave[2], s_wave[3]));
+    const float least = key_value((uint64_t)bound << 32);
+    if (least > -INFINITY) {
+      if (mine >= least) {
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        const int at = base + i * kThreads + t;
-        const uint64_t k = at < a.vocab ? order_key(x[i], at) : 0;
-        if (k >= bound) s_cand[atomicAdd(&s_count, 1)] = k;
+        for (int c = 0; c < CH; ++c) {
+          float most = x[c * V];
+#pragma unroll
+          for (int e = 1; e < V; ++e) most = fmaxf(most, x[c * V + e]);
+          if (most >= least) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+              if (x[c * V + e] >= least) {
+                const int at = atomicAdd(&s_count, 1);
+                if (at < kGather) s_cand[at] = order_key(x[c * V + e], index(c) + e);
+              }
+          }
+        }
       }
+      __syncthreads();
+      count = s_count;
     }
-    __syncthreads();
-    const int count = s_count;
-    uint64_t* out = a.best + slot * a.top;
-    for (int c = t; c < count; c += kThreads) {
-      const uint64_t k = s_cand[c];
-      int rank = 0;
-      for (int i = 0; i < count; ++i) rank += s_cand[i] > k;
-      if (rank < a.top) out[rank] = k;
+    if (count == 0 || count > kGather) {
+      // by keys: of each thread's best the K-th best of the block is reached by K logits, and at most
+      // HELD K reach it
+      uint64_t best = 0;
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) {
+        const int at = index(i / V) + i % V;
+        const uint64_t k = at < a.vocab ? order_key(x[i], at) : 0;
+        best = k > best ? k : best;
+      }
+      s_key[t] = best;
+      if (t == 0) s_bound = 1;  // (fewer than K threads have any: all are taken)
+      __syncthreads();
+      int ahead = 0;
+      for (int i = 0; i < kThreads; ++i) ahead += s_key[i] > best;
+      if (best && ahead == a.top - 1) s_bound = best;
+      __syncthreads();
+      const uint64_t floor = s_bound;
+      if (best >= floor) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) {
+          const int at = index(i / V) + i % V;
+          const uint64_t k = at < a.vocab ? order_key(x[i], at) : 0;
+          if (k >= floor) s_cand[atomicAdd(&s_more, 1)] = k;
+        }
+      }
+      __syncthreads();
+      count = s_more;
     }
-    for (int c = count + t; c < a.top; c += kThreads) out[c] = 0;
   }
   __syncthreads();
+  s = SoftSum{s_stat[0][0], s_stat[0][1], s_stat[0][2]};
+#pragma unroll
+  for (int i = 1; i < 4; ++i) s = soft_join(s, SoftSum{s_stat[i][0], s_stat[i][1], s_stat[i][2]});
+  before = s_before[0] + s_before[1] + s_before[2] + s_before[3];
+  const size_t slot = (size_t)row * a.parts + part;
+  const bool whole = a.parts == 1;
+  const float ll = whole ? log_sum(s) : 0.f;
   if (t == 0) {
-    s = SoftSum{s_stat[0][0], s_stat[0][1], s_stat[0][2]};
-    for (int i = 1; i < 4; ++i) s = soft_join(s, SoftSum{s_stat[i][0], s_stat[i][1], s_stat[i][2]});
-    a.stats[slot * 3] = s.m;
-    a.stats[slot * 3 + 1] = s.l;
-    a.stats[slot * 3 + 2] = s.t;
-    a.before[slot] = s_before[0] + s_before[1] + s_before[2] + s_before[3];
+    if (whole) {
+      finish_row<DT>(a, row, s, ll, before);
+    } else {
+      a.stats[slot * 3] = s.m;
+      a.stats[slot * 3 + 1] = s.l;
+      a.stats[slot * 3 + 2] = s.t;
+      a.before[slot] = before;
+    }
   }
+  for (int c = t; c < count; c += kThreads) {
+    const uint64_t k = s_cand[c];
+    int rank = 0;
+    for (int i = 0; i < count; ++i) rank += s_cand[i] > k;
+    if (rank >= a.top) continue;
+    if (whole) finish_top(a, row, s, ll, rank, k);
+    else a.best[slot * a.top + rank] = k;
+  }
+  if (!whole)
+    for (int c = count + t; c < a.top; c += kThreads) a.best[slot * a.top + c] = 0;  // a last part of fewer logits
 }
 
-// A wave a row.
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t k) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) {
+    const uint64_t o = (uint64_t)(uint32_t)__shfl_xor((int)(k >> 32), m) << 32 | (uint32_t)__shfl_xor((int)k, m);
+    k = o > k ? o : k;
+  }
+  return k;
+}
+
+// A wave a row, a part a lane.  The largest of the parts' K-th keys is a bound that K keys reach.
 template <int DT>
 __global__ __launch_bounds__(64) void logprob_join_kernel(const LogprobArgs a) {
   __shared__ uint64_t s_key[kMaxParts * kTop];
@@ -162,39 +298,43 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(const LogprobArgs a) {
   const size_t slot0 = (size_t)row * a.parts;
   SoftSum s = {-INFINITY, 0.f, 0.f};
   int before = 0;
-  for (int p = lane; p < a.parts; p += 64) {
-    const float* at = a.stats + (slot0 + p) * 3;
-    s = soft_join(s, SoftSum{at[0], at[1], at[2]});
-    before += a.before[slot0 + p];
+  uint64_t bound = 0;
+  if (lane < a.parts) {
+    const float* at = a.stats + (slot0 + lane) * 3;
+    s = SoftSum{at[0], at[1], at[2]};
+    before = a.before[slot0 + lane];
+    if (a.top) bound = a.best[(slot0 + lane + 1) * a.top - 1];
   }
+  const float m = wave_max(s.m), ms = m == -INFINITY ? 0.f : m, f = __expf(s.m - ms);
+  const float part = f > 0.f ? f * fmaf(s.m - ms, s.l, s.t) : 0.f;
+  s = SoftSum{m, wave_sum(s.l * f), wave_sum(part)};
 #pragma unroll
-  for (int m = 32; m; m >>= 1) {
-    s = soft_join(s, SoftSum{__shfl_xor(s.m, m), __shfl_xor(s.l, m), __shfl_xor(s.t, m)});
-    before += __shfl_xor(before, m);
+  for (int k = 32; k; k >>= 1) before += __shfl_xor(before, k);
+  const float ll = log_sum(s);
+  if (lane == 0) finish_row<DT>(a, row, s, ll, before);
+  if (!a.top) return;
+  bound = wave_max_key(bound);
+  if (bound == 0) bound = 1;
+  int count = 0;
+  for (int c = lane; c - lane < a.parts * a.top; c += 64) {
+    const uint64_t k = c < a.parts * a.top ? a.best[slot0 * a.top + c] : 0;
+    const uint64_t reach = __ballot(k >= bound);
+    if (k >= bound) s_key[count + __popcll(reach & ((1ULL << lane) - 1))] = k;
+    count += __popcll(reach);
   }
-  const float ll = s.m == -INFINITY ? NAN : logf(s.l);
-  if (lane == 0) {
-    a.entropy[row] = ll - s.t / s.l;
-    if (a.targets) {
-      const int target = a.targets[row];
-      const bool have = target >= 0 && target < a.vocab;
-      a.logprob[row] = have ? (logit<DT>(a.logits, (size_t)((long long)row * a.stride) + target) - s.m) - ll : NAN;
-      a.rank[row] = have ? before : -1;
-    }
-  }
-  const int count = a.parts * a.top;
-  for (int c = lane; c < count; c += 64) s_key[c] = a.best[slot0 * a.top + c];
   __syncthreads();
   for (int c = lane; c < count; c += 64) {
     const uint64_t k = s_key[c];
-    if (!k) continue;
     int rank = 0;
     for (int i = 0; i < count; ++i) rank += s_key[i] > k;
-    if (rank < a.top) {
-      a.top_logprobs[(size_t)row * a.top + rank] = (key_value(k) - s.m) - ll;
-      a.top_ids[(size_t)row * a.top + rank] = key_index(k);
-    }
+    if (rank < a.top) finish_top(a, row, s, ll, rank, k);
   }
+}
+
+// Logits of a thread: few where the parts would not fill the device.
+int held(int rows, int vocab) {
+  const long long few = (vocab + kThreads * kHeldFew - 1) / (kThreads * kHeldFew);
+  return few <= kMaxParts && rows * few <= 2048 ? kHeldFew : kHeldMost;
 }
 
 struct LogprobLayout {
@@ -203,7 +343,8 @@ struct LogprobLayout {
 };
 LogprobLayout layout(int rows, int vocab, int top) {
   LogprobLayout l;
-  l.parts = (vocab + kPart - 1) / kPart;
+  const int part = kThreads * held(rows, vocab);
+  l.parts = (vocab + part - 1) / part;
   const size_t slots = (size_t)rows * l.parts;
   l.before = align_up(slots * 12, 256);
   l.best = align_up(l.before + slots * 4, 256);
@@ -212,14 +353,17 @@ LogprobLayout layout(int rows, int vocab, int top) {
 }
 
 bool logprob_shape(int rows, int vocab, int top) {
+  constexpr int kPart = kThreads * kHeldMost;
   return rows > 0 && vocab > 0 && vocab <= kMaxParts * kPart && top >= 0 && top <= kTop && top <= vocab &&
          (long long)rows * ((vocab + kPart - 1) / kPart) <= (1 << 23);
 }
 
 template <int DT>
 int launch(const LogprobArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL(logprob_part_kernel<DT>, dim3((unsigned)(a.rows * a.parts)), dim3(kThreads), 0, st, a);
-  hipLaunchKernelGGL(logprob_join_kernel<DT>, dim3((unsigned)a.rows), dim3(64), 0, st, a);
+  const dim3 grid((unsigned)(a.rows * a.parts));
+  if (held(a.rows, a.vocab) == kHeldFew) hipLaunchKernelGGL((logprob_part_kernel<DT, kHeldFew>), grid, dim3(kThreads), 0, st, a);
+  else hipLaunchKernelGGL((logprob_part_kernel<DT, kHeldMost>), grid, dim3(kThreads), 0, st, a);
+  if (a.parts > 1) hipLaunchKernelGGL(logprob_join_kernel<DT>, dim3((unsigned)a.rows), dim3(64), 0, st, a);
   return check_launch();
 }
 

@@ -47,7 +47,7 @@ __device__ __forceinline__ SoftSum soft_sum(float m, F z) {
   for (int i = 0; i < N; ++i) {
     const float d = z(i) - ms, e = __expf(d);
     s.l += e;
-    s.t = e > 0.f ? fmaf(d, e, s.t) : s.t;  // (-Inf x 0 counts as 0)
+    s.t = fmaf(fmaxf(d, -1000.f), e, s.t);  // (e is 0 long before; -Inf x 0 would be NaN)
   }
   return s;
 }
