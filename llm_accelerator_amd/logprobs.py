@@ -54,22 +54,23 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     x = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
     if (vocab > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < vocab):
         x = x.contiguous()
-    rows, dev = x.shape[0], logits.device
-    floats = torch.empty((2, *lead), dtype=torch.float32, device=dev)
-    rank = torch.empty(lead, dtype=torch.int32, device=dev) if targets is not None else None
-    top_logprobs = torch.empty((*lead, top), dtype=torch.float32, device=dev)
-    top_ids = torch.empty((*lead, top), dtype=torch.int32, device=dev)
-    logprob = floats[1] if targets is not None else None
+    rows = x.shape[0]
+    # the results lie side by side in one allocation
+    got = x.new_empty(rows * (3 + 2 * top), dtype=torch.float32)
+    logprob, entropy, rank, top_logprobs, top_ids = got.split((rows, rows, rows, rows * top, rows * top))
     if rows:
-        nbytes = int(_lib.load().q4d_token_logprobs_workspace_bytes(rows, vocab, top))
+        nbytes = _lib.load().q4d_token_logprobs_workspace_bytes(rows, vocab, top)
         if nbytes == 0:
             raise _lib.Q4DecError(-11, "q4d_token_logprobs_workspace_bytes")
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws, at, step, have = x.new_empty(nbytes, dtype=torch.uint8), got.data_ptr(), 4 * rows, targets is not None
         call_on(index, "q4d_token_logprobs", x.data_ptr(), _DTYPES[x.dtype], x.stride(0), rows, vocab,
-                None if targets is None else targets.data_ptr(), top, None if logprob is None else logprob.data_ptr(),
-                None if rank is None else rank.data_ptr(), floats.data_ptr(), top_logprobs.data_ptr() if top else None,
-                top_ids.data_ptr() if top else None, ws.data_ptr(), nbytes)
-    return TokenLogprobs(logprob, rank, floats[0], top_logprobs, top_ids)
+                targets.data_ptr() if have else None, top, at if have else None, at + 2 * step if have else None, at + step,
+                at + 3 * step if top else None, at + (3 + top) * step if top else None, ws.data_ptr(), nbytes)
+    if len(lead) != 1:
+        logprob, entropy, rank = logprob.view(lead), entropy.view(lead), rank.view(lead)
+    wide = (*lead, top)
+    return TokenLogprobs(logprob if targets is not None else None, rank.view(torch.int32) if targets is not None else None, entropy,
+                         top_logprobs.view(wide), top_ids.view(torch.int32).view(wide))
 
 
 __all__ = ["TokenLogprobs", "token_logprobs", "MAX_TOP", "MAX_VOCAB"]

@@ -32,6 +32,10 @@ from ._lib import Q4dKVCache, Q4dLayer, Q4dMatrix, Q4dModel
 
 GROUP_SIZE = 64
 
+# torch.cuda.current_device / current_stream without the objects around them (0.2 us a call instead of 1.6)
+_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
+
 
 @dataclass
 class Qwen3Config:
@@ -346,13 +350,13 @@ def current_stream() -> int:
 def call_on(index: int, name: str, *args) -> None:
     """Entry point ``name`` on device ``index`` and that device's current stream; raises on an error code."""
     call = getattr(_lib.load(), name)
-    here = torch._C._cuda_getDevice()
+    here = _device()
     if here == index:
-        rc = call(*args, torch._C._cuda_getCurrentRawStream(here))
+        rc = call(*args, _stream(here))
     else:
         torch.cuda.set_device(index)
         try:
-            rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = call(*args, _stream(index))
         finally:
             torch.cuda.set_device(here)
     if rc:

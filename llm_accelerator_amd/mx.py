@@ -47,12 +47,16 @@ class MXTensor:
         if packed.device != scale.device:
             raise ValueError(f"packed is on {packed.device}, scale on {scale.device}")
         packed, scale = packed.contiguous(), scale.contiguous()
-        self.packed = packed.clone() if packed.data_ptr() % 16 else packed  # the kernels read 16-byte aligned rows
-        self.scale = scale
-        self.shape = (rows, 2 * half)
-        self._desc = Q4dMX(self.packed.data_ptr(), scale.data_ptr(), rows, 2 * half)
+        if packed.data_ptr() % 16:
+            packed = packed.clone()  # the kernels read 16-byte aligned rows
+        self._setup(packed, scale, rows, 2 * half)
+
+    def _setup(self, packed: torch.Tensor, scale: torch.Tensor, rows: int, cols: int) -> "MXTensor":
+        self.packed, self.scale, self.shape = packed, scale, (rows, cols)
+        self._desc = Q4dMX(packed.data_ptr(), scale.data_ptr(), rows, cols)
         self._ref = ctypes.byref(self._desc)
         self._index = packed.get_device()
+        return self
 
     @property
     def device(self) -> torch.device:
@@ -79,7 +83,7 @@ class MXTensor:
         if dtype not in _DTYPES:
             raise ValueError(f"dtype must be fp32, fp16 or bf16, got {dtype}")
         _on_gpu(self)
-        y = torch.empty(self.shape, dtype=dtype, device=self.device)
+        y = self.packed.new_empty(self.shape, dtype=dtype)
         call_on(self._index, "q4d_mx_dequantize", self._ref, y.data_ptr(), _DTYPES[dtype])
         return y
 
@@ -91,6 +95,9 @@ def _on_gpu(t) -> None:
 
 def _rows(x: torch.Tensor, name: str, cols: int | None = None):
     """(x, its rows, elements from row to row) of x [..., cols], copied only if its rows cannot be read in place."""
+    shape = x.shape
+    if len(shape) == 2 and x.is_cuda and shape[1] == (cols or shape[1]) and x.data_ptr() % 16 == 0 and x.is_contiguous():
+        return x, shape[0], shape[1]  # (cols are multiples of 32, so the rows are aligned as the first is)
     if not x.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor (libq4dec has no CPU path)")
     if x.dim() == 0 or (cols is not None and x.shape[-1] != cols):
@@ -120,11 +127,12 @@ def mx_quantize(x: torch.Tensor, rule: str = "floor") -> MXTensor:
     if rows == 0:
         raise ValueError("expected at least one row")
     cols = x.shape[1]
-    packed = torch.empty((rows, cols // 2), dtype=torch.uint8, device=x.device)
-    scale = torch.empty((rows, cols // BLOCK), dtype=torch.uint8, device=x.device)
-    call_on(x.get_device(), "q4d_mx_quantize", x.data_ptr(), _DTYPES[x.dtype], step, rows, cols, _RULES[rule],
-            packed.data_ptr(), scale.data_ptr())
-    return MXTensor(packed, scale)
+    packed = x.new_empty((rows, cols // 2), dtype=torch.uint8)
+    scale = x.new_empty((rows, cols // BLOCK), dtype=torch.uint8)
+    got = MXTensor.__new__(MXTensor)._setup(packed, scale, rows, cols)
+    call_on(got._index, "q4d_mx_quantize", x.data_ptr(), _DTYPES[x.dtype], step, rows, cols, _RULES[rule],
+            got._desc.w, got._desc.s)
+    return got
 
 
 def mx_linear(x: torch.Tensor | MXTensor, weight: MXTensor, out_dtype: torch.dtype | None = None,
@@ -142,29 +150,32 @@ def mx_linear(x: torch.Tensor | MXTensor, weight: MXTensor, out_dtype: torch.dty
         _on_gpu(x)
         if x.shape[1] != cols:
             raise ValueError(f"x has {x.shape[1]} columns, the weights {cols}")
-        index, lead, kind, m = x._index, (x.shape[0],), torch.bfloat16, x.shape[0]
+        index, lead, kind, m = x._index, x.shape[:1], torch.bfloat16, x.shape[0]
     else:
-        if x.dtype not in (torch.float16, torch.bfloat16):
-            raise ValueError(f"x must be fp16, bf16 or an MXTensor, got {x.dtype}")
-        lead, kind = x.shape[:-1], x.dtype
+        kind = x.dtype
+        if kind is not torch.bfloat16 and kind is not torch.float16:
+            raise ValueError(f"x must be fp16, bf16 or an MXTensor, got {kind}")
+        lead = x.shape[:-1]
         x, m, step = _rows(x, "x", cols)
         index = x.get_device()
     if index != weight._index:
         raise ValueError(f"x is on {x.device}, the weights on {weight.device}")
     if out is None:
-        kind = kind if out_dtype is None else out_dtype
-        if kind not in _DTYPES:
-            raise ValueError(f"out_dtype must be fp32, fp16 or bf16, got {kind}")
-        out = torch.empty((*lead, n), dtype=kind, device=weight.device)
-    elif (out.dtype not in _DTYPES or out_dtype not in (None, out.dtype) or out.shape != (*lead, n) or not out.is_contiguous()
-          or out.get_device() != index or out.data_ptr() % 16):
-        raise ValueError(f"out must be contiguous {tuple((*lead, n))} in fp32, fp16 or bf16 (out_dtype) on {weight.device}, 16-byte aligned")
+        y_kind = kind if out_dtype is None else out_dtype
+        if y_kind not in _DTYPES:
+            raise ValueError(f"out_dtype must be fp32, fp16 or bf16, got {y_kind}")
+        out = weight.packed.new_empty((*lead, n), dtype=y_kind)
+    else:
+        y_kind = out.dtype
+        if (y_kind not in _DTYPES or out_dtype not in (None, y_kind) or out.shape != (*lead, n) or not out.is_contiguous()
+                or out.get_device() != index or out.data_ptr() % 16):
+            raise ValueError(f"out must be contiguous {(*lead, n)} in fp32, fp16 or bf16 (out_dtype) on {weight.device}, 16-byte aligned")
     if m == 0:
         return out
     if codes:
-        call_on(index, "q4d_mx_matmul", weight._ref, x._ref, out.data_ptr(), _DTYPES[out.dtype])
+        call_on(index, "q4d_mx_matmul", weight._ref, x._ref, out.data_ptr(), _DTYPES[y_kind])
     else:
-        call_on(index, "q4d_mx_linear", weight._ref, x.data_ptr(), _DTYPES[x.dtype], step, m, out.data_ptr(), _DTYPES[out.dtype])
+        call_on(index, "q4d_mx_linear", weight._ref, x.data_ptr(), _DTYPES[kind], step, m, out.data_ptr(), _DTYPES[y_kind])
     return out
 
 
@@ -192,10 +203,10 @@ def mx_score(hidden: torch.Tensor, weight: MXTensor, targets: torch.Tensor) -> M
     if targets.dtype != torch.int32 or targets.shape != lead or targets.get_device() != index:
         raise ValueError(f"targets must be int32 {tuple(lead)} on {x.device}")
     targets = targets.contiguous()
-    got = torch.empty((3, *lead), dtype=torch.float32, device=x.device)
+    got = x.new_empty((3, *lead), dtype=torch.float32)
     if m:
-        nbytes = int(_lib.load().q4d_mx_score_workspace_bytes(weight.shape[0], m))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        nbytes = _lib.load().q4d_mx_score_workspace_bytes(weight.shape[0], m)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
         base, row = got.data_ptr(), 4 * m
         call_on(index, "q4d_mx_score", weight._ref, x.data_ptr(), _DTYPES[x.dtype], step, m, targets.data_ptr(), base,
                 base + row, base + 2 * row, ws.data_ptr(), nbytes)
