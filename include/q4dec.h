@@ -530,21 +530,29 @@ int q4d_paged_attention(const q4d_pages_t* pages, int32_t layer, const q4d_ragge
  *
  * A row of cols values (a multiple of 32) is cols / 32 blocks of 32 codes and a scale: value =
  * code 2^(scale - 127), scale 255: NaN.  A code is a sign (bit 3) and one of 0, 0.5, 1, 1.5, 2, 3,
- * 4, 6 (bits 2..0); the even column is in the low nibble (as in q4d_matrix_t). */
+ * 4, 6 (bits 2..0); the even column is in the low nibble (as in q4d_matrix_t), so that a block is 16
+ * bytes.  The kernels keep a matrix in the order in which they read it, tiles of 32 rows x 128
+ * columns: w [ceil(rows / 32)][ceil(cols / 128)][4 blocks][32 rows][16 bytes] and
+ * s [..][..][32 rows][4 blocks].  Columns past cols are zeros, rows past rows anything;
+ * q4d_mx_pack and q4d_mx_unpack take and give plain rows. */
 typedef struct q4d_mx {
-  const uint8_t* w;  /* [rows, cols/2], 16-byte aligned */
-  const uint8_t* s;  /* [rows, cols/32] */
-  int32_t rows;
+  uint8_t* w;    /* q4d_mx_code_bytes(rows, cols), 16-byte aligned */
+  uint8_t* s;    /* q4d_mx_scale_bytes(rows, cols), 4-byte aligned */
+  int32_t rows;  /* up to 2^27 tiles */
   int32_t cols;
 } q4d_mx_t;
+size_t q4d_mx_code_bytes(int32_t rows, int32_t cols);   /* 0: not a shape */
+size_t q4d_mx_scale_bytes(int32_t rows, int32_t cols);
+/* Rows of codes packed [rows, cols/2] (4-byte aligned) and scales [rows, cols/32] into t, and back. */
+int q4d_mx_pack(const uint8_t* packed, const uint8_t* scale, const q4d_mx_t* t, void* stream);
+int q4d_mx_unpack(const q4d_mx_t* t, uint8_t* packed, uint8_t* scale, void* stream);
 
 enum { Q4D_MX_FLOOR = 0, Q4D_MX_CEIL = 1 };
-/* Rows of x (fp32, fp16 or bf16, ld elements apart, 16-byte aligned) as codes and scales.  A block's
+/* The rows of x (fp32, fp16 or bf16, ld elements apart, 16-byte aligned) into t.  A block's
  * exponent is floor(log2(largest magnitude)) - 2 (Q4D_MX_FLOOR: magnitudes past 6 become 6) or the
  * smallest with which none passes 6 (Q4D_MX_CEIL), within -127 .. 127; values go to the nearest code,
  * ties to the even one.  A block with Inf or NaN is NaN (codes 0). */
-int q4d_mx_quantize(const void* x, int32_t dtype, int64_t ld, int32_t rows, int32_t cols, int32_t rule, uint8_t* packed,
-                    uint8_t* scale, void* stream);
+int q4d_mx_quantize(const void* x, int32_t dtype, int64_t ld, int32_t rule, const q4d_mx_t* t, void* stream);
 /* y [rows, cols] = the values, in y_dtype (16-byte aligned): exact in fp32 and bf16 but for what lies past
  * their largest number (Inf), rounded once in fp16. */
 int q4d_mx_dequantize(const q4d_mx_t* t, void* y, int32_t y_dtype, void* stream);
@@ -554,7 +562,7 @@ int q4d_mx_dequantize(const q4d_mx_t* t, void* y, int32_t y_dtype, void* stream)
  * though not on the other rows' values. */
 int q4d_mx_linear(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M, void* y, int32_t y_dtype,
                   void* stream);
-/* The same with x [M, cols] in 4 bits too: products and scales are exact, sums fp32. */
+/* The same with x ([M, cols]) in 4 bits too: products and scales are exact, sums fp32. */
 int q4d_mx_matmul(const q4d_mx_t* w, const q4d_mx_t* x, void* y, int32_t y_dtype, void* stream);
 /* How likely token targets[m] is under the output head w ([vocab, hidden]) at hidden row x[m] (as in
  * q4d_mx_linear), with z = W x[m] in fp32 and never in memory: logprob[m] = z[target] - log sum e^z

@@ -211,7 +211,11 @@ SIGNATURES = {
     "q4d_paged_attention_workspace_init": ([_P, c_size_t, _P], c_int32),
     "q4d_paged_attention": ([_PG, c_int32, _RB, _P, ctypes.c_int64, c_int32, c_float, _P, ctypes.c_int64, _P, c_size_t,
                              _P], c_int32),
-    "q4d_mx_quantize": ([_P, c_int32, ctypes.c_int64, c_int32, c_int32, c_int32, _P, _P, _P], c_int32),
+    "q4d_mx_code_bytes": ([c_int32, c_int32], c_size_t),
+    "q4d_mx_scale_bytes": ([c_int32, c_int32], c_size_t),
+    "q4d_mx_pack": ([_P, _P, _MX, _P], c_int32),
+    "q4d_mx_unpack": ([_MX, _P, _P, _P], c_int32),
+    "q4d_mx_quantize": ([_P, c_int32, ctypes.c_int64, c_int32, _MX, _P], c_int32),
     "q4d_mx_dequantize": ([_MX, _P, c_int32, _P], c_int32),
     "q4d_mx_linear": ([_MX, _P, c_int32, ctypes.c_int64, c_int32, _P, c_int32, _P], c_int32),
     "q4d_mx_matmul": ([_MX, _MX, _P, c_int32, _P], c_int32),

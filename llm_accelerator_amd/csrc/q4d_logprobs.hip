@@ -305,9 +305,7 @@ __global__ __launch_bounds__(64) void logprob_join_kernel(const LogprobArgs a) {
     before = a.before[slot0 + lane];
     if (a.top) bound = a.best[(slot0 + lane + 1) * a.top - 1];
   }
-  const float m = wave_max(s.m), ms = m == -INFINITY ? 0.f : m, f = __expf(s.m - ms);
-  const float part = f > 0.f ? f * fmaf(s.m - ms, s.l, s.t) : 0.f;
-  s = SoftSum{m, wave_sum(s.l * f), wave_sum(part)};
+  s = soft_wave(s);
 #pragma unroll
   for (int k = 32; k; k >>= 1) before += __shfl_xor(before, k);
   const float ll = log_sum(s);

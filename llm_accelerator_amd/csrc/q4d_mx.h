@@ -6,19 +6,19 @@
 namespace q4d {
 
 struct MxProduct {
-  const uint8_t* w;   // [N][K / 2] codes, [N][K / 32] scales
+  const uint8_t* w;   // tiles of codes, of scales
   const uint8_t* ws;
-  const void* x;      // 16-bit rows x_stride elements apart, or codes [M][K / 2]
-  const uint8_t* xs;  // scales of the codes
+  const void* x;      // 16-bit rows x_stride elements apart, or tiles of codes
+  const uint8_t* xs;  // ... of their scales
   long long x_stride;
   int M, N, K;
   void* y;  // [M][N]
   int y_dtype;
   // of a score: row m's target (outside [0, N): none), the target's logit, and of each `parts` range of
-  // the N outputs (max, sum of e^(z - max), sum of (z - max) e^(z - max))
+  // the N outputs (max, sum of e^(z - max), sum of (z - max) e^(z - max), 0)
   const int32_t* targets;
-  float* hit;    // [M]
-  float* stats;  // [parts][M][3]
+  float* hit;  // [M]
+  float __attribute__((ext_vector_type(4)))* stats;  // [M][parts]
 };
 
 enum MxKind { MX_X4 = 0, MX_F16 = 1, MX_BF16 = 2 };  // x: codes or 16-bit floats
@@ -28,7 +28,7 @@ int check_mx(const q4d_mx_t* t);
 // Up to 64 rows a block (q4d_mx_rows.hip) and tiles of many rows (q4d_mx_gemm.hip).
 int launch_mx_rows(const MxProduct& p, MxKind kind, hipStream_t st);
 int launch_mx_gemm(const MxProduct& p, MxKind kind, hipStream_t st);
-int mx_gemm_parts(int N);  // ranges of N that a score's blocks leave
+__host__ __device__ inline int mx_gemm_parts(int N) { return (N + 255) / 256; }  // ranges that a score's blocks leave
 int launch_mx_gemm_score(const MxProduct& p, MxKind kind, hipStream_t st);
 
 }  // namespace q4d

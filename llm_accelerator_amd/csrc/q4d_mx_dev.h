@@ -2,6 +2,12 @@
 // sign, 2 exponent bits and 1 mantissa bit (0, 0.5, 1, 1.5, 2, 3, 4, 6) and one scale byte s that
 // stands for 2^(s - 127), 255 for NaN.  Codes lie two a byte, the even column in the low nibble;
 // 16 bytes are one block.
+//
+// In memory a matrix is tiles of 32 rows x 128 columns, those of 32 rows side by side: codes
+// [4 blocks][32 rows][16 bytes], scales [32 rows][4 blocks].  What a wave loads for a matrix
+// instruction, 64 blocks of 16 or 32 rows, is then 1 KB in one or four pieces (row by row it was 32
+// pieces of 32 bytes: 4096 x 8192 x 4096 in 4 bits took 214 us, all of it waiting).  Rows and columns past the
+// matrix's are there: columns as zeros, rows as anything.
 #pragma once
 
 #include <math.h>
@@ -15,6 +21,13 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kMxRows = 32, kMxCols = 128;              // of a tile
+constexpr int kMxTile = kMxRows * kMxCols / 2;          // bytes of its codes
+constexpr int kMxScales = kMxRows * kMxCols / 32;       // ... and of its scales
+
+__host__ __device__ inline int mx_col_tiles(int cols) { return (cols + kMxCols - 1) / kMxCols; }
+__host__ __device__ inline int mx_row_tiles(int rows) { return (rows + kMxRows - 1) / kMxRows; }
 
 // A scale byte as the conversions take it: they read the exponent field alone, 0 as 2^-127 and 255 as NaN.
 __device__ __forceinline__ float mx_scale(uint32_t s) { return __builtin_bit_cast(float, s << 23); }
@@ -56,6 +69,12 @@ __device__ __forceinline__ SoftSum soft_join(SoftSum a, SoftSum b) {
   const float da = a.m - ms, db = b.m - ms, fa = __expf(da), fb = __expf(db);
   return {m, fmaf(a.l, fa, b.l * fb),
           (fa > 0.f ? fa * fmaf(da, a.l, a.t) : 0.f) + (fb > 0.f ? fb * fmaf(db, b.l, b.t) : 0.f)};
+}
+
+// Of the lanes of a wave, in every lane.
+__device__ __forceinline__ SoftSum soft_wave(SoftSum s) {
+  const float m = wave_max(s.m), d = s.m - (m == -INFINITY ? 0.f : m), f = __expf(d);
+  return {m, wave_sum(s.l * f), wave_sum(f > 0.f ? f * fmaf(d, s.l, s.t) : 0.f)};
 }
 
 // Outputs n .. n + 3 of row m, those below N, rounded once to the output's type.

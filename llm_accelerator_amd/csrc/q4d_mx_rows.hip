@@ -1,7 +1,7 @@
 // Products of a few rows with microscaled 4-bit weights (gfx950, wave64): y = x W^T.
 //
 // A block takes 16 weight rows and up to 16 MT rows of x; its waves share K, 128 columns at a time: lane
-// (r, g) loads the 16 bytes of weight row r's block 4 i + g and the 32 values of x's row r there.  The
+// (r, g) loads the 16 bytes of weight row r's block g and the 32 values of x's row r there.  The
 // order of K inside a product is free, so that both operands go to the matrix unit as they were loaded:
 // four 16x16x32 products of 8 columns a lane after the codes are made 16-bit floats, or with x in 4 bits
 // one 16x16x128 product that takes codes and scales as they are.  The waves' sums meet in LDS.
@@ -14,7 +14,6 @@ namespace {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kRowTile = 16;  // weight rows of a block
-constexpr int kStepK = 128;   // columns of a step
 
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -33,41 +32,40 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(const MxProduct a) {
   const int t = threadIdx.x, lane = t & 63, r = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int n0 = blockIdx.x * kRowTile, m0 = blockIdx.y * (16 * MT);
-  const int blocks = a.K / 32, steps = (blocks + 3) / 4;
-  const int n = min(n0 + r, a.N - 1);  // rows past the last repeat it and are not stored
-  const uint8_t* wp = a.w + (size_t)n * (a.K / 2);
-  const uint8_t* sp = a.ws + (size_t)n * blocks;
+  const int blocks = a.K / 32, steps = mx_col_tiles(a.K);
+  const size_t at = (size_t)(n0 / kMxRows) * steps;  // first tile
+  const uint8_t* wp = a.w + at * kMxTile + g * (kMxRows * 16) + (n0 % kMxRows + r) * 16;
+  const uint8_t* sp = a.ws + at * kMxScales + 4 * (n0 % kMxRows + r) + g;
   const u32x4 none = {0u, 0u, 0u, 0u};
 
   f32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
   for (int it = w; it < steps; it += NW) {
-    const int b = 4 * it + g;
-    const bool in = b < blocks;  // past the last block: codes and x of 0
-    const u32x4 wq = in ? *reinterpret_cast<const u32x4*>(wp + 16 * b) : none;
-    const uint32_t ws = in ? sp[b] : 127u;
+    const u32x4 wq = *reinterpret_cast<const u32x4*>(wp + (size_t)it * kMxTile);
+    const uint32_t ws = sp[(size_t)it * kMxScales];
     if constexpr (KIND == MX_X4) {
       u32x4 x[MT];
       uint32_t xs[MT];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const int m = m0 + 16 * i + r;
-        const bool have = in && m < a.M;
-        x[i] = have ? *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.x) + (size_t)m * (a.K / 2) + 16 * b) : none;
-        xs[i] = have ? a.xs[(size_t)m * blocks + b] : 127u;
+        // (16-row halves of tiles that are there: rows past the last go to outputs that are not stored)
+        const int m = min(m0 + 16 * i, (a.M - 1) & ~15);
+        const size_t tile = (size_t)(m / kMxRows) * steps + it;
+        x[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.x) + tile * kMxTile + g * (kMxRows * 16) + (m % kMxRows + r) * 16);
+        xs[i] = a.xs[tile * kMxScales + 4 * (m % kMxRows + r) + g];
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i)
         acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes_operand(wq), codes_operand(x[i]), acc[i], 4, 4, 0,
                                                                   (int)ws, 0, (int)xs[i]);
     } else {
+      const int b = 4 * it + g;
       u32x4 x[MT][4];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const int m = m0 + 16 * i + r;
-        const bool have = in && m < a.M;
+        const bool have = b < blocks && m < a.M;
         const uint16_t* xp = static_cast<const uint16_t*>(a.x) + (have ? m * a.x_stride + 32 * b : 0);
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[i][j] = have ? *reinterpret_cast<const u32x4*>(xp + 8 * j) : none;

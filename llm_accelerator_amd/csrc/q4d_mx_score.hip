@@ -9,33 +9,34 @@ namespace q4d {
 namespace {
 
 struct JoinArgs {
-  const float* stats;  // [parts][M][3]
+  const f32x4* stats;  // [M][parts]
   const float* hit;    // [M]
   const int32_t* targets;
   int parts, M, N;
   float *logprob, *entropy, *best;
 };
 
-// 16 rows a block, 16 threads a row; a thread's parts in order, then the threads', so that a row's sums
-// do not depend on the other rows.
+// A block a row: a thread's parts in order, then the threads'.
 __global__ __launch_bounds__(256) void mx_score_join_kernel(const JoinArgs a) {
-  __shared__ float s_stat[256][3];
-  const int t = threadIdx.x, m = blockIdx.x * 16 + (t & 15);
+  __shared__ float s_stat[4][3];
+  const int t = threadIdx.x, m = blockIdx.x;
+  const f32x4* at = a.stats + (size_t)m * a.parts;
   SoftSum s = {-INFINITY, 0.f, 0.f};
-  if (m < a.M)
-    for (int p = t >> 4; p < a.parts; p += 16) {
-      const float* at = a.stats + ((size_t)p * a.M + m) * 3;
-      s = soft_join(s, SoftSum{at[0], at[1], at[2]});
-    }
-  s_stat[t][0] = s.m;
-  s_stat[t][1] = s.l;
-  s_stat[t][2] = s.t;
-  __syncthreads();
-  if (t >= 16 || m >= a.M) return;
-  for (int i = 1; i < 16; ++i) {
-    const float* at = s_stat[16 * i + t];
-    s = soft_join(s, SoftSum{at[0], at[1], at[2]});
+#pragma unroll 4
+  for (int p = t; p < a.parts; p += 256) {
+    const f32x4 v = at[p];
+    s = soft_join(s, SoftSum{v[0], v[1], v[2]});
   }
+  s = soft_wave(s);
+  if ((t & 63) == 0) {
+    s_stat[t >> 6][0] = s.m;
+    s_stat[t >> 6][1] = s.l;
+    s_stat[t >> 6][2] = s.t;
+  }
+  __syncthreads();
+  if (t) return;
+#pragma unroll
+  for (int i = 1; i < 4; ++i) s = soft_join(s, SoftSum{s_stat[i][0], s_stat[i][1], s_stat[i][2]});
   const float ll = s.m == -INFINITY ? NAN : logf(s.l);
   const int target = a.targets[m];
   a.logprob[m] = target >= 0 && target < a.N ? (a.hit[m] - s.m) - ll : NAN;
@@ -106,7 +107,7 @@ extern "C" int q4d_mx_matmul(const q4d_mx_t* w, const q4d_mx_t* x, void* y, int3
 
 extern "C" size_t q4d_mx_score_workspace_bytes(int32_t rows, int32_t M) {
   if (rows <= 0 || M <= 0) return 0;
-  return hit_bytes(M) + (size_t)mx_gemm_parts(rows) * M * 12;
+  return hit_bytes(M) + (size_t)mx_gemm_parts(rows) * M * sizeof(f32x4);
 }
 
 extern "C" int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M,
@@ -129,10 +130,10 @@ extern "C" int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, i
   p.K = w->cols;
   p.targets = targets;
   p.hit = ws_ptr<float>(ws, 0);
-  p.stats = ws_ptr<float>(ws, hit_bytes(M));
+  p.stats = ws_ptr<f32x4>(ws, hit_bytes(M));
   const int parts = mx_gemm_parts(p.N);
   if ((rc = launch_mx_gemm_score(p, kind_of(x_dtype), st))) return rc;
   const JoinArgs j = {p.stats, p.hit, targets, parts, M, p.N, logprob, entropy, best};
-  hipLaunchKernelGGL(mx_score_join_kernel, dim3((unsigned)((M + 15) / 16)), dim3(256), 0, st, j);
+  hipLaunchKernelGGL(mx_score_join_kernel, dim3((unsigned)M), dim3(256), 0, st, j);
   return check_launch();
 }

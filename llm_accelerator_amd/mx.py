@@ -32,45 +32,90 @@ _DTYPES = {torch.float16: Q4D_F16, torch.bfloat16: Q4D_BF16, torch.float32: Q4D_
 _RULES = {"floor": 0, "ceil": 1}
 
 
+TILE_ROWS, TILE_COLS = 32, 128  # of the order in memory (q4d_mx_t)
+
+
+def _order(rows_bytes: torch.Tensor, width: int) -> torch.Tensor:
+    """[rows, blocks * width] bytes as [row tiles, column tiles, 32 rows, 4 blocks, width], zeros past both ends."""
+    rows, n = rows_bytes.shape[0], rows_bytes.shape[1] // width
+    rt, kt = -(-rows // TILE_ROWS), -(-n // 4)
+    full = rows_bytes.new_zeros((rt * TILE_ROWS, kt * 4, width))
+    full[:rows, :n] = rows_bytes.view(rows, n, width)
+    return full.view(rt, TILE_ROWS, kt, 4, width).transpose(1, 2)
+
+
 class MXTensor:
-    """A matrix of microscaled 4-bit floats: ``packed`` uint8 [rows, cols/2] (the even column in the low
-    nibble) and ``scale`` uint8 [rows, cols/32] (2^(scale - 127); 255: NaN)."""
+    """A matrix of microscaled 4-bit floats, from rows of codes ``packed`` uint8 [rows, cols/2] (the even
+    column in the low nibble) and ``scale`` uint8 [rows, cols/32] (2^(scale - 127); 255: NaN).
+
+    It keeps a copy of its own in the order that the kernels read (``codes`` and ``scales``, tiles of 32
+    rows and 128 columns); :attr:`packed` and :attr:`scale` are the rows again, made at each access."""
 
     def __init__(self, packed: torch.Tensor, scale: torch.Tensor):
         if packed.dtype != torch.uint8 or scale.dtype != torch.uint8:
             raise TypeError("MXTensor needs uint8 packed codes and uint8 scales")
         if packed.dim() != 2 or packed.shape[0] == 0 or packed.shape[1] == 0 or packed.shape[1] % (BLOCK // 2):
             raise ValueError(f"packed must be [rows, cols/2] with cols a multiple of {BLOCK}, got {tuple(packed.shape)}")
-        rows, half = packed.shape
-        if scale.shape != (rows, 2 * half // BLOCK):
+        rows, cols = packed.shape[0], 2 * packed.shape[1]
+        if scale.shape != (rows, cols // BLOCK):
             raise ValueError(f"scale shape {tuple(scale.shape)} does not match packed {tuple(packed.shape)}")
         if packed.device != scale.device:
             raise ValueError(f"packed is on {packed.device}, scale on {scale.device}")
         packed, scale = packed.contiguous(), scale.contiguous()
-        if packed.data_ptr() % 16:
-            packed = packed.clone()  # the kernels read 16-byte aligned rows
-        self._setup(packed, scale, rows, 2 * half)
+        if not packed.is_cuda:
+            self._setup(_order(packed, 16).transpose(2, 3).reshape(-1), _order(scale, 1).reshape(-1), rows, cols)
+            return
+        if packed.data_ptr() % 4:
+            packed = packed.clone()
+        self._new(packed, rows, cols)
+        call_on(self._index, "q4d_mx_pack", packed.data_ptr(), scale.data_ptr(), self._ref)
 
-    def _setup(self, packed: torch.Tensor, scale: torch.Tensor, rows: int, cols: int) -> "MXTensor":
-        self.packed, self.scale, self.shape = packed, scale, (rows, cols)
-        self._desc = Q4dMX(packed.data_ptr(), scale.data_ptr(), rows, cols)
+    def _setup(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int) -> "MXTensor":
+        self.codes, self.scales, self.shape = codes, scales, (rows, cols)
+        self._desc = Q4dMX(codes.data_ptr(), scales.data_ptr(), rows, cols)
         self._ref = ctypes.byref(self._desc)
-        self._index = packed.get_device()
+        self._index = codes.get_device()
         return self
+
+    def _new(self, like: torch.Tensor, rows: int, cols: int) -> "MXTensor":
+        """Memory for rows x cols on the device of ``like``."""
+        tiles = -(-rows // TILE_ROWS) * -(-cols // TILE_COLS)
+        return self._setup(like.new_empty(tiles * 2048, dtype=torch.uint8), like.new_empty(tiles * 128, dtype=torch.uint8), rows, cols)
+
+    def _rows(self) -> tuple[torch.Tensor, torch.Tensor]:
+        rows, cols = self.shape
+        if self._index >= 0:
+            packed = self.codes.new_empty((rows, cols // 2))
+            scale = self.codes.new_empty((rows, cols // BLOCK))
+            call_on(self._index, "q4d_mx_unpack", self._ref, packed.data_ptr(), scale.data_ptr())
+            return packed, scale
+        rt, kt = -(-rows // TILE_ROWS), -(-cols // TILE_COLS)
+        packed = self.codes.view(rt, kt, 4, TILE_ROWS, 16).permute(0, 3, 1, 2, 4).reshape(rt * TILE_ROWS, -1)
+        scale = self.scales.view(rt, kt, TILE_ROWS, 4).permute(0, 2, 1, 3).reshape(rt * TILE_ROWS, -1)
+        return packed[:rows, :cols // 2].contiguous(), scale[:rows, :cols // BLOCK].contiguous()
+
+    @property
+    def packed(self) -> torch.Tensor:
+        return self._rows()[0]
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return self._rows()[1]
 
     @property
     def device(self) -> torch.device:
-        return self.packed.device
+        return self.codes.device
 
     @property
     def nbytes(self) -> int:
-        return self.packed.numel() + self.scale.numel()
+        return self.codes.numel() + self.scales.numel()
 
     def to(self, device) -> "MXTensor":
-        return MXTensor(self.packed.to(device), self.scale.to(device))
+        return MXTensor.__new__(MXTensor)._setup(self.codes.to(device), self.scales.to(device), *self.shape)
 
     def numpy(self) -> tuple[np.ndarray, np.ndarray]:
-        return self.packed.cpu().numpy(), self.scale.cpu().numpy()
+        packed, scale = self._rows()
+        return packed.cpu().numpy(), scale.cpu().numpy()
 
     @classmethod
     def from_numpy(cls, packed: np.ndarray, scale: np.ndarray, device="cpu") -> "MXTensor":
@@ -83,7 +128,7 @@ class MXTensor:
         if dtype not in _DTYPES:
             raise ValueError(f"dtype must be fp32, fp16 or bf16, got {dtype}")
         _on_gpu(self)
-        y = self.packed.new_empty(self.shape, dtype=dtype)
+        y = self.codes.new_empty(self.shape, dtype=dtype)
         call_on(self._index, "q4d_mx_dequantize", self._ref, y.data_ptr(), _DTYPES[dtype])
         return y
 
@@ -127,11 +172,8 @@ def mx_quantize(x: torch.Tensor, rule: str = "floor") -> MXTensor:
     if rows == 0:
         raise ValueError("expected at least one row")
     cols = x.shape[1]
-    packed = x.new_empty((rows, cols // 2), dtype=torch.uint8)
-    scale = x.new_empty((rows, cols // BLOCK), dtype=torch.uint8)
-    got = MXTensor.__new__(MXTensor)._setup(packed, scale, rows, cols)
-    call_on(got._index, "q4d_mx_quantize", x.data_ptr(), _DTYPES[x.dtype], step, rows, cols, _RULES[rule],
-            got._desc.w, got._desc.s)
+    got = MXTensor.__new__(MXTensor)._new(x, rows, cols)
+    call_on(got._index, "q4d_mx_quantize", x.data_ptr(), _DTYPES[x.dtype], step, _RULES[rule], got._ref)
     return got
 
 
@@ -164,7 +206,7 @@ def mx_linear(x: torch.Tensor | MXTensor, weight: MXTensor, out_dtype: torch.dty
         y_kind = kind if out_dtype is None else out_dtype
         if y_kind not in _DTYPES:
             raise ValueError(f"out_dtype must be fp32, fp16 or bf16, got {y_kind}")
-        out = weight.packed.new_empty((*lead, n), dtype=y_kind)
+        out = weight.codes.new_empty((*lead, n), dtype=y_kind)
     else:
         y_kind = out.dtype
         if (y_kind not in _DTYPES or out_dtype not in (None, y_kind) or out.shape != (*lead, n) or not out.is_contiguous()

@@ -106,6 +106,30 @@ def test_every_code_and_scale_comes_back(dev, dtype):
     np.testing.assert_array_equal(got.float().cpu().numpy(), want.float().numpy())
 
 
+@pytest.mark.parametrize("rows,cols", [(1, 32), (5, 96), (33, 160), (70, 288), (1000, 1056)])
+def test_pack_on_the_device_is_the_hosts(dev, rows, cols):
+    p, s = mx_ref.random_mx(np.random.default_rng(cols), rows, cols)
+    host, here = MXTensor.from_numpy(p, s), MXTensor.from_numpy(p, s, device=dev)
+    p2, s2 = here.numpy()
+    assert (p2 == p).all() and (s2 == s).all()
+    back = here.to("cpu")
+    assert all((a == b).all() for a, b in zip(back.numpy(), (p, s)))
+    v = host.to(dev).dequantize().cpu().numpy()
+    np.testing.assert_array_equal(v, mx_ref.values(p, s))
+
+
+def test_pads_are_zeros_whatever_was_there(dev):
+    """Columns past the last, which products read, in memory that held NaN scales."""
+    junk = torch.full((1 << 20,), 255, dtype=torch.uint8, device=dev)
+    del junk
+    x = torch.randn(40, 160, device=dev)
+    got = mx_quantize(x)
+    rows = torch.arange(40, device=dev)
+    sc = got.scales.view(2, 2, 32, 4).permute(0, 2, 1, 3).reshape(64, 8)[rows]
+    codes = got.codes.view(2, 2, 4, 32, 16).permute(0, 3, 1, 2, 4).reshape(64, 8, 16)[rows]
+    assert not sc[:, 5:].any() and not codes[:, 5:].any()
+
+
 def test_a_large_matrix_and_its_last_rows(dev):
     """More groups than the grid has threads in a round."""
     x = torch.randn(40001, 1056, device=dev, dtype=torch.bfloat16)

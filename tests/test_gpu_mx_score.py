@@ -57,8 +57,9 @@ def test_shapes(dev, m, n, k, kind):
 
 def test_one_token_certain(dev):
     """One logit far above the others: entropy near 0, never NaN."""
-    w = MXTensor(torch.zeros(700, 32, dtype=torch.uint8, device=dev), torch.full((700, 2), 127, dtype=torch.uint8, device=dev))
-    w.packed[37, 0] = 7  # 6
+    packed = torch.zeros(700, 32, dtype=torch.uint8, device=dev)
+    packed[37, 0] = 7  # 6
+    w = MXTensor(packed, torch.full((700, 2), 127, dtype=torch.uint8, device=dev))
     x = torch.zeros(3, 64, device=dev, dtype=torch.bfloat16)
     x[1, 0], x[2, 0] = 100.0, -100.0
     t = torch.tensor([37, 37, 37], device=dev, dtype=torch.int32)

@@ -54,14 +54,29 @@ def test_reference_round_trip_of_every_code():
     assert (mx_ref.values(back, s) == v).all()
 
 
+def test_sizes(lib):
+    assert lib.q4d_mx_code_bytes(1, 32) == lib.q4d_mx_code_bytes(32, 128) == 2048 and lib.q4d_mx_scale_bytes(1, 32) == 128
+    assert lib.q4d_mx_code_bytes(33, 160) == 4 * 2048 and lib.q4d_mx_scale_bytes(33, 160) == 4 * 128
+    assert lib.q4d_mx_code_bytes(151936, 1024) == 151936 * 512
+    assert lib.q4d_mx_code_bytes(2 ** 31 - 1, 128) == lib.q4d_mx_code_bytes(32, 2 ** 31 - 32) == 0
+    assert lib.q4d_mx_code_bytes(2 ** 27, 4096) == 2 ** 38 and lib.q4d_mx_code_bytes(2 ** 27, 4128) == 0
+
+
 def test_quantize_refusals(lib):
     def call(x=FAKE, dt=BF16, ld=64, rows=48, cols=64, rule=0, p=FAKE, s=FAKE):
-        return lib.q4d_mx_quantize(x, dt, ld, rows, cols, rule, p, s, None)
-    assert call(x=None) == call(p=None) == call(s=None) == NULL
+        return lib.q4d_mx_quantize(x, dt, ld, rule, mx(rows, cols, p, s), None)
+    assert call(x=None) == call(p=None) == call(s=None) == lib.q4d_mx_quantize(FAKE, BF16, 64, 0, None, None) == NULL
     assert call(dt=3) == DTYPE
     assert call(rows=0) == call(cols=48, ld=48) == call(cols=0) == call(ld=32) == call(rule=2) == call(rule=-1) == SHAPE
-    assert call(rows=2 ** 31 - 1, cols=1024, ld=1024) == SHAPE  # more than 2^32 groups of 8
+    assert call(rows=2 ** 31 - 1, cols=1024, ld=1024) == SHAPE  # more tiles than 32 bits count
     assert call(x=FAKE + 8) == call(p=FAKE + 8) == call(ld=68) == call(dt=F32, ld=66) == ADDR
+
+
+def test_pack_refusals(lib):
+    for call in (lambda p, s, t: lib.q4d_mx_pack(p, s, t, None), lambda p, s, t: lib.q4d_mx_unpack(t, p, s, None)):
+        assert call(None, FAKE, mx()) == call(FAKE, None, mx()) == call(FAKE, FAKE, None) == call(FAKE, FAKE, mx(w=None)) == NULL
+        assert call(FAKE, FAKE, mx(cols=33)) == SHAPE
+        assert call(FAKE + 2, FAKE, mx()) == call(FAKE, FAKE, mx(w=FAKE + 8)) == call(FAKE, FAKE, mx(s=FAKE + 2)) == ADDR
 
 
 def test_dequantize_refusals(lib):
@@ -136,7 +151,7 @@ def test_python_refuses_host_tensors_and_shapes():
     with pytest.raises(ValueError, match="multiple"):
         MXTensor(torch.zeros(4, 8, dtype=torch.uint8), torch.zeros(4, 0, dtype=torch.uint8))
     w = MXTensor(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8))
-    assert w.shape == (4, 64) and w.nbytes == 4 * 34
+    assert w.shape == (4, 64) and w.nbytes == 2048 + 128  # one tile
     for call in (lambda: w.dequantize(), lambda: mx_linear(x.half(), w), lambda: mx_score(x.half(), w, torch.zeros(4, dtype=torch.int32))):
         with pytest.raises(ValueError, match="GPU"):
             call()
@@ -144,8 +159,21 @@ def test_python_refuses_host_tensors_and_shapes():
         mx_linear(x.half(), x)
 
 
-def test_numpy_round_trip():
+@pytest.mark.parametrize("rows,cols", [(1, 32), (5, 96), (32, 128), (33, 160), (70, 288)])
+def test_order_in_memory_and_back(rows, cols):
     rng = np.random.default_rng(0)
-    p, s = mx_ref.random_mx(rng, 5, 96)
-    p2, s2 = MXTensor.from_numpy(p, s).numpy()
+    p, s = mx_ref.random_mx(rng, rows, cols)
+    t = MXTensor.from_numpy(p, s)
+    p2, s2 = t.numpy()
     assert (p == p2).all() and (s == s2).all()
+    codes, scales, kt = t.codes.numpy(), t.scales.numpy(), -(-cols // 128)
+    for row, block in ((0, 0), (rows - 1, cols // 32 - 1), (rows // 2, cols // 64)):
+        tile = row // 32 * kt + block // 4
+        at = tile * 2048 + block % 4 * 512 + row % 32 * 16
+        assert (codes[at:at + 16] == p[row, 16 * block:16 * block + 16]).all()
+        assert scales[tile * 128 + row % 32 * 4 + block % 4] == s[row, block]
+    for row in range(rows):  # columns past the last are zeros
+        for block in range(cols // 32, 4 * kt):
+            tile = row // 32 * kt + block // 4
+            at = tile * 2048 + block % 4 * 512 + row % 32 * 16
+            assert not codes[at:at + 16].any() and scales[tile * 128 + row % 32 * 4 + block % 4] == 0
