@@ -8,6 +8,7 @@
 // columns a lane after the codes are made 16-bit floats, with x in 4 bits one 32x32x64 product that
 // takes codes and scales as they are.
 // The weights are the first operand, so that a lane holds outputs of one row of x.
+#include <float.h>
 #include <math.h>
 
 #include <type_traits>
@@ -22,6 +23,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTileN = 256;
+constexpr float kLog2e = 1.44269504f;
 constexpr int kXcds = 8;
 
 template <bool BF>
@@ -140,8 +142,10 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
   const auto ready = [&]() {
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): this wave's rows of x are there
-    __builtin_amdgcn_s_barrier();        // everybody's are, and the other stage is read
+    // this wave's rows of x are there: lgkmcnt(0) and vmcnt(0), or with x in 4 bits vmcnt(8), the weights'
+    // loads of a stage that follow those of x (of the last stage fewer, after which nothing waits here)
+    __builtin_amdgcn_s_waitcnt(X4 ? 0x0078 : 0x0070);
+    __builtin_amdgcn_s_barrier();  // everybody's are, and the other stage is read
     asm volatile("" ::: "memory");
   };
   if constexpr (X4) {
@@ -203,16 +207,19 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
       for (int k = 0; k < 2; ++k) s[k] = *reinterpret_cast<const uint32_t*>(sp[k] + (size_t)kt * kMxScales + 4 * r);
     };
     u32x4 q[2][2];  // [stage of a tile][weight rows]
-    uint32_t s[2];
+    uint32_t s[2], s_next[2];
     const int last = stages - 1;
     issue_x(0, 0);
     load_q(0, q[0]);
-    load_q(min(1, last), q[1]);
     load_s(0, s);
     const auto take = [&](int st, auto c_) {
       constexpr int C = decltype(c_)::value;
       ready();
-      if (st < last) issue_x(st + 1, C ^ 1);
+      if (st < last) {
+        issue_x(st + 1, C ^ 1);
+        load_q(st + 1, q[C ^ 1]);
+        if (C == 1) load_s((st + 1) / 2, s_next);
+      }
       const char* xt = lds + C * kStageAll + r * 128;
       float f[2];
 #pragma unroll
@@ -229,8 +236,10 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
           for (int k = 0; k < 2; ++k) acc[k][j] = mfma32<KIND == MX_BF16>(wd[k], x, acc[k][j]);
         }
       }
-      load_q(min(st + 2, last), q[C]);
-      if (C == 1) load_s(min(st / 2 + 1, col_tiles - 1), s);
+      if (C == 1) {
+        s[0] = s_next[0];
+        s[1] = s_next[1];
+      }
     };
     for (int st = 0; st < stages; st += 2) {
       take(st, std::integral_constant<int, 0>());
@@ -256,29 +265,48 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
   } else {
     __syncthreads();  // everybody is done with x's tiles
     float* s_stat = reinterpret_cast<float*>(lds);  // [4 waves][32 MT rows][3]
+    const bool part = n0 + kTileN > a.N;            // outputs past the last have the weight 0
+    const bool none = n0 + 64 * w >= a.N;           // ... and are all that the wave has
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       const int m = m0 + 32 * j + r;
-      const int target = m < a.M ? a.targets[m] : -1;
-      const bool mine = target >= n0 + 64 * w && target < n0 + 64 * w + 64;
-      float top = -INFINITY;
+      const int hit = m < a.M ? a.targets[m] - nb : -1;  // 32 i + 8 (e / 4) + e % 4 of the lane's
+      if (__ballot((unsigned)hit < 64u)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (hit == 32 * i + 8 * (e >> 2) + (e & 3) && nb + hit < a.N) a.hit[m] = acc[i][j][e];
+      }
+      if (part) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (nb + 32 * i + 8 * (e >> 2) + (e & 3) >= a.N) acc[i][j][e] = -1e30f;
+      }
+      float top = -FLT_MAX;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, acc[i][j][e]);
+      top = halves<false>(top);
+      float l = 0.f, u = 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int n = nb + 32 * i + 8 * (e >> 2) + (e & 3);
-          if (mine && n == target && n < a.N) a.hit[m] = acc[i][j][e];
-          if (n >= a.N) acc[i][j][e] = -INFINITY;
-          top = fmaxf(top, acc[i][j][e]);
+          const float d = acc[i][j][e] - top, p = __builtin_amdgcn_exp2f(d * kLog2e);
+          l += p;
+          u = fmaf(p, d, u);
         }
-      top = halves<false>(top);
-      const SoftSum s = soft_sum<32>(top, [&](int k) { return acc[k >> 4][j][k & 15]; });
-      const float l = halves<true>(s.l), u = halves<true>(s.t);
+      l = halves<true>(l);
+      u = halves<true>(u);
       if (h == 0) {
         float* at = s_stat + (w * kTileM + 32 * j + r) * 3;
-        at[0] = top;
-        at[1] = l;
-        at[2] = u;
+        at[0] = none ? -INFINITY : top;
+        at[1] = none ? 0.f : l;
+        at[2] = none ? 0.f : u;
       }
     }
     __syncthreads();
