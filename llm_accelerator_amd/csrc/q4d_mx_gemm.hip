@@ -66,11 +66,13 @@ template <MxKind KIND, bool SCORE, int MT>
 __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
   constexpr bool X4 = KIND == MX_X4;
   constexpr int kTileM = 32 * MT;
-  constexpr int kCols = X4 ? 256 : 64;             // columns of a stage
-  constexpr int kStage = kTileM * 128;             // bytes of x's values or codes
-  constexpr int kStageAll = kStage + (X4 ? 1024 : 0);  // ... and scales [MT][2 tiles][32 rows][4]
+  constexpr int kCols = X4 ? 128 : 64;                     // columns of a stage
+  // bytes of a stage: x (16 bits: 128 a row; 4 bits: tiles), weights, their scales and x's, 256 a wave
+  constexpr int kX = kTileM * (X4 ? 64 : 128), kW = 8 * kMxTile * kCols / kMxCols, kS = 1024;
+  constexpr int kStage = kX + kW + kS * (X4 ? 2 : 1), kRing = 3;
+  constexpr int kLoads = X4 ? 8 : 7;                       // DMA instructions of a wave and stage
   static_assert(MT == 4, "a wave moves 32 rows of x");
-  __shared__ __attribute__((aligned(16))) char lds[2 * kStageAll];
+  __shared__ __attribute__((aligned(16))) char lds[kRing * kStage];
   const int t = threadIdx.x, lane = t & 63, r = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int tm = (a.M + kTileM - 1) / kTileM, tiles = gridDim.x;
@@ -80,10 +82,10 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
   const int n0 = tile / tm * kTileN, m0 = tile % tm * kTileM;
   const int col_tiles = mx_col_tiles(a.K), stages = (a.K + kCols - 1) / kCols;
 
-  // ---- x to LDS ----------------------------------------------------------------------------------
+  // ---- to LDS ------------------------------------------------------------------------------------
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
-  // 16 bits: 128 bytes a row, slot s of row i holds the row's 16-byte group s ^ (i / 2 & 7), so that 16 rows'
-  // same group falls on all banks.  4 bits: the tiles as they are.
+  // x in 16 bits: slot s of row i holds the row's 16-byte group s ^ (i / 2 & 7), so that 16 rows' same group
+  // falls on all banks.  Tiles lie as they are.
   const size_t x_row = 2 * (size_t)a.x_stride;
   const char* xb = static_cast<const char*>(a.x) + (X4 ? 0 : m0 * x_row);
   const auto group = [&](int j) { return (lane & 7) ^ ((4 * j + (lane >> 4)) & 7); };
@@ -93,45 +95,43 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
     for (int j = 0; j < 4; ++j) from[j] = (uint32_t)(min(32 * w + 8 * j + (lane >> 3), a.M - 1 - m0) * x_row) + 16 * group(j);
   }
   const size_t x_tile = (size_t)min(m0 / kMxRows + w, (a.M - 1) / kMxRows) * col_tiles;  // this wave's first
-  const auto issue_x = [&](int st, int sg) {
-    const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + sg * kStageAll + 4096 * w);
+  // the wave's two tiles of weight rows (past the last: the last, not stored)
+  const int w_tiles = mx_row_tiles(a.N), wt0 = min(n0 / kMxRows + 2 * w, w_tiles - 1), wt1 = min(wt0 + 1, w_tiles - 1);
+  const uint8_t* const wp0 = a.w + (size_t)wt0 * col_tiles * kMxTile;
+  const uint8_t* const wp1 = a.w + (size_t)wt1 * col_tiles * kMxTile;
+  const uint8_t* const sp = a.ws + (size_t)wt0 * col_tiles * kMxScales;
+  const uint32_t sfrom = 4 * r + h * (wt1 - wt0) * col_tiles * kMxScales;
+  const auto issue = [&](int st, int at) {
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + at);
     if constexpr (X4) {
-      const int second = min(2 * st + 1, col_tiles - 1);  // (past the last: not used)
-      const uint8_t* p0 = static_cast<const uint8_t*>(a.x) + (x_tile + 2 * st) * kMxTile;
-      const uint8_t* p1 = static_cast<const uint8_t*>(a.x) + (x_tile + second) * kMxTile;
-      dma16(p0, 16 * lane, to);
-      dma16(p0, 16 * lane + 1024, to + 1024);
-      dma16(p1, 16 * lane, to + 2048);
-      dma16(p1, 16 * lane + 1024, to + 3072);
-      const uint32_t scales = __builtin_amdgcn_readfirstlane(lds0 + sg * kStageAll + kStage + 256 * w);
-      dma4(a.xs + (x_tile + 2 * st) * kMxScales, 4 * r + h * ((second - 2 * st) * kMxScales), scales);
+      const uint8_t* p = static_cast<const uint8_t*>(a.x) + (x_tile + st) * kMxTile;
+      dma16(p, 16 * lane, to + 2048 * w);
+      dma16(p, 16 * lane + 1024, to + 2048 * w + 1024);
+      dma16(wp0 + (size_t)st * kMxTile, 16 * lane, to + kX + 4096 * w);
+      dma16(wp0 + (size_t)st * kMxTile, 16 * lane + 1024, to + kX + 4096 * w + 1024);
+      dma16(wp1 + (size_t)st * kMxTile, 16 * lane, to + kX + 4096 * w + 2048);
+      dma16(wp1 + (size_t)st * kMxTile, 16 * lane + 1024, to + kX + 4096 * w + 3072);
+      dma4(sp + (size_t)st * kMxScales, sfrom, to + kX + kW + 256 * w);
+      dma4(a.xs + (x_tile + st) * kMxScales, 4 * r, to + kX + kW + kS + 256 * w);
     } else {
       const char* base = xb + (size_t)st * 128;
       const int have = a.K / 8 - 8 * st;  // groups left in the row
       if (have >= 8) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) dma16(base, from[j], to + 1024 * j);
+        for (int j = 0; j < 4; ++j) dma16(base, from[j], to + 4096 * w + 1024 * j);
       } else {  // groups past the row's end are zeros
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           u32x4 v = {0u, 0u, 0u, 0u};
           if (group(j) < have) v = *reinterpret_cast<const u32x4*>(base + from[j]);
-          *reinterpret_cast<u32x4*>(lds + sg * kStageAll + 4096 * w + 1024 * j + 16 * lane) = v;
+          *reinterpret_cast<u32x4*>(lds + at + 4096 * w + 1024 * j + 16 * lane) = v;
         }
       }
+      dma16(wp0 + (size_t)st * (kMxTile / 2), 16 * lane, to + kX + 2048 * w);
+      dma16(wp1 + (size_t)st * (kMxTile / 2), 16 * lane, to + kX + 2048 * w + 1024);
+      dma4(sp + (size_t)(st / 2) * kMxScales, sfrom, to + kX + kW + 256 * w);
     }
   };
-
-  // ---- weights to registers --------------------------------------------------------------------
-  const int w_tiles = mx_row_tiles(a.N);
-  const uint8_t* wp[2];
-  const uint8_t* sp[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const size_t at = (size_t)min(n0 / kMxRows + 2 * w + i, w_tiles - 1) * col_tiles;  // (past the last: not stored)
-    wp[i] = a.w + at * kMxTile;
-    sp[i] = a.ws + at * kMxScales;
-  }
 
   f32x16 acc[2][MT];
 #pragma unroll
@@ -141,110 +141,61 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  const auto ready = [&]() {
-    // this wave's rows of x are there: lgkmcnt(0) and vmcnt(0), or with x in 4 bits vmcnt(8), the weights'
-    // loads of a stage that follow those of x (of the last stage fewer, after which nothing waits here)
-    __builtin_amdgcn_s_waitcnt(X4 ? 0x0078 : 0x0070);
-    __builtin_amdgcn_s_barrier();  // everybody's are, and the other stage is read
+  issue(0, 0);
+  if (stages > 1) issue(1, kStage);
+  int at = 0, ahead = 2 * kStage;  // of this stage in the ring, and of the one after the next
+  for (int st = 0; st < stages; ++st) {
+    // this wave's part of the stage is there (the next stage's loads may be under way), then everybody's,
+    // and the stage before is read
+    if (st + 1 < stages) __builtin_amdgcn_s_waitcnt(0x0070 | kLoads);  // vmcnt(kLoads) lgkmcnt(0)
+    else __builtin_amdgcn_s_waitcnt(0x0070);
+    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-  };
-  if constexpr (X4) {
-    // blocks 2 i + h of a tile, and the tile's scales
-    const auto load_q = [&](int kt, int i, u32x4 (&q)[2]) {
+    if (st + 2 < stages) issue(st + 2, ahead);
+    const char* stage = lds + at;
+    if constexpr (X4) {
+      uint32_t xs[MT], ws[2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) q[k] = *reinterpret_cast<const u32x4*>(wp[k] + (size_t)kt * kMxTile + 1024 * i + 16 * lane);
-    };
-    const auto load_s = [&](int kt, uint32_t (&s)[2]) {
+      for (int j = 0; j < MT; ++j) xs[j] = *reinterpret_cast<const uint32_t*>(stage + kX + kW + kS + 256 * j + 4 * r) >> (8 * h);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) s[k] = *reinterpret_cast<const uint32_t*>(sp[k] + (size_t)kt * kMxScales + 4 * r);
-    };
-    u32x4 q[2][2][2];  // [tile of the stage][step of the tile][weight rows]
-    uint32_t s[2][2];
-    issue_x(0, 0);
+      for (int k = 0; k < 2; ++k) ws[k] = *reinterpret_cast<const uint32_t*>(stage + kX + kW + 256 * w + 128 * k + 4 * r) >> (8 * h);
+      const auto step = [&](auto i_) {
+        constexpr int I = decltype(i_)::value;
+        u32x4 q[2];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int kt = min(c, col_tiles - 1);
-      load_q(kt, 0, q[c][0]);
-      load_q(kt, 1, q[c][1]);
-      load_s(kt, s[c]);
-    }
-    for (int st = 0; st < stages; ++st) {
-      ready();
-      if (st + 1 < stages) issue_x(st + 1, (st + 1) & 1);
-      const char* stage = lds + (st & 1) * kStageAll;
-      const auto tile_of = [&](auto c_) {
-        constexpr int C = decltype(c_)::value;
-        uint32_t xs[MT], ws[2];
+        for (int k = 0; k < 2; ++k) q[k] = *reinterpret_cast<const u32x4*>(stage + kX + 4096 * w + 2048 * k + 1024 * I + 16 * lane);
 #pragma unroll
-        for (int j = 0; j < MT; ++j) xs[j] = *reinterpret_cast<const uint32_t*>(stage + kStage + 256 * j + 128 * C + 4 * r) >> (8 * h);
+        for (int j = 0; j < MT; ++j) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(stage + 2048 * j + 1024 * I + 16 * lane);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) ws[k] = s[C][k] >> (8 * h);
-        const int next = min(2 * st + 2 + C, col_tiles - 1);
-        const auto step = [&](auto i_) {
-          constexpr int I = decltype(i_)::value;
-#pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(stage + 4096 * j + 2048 * C + 1024 * I + 16 * lane);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) acc[k][j] = mfma_codes<I>(q[C][I][k], ws[k], x, xs[j], acc[k][j]);
-          }
-          load_q(next, I, q[C][I]);
-        };
-        step(std::integral_constant<int, 0>());
-        step(std::integral_constant<int, 1>());
-        load_s(next, s[C]);
+          for (int k = 0; k < 2; ++k) acc[k][j] = mfma_codes<I>(q[k], ws[k], x, xs[j], acc[k][j]);
+        }
       };
-      tile_of(std::integral_constant<int, 0>());
-      if (2 * st + 1 < col_tiles) tile_of(std::integral_constant<int, 1>());
-    }
-  } else {
-    const auto load_q = [&](int st, u32x4 (&q)[2]) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) q[k] = *reinterpret_cast<const u32x4*>(wp[k] + (size_t)st * (kMxTile / 2) + 16 * lane);
-    };
-    const auto load_s = [&](int kt, uint32_t (&s)[2]) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) s[k] = *reinterpret_cast<const uint32_t*>(sp[k] + (size_t)kt * kMxScales + 4 * r);
-    };
-    u32x4 q[2][2];  // [stage of a tile][weight rows]
-    uint32_t s[2], s_next[2];
-    const int last = stages - 1;
-    issue_x(0, 0);
-    load_q(0, q[0]);
-    load_s(0, s);
-    const auto take = [&](int st, auto c_) {
-      constexpr int C = decltype(c_)::value;
-      ready();
-      if (st < last) {
-        issue_x(st + 1, C ^ 1);
-        load_q(st + 1, q[C ^ 1]);
-        if (C == 1) load_s((st + 1) / 2, s_next);
-      }
-      const char* xt = lds + C * kStageAll + r * 128;
+      step(std::integral_constant<int, 0>());
+      step(std::integral_constant<int, 1>());
+    } else {
+      u32x4 q[2];
       float f[2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) f[k] = mx_scale(s[k] >> (16 * C + 8 * h) & 255u);
+      for (int k = 0; k < 2; ++k) {
+        q[k] = *reinterpret_cast<const u32x4*>(stage + kX + 2048 * w + 1024 * k + 16 * lane);
+        f[k] = mx_scale(*reinterpret_cast<const uint32_t*>(stage + kX + kW + 256 * w + 128 * k + 4 * r) >> (16 * (st & 1) + 8 * h) & 255u);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         u32x4 wd[2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) wd[k] = mx_dequant8<KIND == MX_BF16>(q[C][k][i], f[k]);
+        for (int k = 0; k < 2; ++k) wd[k] = mx_dequant8<KIND == MX_BF16>(q[k][i], f[k]);
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(xt + 4096 * j + (((4 * h + i) ^ (r >> 1 & 7)) << 4));
+          const u32x4 x = *reinterpret_cast<const u32x4*>(stage + 128 * r + 4096 * j + (((4 * h + i) ^ (r >> 1 & 7)) << 4));
 #pragma unroll
           for (int k = 0; k < 2; ++k) acc[k][j] = mfma32<KIND == MX_BF16>(wd[k], x, acc[k][j]);
         }
       }
-      if (C == 1) {
-        s[0] = s_next[0];
-        s[1] = s_next[1];
-      }
-    };
-    for (int st = 0; st < stages; st += 2) {
-      take(st, std::integral_constant<int, 0>());
-      if (st < last) take(st + 1, std::integral_constant<int, 1>());
     }
+    at = at == 2 * kStage ? 0 : at + kStage;
+    ahead = ahead == 2 * kStage ? 0 : ahead + kStage;
   }
 
   // lane (r, h) holds outputs n0 + 64 w + 32 i + 8 (e / 4) + 4 h + e % 4 of x's row m0 + 32 j + r
