@@ -25,10 +25,14 @@ enum MxKind { MX_X4 = 0, MX_F16 = 1, MX_BF16 = 2 };  // x: codes or 16-bit float
 
 int check_mx(const q4d_mx_t* t);
 
-// Up to 64 rows a block (q4d_mx_rows.hip) and tiles of many rows (q4d_mx_gemm.hip).
+// Few rows (q4d_mx_rows.hip; a score: up to kMxFewRows) and tiles of many (q4d_mx_gemm.hip), and the ranges of N
+// that a score's blocks leave.
+constexpr int kMxFewRows = 64;
 int launch_mx_rows(const MxProduct& p, MxKind kind, hipStream_t st);
+int launch_mx_rows_score(const MxProduct& p, MxKind kind, hipStream_t st);
+int mx_rows_parts(int M, int N);
 int launch_mx_gemm(const MxProduct& p, MxKind kind, hipStream_t st);
-__host__ __device__ inline int mx_gemm_parts(int N) { return (N + 255) / 256; }  // ranges that a score's blocks leave
+__host__ __device__ inline int mx_gemm_parts(int N) { return (int)((N + 255LL) / 256); }
 int launch_mx_gemm_score(const MxProduct& p, MxKind kind, hipStream_t st);
 
 }  // namespace q4d

@@ -1,6 +1,7 @@
-// Products of a few rows with microscaled 4-bit weights (gfx950, wave64): y = x W^T.
+// Products of a few rows with microscaled 4-bit weights (gfx950, wave64): y = x W^T, and the score of
+// given outputs (see q4d_mx_gemm.hip).
 //
-// A block takes 16 weight rows and up to 16 MT rows of x; its waves share K, 128 columns at a time: lane
+// A block takes 16 NT weight rows and 16 MT rows of x; its waves share K, 128 columns at a time: lane
 // (r, g) loads the 16 bytes of weight row r's block g and the 32 values of x's row r there.  The
 // order of K inside a product is free, so that both operands go to the matrix unit as they were loaded:
 // four 16x16x32 products of 8 columns a lane after the codes are made 16-bit floats, or with x in 4 bits
@@ -13,8 +14,6 @@ namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kRowTile = 16;  // weight rows of a block
-
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   if constexpr (BF)
@@ -26,88 +25,163 @@ __device__ __forceinline__ i32x8 codes_operand(u32x4 v) {
   return i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
 }
 
-template <MxKind KIND, int MT, int NW>
+template <MxKind KIND, int MT, int NT>
+struct RowsStep {  // a wave's operands of 128 columns
+  u32x4 w[NT];
+  uint32_t ws[NT];
+  u32x4 x[MT][KIND == MX_X4 ? 1 : 4];
+  uint32_t xs[KIND == MX_X4 ? MT : 1];
+};
+
+template <MxKind KIND, int MT, int NT, int NW, bool SCORE>
 __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(const MxProduct a) {
-  __shared__ f32x4 part[NW][MT][64];
+  __shared__ f32x4 part[NW][NT][MT][64];
   const int t = threadIdx.x, lane = t & 63, r = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int n0 = blockIdx.x * kRowTile, m0 = blockIdx.y * (16 * MT);
-  const int blocks = a.K / 32, steps = mx_col_tiles(a.K);
-  const size_t at = (size_t)(n0 / kMxRows) * steps;  // first tile
-  const uint8_t* wp = a.w + at * kMxTile + g * (kMxRows * 16) + (n0 % kMxRows + r) * 16;
-  const uint8_t* sp = a.ws + at * kMxScales + 4 * (n0 % kMxRows + r) + g;
-  const u32x4 none = {0u, 0u, 0u, 0u};
-
-  f32x4 acc[MT];
+  const int n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT);
+  const int blocks = a.K / 32, steps = mx_col_tiles(a.K), row_tiles = mx_row_tiles(a.N);
+  const auto load = [&](int it, RowsStep<KIND, MT, NT>& s) {
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int it = w; it < steps; it += NW) {
-    const u32x4 wq = *reinterpret_cast<const u32x4*>(wp + (size_t)it * kMxTile);
-    const uint32_t ws = sp[(size_t)it * kMxScales];
+    for (int k = 0; k < NT; ++k) {
+      // (16-row halves of tiles that are there: outputs past the last are not stored)
+      const int half = min(n0 / 16 + k, 2 * row_tiles - 1), row = 16 * (half & 1) + r;
+      const size_t tile = (size_t)(half >> 1) * steps + it;
+      s.w[k] = *reinterpret_cast<const u32x4*>(a.w + tile * kMxTile + g * (kMxRows * 16) + row * 16);
+      s.ws[k] = a.ws[tile * kMxScales + 4 * row + g];
+    }
     if constexpr (KIND == MX_X4) {
-      u32x4 x[MT];
-      uint32_t xs[MT];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        // (16-row halves of tiles that are there: rows past the last go to outputs that are not stored)
         const int m = min(m0 + 16 * i, (a.M - 1) & ~15);
         const size_t tile = (size_t)(m / kMxRows) * steps + it;
-        x[i] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.x) + tile * kMxTile + g * (kMxRows * 16) + (m % kMxRows + r) * 16);
-        xs[i] = a.xs[tile * kMxScales + 4 * (m % kMxRows + r) + g];
+        s.x[i][0] = *reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(a.x) + tile * kMxTile + g * (kMxRows * 16) + (m % kMxRows + r) * 16);
+        s.xs[i] = a.xs[tile * kMxScales + 4 * (m % kMxRows + r) + g];
       }
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes_operand(wq), codes_operand(x[i]), acc[i], 4, 4, 0,
-                                                                  (int)ws, 0, (int)xs[i]);
     } else {
       const int b = 4 * it + g;
-      u32x4 x[MT][4];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const int m = m0 + 16 * i + r;
-        const bool have = b < blocks && m < a.M;
-        const uint16_t* xp = static_cast<const uint16_t*>(a.x) + (have ? m * a.x_stride + 32 * b : 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[i][j] = have ? *reinterpret_cast<const u32x4*>(xp + 8 * j) : none;
-      }
-      const float f = mx_scale(ws);
+        for (int j = 0; j < 4; ++j) s.x[i][j] = u32x4{0u, 0u, 0u, 0u};
+        if (b < blocks && m < a.M) {
+          const uint16_t* p = static_cast<const uint16_t*>(a.x) + m * a.x_stride + 32 * b;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u32x4 v = mx_dequant8<KIND == MX_BF16>(wq[j], f);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i] = mfma16<KIND == MX_BF16>(v, x[i][j], acc[i]);
+          for (int j = 0; j < 4; ++j) s.x[i][j] = *reinterpret_cast<const u32x4*>(p + 8 * j);
+        }
       }
     }
+  };
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int k = 0; k < NT; ++k)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[k][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const auto take = [&](const RowsStep<KIND, MT, NT>& s) {
+    if constexpr (KIND == MX_X4) {
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          acc[k][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(codes_operand(s.w[k]), codes_operand(s.x[i][0]), acc[k][i],
+                                                                       4, 4, 0, (int)s.ws[k], 0, (int)s.xs[i]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        const float f = mx_scale(s.ws[k]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u32x4 v = mx_dequant8<KIND == MX_BF16>(s.w[k][j], f);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) acc[k][i] = mfma16<KIND == MX_BF16>(v, s.x[i][j], acc[k][i]);
+        }
+      }
+    }
+  };
+  // two steps' loads in flight
+  for (int it = w; it < steps; it += 2 * NW) {
+    RowsStep<KIND, MT, NT> s0, s1;
+    load(it, s0);
+    if (it + NW < steps) load(it + NW, s1);
+    take(s0);
+    if (it + NW < steps) take(s1);
   }
 #pragma unroll
-  for (int i = 0; i < MT; ++i) part[w][i][lane] = acc[i];
+  for (int k = 0; k < NT; ++k)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) part[w][k][i][lane] = acc[k][i];
   __syncthreads();
-  // lane (r, g) of row tile i: outputs 4 g .. + 3 of x's row 16 i + r
-  for (int i = w; i < MT; i += NW) {
-    f32x4 s = part[0][i][lane];
+  // lane (r, g) of row tiles (k, i): outputs 16 k + 4 g .. + 3 of x's row 16 i + r
+  const auto sum = [&](int k, int i) {
+    f32x4 s = part[0][k][i][lane];
 #pragma unroll
-    for (int k = 1; k < NW; ++k) {
-      const f32x4 v = part[k][i][lane];
+    for (int v = 1; v < NW; ++v)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] += v[e];
+      for (int e = 0; e < 4; ++e) s[e] += part[v][k][i][lane][e];
+    return s;
+  };
+  if constexpr (!SCORE) {
+    for (int c = w; c < NT * MT; c += NW) {
+      const int k = c / MT, i = c - k * MT, m = m0 + 16 * i + r, n = n0 + 16 * k + 4 * g;
+      const f32x4 s = sum(k, i);
+      if (m < a.M && n < a.N) store_out4(a, m, n, s);
     }
-    const int m = m0 + 16 * i + r, at = n0 + 4 * g;
-    if (m < a.M) store_out4(a, m, at, s);
+  } else {
+    for (int i = w; i < MT; i += NW) {
+      const int m = m0 + 16 * i + r, hit = m < a.M ? a.targets[m] - n0 - 4 * g : -1;  // 16 k + e of the lane's
+      float z[4 * NT], top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        const f32x4 s = sum(k, i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool have = n0 + 16 * k + 4 * g + e < a.N;
+          if (have && hit == 16 * k + e) a.hit[m] = s[e];
+          z[4 * k + e] = have ? s[e] : -INFINITY;
+          top = fmaxf(top, z[4 * k + e]);
+        }
+      }
+      SoftSum s = soft_sum<4 * NT>(top, [&](int c) { return z[c]; });
+#pragma unroll
+      for (int v = 16; v <= 32; v *= 2) s = soft_join(s, SoftSum{__shfl_xor(s.m, v), __shfl_xor(s.l, v), __shfl_xor(s.t, v)});
+      if (g == 0 && m < a.M) a.stats[(size_t)m * gridDim.x + blockIdx.x] = f32x4{s.m, s.l, s.t, 0.f};
+    }
   }
 }
 
+template <MxKind KIND, int MT, int NT, int NW>
+int launch(const MxProduct& p, hipStream_t st) {
+  const dim3 grid((unsigned)((p.N + 16LL * NT - 1) / (16 * NT)), (unsigned)((p.M + 16 * MT - 1) / (16 * MT)));
+  if (grid.y > 65535u) return Q4D_ERR_SHAPE;
+  hipLaunchKernelGGL((mx_rows_kernel<KIND, MT, NT, NW, false>), grid, dim3(64 * NW), 0, st, p);
+  return check_launch();
+}
 template <MxKind KIND, int MT>
 int launch(const MxProduct& p, hipStream_t st) {
-  const dim3 grid((unsigned)((p.N + kRowTile - 1) / kRowTile), (unsigned)((p.M + 16 * MT - 1) / (16 * MT)));
-  if (grid.y > 65535u) return Q4D_ERR_SHAPE;
-  hipLaunchKernelGGL((mx_rows_kernel<KIND, MT, 4>), grid, dim3(256), 0, st, p);
-  return check_launch();
+  // Many weight rows: four or two tiles of them share what is loaded of x.
+  if (p.N >= 32768) return launch<KIND, MT, MT == 4 ? 2 : 4, 4>(p, st);
+  return p.K > 1024 ? launch<KIND, MT, 1, 8>(p, st) : launch<KIND, MT, 1, 4>(p, st);
 }
 template <MxKind KIND>
 int launch(const MxProduct& p, hipStream_t st) {
-  if (p.M <= 16) return launch<KIND, 1>(p, st);
-  if (p.M <= 32) return launch<KIND, 2>(p, st);
+  // the fewest rows a block that leave no more blocks than two a CU
+  const long long tiles = (p.N + 15LL) / 16, most = 2LL * device_cus();
+  if (p.M <= 16 || tiles * ((p.M + 15) / 16) <= most) return launch<KIND, 1>(p, st);
+  if (p.M <= 32 || tiles * ((p.M + 31) / 32) <= most) return launch<KIND, 2>(p, st);
   return launch<KIND, 4>(p, st);
+}
+
+template <MxKind KIND, int MT, int NT>
+int launch_score(const MxProduct& p, hipStream_t st) {
+  const dim3 grid((unsigned)((p.N + 16LL * NT - 1) / (16 * NT)));
+  hipLaunchKernelGGL((mx_rows_kernel<KIND, MT, NT, 4, true>), grid, dim3(256), 0, st, p);
+  return check_launch();
+}
+template <MxKind KIND>
+int launch_score(const MxProduct& p, hipStream_t st) {
+  if (p.M <= 16) return launch_score<KIND, 1, 4>(p, st);
+  if (p.M <= 32) return launch_score<KIND, 2, 4>(p, st);
+  return launch_score<KIND, 4, 2>(p, st);
 }
 
 }  // namespace
@@ -116,5 +190,9 @@ int launch_mx_rows(const MxProduct& p, MxKind kind, hipStream_t st) {
   if (kind == MX_X4) return launch<MX_X4>(p, st);
   return kind == MX_BF16 ? launch<MX_BF16>(p, st) : launch<MX_F16>(p, st);
 }
+int launch_mx_rows_score(const MxProduct& p, MxKind kind, hipStream_t st) {
+  return kind == MX_BF16 ? launch_score<MX_BF16>(p, st) : launch_score<MX_F16>(p, st);
+}
+int mx_rows_parts(int M, int N) { return (int)((N + (M <= 32 ? 63LL : 31LL)) / (M <= 32 ? 64 : 32)); }
 
 }  // namespace q4d

@@ -44,9 +44,6 @@ __global__ __launch_bounds__(256) void mx_score_join_kernel(const JoinArgs a) {
   a.best[m] = -ll;
 }
 
-// Batches of up to this many rows take the kernel of few rows.
-constexpr int kFewRows = 64;
-
 int check_x(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M) {
   if (const int rc = check_mx(w)) return rc;
   if (!x) return Q4D_ERR_NULL;
@@ -60,11 +57,12 @@ int check_y(const void* y, int32_t y_dtype) {
   return aligned(y, 16) ? Q4D_OK : Q4D_ERR_BAD_ADDR;
 }
 int product(const MxProduct& p, MxKind kind, hipStream_t st) {
-  return p.M <= kFewRows ? launch_mx_rows(p, kind, st) : launch_mx_gemm(p, kind, st);
+  return p.M <= kMxFewRows ? launch_mx_rows(p, kind, st) : launch_mx_gemm(p, kind, st);
 }
 MxKind kind_of(int32_t x_dtype) { return x_dtype == Q4D_BF16 ? MX_BF16 : MX_F16; }
 
 size_t hit_bytes(int M) { return align_up((size_t)M * 4, 256); }
+int score_parts(int M, int N) { return M <= kMxFewRows ? mx_rows_parts(M, N) : mx_gemm_parts(N); }
 
 }  // namespace
 }  // namespace q4d
@@ -107,7 +105,7 @@ extern "C" int q4d_mx_matmul(const q4d_mx_t* w, const q4d_mx_t* x, void* y, int3
 
 extern "C" size_t q4d_mx_score_workspace_bytes(int32_t rows, int32_t M) {
   if (rows <= 0 || M <= 0) return 0;
-  return hit_bytes(M) + (size_t)mx_gemm_parts(rows) * M * sizeof(f32x4);
+  return hit_bytes(M) + (size_t)score_parts(M, rows) * M * sizeof(f32x4);
 }
 
 extern "C" int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M,
@@ -131,8 +129,8 @@ extern "C" int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, i
   p.targets = targets;
   p.hit = ws_ptr<float>(ws, 0);
   p.stats = ws_ptr<f32x4>(ws, hit_bytes(M));
-  const int parts = mx_gemm_parts(p.N);
-  if ((rc = launch_mx_gemm_score(p, kind_of(x_dtype), st))) return rc;
+  const int parts = score_parts(M, p.N);
+  if ((rc = M <= kMxFewRows ? launch_mx_rows_score(p, kind_of(x_dtype), st) : launch_mx_gemm_score(p, kind_of(x_dtype), st))) return rc;
   const JoinArgs j = {p.stats, p.hit, targets, parts, M, p.N, logprob, entropy, best};
   hipLaunchKernelGGL(mx_score_join_kernel, dim3((unsigned)M), dim3(256), 0, st, j);
   return check_launch();
