@@ -1,14 +1,14 @@
 // Log probabilities of given tokens, ranks, entropy and the most likely alternatives out of logits
 // (gfx950, wave64), in one pass over them.
 //
-// A row is cut into parts of 256 x HELD logits; a block holds a part in registers, HELD logits a thread, and
-// leaves the part's softmax sums, how many of its logits come before the target, and its K best.  A row
+// A row is cut into parts of 64 W x HELD logits; a block of W waves holds a part in registers, HELD logits a
+// thread, and leaves the part's softmax sums, how many of its logits come before the target, and its K best.  A row
 // of one part is finished there; else a second kernel joins a row's parts, a wave a row.
 //
-// The K best: in each wave the K-th largest of the lanes' own maxima is a bound that K logits reach, found
-// bit by bit with ballots; the few logits of the part that reach the largest such bound are gathered in
-// LDS and ordered by counting.  Where they are too many (equal logits, masks) or NaN matters the bound
-// is found again among keys of value and index, which no two logits share.
+// The K best: of the lanes' own maxima in a wave the K-th largest, found bit by bit with ballots, is reached by
+// K logits, and so is the smallest of the waves' K/W-th largest; the larger of such bounds serves.  The
+// few logits that reach it are gathered in LDS and ordered by counting.  Where they are too many (equal logits, masks) or NaN matters the bound is found again
+// among keys of value and index, which no two logits share.  The parts' lists are joined the same way.
 //
 // Logits are ordered by value, then by index, the lower first; NaN comes last, after -Inf.
 #include <math.h>
@@ -19,9 +19,9 @@
 namespace q4d {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kHeldMost = 64;                 // logits of a thread
-constexpr int kHeldFew = 16;                  // ... where there are few parts
+constexpr int kJoinThreads = 256;
+constexpr int kHeldMost = 64;                 // logits of a thread, kHeldFew where there are few parts or short rows
+constexpr int kHeldFew = 16;
 constexpr int kTop = 32;                      // alternatives at most
 constexpr int kMaxParts = 64;                 // of a row: vocabularies of up to 2^20
 constexpr int kGather = 256;                  // logits that are ordered without a second bound
@@ -81,8 +81,20 @@ __device__ __forceinline__ void load_logits(const void* p, size_t i, float* x) {
     }
   }
 }
-template <bool SUM>
-__device__ __forceinline__ float wave_all(float v) { return SUM ? wave_sum(v) : wave_max(v); }
+// A number that at least n of the lanes' u reach, and not many more: their n-th largest but for lower bits
+// that do not tell them apart.
+__device__ __forceinline__ uint32_t wave_reach(uint32_t u, int n) {
+  uint32_t bound = 0;
+  for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+    const int reach = __popcll(__ballot(u >= (bound | bit)));
+    if (reach >= n) bound |= bit;
+    if (reach == n) break;
+  }
+  return bound;
+}
+
+// Sum of a count of up to 2^8 a lane: exact in fp32.
+__device__ __forceinline__ int wave_count(int c) { return (int)wave_all<true>((float)c); }
 
 // What a row's outputs are once its sums are whole.
 template <int DT>
@@ -100,14 +112,15 @@ __device__ __forceinline__ void finish_top(const LogprobArgs& a, int row, const 
 }
 __device__ __forceinline__ float log_sum(const SoftSum& s) { return s.m == -INFINITY ? NAN : logf(s.l); }
 
-template <int DT, int HELD>
-__global__ __launch_bounds__(kThreads) void logprob_part_kernel(const LogprobArgs a) {
+template <int DT, int HELD, int W>
+__global__ __launch_bounds__(64 * W) void logprob_part_kernel(const LogprobArgs a) {
+  constexpr int kThreads = 64 * W;
   constexpr int V = DT == Q4D_F32 ? 4 : 8, CH = HELD / V, kPart = kThreads * HELD;
   constexpr int kCand = HELD * kTop;
   static_assert(kCand >= kGather, "");
-  __shared__ float s_stat[4][3];
-  __shared__ int s_before[4];
-  __shared__ uint32_t s_wave[4];
+  __shared__ float s_stat[W][3];
+  __shared__ int s_before[W];
+  __shared__ uint32_t s_wave[2][W];
   __shared__ uint64_t s_key[kThreads];
   __shared__ uint64_t s_cand[kCand];
   __shared__ uint64_t s_bound;
@@ -117,6 +130,17 @@ __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const LogprobArg
   const int base = part * kPart;
   const size_t row0 = (size_t)((long long)row * a.stride);
   const auto index = [&](int c) { return base + (c * kThreads + t) * V; };  // of a thread's chunk
+  // Chunk c again from memory, for what is seldom needed: kept in registers, its masks and keys were spilled.
+  const auto again = [&](int c, float (&v)[V]) {
+    const int at = index(c);
+    if (at + V <= a.vocab) {
+      load_logits<DT, V>(a.logits, row0 + at, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = at + e < a.vocab ? logit<DT>(a.logits, row0 + at + e) : -INFINITY;
+    }
+  };
+  const auto key_of = [&](const float (&v)[V], int c, int e) { return index(c) + e < a.vocab ? order_key(v[e], index(c) + e) : 0; };
 
   float x[HELD];
   if (base + kPart <= a.vocab) {
@@ -144,41 +168,51 @@ __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const LogprobArg
   if (t == 0) s_count = s_more = 0;
 
   // ---- softmax sums --------------------------------------------------------------------------
-  float mine = x[0];
+  float most[CH], mine = -INFINITY;  // of the chunks, of the thread
 #pragma unroll
-  for (int i = 1; i < HELD; ++i) mine = fmaxf(mine, x[i]);
+  for (int c = 0; c < CH; ++c) {
+    most[c] = x[c * V];
+#pragma unroll
+    for (int e = 1; e < V; ++e) most[c] = fmaxf(most[c], x[c * V + e]);
+    mine = fmaxf(mine, most[c]);
+  }
   const float top = wave_all<false>(mine);
   SoftSum s = soft_sum<HELD>(top, [&](int i) { return x[i]; });
   s.l = wave_all<true>(s.l);
   s.t = wave_all<true>(s.t);
 
   // ---- logits before the target ----------------------------------------------------------------
+  // (of the wave: a comparison's lanes are counted by the scalar unit)
   int before = 0;
   if (target >= 0) {
     if (goal != goal) {  // NaN: all that are not, and the NaN of lower index
+#pragma unroll 1
+      for (int c = 0; c < CH; ++c) {
+        float v[V];
+        again(c, v);
 #pragma unroll
-      for (int i = 0; i < HELD; ++i) {
-        const int at = index(i / V) + i % V;
-        before += at < a.vocab && (x[i] == x[i] || at < target);
+        for (int e = 0; e < V; ++e) before += __popcll(__ballot(index(c) + e < a.vocab && (v[e] == v[e] || index(c) + e < target)));
       }
     } else {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        const int first = base + (c * kThreads + 64 * w) * V;  // of the wave's 64 V
-        if (first + 64 * V <= target) {
+        const int last = base + (c * kThreads + 64 * w + 64) * V;  // of the wave's 64 V
+        if (last <= target) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) before += x[c * V + e] >= goal;
-        } else if (first > target) {  // (what lies past the row's end is -Inf, above which no goal lies)
+          for (int e = 0; e < V; ++e) before += __popcll(__ballot(x[c * V + e] >= goal));
+        } else {  // (what lies past the row's end is -Inf, above which no goal lies)
 #pragma unroll
-          for (int e = 0; e < V; ++e) before += x[c * V + e] > goal;
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) before += x[c * V + e] > goal || (x[c * V + e] == goal && index(c) + e < target);
+          for (int e = 0; e < V; ++e) before += __popcll(__ballot(x[c * V + e] > goal));
         }
       }
-    }
+      const int c = (target - base) / (kThreads * V);  // the target's own: equal ones of lower index
+      if (target >= base && target - base < kPart && (target - base) / (64 * V) % W == w) {
+        float v[V];
+        again(c, v);
 #pragma unroll
-    for (int m = 32; m; m >>= 1) before += __shfl_xor(before, m);
+        for (int e = 0; e < V; ++e) before += __popcll(__ballot(v[e] == goal && index(c) + e < target));
+      }
+    }
   }
   if (lane == 0) {
     s_stat[w][0] = s.m;
@@ -190,25 +224,33 @@ __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const LogprobArg
   // ---- the K best ------------------------------------------------------------------------------
   int count = 0;
   if (a.top) {
-    const uint32_t u = order_bits(mine);  // (of a thread without a number: of -Inf or NaN, which the keys tell apart)
-    uint32_t bound = 0;
-    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-      const int reach = __popcll(__ballot(u >= (bound | bit)));
-      if (reach >= a.top) bound |= bit;
-      if (reach == a.top) break;
+    // (a thread without a number has the bits of -Inf or NaN, which the keys tell apart)
+    const uint32_t u = order_bits(mine);
+    uint32_t bound = wave_reach(u, a.top);
+    if constexpr (W > 1) {
+      // (the second for more than a few, of which one wave's K best are not the part's)
+      const uint32_t share = a.top >= W ? wave_reach(u, (a.top + W - 1) / W) : 0;
+      if (lane == 0) {
+        s_wave[0][w] = bound;
+        s_wave[1][w] = share;
+      }
+      __syncthreads();
+      uint32_t least = s_wave[1][0];
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        bound = max(bound, s_wave[0][i]);
+        least = min(least, s_wave[1][i]);
+      }
+      bound = max(bound, least);
+    } else {
+      __syncthreads();  // (s_count is set)
     }
-    if (lane == 0) s_wave[w] = bound;
-    __syncthreads();
-    bound = max(max(s_wave[0], s_wave[1]), max(s_wave[2], s_wave[3]));
     const float least = key_value((uint64_t)bound << 32);
     if (least > -INFINITY) {
       if (mine >= least) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          float most = x[c * V];
-#pragma unroll
-          for (int e = 1; e < V; ++e) most = fmaxf(most, x[c * V + e]);
-          if (most >= least) {
+          if (most[c] >= least) {
 #pragma unroll
             for (int e = 0; e < V; ++e)
               if (x[c * V + e] >= least) {
@@ -225,11 +267,15 @@ __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const LogprobArg
       // by keys: of each thread's best the K-th best of the block is reached by K logits, and at most
       // HELD K reach it
       uint64_t best = 0;
+#pragma unroll 1
+      for (int c = 0; c < CH; ++c) {
+        float v[V];
+        again(c, v);
 #pragma unroll
-      for (int i = 0; i < HELD; ++i) {
-        const int at = index(i / V) + i % V;
-        const uint64_t k = at < a.vocab ? order_key(x[i], at) : 0;
-        best = k > best ? k : best;
+        for (int e = 0; e < V; ++e) {
+          const uint64_t k = key_of(v, c, e);
+          best = k > best ? k : best;
+        }
       }
       s_key[t] = best;
       if (t == 0) s_bound = 1;  // (fewer than K threads have any: all are taken)
@@ -240,11 +286,15 @@ __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const LogprobArg
       __syncthreads();
       const uint64_t floor = s_bound;
       if (best >= floor) {
+#pragma unroll 1
+        for (int c = 0; c < CH; ++c) {
+          float v[V];
+          again(c, v);
 #pragma unroll
-        for (int i = 0; i < HELD; ++i) {
-          const int at = index(i / V) + i % V;
-          const uint64_t k = at < a.vocab ? order_key(x[i], at) : 0;
-          if (k >= floor) s_cand[atomicAdd(&s_more, 1)] = k;
+          for (int e = 0; e < V; ++e) {
+            const uint64_t k = key_of(v, c, e);
+            if (k >= floor) s_cand[atomicAdd(&s_more, 1)] = k;
+          }
         }
       }
       __syncthreads();
@@ -254,8 +304,10 @@ __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const LogprobArg
   __syncthreads();
   s = SoftSum{s_stat[0][0], s_stat[0][1], s_stat[0][2]};
 #pragma unroll
-  for (int i = 1; i < 4; ++i) s = soft_join(s, SoftSum{s_stat[i][0], s_stat[i][1], s_stat[i][2]});
-  before = s_before[0] + s_before[1] + s_before[2] + s_before[3];
+  for (int i = 1; i < W; ++i) s = soft_join(s, SoftSum{s_stat[i][0], s_stat[i][1], s_stat[i][2]});
+  before = s_before[0];
+#pragma unroll
+  for (int i = 1; i < W; ++i) before += s_before[i];
   const size_t slot = (size_t)row * a.parts + part;
   const bool whole = a.parts == 1;
   const float ll = whole ? log_sum(s) : 0.f;
@@ -272,6 +324,7 @@ __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const LogprobArg
   for (int c = t; c < count; c += kThreads) {
     const uint64_t k = s_cand[c];
     int rank = 0;
+#pragma unroll 4
     for (int i = 0; i < count; ++i) rank += s_cand[i] > k;
     if (rank >= a.top) continue;
     if (whole) finish_top(a, row, s, ll, rank, k);
@@ -281,69 +334,69 @@ __global__ __launch_bounds__(kThreads) void logprob_part_kernel(const LogprobArg
     for (int c = count + t; c < a.top; c += kThreads) a.best[slot * a.top + c] = 0;  // a last part of fewer logits
 }
 
-__device__ __forceinline__ uint64_t wave_max_key(uint64_t k) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) {
-    const uint64_t o = (uint64_t)(uint32_t)__shfl_xor((int)(k >> 32), m) << 32 | (uint32_t)__shfl_xor((int)k, m);
-    k = o > k ? o : k;
-  }
-  return k;
-}
-
-// A wave a row, a part a lane.  The largest of the parts' K-th keys is a bound that K keys reach.
+// A block a row, a part a lane of each wave.  Of the parts' J-th best keys as many as K / J reach their K/J-th
+// largest, and so do K keys; J such that this is about the middle one.
 template <int DT>
-__global__ __launch_bounds__(64) void logprob_join_kernel(const LogprobArgs a) {
+__global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(const LogprobArgs a) {
+  constexpr int kEach = kMaxParts * kTop / kJoinThreads;  // keys of a thread
   __shared__ uint64_t s_key[kMaxParts * kTop];
-  const int row = blockIdx.x, lane = threadIdx.x;
+  __shared__ int s_count;
+  const int row = blockIdx.x, t = threadIdx.x, lane = t & 63;
   const size_t slot0 = (size_t)row * a.parts;
+  const int all = a.parts * a.top;
+  uint64_t key[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) key[i] = i * kJoinThreads + t < all ? a.best[slot0 * a.top + i * kJoinThreads + t] : 0;
   SoftSum s = {-INFINITY, 0.f, 0.f};
   int before = 0;
-  uint64_t bound = 0;
+  uint32_t bound = 0;
+  const int nth = min(a.top, (2 * a.top + a.parts - 1) / a.parts);
   if (lane < a.parts) {
     const float* at = a.stats + (slot0 + lane) * 3;
     s = SoftSum{at[0], at[1], at[2]};
     before = a.before[slot0 + lane];
-    if (a.top) bound = a.best[(slot0 + lane + 1) * a.top - 1];
+    if (a.top) bound = (uint32_t)(a.best[(slot0 + lane) * a.top + nth - 1] >> 32);
   }
   s = soft_wave(s);
-#pragma unroll
-  for (int k = 32; k; k >>= 1) before += __shfl_xor(before, k);
+  before = wave_count(before & 0xFFFF) + (wave_count(before >> 16) << 16);
   const float ll = log_sum(s);
-  if (lane == 0) finish_row<DT>(a, row, s, ll, before);
+  if (t == 0) finish_row<DT>(a, row, s, ll, before);
   if (!a.top) return;
-  bound = wave_max_key(bound);
-  if (bound == 0) bound = 1;
-  int count = 0;
-  for (int c = lane; c - lane < a.parts * a.top; c += 64) {
-    const uint64_t k = c < a.parts * a.top ? a.best[slot0 * a.top + c] : 0;
-    const uint64_t reach = __ballot(k >= bound);
-    if (k >= bound) s_key[count + __popcll(reach & ((1ULL << lane) - 1))] = k;
-    count += __popcll(reach);
-  }
+  // (by value alone: keys of the bound's value all reach it)
+  const uint32_t least = wave_reach(bound, (a.top + nth - 1) / nth);
+  if (t == 0) s_count = 0;
   __syncthreads();
-  for (int c = lane; c < count; c += 64) {
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (key[i] && (uint32_t)(key[i] >> 32) >= least) s_key[atomicAdd(&s_count, 1)] = key[i];
+  __syncthreads();
+  const int count = s_count;
+  for (int c = t; c < count; c += kJoinThreads) {
     const uint64_t k = s_key[c];
     int rank = 0;
+#pragma unroll 4
     for (int i = 0; i < count; ++i) rank += s_key[i] > k;
     if (rank < a.top) finish_top(a, row, s, ll, rank, k);
   }
 }
 
-// Logits of a thread: few where the parts would not fill the device.
-int held(int rows, int vocab) {
-  const long long few = (vocab + kThreads * kHeldFew - 1) / (kThreads * kHeldFew);
-  return few <= kMaxParts && rows * few <= 2048 ? kHeldFew : kHeldMost;
+// How a row is cut: short rows are a wave's, others parts of four waves.
+struct Cut {
+  int held, waves, parts;
+};
+Cut cut(int rows, int vocab) {
+  if (vocab <= 64 * kHeldFew) return {kHeldFew, 1, 1};
+  const auto parts = [&](int held) { return (vocab + 256 * held - 1) / (256 * held); };
+  const bool few = parts(kHeldFew) <= kMaxParts && (parts(kHeldFew) == 1 || (long long)rows * parts(kHeldFew) <= 2048);
+  return {few ? kHeldFew : kHeldMost, 4, parts(few ? kHeldFew : kHeldMost)};
 }
 
 struct LogprobLayout {
   size_t before, best, total;
-  int parts;
 };
-LogprobLayout layout(int rows, int vocab, int top) {
+LogprobLayout layout(int rows, int parts, int top) {
   LogprobLayout l;
-  const int part = kThreads * held(rows, vocab);
-  l.parts = (vocab + part - 1) / part;
-  const size_t slots = (size_t)rows * l.parts;
+  const size_t slots = (size_t)rows * parts;
   l.before = align_up(slots * 12, 256);
   l.best = align_up(l.before + slots * 4, 256);
   l.total = l.best + slots * top * 8;
@@ -351,17 +404,18 @@ LogprobLayout layout(int rows, int vocab, int top) {
 }
 
 bool logprob_shape(int rows, int vocab, int top) {
-  constexpr int kPart = kThreads * kHeldMost;
+  constexpr int kPart = 256 * kHeldMost;
   return rows > 0 && vocab > 0 && vocab <= kMaxParts * kPart && top >= 0 && top <= kTop && top <= vocab &&
          (long long)rows * ((vocab + kPart - 1) / kPart) <= (1 << 23);
 }
 
 template <int DT>
-int launch(const LogprobArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)(a.rows * a.parts));
-  if (held(a.rows, a.vocab) == kHeldFew) hipLaunchKernelGGL((logprob_part_kernel<DT, kHeldFew>), grid, dim3(kThreads), 0, st, a);
-  else hipLaunchKernelGGL((logprob_part_kernel<DT, kHeldMost>), grid, dim3(kThreads), 0, st, a);
-  if (a.parts > 1) hipLaunchKernelGGL(logprob_join_kernel<DT>, dim3((unsigned)a.rows), dim3(64), 0, st, a);
+int launch(const LogprobArgs& a, const Cut& c, hipStream_t st) {
+  const dim3 grid((unsigned)(a.rows * a.parts)), block(64 * c.waves);
+  if (c.waves == 1) hipLaunchKernelGGL((logprob_part_kernel<DT, kHeldFew, 1>), grid, block, 0, st, a);
+  else if (c.held == kHeldFew) hipLaunchKernelGGL((logprob_part_kernel<DT, kHeldFew, 4>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((logprob_part_kernel<DT, kHeldMost, 4>), grid, block, 0, st, a);
+  if (a.parts > 1) hipLaunchKernelGGL(logprob_join_kernel<DT>, dim3((unsigned)a.rows), dim3(kJoinThreads), 0, st, a);
   return check_launch();
 }
 
@@ -371,7 +425,8 @@ int launch(const LogprobArgs& a, hipStream_t st) {
 using namespace q4d;
 
 extern "C" size_t q4d_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top) {
-  return logprob_shape(rows, vocab, top) ? layout(rows, vocab, top).total : 0;
+  if (!logprob_shape(rows, vocab, top)) return 0;
+  return layout(rows, cut(rows, vocab).parts, top).total;
 }
 
 extern "C" int q4d_token_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_t rows, int32_t vocab,
@@ -383,11 +438,12 @@ extern "C" int q4d_token_logprobs(const void* logits, int32_t dtype, int64_t str
   if (!aligned(logits, dtype == Q4D_F32 ? 4 : 2) || !aligned(targets, 4) || !aligned(logprob, 4) || !aligned(rank, 4) ||
       !aligned(entropy, 4) || !aligned(top_logprobs, 4) || !aligned(top_ids, 4) || !aligned(ws, 256))
     return Q4D_ERR_BAD_ADDR;
-  const LogprobLayout l = layout(rows, vocab, top);
+  const Cut c = cut(rows, vocab);
+  const LogprobLayout l = layout(rows, c.parts, top);
   if (ws_bytes < l.total) return Q4D_ERR_CAPACITY;
-  const LogprobArgs a = {logits, stride, rows, vocab, l.parts, top, targets, ws_ptr<float>(ws, 0), ws_ptr<int32_t>(ws, l.before),
+  const LogprobArgs a = {logits, stride, rows, vocab, c.parts, top, targets, ws_ptr<float>(ws, 0), ws_ptr<int32_t>(ws, l.before),
                          ws_ptr<uint64_t>(ws, l.best), logprob, rank, entropy, top_logprobs, top_ids};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == Q4D_F32) return launch<Q4D_F32>(a, st);
-  return dtype == Q4D_BF16 ? launch<Q4D_BF16>(a, st) : launch<Q4D_F16>(a, st);
+  if (dtype == Q4D_F32) return launch<Q4D_F32>(a, c, st);
+  return dtype == Q4D_BF16 ? launch<Q4D_BF16>(a, c, st) : launch<Q4D_F16>(a, c, st);
 }

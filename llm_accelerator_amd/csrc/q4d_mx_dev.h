@@ -45,12 +45,33 @@ __device__ __forceinline__ u32x4 mx_dequant8(uint32_t w, float scale) {
   return u32x4{mx_pair<0, BF>(w, scale), mx_pair<1, BF>(w, scale), mx_pair<2, BF>(w, scale), mx_pair<3, BF>(w, scale)};
 }
 
+// Sum / maximum of a wave, in every lane: in the 16-lane rows by DPP, then over the rows by lane swaps (shuffles
+// through LDS would be a few hundred clocks of a chain).
+template <bool SUM>
+__device__ __forceinline__ float wave_all(float v) {
+  const auto op = [](float a, float b) { return SUM ? a + b : fmaxf(a, b); };
+  v = op(v, dpp_f<kDppQuadSwap1>(v));
+  v = op(v, dpp_f<kDppQuadSwap2>(v));
+  v = op(v, dpp_f<kDppRowHalfMirror>(v));
+  v = op(v, dpp_f<kDppRowMirror>(v));
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  const uint32_t x = __builtin_bit_cast(uint32_t, op(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return op(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+
 // A softmax's sums over some logits z: the maximum m, l = sum e^(z - m) and t = sum (z - m) e^(z - m), from
 // which log(sum e^z) = m + log l and the entropy log l - t / l.  fp32; a NaN among the logits makes l NaN,
 // and where all are -Inf l is 0 (and the joined l NaN at the end, as the softmax is).
 struct SoftSum {
   float m, l, t;
 };
+// e^d, d <= 0, by the hardware's 2^x (what would be subnormal is 0).
+constexpr float kLog2e = 1.44269504f;
+__device__ __forceinline__ float exp_neg(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 // The sums of N logits given their maximum.
 template <int N, class F>
 __device__ __forceinline__ SoftSum soft_sum(float m, F z) {
@@ -58,7 +79,7 @@ __device__ __forceinline__ SoftSum soft_sum(float m, F z) {
   SoftSum s = {m, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const float d = z(i) - ms, e = __expf(d);
+    const float d = z(i) - ms, e = exp_neg(d);
     s.l += e;
     s.t = fmaf(fmaxf(d, -1000.f), e, s.t);  // (e is 0 long before; -Inf x 0 would be NaN)
   }
@@ -66,15 +87,15 @@ __device__ __forceinline__ SoftSum soft_sum(float m, F z) {
 }
 __device__ __forceinline__ SoftSum soft_join(SoftSum a, SoftSum b) {
   const float m = fmaxf(a.m, b.m), ms = m == -INFINITY ? 0.f : m;
-  const float da = a.m - ms, db = b.m - ms, fa = __expf(da), fb = __expf(db);
+  const float da = a.m - ms, db = b.m - ms, fa = exp_neg(da), fb = exp_neg(db);
   return {m, fmaf(a.l, fa, b.l * fb),
           (fa > 0.f ? fa * fmaf(da, a.l, a.t) : 0.f) + (fb > 0.f ? fb * fmaf(db, b.l, b.t) : 0.f)};
 }
 
 // Of the lanes of a wave, in every lane.
 __device__ __forceinline__ SoftSum soft_wave(SoftSum s) {
-  const float m = wave_max(s.m), d = s.m - (m == -INFINITY ? 0.f : m), f = __expf(d);
-  return {m, wave_sum(s.l * f), wave_sum(f > 0.f ? f * fmaf(d, s.l, s.t) : 0.f)};
+  const float m = wave_all<false>(s.m), d = s.m - (m == -INFINITY ? 0.f : m), f = exp_neg(d);
+  return {m, wave_all<true>(s.l * f), wave_all<true>(f > 0.f ? f * fmaf(d, s.l, s.t) : 0.f)};
 }
 
 // Outputs n .. n + 3 of row m, those below N, rounded once to the output's type.

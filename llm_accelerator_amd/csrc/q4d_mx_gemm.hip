@@ -23,7 +23,6 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTileN = 256;
-constexpr float kLog2e = 1.44269504f;
 constexpr int kXcds = 8;
 
 template <bool BF>
@@ -247,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float d = acc[i][j][e] - top, p = __builtin_amdgcn_exp2f(d * kLog2e);
+          const float d = acc[i][j][e] - top, p = exp_neg(d);
           l += p;
           u = fmaf(p, d, u);
         }
