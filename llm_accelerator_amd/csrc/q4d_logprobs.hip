@@ -93,7 +93,7 @@ __device__ __forceinline__ uint32_t wave_reach(uint32_t u, int n) {
   return bound;
 }
 
-// Sum of a count of up to 2^8 a lane: exact in fp32.
+// Sum of a count of up to 2^16 a lane: exact in fp32.
 __device__ __forceinline__ int wave_count(int c) { return (int)wave_all<true>((float)c); }
 
 // What a row's outputs are once its sums are whole.
@@ -226,10 +226,10 @@ __global__ __launch_bounds__(64 * W) void logprob_part_kernel(const LogprobArgs 
   if (a.top) {
     // (a thread without a number has the bits of -Inf or NaN, which the keys tell apart)
     const uint32_t u = order_bits(mine);
-    uint32_t bound = wave_reach(u, a.top);
+    uint32_t bound = a.top == 1 ? order_bits(top) : wave_reach(u, a.top);
     if constexpr (W > 1) {
       // (the second for more than a few, of which one wave's K best are not the part's)
-      const uint32_t share = a.top >= W ? wave_reach(u, (a.top + W - 1) / W) : 0;
+      const uint32_t share = a.top > W ? wave_reach(u, (a.top + W - 1) / W) : 0;
       if (lane == 0) {
         s_wave[0][w] = bound;
         s_wave[1][w] = share;
@@ -387,7 +387,7 @@ struct Cut {
 Cut cut(int rows, int vocab) {
   if (vocab <= 64 * kHeldFew) return {kHeldFew, 1, 1};
   const auto parts = [&](int held) { return (vocab + 256 * held - 1) / (256 * held); };
-  const bool few = parts(kHeldFew) <= kMaxParts && (parts(kHeldFew) == 1 || (long long)rows * parts(kHeldFew) <= 2048);
+  const bool few = parts(kHeldFew) <= kMaxParts && (parts(kHeldFew) == 1 || (long long)rows * parts(kHeldFew) <= 4096);
   return {few ? kHeldFew : kHeldMost, 4, parts(few ? kHeldFew : kHeldMost)};
 }
 
