@@ -568,8 +568,8 @@ int q4d_mx_matmul(const q4d_mx_t* w, const q4d_mx_t* x, void* y, int32_t y_dtype
  * q4d_mx_linear), with z = W x[m] in fp32 and never in memory: logprob[m] = z[target] - log sum e^z
  * (a target outside the vocabulary, a padded row's: NaN), entropy[m] of the distribution, best[m] =
  * the largest log probability.  A row whose z hold NaN or +Inf gives NaN.  ws: 256-byte aligned,
- * q4d_mx_score_workspace_bytes(w->rows, M) bytes, holds nothing between calls. */
-size_t q4d_mx_score_workspace_bytes(int32_t rows, int32_t M);
+ * q4d_mx_score_workspace_bytes(w->rows, w->cols, M) bytes, holds nothing between calls. */
+size_t q4d_mx_score_workspace_bytes(int32_t rows, int32_t cols, int32_t M);
 int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M, const int32_t* targets,
                  float* logprob, float* entropy, float* best, void* ws, size_t ws_bytes, void* stream);
 /* Of logits (fp32, fp16 or bf16, row i at i * stride elements, vocab up to 2^20): the entropy [rows]; with

@@ -219,7 +219,7 @@ SIGNATURES = {
     "q4d_mx_dequantize": ([_MX, _P, c_int32, _P], c_int32),
     "q4d_mx_linear": ([_MX, _P, c_int32, ctypes.c_int64, c_int32, _P, c_int32, _P], c_int32),
     "q4d_mx_matmul": ([_MX, _MX, _P, c_int32, _P], c_int32),
-    "q4d_mx_score_workspace_bytes": ([c_int32, c_int32], c_size_t),
+    "q4d_mx_score_workspace_bytes": ([c_int32, c_int32, c_int32], c_size_t),
     "q4d_mx_score": ([_MX, _P, c_int32, ctypes.c_int64, c_int32, _P, _P, _P, _P, _P, c_size_t, _P], c_int32),
     "q4d_token_logprobs_workspace_bytes": ([c_int32, c_int32, c_int32], c_size_t),
     "q4d_token_logprobs": ([_P, c_int32, ctypes.c_int64, c_int32, c_int32, _P, c_int32, _P, _P, _P, _P, _P, _P, c_size_t,

@@ -23,6 +23,7 @@ struct MxProduct {
 
 enum MxKind { MX_X4 = 0, MX_F16 = 1, MX_BF16 = 2 };  // x: codes or 16-bit floats
 
+bool mx_shape(int32_t rows, int32_t cols);
 int check_mx(const q4d_mx_t* t);
 
 // Few rows (q4d_mx_rows.hip; a score: up to kMxFewRows) and tiles of many (q4d_mx_gemm.hip), and the ranges of N
@@ -31,6 +32,11 @@ constexpr int kMxFewRows = 64;
 int launch_mx_rows(const MxProduct& p, MxKind kind, hipStream_t st);
 int launch_mx_rows_score(const MxProduct& p, MxKind kind, hipStream_t st);
 int mx_rows_parts(int M, int N);
+// Few rows and many weights (q4d_mx_head.hip), where x fits in LDS.
+bool mx_head_fits(int M, int K);
+int mx_head_parts(int M, int N, int K);
+int launch_mx_head(const MxProduct& p, MxKind kind, hipStream_t st);
+int launch_mx_head_score(const MxProduct& p, MxKind kind, hipStream_t st);
 int launch_mx_gemm(const MxProduct& p, MxKind kind, hipStream_t st);
 __host__ __device__ inline int mx_gemm_parts(int N) { return (int)((N + 255LL) / 256); }
 int launch_mx_gemm_score(const MxProduct& p, MxKind kind, hipStream_t st);

@@ -189,11 +189,6 @@ __global__ __launch_bounds__(256) void mx_rows_tiles_kernel(const MxArgs a) {
 
 bool mx_kind(int dtype) { return dtype == Q4D_F16 || dtype == Q4D_BF16 || dtype == Q4D_F32; }
 
-// Up to 2^27 tiles (2^38 codes): groups, and a round past the last, are counted in 32 bits.
-bool mx_shape(int32_t rows, int32_t cols) {
-  return rows > 0 && cols > 0 && cols % 32 == 0 && rows <= 0x7FFFFF00 && cols <= 0x7FFFFF00 &&
-         (long long)mx_row_tiles(rows) * mx_col_tiles(cols) <= 1LL << 27;
-}
 MxArgs mx_args(const void* w, const void* s, int32_t rows, int32_t cols) {
   MxArgs a = {};
   a.codes = static_cast<uint32_t*>(const_cast<void*>(w));
@@ -217,6 +212,11 @@ void quantize(const MxArgs& a, bool ceil, hipStream_t st) {
 
 }  // namespace
 
+// Up to 2^27 tiles (2^38 codes): groups, and a round past the last, are counted in 32 bits.
+bool mx_shape(int32_t rows, int32_t cols) {
+  return rows > 0 && cols > 0 && cols % 32 == 0 && rows <= 0x7FFFFF00 && cols <= 0x7FFFFF00 &&
+         (long long)mx_row_tiles(rows) * mx_col_tiles(cols) <= 1LL << 27;
+}
 int check_mx(const q4d_mx_t* t) {
   if (!t || !t->w || !t->s) return Q4D_ERR_NULL;
   if (!mx_shape(t->rows, t->cols)) return Q4D_ERR_SHAPE;

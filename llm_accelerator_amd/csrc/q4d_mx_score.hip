@@ -56,13 +56,19 @@ int check_y(const void* y, int32_t y_dtype) {
   if (y_dtype != Q4D_F16 && y_dtype != Q4D_BF16 && y_dtype != Q4D_F32) return Q4D_ERR_DTYPE;
   return aligned(y, 16) ? Q4D_OK : Q4D_ERR_BAD_ADDR;
 }
+constexpr int kHeadRows = 32768;  // weight rows from which q4d_mx_head.hip takes a few rows
+bool use_head(int M, int N, int K) { return M <= kMxFewRows && N >= kHeadRows && mx_head_fits(M, K); }
 int product(const MxProduct& p, MxKind kind, hipStream_t st) {
+  if (kind != MX_X4 && use_head(p.M, p.N, p.K)) return launch_mx_head(p, kind, st);
   return p.M <= kMxFewRows ? launch_mx_rows(p, kind, st) : launch_mx_gemm(p, kind, st);
 }
 MxKind kind_of(int32_t x_dtype) { return x_dtype == Q4D_BF16 ? MX_BF16 : MX_F16; }
 
 size_t hit_bytes(int M) { return align_up((size_t)M * 4, 256); }
-int score_parts(int M, int N) { return M <= kMxFewRows ? mx_rows_parts(M, N) : mx_gemm_parts(N); }
+int score_parts(int M, int N, int K) {
+  if (use_head(M, N, K)) return mx_head_parts(M, N, K);
+  return M <= kMxFewRows ? mx_rows_parts(M, N) : mx_gemm_parts(N);
+}
 
 }  // namespace
 }  // namespace q4d
@@ -103,9 +109,9 @@ extern "C" int q4d_mx_matmul(const q4d_mx_t* w, const q4d_mx_t* x, void* y, int3
   return product(p, MX_X4, reinterpret_cast<hipStream_t>(stream));
 }
 
-extern "C" size_t q4d_mx_score_workspace_bytes(int32_t rows, int32_t M) {
-  if (rows <= 0 || M <= 0) return 0;
-  return hit_bytes(M) + (size_t)score_parts(M, rows) * M * sizeof(f32x4);
+extern "C" size_t q4d_mx_score_workspace_bytes(int32_t rows, int32_t cols, int32_t M) {
+  if (!mx_shape(rows, cols) || M <= 0) return 0;
+  return hit_bytes(M) + (size_t)score_parts(M, rows, cols) * M * sizeof(f32x4);
 }
 
 extern "C" int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M,
@@ -116,7 +122,7 @@ extern "C" int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, i
   if (!targets || !logprob || !entropy || !best || !ws) return Q4D_ERR_NULL;
   if (!aligned(targets, 4) || !aligned(logprob, 4) || !aligned(entropy, 4) || !aligned(best, 4) || !aligned(ws, 256))
     return Q4D_ERR_BAD_ADDR;
-  if (ws_bytes < q4d_mx_score_workspace_bytes(w->rows, M)) return Q4D_ERR_CAPACITY;
+  if (ws_bytes < q4d_mx_score_workspace_bytes(w->rows, w->cols, M)) return Q4D_ERR_CAPACITY;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   MxProduct p = {};
   p.w = w->w;
@@ -129,8 +135,11 @@ extern "C" int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, i
   p.targets = targets;
   p.hit = ws_ptr<float>(ws, 0);
   p.stats = ws_ptr<f32x4>(ws, hit_bytes(M));
-  const int parts = score_parts(M, p.N);
-  if ((rc = M <= kMxFewRows ? launch_mx_rows_score(p, kind_of(x_dtype), st) : launch_mx_gemm_score(p, kind_of(x_dtype), st))) return rc;
+  const int parts = score_parts(M, p.N, p.K);
+  const MxKind kind = kind_of(x_dtype);
+  if (use_head(M, p.N, p.K)) rc = launch_mx_head_score(p, kind, st);
+  else rc = M <= kMxFewRows ? launch_mx_rows_score(p, kind, st) : launch_mx_gemm_score(p, kind, st);
+  if (rc) return rc;
   const JoinArgs j = {p.stats, p.hit, targets, parts, M, p.N, logprob, entropy, best};
   hipLaunchKernelGGL(mx_score_join_kernel, dim3((unsigned)M), dim3(256), 0, st, j);
   return check_launch();

@@ -247,7 +247,7 @@ def mx_score(hidden: torch.Tensor, weight: MXTensor, targets: torch.Tensor) -> M
     targets = targets.contiguous()
     got = x.new_empty((3, *lead), dtype=torch.float32)
     if m:
-        nbytes = _lib.load().q4d_mx_score_workspace_bytes(weight.shape[0], m)
+        nbytes = _lib.load().q4d_mx_score_workspace_bytes(*weight.shape, m)
         ws = x.new_empty(nbytes, dtype=torch.uint8)
         base, row = got.data_ptr(), 4 * m
         call_on(index, "q4d_mx_score", weight._ref, x.data_ptr(), _DTYPES[x.dtype], step, m, targets.data_ptr(), base,

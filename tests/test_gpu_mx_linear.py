@@ -34,7 +34,7 @@ def compare(y, x, w):
 SHAPES = [(1, 1, 32), (1, 16, 64), (1, 2048, 1024), (2, 17, 96), (3, 255, 160), (5, 64, 2048), (15, 33, 128), (16, 1000, 1056),
           (17, 48, 224), (31, 129, 288), (33, 16, 512), (48, 1024, 2048), (63, 257, 320), (64, 70, 4096), (65, 256, 64),
           (100, 3, 1024), (127, 255, 96), (128, 256, 256), (129, 257, 288), (200, 1000, 1024), (257, 513, 1056), (300, 64, 32),
-          (513, 2048, 192)]
+          (513, 2048, 192), (1, 33001, 160), (7, 32768, 1024), (30, 32800, 1056), (64, 32769, 1024), (64, 32770, 1056), (40, 33000, 64)]
 
 
 @pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16, "mx"])

@@ -43,7 +43,8 @@ def check(got, x, w, targets):
 @pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 32), (1, 5000, 1024), (2, 2, 64), (7, 257, 96), (16, 4096, 1024), (17, 300, 160), (21, 20000, 1024),
                                    (33, 16, 288), (48, 3001, 512), (64, 1000, 2048), (65, 255, 64), (128, 256, 1024), (131, 9001, 224),
-                                   (300, 2000, 1056)])
+                                   (300, 2000, 1056), (5, 33000, 1024), (32, 40001, 96), (33, 32768, 1024), (64, 33333, 992), (2, 32800, 4096),
+                                   (20, 32801, 4096), (64, 32799, 2048)])
 def test_shapes(dev, m, n, k, kind):
     rng = np.random.default_rng(m + 3 * n + 5 * k)
     w, wv = head(rng, n, k, dev)

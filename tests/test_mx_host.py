@@ -104,8 +104,9 @@ def test_matmul_refusals(lib):
 
 
 def test_score_refusals(lib):
-    need = lib.q4d_mx_score_workspace_bytes(48, 3)
-    assert need > 0 and lib.q4d_mx_score_workspace_bytes(0, 3) == lib.q4d_mx_score_workspace_bytes(48, 0) == 0
+    need = lib.q4d_mx_score_workspace_bytes(48, 64, 3)
+    assert need > 0 and lib.q4d_mx_score_workspace_bytes(0, 64, 3) == lib.q4d_mx_score_workspace_bytes(48, 64, 0) == 0
+    assert lib.q4d_mx_score_workspace_bytes(48, 40, 3) == 0
 
     def call(w=mx(), x=FAKE, dt=F16, stride=64, m=3, targets=FAKE, out=FAKE, ws=FAKE, nbytes=need):
         return lib.q4d_mx_score(w, x, dt, stride, m, targets, out, out, out, ws, nbytes, None)
