@@ -98,12 +98,21 @@ __device__ __forceinline__ SoftSum soft_wave(SoftSum s) {
   return {m, wave_all<true>(s.l * f), wave_all<true>(f > 0.f ? f * fmaf(d, s.l, s.t) : 0.f)};
 }
 
+// Four outputs rounded once to a 16-bit type.
+__device__ __forceinline__ u32x2 pack_out4(int dtype, f32x4 v) {
+  uint32_t u[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    u[e] = dtype == Q4D_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)v[e]) : __builtin_bit_cast(uint16_t, (_Float16)v[e]);
+  return u32x2{u[0] | u[1] << 16, u[2] | u[3] << 16};
+}
 // Outputs n .. n + 3 of row m, those below N, rounded once to the output's type.
 __device__ __forceinline__ void store_out4(const MxProduct& a, int m, int n, f32x4 v) {
   const size_t at = (size_t)m * a.N + n;
+  const bool whole = n + 4 <= a.N && a.N % 4 == 0;
   if (a.y_dtype == Q4D_F32) {
     float* y = static_cast<float*>(a.y) + at;
-    if (n + 4 <= a.N && a.N % 4 == 0) {
+    if (whole) {
       *reinterpret_cast<f32x4*>(y) = v;
     } else {
 #pragma unroll
@@ -112,17 +121,14 @@ __device__ __forceinline__ void store_out4(const MxProduct& a, int m, int n, f32
     }
     return;
   }
-  uint32_t u[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    u[e] = a.y_dtype == Q4D_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)v[e]) : __builtin_bit_cast(uint16_t, (_Float16)v[e]);
+  const u32x2 u = pack_out4(a.y_dtype, v);
   uint16_t* y = static_cast<uint16_t*>(a.y) + at;
-  if (n + 4 <= a.N && a.N % 4 == 0) {
-    *reinterpret_cast<u32x2*>(y) = u32x2{u[0] | u[1] << 16, u[2] | u[3] << 16};
+  if (whole) {
+    *reinterpret_cast<u32x2*>(y) = u;
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (n + e < a.N) y[e] = (uint16_t)u[e];
+      if (n + e < a.N) y[e] = (uint16_t)(u[e / 2] >> (16 * (e & 1)));
   }
 }
 

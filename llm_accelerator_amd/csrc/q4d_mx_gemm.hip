@@ -1,12 +1,11 @@
 // Products of many rows with microscaled 4-bit weights (gfx950, wave64): y = x W^T, and the score of
 // given outputs, which keeps of each row's products only the sums of a softmax.
 //
-// A block takes 256 weight rows and 32 MT rows of x, a wave 64 weight rows and all of x's.  x goes to LDS
-// by DMA a stage ahead (64 columns of 16 bits, 256 of 4); weights go from memory to the registers of the
-// one wave that needs them: lane (r, h) loads row r's block 2 i + h, and since the order of K inside a
-// product is free, its 32 columns are the lane's share of 64: with 16-bit x four 32x32x16 products of 8
-// columns a lane after the codes are made 16-bit floats, with x in 4 bits one 32x32x64 product that
-// takes codes and scales as they are.
+// A block takes 128 NT weight rows and 32 MT rows of x, a wave 32 NT weight rows and all of x's.  Both go to
+// LDS by DMA, RING - 1 stages ahead (64 columns with x in 16 bits, 128 in 4).  Lane (r, h) takes row r's block
+// 2 i + h, and since the order of K inside a product is free, its 32 columns are the lane's share of 64:
+// with 16-bit x four 32x32x16 products of 8 columns a lane after the codes are made 16-bit floats, with x
+// in 4 bits one 32x32x64 product that takes codes and scales as they are.
 // The weights are the first operand, so that a lane holds outputs of one row of x.
 #include <float.h>
 #include <math.h>
@@ -22,7 +21,6 @@ namespace {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kTileN = 256;
 constexpr int kXcds = 8;
 
 template <bool BF>
@@ -61,17 +59,25 @@ __device__ __forceinline__ float halves(float v) {  // of lanes l and l ^ 32, in
   return SUM ? x0 + x1 : fmaxf(x0, x1);
 }
 
-template <MxKind KIND, bool SCORE, int MT>
-__global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
+// s_waitcnt vmcnt(N) lgkmcnt(0)
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
+}
+
+template <MxKind KIND, bool SCORE, int NT, int MT, int RING, int PER_CU>
+__global__ __launch_bounds__(256, PER_CU) void mx_gemm_kernel(const MxProduct a) {
   constexpr bool X4 = KIND == MX_X4;
-  constexpr int kTileM = 32 * MT;
+  constexpr int kTileN = 128 * NT, kTileM = 32 * MT;
   constexpr int kCols = X4 ? 128 : 64;                     // columns of a stage
   // bytes of a stage: x (16 bits: 128 a row; 4 bits: tiles), weights, their scales and x's, 256 a wave
-  constexpr int kX = kTileM * (X4 ? 64 : 128), kW = 8 * kMxTile * kCols / kMxCols, kS = 1024;
-  constexpr int kStage = kX + kW + kS * (X4 ? 2 : 1), kRing = 3;
-  constexpr int kLoads = X4 ? 8 : 7;                       // DMA instructions of a wave and stage
-  static_assert(MT == 4, "a wave moves 32 rows of x");
-  __shared__ __attribute__((aligned(16))) char lds[kRing * kStage];
+  constexpr int kWaveX = kTileM * (X4 ? 64 : 128) / 4, kWaveW = NT * kMxTile * kCols / kMxCols;  // of a wave
+  constexpr int kX = 4 * kWaveX, kW = 4 * kWaveW, kS = 1024;
+  constexpr int kStage = kX + kW + kS * (X4 ? 2 : 1);
+  constexpr int kLoads = (kWaveX + kWaveW) / 1024 + (X4 ? 2 : 1);  // DMA instructions of a wave and stage
+  static_assert((MT == 2 || MT == 4) && RING >= 3 && RING <= 6 && kLoads * (RING - 2) < 64 && RING * kStage * PER_CU <= 160 << 10, "");
+  static_assert(!SCORE || (NT == 2 && 4 * kTileM * 12 <= RING * kStage), "");
+  __shared__ __attribute__((aligned(16))) char lds[RING * kStage];
   const int t = threadIdx.x, lane = t & 63, r = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int tm = (a.M + kTileM - 1) / kTileM, tiles = gridDim.x;
@@ -88,14 +94,14 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
   const size_t x_row = 2 * (size_t)a.x_stride;
   const char* xb = static_cast<const char*>(a.x) + (X4 ? 0 : m0 * x_row);
   const auto group = [&](int j) { return (lane & 7) ^ ((4 * j + (lane >> 4)) & 7); };
-  uint32_t from[4];
+  uint32_t from[MT];
   if constexpr (!X4) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) from[j] = (uint32_t)(min(32 * w + 8 * j + (lane >> 3), a.M - 1 - m0) * x_row) + 16 * group(j);
+    for (int j = 0; j < MT; ++j) from[j] = (uint32_t)(min(8 * (MT * w + j) + (lane >> 3), a.M - 1 - m0) * x_row) + 16 * group(MT * w + j);
   }
-  const size_t x_tile = (size_t)min(m0 / kMxRows + w, (a.M - 1) / kMxRows) * col_tiles;  // this wave's first
-  // the wave's two tiles of weight rows (past the last: the last, not stored)
-  const int w_tiles = mx_row_tiles(a.N), wt0 = min(n0 / kMxRows + 2 * w, w_tiles - 1), wt1 = min(wt0 + 1, w_tiles - 1);
+  const size_t x_tile = (size_t)min(m0 / kMxRows + w * MT / 4, (a.M - 1) / kMxRows) * col_tiles;  // this wave's first
+  // the wave's tiles of weight rows (past the last: the last, not stored)
+  const int w_tiles = mx_row_tiles(a.N), wt0 = min(n0 / kMxRows + NT * w, w_tiles - 1), wt1 = min(wt0 + NT - 1, w_tiles - 1);
   const uint8_t* const wp0 = a.w + (size_t)wt0 * col_tiles * kMxTile;
   const uint8_t* const wp1 = a.w + (size_t)wt1 * col_tiles * kMxTile;
   const uint8_t* const sp = a.ws + (size_t)wt0 * col_tiles * kMxScales;
@@ -103,13 +109,12 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
   const auto issue = [&](int st, int at) {
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + at);
     if constexpr (X4) {
-      const uint8_t* p = static_cast<const uint8_t*>(a.x) + (x_tile + st) * kMxTile;
-      dma16(p, 16 * lane, to + 2048 * w);
-      dma16(p, 16 * lane + 1024, to + 2048 * w + 1024);
-      dma16(wp0 + (size_t)st * kMxTile, 16 * lane, to + kX + 4096 * w);
-      dma16(wp0 + (size_t)st * kMxTile, 16 * lane + 1024, to + kX + 4096 * w + 1024);
-      dma16(wp1 + (size_t)st * kMxTile, 16 * lane, to + kX + 4096 * w + 2048);
-      dma16(wp1 + (size_t)st * kMxTile, 16 * lane + 1024, to + kX + 4096 * w + 3072);
+      const uint8_t* p = static_cast<const uint8_t*>(a.x) + (x_tile + st) * kMxTile + (MT == 2 ? 1024 * (w & 1) : 0);
+#pragma unroll
+      for (int j = 0; j < kWaveX / 1024; ++j) dma16(p, 16 * lane + 1024 * j, to + kWaveX * w + 1024 * j);
+#pragma unroll
+      for (int j = 0; j < 2 * NT; ++j)
+        dma16((j < 2 ? wp0 : wp1) + (size_t)st * kMxTile, 16 * lane + 1024 * (j & 1), to + kX + kWaveW * w + 1024 * j);
       dma4(sp + (size_t)st * kMxScales, sfrom, to + kX + kW + 256 * w);
       dma4(a.xs + (x_tile + st) * kMxScales, 4 * r, to + kX + kW + kS + 256 * w);
     } else {
@@ -117,100 +122,143 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
       const int have = a.K / 8 - 8 * st;  // groups left in the row
       if (have >= 8) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) dma16(base, from[j], to + 4096 * w + 1024 * j);
+        for (int j = 0; j < MT; ++j) dma16(base, from[j], to + kWaveX * w + 1024 * j);
       } else {  // groups past the row's end are zeros
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < MT; ++j) {
           u32x4 v = {0u, 0u, 0u, 0u};
-          if (group(j) < have) v = *reinterpret_cast<const u32x4*>(base + from[j]);
-          *reinterpret_cast<u32x4*>(lds + at + 4096 * w + 1024 * j + 16 * lane) = v;
+          if (group(MT * w + j) < have) v = *reinterpret_cast<const u32x4*>(base + from[j]);
+          *reinterpret_cast<u32x4*>(lds + at + kWaveX * w + 1024 * j + 16 * lane) = v;
         }
       }
-      dma16(wp0 + (size_t)st * (kMxTile / 2), 16 * lane, to + kX + 2048 * w);
-      dma16(wp1 + (size_t)st * (kMxTile / 2), 16 * lane, to + kX + 2048 * w + 1024);
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        dma16((j ? wp1 : wp0) + (size_t)st * (kMxTile / 2), 16 * lane, to + kX + kWaveW * w + 1024 * j);
       dma4(sp + (size_t)(st / 2) * kMxScales, sfrom, to + kX + kW + 256 * w);
     }
   };
 
-  f32x16 acc[2][MT];
+  f32x16 acc[NT][MT];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < MT; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  issue(0, 0);
-  if (stages > 1) issue(1, kStage);
-  int at = 0, ahead = 2 * kStage;  // of this stage in the ring, and of the one after the next
+#pragma unroll
+  for (int c = 0; c < RING - 1; ++c)
+    if (c < stages) issue(c, c * kStage);
+  int at = 0, ahead = (RING - 1) * kStage;  // of this stage in the ring, and of the one to load next
   for (int st = 0; st < stages; ++st) {
-    // this wave's part of the stage is there (the next stage's loads may be under way), then everybody's,
+    // this wave's part of the stage is there (the loads of later ones may be under way), then everybody's,
     // and the stage before is read
-    if (st + 1 < stages) __builtin_amdgcn_s_waitcnt(0x0070 | kLoads);  // vmcnt(kLoads) lgkmcnt(0)
-    else __builtin_amdgcn_s_waitcnt(0x0070);
+    const int later = min(stages - 1 - st, RING - 2);
+    if (later >= 4) wait_loads<4 * kLoads>();
+    else if (later == 3) wait_loads<3 * kLoads>();
+    else if (later == 2) wait_loads<2 * kLoads>();
+    else if (later == 1) wait_loads<kLoads>();
+    else wait_loads<0>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (st + 2 < stages) issue(st + 2, ahead);
+    if (st + RING - 1 < stages) issue(st + RING - 1, ahead);
     const char* stage = lds + at;
     if constexpr (X4) {
-      uint32_t xs[MT], ws[2];
+      uint32_t xs[MT], ws[NT];
 #pragma unroll
-      for (int j = 0; j < MT; ++j) xs[j] = *reinterpret_cast<const uint32_t*>(stage + kX + kW + kS + 256 * j + 4 * r) >> (8 * h);
+      for (int j = 0; j < MT; ++j) xs[j] = *reinterpret_cast<const uint32_t*>(stage + kX + kW + kS + 256 * (j * 4 / MT) + 4 * r) >> (8 * h);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) ws[k] = *reinterpret_cast<const uint32_t*>(stage + kX + kW + 256 * w + 128 * k + 4 * r) >> (8 * h);
+      for (int k = 0; k < NT; ++k) ws[k] = *reinterpret_cast<const uint32_t*>(stage + kX + kW + 256 * w + 128 * k + 4 * r) >> (8 * h);
       const auto step = [&](auto i_) {
         constexpr int I = decltype(i_)::value;
-        u32x4 q[2];
+        u32x4 q[NT];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) q[k] = *reinterpret_cast<const u32x4*>(stage + kX + 4096 * w + 2048 * k + 1024 * I + 16 * lane);
+        for (int k = 0; k < NT; ++k) q[k] = *reinterpret_cast<const u32x4*>(stage + kX + kWaveW * w + 2048 * k + 1024 * I + 16 * lane);
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
           const u32x4 x = *reinterpret_cast<const u32x4*>(stage + 2048 * j + 1024 * I + 16 * lane);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) acc[k][j] = mfma_codes<I>(q[k], ws[k], x, xs[j], acc[k][j]);
+          for (int k = 0; k < NT; ++k) acc[k][j] = mfma_codes<I>(q[k], ws[k], x, xs[j], acc[k][j]);
         }
       };
       step(std::integral_constant<int, 0>());
       step(std::integral_constant<int, 1>());
     } else {
-      u32x4 q[2];
-      float f[2];
+      u32x4 q[NT];
+      float f[NT];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        q[k] = *reinterpret_cast<const u32x4*>(stage + kX + 2048 * w + 1024 * k + 16 * lane);
+      for (int k = 0; k < NT; ++k) {
+        q[k] = *reinterpret_cast<const u32x4*>(stage + kX + kWaveW * w + 1024 * k + 16 * lane);
         f[k] = mx_scale(*reinterpret_cast<const uint32_t*>(stage + kX + kW + 256 * w + 128 * k + 4 * r) >> (16 * (st & 1) + 8 * h) & 255u);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        u32x4 wd[2];
+        u32x4 wd[NT];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) wd[k] = mx_dequant8<KIND == MX_BF16>(q[k][i], f[k]);
+        for (int k = 0; k < NT; ++k) wd[k] = mx_dequant8<KIND == MX_BF16>(q[k][i], f[k]);
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
           const u32x4 x = *reinterpret_cast<const u32x4*>(stage + 128 * r + 4096 * j + (((4 * h + i) ^ (r >> 1 & 7)) << 4));
 #pragma unroll
-          for (int k = 0; k < 2; ++k) acc[k][j] = mfma32<KIND == MX_BF16>(wd[k], x, acc[k][j]);
+          for (int k = 0; k < NT; ++k) acc[k][j] = mfma32<KIND == MX_BF16>(wd[k], x, acc[k][j]);
         }
       }
     }
-    at = at == 2 * kStage ? 0 : at + kStage;
-    ahead = ahead == 2 * kStage ? 0 : ahead + kStage;
+    at = at == (RING - 1) * kStage ? 0 : at + kStage;
+    ahead = ahead == (RING - 1) * kStage ? 0 : ahead + kStage;
   }
 
-  // lane (r, h) holds outputs n0 + 64 w + 32 i + 8 (e / 4) + 4 h + e % 4 of x's row m0 + 32 j + r
-  const int nb = n0 + 64 * w + 4 * h;
+  // lane (r, h) holds outputs n0 + 32 NT w + 32 i + 8 (e / 4) + 4 h + e % 4 of x's row m0 + 32 j + r
+  const int nb = n0 + 32 * NT * w + 4 * h;
   if constexpr (!SCORE) {
+    // Through LDS, so that a row's outputs leave as 64 or 128 bytes together (straight from the registers, 8 bytes
+    // of 32 rows an instruction, 2000 x 16384 x 1024 in 4 bits took 61 us).
+    __syncthreads();  // everybody is done with the last stage
+    constexpr int kPitch = 64 * NT + 16;  // bytes of a row of 32 NT 16-bit outputs, or of 16 NT floats
+    char* own = lds + w * (32 * kPitch);
+    const bool wide = a.y_dtype == Q4D_F32;
+    const int size = wide ? 4 : 2;
+    const bool whole = a.N % (16 / size) == 0;  // rows of 16-byte pieces
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
-      const int m = m0 + 32 * j + r;
-      if (m >= a.M) continue;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int pass = 0; pass < 2; ++pass) {
+        if (!whole) {
+          const int m = m0 + 32 * j + r;
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const int n = nb + 32 * i + 2 * e;
-          if (n < a.N) store_out4(a, m, n, f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]});
+          for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 8 * pass; e < 8 * pass + 8; e += 4) {
+              const int n = nb + 32 * i + 2 * e;
+              if (m < a.M && n < a.N) store_out4(a, m, n, f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]});
+            }
+          continue;
         }
+        if (pass && !wide) continue;
+        // a pass: 16 columns of each tile of 32 as floats, all of them in 16 bits
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            if (wide) {
+              if (e / 8 == pass)
+                *reinterpret_cast<f32x4*>(own + r * kPitch + 64 * i + 4 * (2 * e - 16 * pass + 4 * h)) =
+                    f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+            } else {
+              *reinterpret_cast<u32x2*>(own + r * kPitch + 64 * i + 2 * (2 * e + 4 * h)) =
+                  pack_out4(a.y_dtype, f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]});
+            }
+          }
+#pragma unroll
+        for (int c = 0; c < 2 * NT; ++c) {  // 16 bytes a lane, 4 NT lanes a row
+          const int row = (64 * c + lane) / (4 * NT), col = (64 * c + lane) % (4 * NT);  // (in order: LDS answers a wave so)
+          const int m = m0 + 32 * j + row;
+          // of tile col / 4: floats 16 pass + 4 (col % 4) .., or 16-bit outputs 8 (col % 4) ..
+          const int n = n0 + 32 * NT * w + 32 * (col / 4) + (wide ? 16 * pass + 4 * (col % 4) : 8 * (col % 4));
+          const u32x4 v = *reinterpret_cast<const u32x4*>(own + row * kPitch + 16 * col);
+          if (m < a.M && n < a.N) *reinterpret_cast<u32x4*>(static_cast<char*>(a.y) + ((size_t)m * a.N + n) * size) = v;
+        }
+      }
     }
   } else {
     __syncthreads();  // everybody is done with x's tiles
@@ -272,26 +320,32 @@ __global__ __launch_bounds__(256, 2) void mx_gemm_kernel(const MxProduct a) {
   }
 }
 
-template <bool SCORE>
-int launch(const MxProduct& p, MxKind kind, hipStream_t st) {
-  constexpr int MT = 4;
-  const long long tiles = ((long long)p.N + kTileN - 1) / kTileN * ((p.M + 32LL * MT - 1) / (32 * MT));
-  if (tiles > (1 << 23) || (kind != MX_X4 && 2 * p.x_stride * 32 * MT > 0x7FFFFFFFLL)) return Q4D_ERR_SHAPE;  // a tile's offsets are 32 bits
-  const dim3 grid((unsigned)tiles);
-  if (kind == MX_X4) {
-    if constexpr (SCORE) return Q4D_ERR_DTYPE;
-    else hipLaunchKernelGGL((mx_gemm_kernel<MX_X4, false, MT>), grid, dim3(256), 0, st, p);
-  } else if (kind == MX_BF16) {
-    hipLaunchKernelGGL((mx_gemm_kernel<MX_BF16, SCORE, MT>), grid, dim3(256), 0, st, p);
-  } else {
-    hipLaunchKernelGGL((mx_gemm_kernel<MX_F16, SCORE, MT>), grid, dim3(256), 0, st, p);
-  }
+// 256 x 128 tiles two a CU; where those are fewer than the device holds, 256 x 64 three a CU; where those
+// leave CUs idle 128 x 64.
+template <MxKind KIND, bool SCORE, int NT, int MT, int RING, int PER_CU>
+int launch(const MxProduct& p, hipStream_t st) {
+  const long long tiles = (p.N + 128LL * NT - 1) / (128 * NT) * ((p.M + 32LL * MT - 1) / (32 * MT));
+  if (tiles > (1 << 23) || (KIND != MX_X4 && 2 * p.x_stride * 32 * MT > 0x7FFFFFFFLL)) return Q4D_ERR_SHAPE;  // a tile's offsets are 32 bits
+  hipLaunchKernelGGL((mx_gemm_kernel<KIND, SCORE, NT, MT, RING, PER_CU>), dim3((unsigned)tiles), dim3(256), 0, st, p);
   return check_launch();
+}
+template <MxKind KIND>
+int launch(const MxProduct& p, hipStream_t st) {
+  const auto tiles = [&](int n, int m) { return (p.N + (long long)n - 1) / n * ((p.M + (long long)m - 1) / m); };
+  const int cus = device_cus();
+  if (tiles(256, 128) >= 2 * cus) return launch<KIND, false, 2, 4, 3, 2>(p, st);
+  if (tiles(256, 64) >= cus) return launch<KIND, false, 2, 2, 3, KIND == MX_X4 ? 2 : 3>(p, st);
+  return launch<KIND, false, 1, 2, KIND == MX_X4 ? 5 : 6, 2>(p, st);
 }
 
 }  // namespace
 
-int launch_mx_gemm(const MxProduct& p, MxKind kind, hipStream_t st) { return launch<false>(p, kind, st); }
-int launch_mx_gemm_score(const MxProduct& p, MxKind kind, hipStream_t st) { return launch<true>(p, kind, st); }
+int launch_mx_gemm(const MxProduct& p, MxKind kind, hipStream_t st) {
+  if (kind == MX_X4) return launch<MX_X4>(p, st);
+  return kind == MX_BF16 ? launch<MX_BF16>(p, st) : launch<MX_F16>(p, st);
+}
+int launch_mx_gemm_score(const MxProduct& p, MxKind kind, hipStream_t st) {
+  return kind == MX_BF16 ? launch<MX_BF16, true, 2, 4, 3, 2>(p, st) : launch<MX_F16, true, 2, 4, 3, 2>(p, st);
+}
 
 }  // namespace q4d
