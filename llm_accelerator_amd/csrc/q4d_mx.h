@@ -34,7 +34,7 @@ int launch_mx_rows_score(const MxProduct& p, MxKind kind, hipStream_t st);
 int mx_rows_parts(int M, int N);
 // Few rows and many weights (q4d_mx_head.hip), where x fits in LDS.
 bool mx_head_fits(int M, int K);
-int mx_head_parts(int M, int N, int K);
+int mx_head_parts(int N);
 int launch_mx_head(const MxProduct& p, MxKind kind, hipStream_t st);
 int launch_mx_head_score(const MxProduct& p, MxKind kind, hipStream_t st);
 int launch_mx_gemm(const MxProduct& p, MxKind kind, hipStream_t st);

@@ -320,8 +320,6 @@ __global__ __launch_bounds__(256, PER_CU) void mx_gemm_kernel(const MxProduct a)
   }
 }
 
-// 256 x 128 tiles two a CU; where those are fewer than the device holds, 256 x 64 three a CU; where those
-// leave CUs idle 128 x 64.
 template <MxKind KIND, bool SCORE, int NT, int MT, int RING, int PER_CU>
 int launch(const MxProduct& p, hipStream_t st) {
   const long long tiles = (p.N + 128LL * NT - 1) / (128 * NT) * ((p.M + 32LL * MT - 1) / (32 * MT));
@@ -329,12 +327,19 @@ int launch(const MxProduct& p, hipStream_t st) {
   hipLaunchKernelGGL((mx_gemm_kernel<KIND, SCORE, NT, MT, RING, PER_CU>), dim3((unsigned)tiles), dim3(256), 0, st, p);
   return check_launch();
 }
+// Tiles of 256 x 64, three blocks a CU (two with x in 4 bits); 128 x 64 where those are no more than one a CU:
+// 1024 x 4096 x 4096 in 16 bits 42 / 39 us, 512 x 16384 x 1024 (two a CU) 20 / 24.  With x in 4 bits, whose
+// products take a quarter of the time their operands are moved for, 256 x 128 where that gives two a CU:
+// 4096 x 8192 x 4096 78 instead of 98 us, 2000 x 4096 x 4096 (one a CU) 31 instead of 28; in 16 bits the
+// larger tile is no faster (8192 x 8192 x 8192 864 instead of 844, 2000 x 16384 x 1024 66 instead of 68).
 template <MxKind KIND>
 int launch(const MxProduct& p, hipStream_t st) {
   const auto tiles = [&](int n, int m) { return (p.N + (long long)n - 1) / n * ((p.M + (long long)m - 1) / m); };
   const int cus = device_cus();
-  if (tiles(256, 128) >= 2 * cus) return launch<KIND, false, 2, 4, 3, 2>(p, st);
-  if (tiles(256, 64) >= cus) return launch<KIND, false, 2, 2, 3, KIND == MX_X4 ? 2 : 3>(p, st);
+  if constexpr (KIND == MX_X4) {
+    if (tiles(256, 128) >= 2 * cus) return launch<KIND, false, 2, 4, 3, 2>(p, st);
+  }
+  if (tiles(256, 64) > cus) return launch<KIND, false, 2, 2, 3, KIND == MX_X4 ? 2 : 3>(p, st);
   return launch<KIND, false, 1, 2, KIND == MX_X4 ? 5 : 6, 2>(p, st);
 }
 
@@ -345,7 +350,10 @@ int launch_mx_gemm(const MxProduct& p, MxKind kind, hipStream_t st) {
   return kind == MX_BF16 ? launch<MX_BF16>(p, st) : launch<MX_F16>(p, st);
 }
 int launch_mx_gemm_score(const MxProduct& p, MxKind kind, hipStream_t st) {
-  return kind == MX_BF16 ? launch<MX_BF16, true, 2, 4, 3, 2>(p, st) : launch<MX_F16, true, 2, 4, 3, 2>(p, st);
+  // (the larger tile where it gives two a CU, which leaves fewer sums: 2000 rows of 151936 x 1024 540 instead of 560 us)
+  if ((p.N + 255LL) / 256 * ((p.M + 127LL) / 128) >= 2LL * device_cus())
+    return kind == MX_BF16 ? launch<MX_BF16, true, 2, 4, 3, 2>(p, st) : launch<MX_F16, true, 2, 4, 3, 2>(p, st);
+  return kind == MX_BF16 ? launch<MX_BF16, true, 2, 2, 3, 3>(p, st) : launch<MX_F16, true, 2, 2, 3, 3>(p, st);
 }
 
 }  // namespace q4d

@@ -1,8 +1,8 @@
 // Products of up to 64 rows of 16-bit x with many microscaled 4-bit weights, as an output head's (gfx950,
 // wave64): y = x W^T, and the score of given outputs (see q4d_mx_gemm.hip).
 //
-// x lies in LDS as the matrix instruction's operands, made once a block; a wave streams tiles of 32
-// weight rows through registers, kAhead tile columns ahead (2 KB each), and needs no other wave until its
+// x lies in LDS as the matrix instruction's operands, made once a block; a wave streams units of 16 NT
+// weight rows through registers, kAhead tile columns ahead (1 KB a unit), and needs no other wave until its
 // end.  The operands and their order are those of q4d_mx_rows.hip.  A score's waves keep the softmax's
 // sums of their outputs, so that a block leaves one set a row.
 // Bound by the weight stream.
@@ -16,9 +16,9 @@
 namespace q4d {
 namespace {
 
-constexpr int kAhead = 8;
+constexpr int kAhead = 4;
 constexpr int kHeadLds = 128 << 10;  // x's operands at most
-constexpr int kHeadBlocks = 256;     // one or two a CU
+constexpr int kHeadBlocks = 256;     // one a CU
 
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -28,31 +28,32 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <bool BF, int MT, int NW, bool SCORE>
+template <bool BF, int MT, int NT, int NW, bool SCORE>
 __global__ __launch_bounds__(64 * NW) void mx_head_kernel(const MxProduct a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];  // [column tile][4 parts j][MT][64 lanes][16 bytes]
   const int t = threadIdx.x, lane = t & 63, r = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int steps = mx_col_tiles(a.K), tiles = mx_row_tiles(a.N), stride = gridDim.x * NW;
+  const int steps = mx_col_tiles(a.K), units = (a.N + 16 * NT - 1) / (16 * NT), stride = gridDim.x * NW;
 
   struct Step {
-    u32x4 w[2];
-    uint32_t s[2];
+    u32x4 w[NT];
+    uint32_t s[NT];
   } ring[kAhead];
-  // The wave's steps in order: (tile, column tile); `ahead` names the next to load.
-  int tile = blockIdx.x * NW + w, ahead_tile = tile, ahead = 0;
+  // The wave's steps in order: (unit, column tile); `ahead` names the next to load.
+  int unit = blockIdx.x * NW + w, ahead_unit = unit, ahead = 0;
   const auto load = [&](Step& s) {
-    const size_t at = (size_t)min(ahead_tile, tiles - 1) * steps + ahead;  // (past the last: not used)
-    const uint8_t* p = a.w + at * kMxTile + g * (kMxRows * 16) + r * 16;
-    const uint8_t* q = a.ws + at * kMxScales + 4 * r + g;
+    const int u = min(ahead_unit, units - 1), half = NT == 1 ? u & 1 : 0;  // (past the last: not used)
+    const size_t at = (size_t)(NT == 1 ? u >> 1 : u) * steps + ahead;
+    const uint8_t* p = a.w + at * kMxTile + g * (kMxRows * 16) + (16 * half + r) * 16;
+    const uint8_t* q = a.ws + at * kMxScales + 4 * (16 * half + r) + g;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < NT; ++k) {
       s.w[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + 256 * k));
       s.s[k] = q[64 * k];
     }
     if (++ahead == steps) {
       ahead = 0;
-      ahead_tile += stride;
+      ahead_unit += stride;
     }
   };
 #pragma unroll
@@ -67,10 +68,10 @@ __global__ __launch_bounds__(64 * NW) void mx_head_kernel(const MxProduct a) {
   }
   __syncthreads();
 
-  f32x4 acc[2][MT];
+  f32x4 acc[NT][MT];
   const auto clear = [&]() {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < NT; ++k)
 #pragma unroll
       for (int i = 0; i < MT; ++i) acc[k][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   };
@@ -83,46 +84,47 @@ __global__ __launch_bounds__(64 * NW) void mx_head_kernel(const MxProduct a) {
       target[i] = 16 * i + r < a.M ? a.targets[16 * i + r] : -1;
     }
   }
-  // lane (r, g) holds outputs 32 tile + 16 k + 4 g .. + 3 of x's row 16 i + r
+  // lane (r, g) holds outputs 16 (NT unit + k) + 4 g .. + 3 of x's row 16 i + r
   const auto finish = [&]() {
-    const int n0 = kMxRows * tile + 4 * g;
+    const int n0 = 16 * NT * unit + 4 * g;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       if constexpr (!SCORE) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < NT; ++k)
           if (16 * i + r < a.M && n0 + 16 * k < a.N) store_out4(a, 16 * i + r, n0 + 16 * k, acc[k][i]);
       } else {
-        float z[8], top = -INFINITY;
+        float z[4 * NT], top = -INFINITY;
         const int hit = target[i] - n0;  // 16 k + e of the lane's
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < 4 * NT; ++c) {
           const int n = 16 * (c >> 2) + (c & 3);
           if (hit == n && n0 + n < a.N) a.hit[16 * i + r] = acc[c >> 2][i][c & 3];
           z[c] = n0 + n < a.N ? acc[c >> 2][i][c & 3] : -INFINITY;
           top = fmaxf(top, z[c]);
         }
-        sums[i] = soft_join(sums[i], soft_sum<8>(top, [&](int c) { return z[c]; }));
+        sums[i] = soft_join(sums[i], soft_sum<4 * NT>(top, [&](int c) { return z[c]; }));
       }
     }
   };
 
   clear();
   int step = 0;
-  while (tile < tiles) {
+  while (unit < units) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (tile >= tiles) break;
+      if (unit >= units) break;
       const char* x = lds + step * (4 * MT * 1024) + 16 * lane;
-      const float f0 = mx_scale(ring[u].s[0]), f1 = mx_scale(ring[u].s[1]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const u32x4 v0 = mx_dequant8<BF>(ring[u].w[0][j], f0), v1 = mx_dequant8<BF>(ring[u].w[1][j], f1);
+        u32x4 v[NT];
+#pragma unroll
+        for (int k = 0; k < NT; ++k) v[k] = mx_dequant8<BF>(ring[u].w[k][j], mx_scale(ring[u].s[k]));
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           const u32x4 xv = *reinterpret_cast<const u32x4*>(x + (j * MT + i) * 1024);
-          acc[0][i] = mfma16<BF>(v0, xv, acc[0][i]);
-          acc[1][i] = mfma16<BF>(v1, xv, acc[1][i]);
+#pragma unroll
+          for (int k = 0; k < NT; ++k) acc[k][i] = mfma16<BF>(v[k], xv, acc[k][i]);
         }
       }
       load(ring[u]);
@@ -130,7 +132,7 @@ __global__ __launch_bounds__(64 * NW) void mx_head_kernel(const MxProduct a) {
         finish();
         clear();
         step = 0;
-        tile += stride;
+        unit += stride;
       }
     }
   }
@@ -165,22 +167,19 @@ __global__ __launch_bounds__(64 * NW) void mx_head_kernel(const MxProduct a) {
 
 int row_tiles16(int M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
 size_t lds_bytes(int M, int K) { return (size_t)mx_col_tiles(K) * 4 * row_tiles16(M) * 1024; }
-// Waves of a block, and blocks: as many as fit, but no wave without a tile.
-constexpr int kWaves = 4, kWavesMost = 8;
-int head_waves(int M) { return row_tiles16(M) == 4 ? kWavesMost : kWaves; }
-int head_blocks(int M, int N, int K) {
-  const int waves = head_waves(M), fit = lds_bytes(M, K) <= 72 << 10 ? 2 : 1;
-  return std::max(1, std::min(kHeadBlocks * fit, (mx_row_tiles(N) + waves - 1) / waves));
+constexpr int kWaves = 8, kUnit = 2;  // waves of a block, NT
+int head_blocks(int N) {
+  return (int)std::min((long long)kHeadBlocks, (N + 16LL * kUnit * kWaves - 1) / (16 * kUnit * kWaves));
 }
 
 template <bool BF, bool SCORE>
 int launch(const MxProduct& p, hipStream_t st) {
-  const dim3 grid((unsigned)head_blocks(p.M, p.N, p.K));
+  const dim3 grid((unsigned)head_blocks(p.N)), block(64 * kWaves);
   const size_t bytes = lds_bytes(p.M, p.K);
   switch (row_tiles16(p.M)) {
-    case 1: hipLaunchKernelGGL((mx_head_kernel<BF, 1, kWaves, SCORE>), grid, dim3(64 * kWaves), bytes, st, p); break;
-    case 2: hipLaunchKernelGGL((mx_head_kernel<BF, 2, kWaves, SCORE>), grid, dim3(64 * kWaves), bytes, st, p); break;
-    default: hipLaunchKernelGGL((mx_head_kernel<BF, 4, kWavesMost, SCORE>), grid, dim3(64 * kWavesMost), bytes, st, p);
+    case 1: hipLaunchKernelGGL((mx_head_kernel<BF, 1, kUnit, kWaves, SCORE>), grid, block, bytes, st, p); break;
+    case 2: hipLaunchKernelGGL((mx_head_kernel<BF, 2, kUnit, kWaves, SCORE>), grid, block, bytes, st, p); break;
+    default: hipLaunchKernelGGL((mx_head_kernel<BF, 4, kUnit, kWaves, SCORE>), grid, block, bytes, st, p);
   }
   return check_launch();
 }
@@ -188,7 +187,7 @@ int launch(const MxProduct& p, hipStream_t st) {
 }  // namespace
 
 bool mx_head_fits(int M, int K) { return M <= 64 && lds_bytes(M, K) <= (size_t)kHeadLds; }
-int mx_head_parts(int M, int N, int K) { return head_blocks(M, N, K); }
+int mx_head_parts(int N) { return head_blocks(N); }
 int launch_mx_head(const MxProduct& p, MxKind kind, hipStream_t st) {
   return kind == MX_BF16 ? launch<true, false>(p, st) : launch<false, false>(p, st);
 }

@@ -156,11 +156,16 @@ int launch(const MxProduct& p, hipStream_t st) {
   hipLaunchKernelGGL((mx_rows_kernel<KIND, MT, NT, NW, false>), grid, dim3(64 * NW), 0, st, p);
   return check_launch();
 }
+// 16 weight rows a block where those are at most one a CU, else 32, which share what is loaded of x: one row of
+// 4096 x 1024 3.2 / 3.4 us, 16 of 8192 x 1024 4.7 / 4.1, 64 of 4096 x 4096 17.8 / 11.3.  64 for very many (16 rows
+// of 24000 x 1024 6.7 / 6.6).  Eight waves where K is long (one row of 8192 x 8192 10.2 instead of 12.5 us).
 template <MxKind KIND, int MT>
 int launch(const MxProduct& p, hipStream_t st) {
-  // Many weight rows: four or two tiles of them share what is loaded of x.
-  if (p.N >= 32768) return launch<KIND, MT, MT == 4 ? 2 : 4, 4>(p, st);
-  return p.K > 1024 ? launch<KIND, MT, 1, 8>(p, st) : launch<KIND, MT, 1, 4>(p, st);
+  const long long blocks = (p.N + 15LL) / 16 * ((p.M + 16LL * MT - 1) / (16 * MT));
+  const bool deep = p.K > 1024;
+  if (p.N >= 32768 && !deep) return launch<KIND, MT, MT == 4 ? 2 : 4, 4>(p, st);
+  if (blocks > device_cus()) return deep ? launch<KIND, MT, 2, 8>(p, st) : launch<KIND, MT, 2, 4>(p, st);
+  return deep ? launch<KIND, MT, 1, 8>(p, st) : launch<KIND, MT, 1, 4>(p, st);
 }
 template <MxKind KIND>
 int launch(const MxProduct& p, hipStream_t st) {

@@ -56,18 +56,33 @@ int check_y(const void* y, int32_t y_dtype) {
   if (y_dtype != Q4D_F16 && y_dtype != Q4D_BF16 && y_dtype != Q4D_F32) return Q4D_ERR_DTYPE;
   return aligned(y, 16) ? Q4D_OK : Q4D_ERR_BAD_ADDR;
 }
-constexpr int kHeadRows = 32768;  // weight rows from which q4d_mx_head.hip takes a few rows
-bool use_head(int M, int N, int K) { return M <= kMxFewRows && N >= kHeadRows && mx_head_fits(M, K); }
+// Few outputs go to the kernel of few rows, which reads x once a weight tile but whose waves share K: with 16-bit
+// x up to 750000 (64 rows of 8192 x 1024 7.6 us, tiles of many rows 9.8; 64 of 16384 11.6 / 10.1; 128 of 4096 x 4096
+// 21 / 28), with x in 4 bits, a quarter of the bytes, up to a million or 16 rows (64 of 16384 x 1024 5.3 / 6.0, 128 of
+// 16384 9.0 / 6.4, 16 of 151936 18.2 / 19.8).  Up to 32 rows of many more weights: the kernel that holds x in
+// LDS (24 rows of 151936 x 1024 22 us, tiles 29; 48 rows 32 / 31).
+constexpr long long kFewOutputs = 750000, kFewOutputs4 = 1000000;
+constexpr int kHeadRows = 49152;
 int product(const MxProduct& p, MxKind kind, hipStream_t st) {
-  if (kind != MX_X4 && use_head(p.M, p.N, p.K)) return launch_mx_head(p, kind, st);
-  return p.M <= kMxFewRows ? launch_mx_rows(p, kind, st) : launch_mx_gemm(p, kind, st);
+  const long long outputs = (long long)p.M * p.N;
+  if (kind == MX_X4) return outputs <= kFewOutputs4 || p.M <= 16 ? launch_mx_rows(p, kind, st) : launch_mx_gemm(p, kind, st);
+  if (outputs <= kFewOutputs) return launch_mx_rows(p, kind, st);
+  return p.M <= 32 && p.N >= kHeadRows && mx_head_fits(p.M, p.K) ? launch_mx_head(p, kind, st) : launch_mx_gemm(p, kind, st);
+}
+// A score's kernels: the same three, few outputs being up to 1100000 and 64 rows (32 rows of 32000 x 1024 13.8 us,
+// tiles 15.2; 48 rows 22 / 16; 64 of 8000 x 1024 10.9 / 15.6).
+constexpr long long kFewScores = 1100000;
+enum ScorePath { SCORE_ROWS, SCORE_HEAD, SCORE_TILES };
+ScorePath score_path(int M, int N, int K) {
+  if (M <= 32 && N >= kHeadRows && mx_head_fits(M, K)) return SCORE_HEAD;
+  return M <= 16 || (M <= kMxFewRows && (long long)M * N <= kFewScores) ? SCORE_ROWS : SCORE_TILES;
 }
 MxKind kind_of(int32_t x_dtype) { return x_dtype == Q4D_BF16 ? MX_BF16 : MX_F16; }
 
 size_t hit_bytes(int M) { return align_up((size_t)M * 4, 256); }
 int score_parts(int M, int N, int K) {
-  if (use_head(M, N, K)) return mx_head_parts(M, N, K);
-  return M <= kMxFewRows ? mx_rows_parts(M, N) : mx_gemm_parts(N);
+  const ScorePath path = score_path(M, N, K);
+  return path == SCORE_HEAD ? mx_head_parts(N) : path == SCORE_ROWS ? mx_rows_parts(M, N) : mx_gemm_parts(N);
 }
 
 }  // namespace
@@ -137,8 +152,9 @@ extern "C" int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, i
   p.stats = ws_ptr<f32x4>(ws, hit_bytes(M));
   const int parts = score_parts(M, p.N, p.K);
   const MxKind kind = kind_of(x_dtype);
-  if (use_head(M, p.N, p.K)) rc = launch_mx_head_score(p, kind, st);
-  else rc = M <= kMxFewRows ? launch_mx_rows_score(p, kind, st) : launch_mx_gemm_score(p, kind, st);
+  const ScorePath path = score_path(M, p.N, p.K);
+  if (path == SCORE_HEAD) rc = launch_mx_head_score(p, kind, st);
+  else rc = path == SCORE_ROWS ? launch_mx_rows_score(p, kind, st) : launch_mx_gemm_score(p, kind, st);
   if (rc) return rc;
   const JoinArgs j = {p.stats, p.hit, targets, parts, M, p.N, logprob, entropy, best};
   hipLaunchKernelGGL(mx_score_join_kernel, dim3((unsigned)M), dim3(256), 0, st, j);
