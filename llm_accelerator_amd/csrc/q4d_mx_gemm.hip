@@ -350,9 +350,6 @@ int launch_mx_gemm(const MxProduct& p, MxKind kind, hipStream_t st) {
   return kind == MX_BF16 ? launch<MX_BF16>(p, st) : launch<MX_F16>(p, st);
 }
 int launch_mx_gemm_score(const MxProduct& p, MxKind kind, hipStream_t st) {
-  // (the larger tile where it gives two a CU, which leaves fewer sums: 2000 rows of 151936 x 1024 540 instead of 560 us)
-  if ((p.N + 255LL) / 256 * ((p.M + 127LL) / 128) >= 2LL * device_cus())
-    return kind == MX_BF16 ? launch<MX_BF16, true, 2, 4, 3, 2>(p, st) : launch<MX_F16, true, 2, 4, 3, 2>(p, st);
   return kind == MX_BF16 ? launch<MX_BF16, true, 2, 2, 3, 3>(p, st) : launch<MX_F16, true, 2, 2, 3, 3>(p, st);
 }
 

@@ -1,4 +1,4 @@
-// Products of up to 64 rows of 16-bit x with many microscaled 4-bit weights, as an output head's (gfx950,
+// Products of up to 32 rows of 16-bit x with many microscaled 4-bit weights, as an output head's (gfx950,
 // wave64): y = x W^T, and the score of given outputs (see q4d_mx_gemm.hip).
 //
 // x lies in LDS as the matrix instruction's operands, made once a block; a wave streams units of 16 NT
@@ -16,9 +16,10 @@
 namespace q4d {
 namespace {
 
-constexpr int kAhead = 4;
+constexpr int kAhead = 3;
 constexpr int kHeadLds = 128 << 10;  // x's operands at most
 constexpr int kHeadBlocks = 256;     // one a CU
+constexpr int kWavesLeast = 8, kWavesMost = 16;
 
 template <bool BF>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -28,19 +29,19 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <bool BF, int MT, int NT, int NW, bool SCORE>
-__global__ __launch_bounds__(64 * NW) void mx_head_kernel(const MxProduct a) {
+template <bool BF, int MT, int NT, bool SCORE>
+__global__ __launch_bounds__(64 * kWavesMost) void mx_head_kernel(const MxProduct a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];  // [column tile][4 parts j][MT][64 lanes][16 bytes]
   const int t = threadIdx.x, lane = t & 63, r = lane & 15, g = lane >> 4;
-  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int steps = mx_col_tiles(a.K), units = (a.N + 16 * NT - 1) / (16 * NT), stride = gridDim.x * NW;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6), waves = blockDim.x >> 6;
+  const int steps = mx_col_tiles(a.K), units = (a.N + 16 * NT - 1) / (16 * NT), stride = gridDim.x * waves;
 
   struct Step {
     u32x4 w[NT];
     uint32_t s[NT];
   } ring[kAhead];
   // The wave's steps in order: (unit, column tile); `ahead` names the next to load.
-  int unit = blockIdx.x * NW + w, ahead_unit = unit, ahead = 0;
+  int unit = blockIdx.x * waves + w, ahead_unit = unit, ahead = 0;
   const auto load = [&](Step& s) {
     const int u = min(ahead_unit, units - 1), half = NT == 1 ? u & 1 : 0;  // (past the last: not used)
     const size_t at = (size_t)(NT == 1 ? u >> 1 : u) * steps + ahead;
@@ -59,7 +60,7 @@ __global__ __launch_bounds__(64 * NW) void mx_head_kernel(const MxProduct a) {
 #pragma unroll
   for (int u = 0; u < kAhead; ++u) load(ring[u]);
 
-  for (int c = t; c < steps * 16 * (16 * MT); c += 64 * NW) {  // 16-byte groups of x, along its rows
+  for (int c = t; c < steps * 16 * (16 * MT); c += blockDim.x) {  // 16-byte groups of x, along its rows
     const int m = c / (steps * 16), k = c - m * (steps * 16);
     u32x4 v = {0u, 0u, 0u, 0u};
     if (m < a.M && 8 * k < a.K) v = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.x) + m * a.x_stride + 8 * k);
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(64 * NW) void mx_head_kernel(const MxProduct a) {
 
   if constexpr (SCORE) {
     __syncthreads();  // everybody is done with x
-    float* s_stat = reinterpret_cast<float*>(lds);  // [NW][16 MT][3]
+    float* s_stat = reinterpret_cast<float*>(lds);  // [waves][16 MT][3]
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       SoftSum s = sums[i];
@@ -155,8 +156,7 @@ __global__ __launch_bounds__(64 * NW) void mx_head_kernel(const MxProduct a) {
     __syncthreads();
     if (t < 16 * MT && t < a.M) {
       SoftSum s = {s_stat[t * 3], s_stat[t * 3 + 1], s_stat[t * 3 + 2]};
-#pragma unroll
-      for (int v = 1; v < NW; ++v) {
+      for (int v = 1; v < waves; ++v) {
         const float* at = s_stat + (v * 16 * MT + t) * 3;
         s = soft_join(s, SoftSum{at[0], at[1], at[2]});
       }
@@ -165,29 +165,36 @@ __global__ __launch_bounds__(64 * NW) void mx_head_kernel(const MxProduct a) {
   }
 }
 
-int row_tiles16(int M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }
-size_t lds_bytes(int M, int K) { return (size_t)mx_col_tiles(K) * 4 * row_tiles16(M) * 1024; }
-constexpr int kWaves = 8, kUnit = 2;  // waves of a block, NT
-int head_blocks(int N) {
-  return (int)std::min((long long)kHeadBlocks, (N + 16LL * kUnit * kWaves - 1) / (16 * kUnit * kWaves));
+constexpr int kUnit = 2;  // NT
+size_t lds_bytes(int M, int K) { return (size_t)mx_col_tiles(K) * 4 * (M <= 16 ? 1 : 2) * 1024; }
+struct Shape {
+  int blocks, waves;
+};
+// One block a CU, of as many waves as leave the fewest places without a unit in the last round (an LM head of 151936
+// rows: 10 waves have two rounds, 93 % full; 8 would have three, 77 %).
+Shape head_shape(int N) {
+  const int units = (int)((N + 16LL * kUnit - 1) / (16 * kUnit));
+  const int blocks = std::min(kHeadBlocks, (units + kWavesLeast - 1) / kWavesLeast), each = (units + blocks - 1) / blocks;
+  int best = kWavesLeast;
+  for (int w = kWavesLeast; w <= kWavesMost; ++w)
+    if ((each + w - 1) / w * w < (each + best - 1) / best * best) best = w;
+  return {blocks, best};
 }
 
 template <bool BF, bool SCORE>
 int launch(const MxProduct& p, hipStream_t st) {
-  const dim3 grid((unsigned)head_blocks(p.N)), block(64 * kWaves);
+  const Shape s = head_shape(p.N);
+  const dim3 grid(s.blocks), block(64 * s.waves);
   const size_t bytes = lds_bytes(p.M, p.K);
-  switch (row_tiles16(p.M)) {
-    case 1: hipLaunchKernelGGL((mx_head_kernel<BF, 1, kUnit, kWaves, SCORE>), grid, block, bytes, st, p); break;
-    case 2: hipLaunchKernelGGL((mx_head_kernel<BF, 2, kUnit, kWaves, SCORE>), grid, block, bytes, st, p); break;
-    default: hipLaunchKernelGGL((mx_head_kernel<BF, 4, kUnit, kWaves, SCORE>), grid, block, bytes, st, p);
-  }
+  if (p.M <= 16) hipLaunchKernelGGL((mx_head_kernel<BF, 1, kUnit, SCORE>), grid, block, bytes, st, p);
+  else hipLaunchKernelGGL((mx_head_kernel<BF, 2, kUnit, SCORE>), grid, block, bytes, st, p);
   return check_launch();
 }
 
 }  // namespace
 
-bool mx_head_fits(int M, int K) { return M <= 64 && lds_bytes(M, K) <= (size_t)kHeadLds; }
-int mx_head_parts(int N) { return head_blocks(N); }
+bool mx_head_fits(int M, int K) { return M <= 32 && lds_bytes(M, K) <= (size_t)kHeadLds; }
+int mx_head_parts(int N) { return head_shape(N).blocks; }
 int launch_mx_head(const MxProduct& p, MxKind kind, hipStream_t st) {
   return kind == MX_BF16 ? launch<true, false>(p, st) : launch<false, false>(p, st);
 }

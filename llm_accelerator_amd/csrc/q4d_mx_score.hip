@@ -67,14 +67,14 @@ int product(const MxProduct& p, MxKind kind, hipStream_t st) {
   const long long outputs = (long long)p.M * p.N;
   if (kind == MX_X4) return outputs <= kFewOutputs4 || p.M <= 16 ? launch_mx_rows(p, kind, st) : launch_mx_gemm(p, kind, st);
   if (outputs <= kFewOutputs) return launch_mx_rows(p, kind, st);
-  return p.M <= 32 && p.N >= kHeadRows && mx_head_fits(p.M, p.K) ? launch_mx_head(p, kind, st) : launch_mx_gemm(p, kind, st);
+  return p.N >= kHeadRows && mx_head_fits(p.M, p.K) ? launch_mx_head(p, kind, st) : launch_mx_gemm(p, kind, st);
 }
 // A score's kernels: the same three, few outputs being up to 1100000 and 64 rows (32 rows of 32000 x 1024 13.8 us,
 // tiles 15.2; 48 rows 22 / 16; 64 of 8000 x 1024 10.9 / 15.6).
 constexpr long long kFewScores = 1100000;
 enum ScorePath { SCORE_ROWS, SCORE_HEAD, SCORE_TILES };
 ScorePath score_path(int M, int N, int K) {
-  if (M <= 32 && N >= kHeadRows && mx_head_fits(M, K)) return SCORE_HEAD;
+  if (N >= kHeadRows && mx_head_fits(M, K)) return SCORE_HEAD;
   return M <= 16 || (M <= kMxFewRows && (long long)M * N <= kFewScores) ? SCORE_ROWS : SCORE_TILES;
 }
 MxKind kind_of(int32_t x_dtype) { return x_dtype == Q4D_BF16 ? MX_BF16 : MX_F16; }
