@@ -131,15 +131,16 @@ def test_two_graphs_side_by_side(dev):
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             out = all_calls(x, head, t, logits)
-        made.append((g, out, [v.clone() for v in all_calls(x, head, t, logits)]))
+        # (the graph reads x, t and logits where they are: they are kept)
+        made.append((g, out, [v.clone() for v in all_calls(x, head, t, logits)], (x, t, logits)))
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in made]
     for _ in range(5):
-        for s, (g, _, _) in zip(streams, made):
+        for s, (g, _, _, _) in zip(streams, made):
             with torch.cuda.stream(s):
                 g.replay()
     torch.cuda.synchronize()
-    for _, out, want in made:
+    for _, out, want, _ in made:
         for a, b in zip(out, want):
             assert torch.equal(a.nan_to_num(nan=7.0) if a.is_floating_point() else a, b.nan_to_num(nan=7.0) if b.is_floating_point() else b)
 
