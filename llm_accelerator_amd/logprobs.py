@@ -19,6 +19,7 @@ from .model import call_on
 
 MAX_TOP = 32
 MAX_VOCAB = 1 << 20
+SMALL_WORKSPACE = 1 << 15  # bytes that the results may keep alive beside them
 _DTYPES = {torch.float16: Q4D_F16, torch.bfloat16: Q4D_BF16, torch.float32: Q4D_F32}
 
 
@@ -54,23 +55,24 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     x = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
     if (vocab > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < vocab):
         x = x.contiguous()
-    rows = x.shape[0]
-    # the results lie side by side in one allocation
-    got = x.new_empty(rows * (3 + 2 * top), dtype=torch.float32)
-    logprob, entropy, rank, top_logprobs, top_ids = got.split((rows, rows, rows, rows * top, rows * top))
+    rows, have = x.shape[0], targets is not None
+    nbytes = _lib.load().q4d_token_logprobs_workspace_bytes(rows, vocab, top) if rows else 0
+    if rows and nbytes == 0:
+        raise _lib.Q4DecError(-11, "q4d_token_logprobs_workspace_bytes")
+    # the results lie side by side in one allocation, behind the workspace if that is small
+    inside = (nbytes + 3) // 4 if nbytes <= SMALL_WORKSPACE else 0
+    got = x.new_empty(inside + rows * (3 + 2 * top), dtype=torch.float32)
+    _, logprob, entropy, rank, top_logprobs, top_ids = got.split((inside, rows, rows, rows, rows * top, rows * top))
     if rows:
-        nbytes = _lib.load().q4d_token_logprobs_workspace_bytes(rows, vocab, top)
-        if nbytes == 0:
-            raise _lib.Q4DecError(-11, "q4d_token_logprobs_workspace_bytes")
-        ws, at, step, have = x.new_empty(nbytes, dtype=torch.uint8), got.data_ptr(), 4 * rows, targets is not None
+        ws = got if inside else x.new_empty(nbytes, dtype=torch.uint8)
+        at, step = got.data_ptr() + 4 * inside, 4 * rows
         call_on(index, "q4d_token_logprobs", x.data_ptr(), _DTYPES[x.dtype], x.stride(0), rows, vocab,
                 targets.data_ptr() if have else None, top, at if have else None, at + 2 * step if have else None, at + step,
                 at + 3 * step if top else None, at + (3 + top) * step if top else None, ws.data_ptr(), nbytes)
     if len(lead) != 1:
         logprob, entropy, rank = logprob.view(lead), entropy.view(lead), rank.view(lead)
     wide = (*lead, top)
-    return TokenLogprobs(logprob if targets is not None else None, rank.view(torch.int32) if targets is not None else None, entropy,
-                         top_logprobs.view(wide), top_ids.view(torch.int32).view(wide))
+    return TokenLogprobs(logprob if have else None, rank.view(torch.int32) if have else None, entropy, top_logprobs.view(wide), top_ids.view(torch.int32).view(wide))
 
 
 __all__ = ["TokenLogprobs", "token_logprobs", "MAX_TOP", "MAX_VOCAB"]

@@ -48,8 +48,8 @@ class MXTensor:
     """A matrix of microscaled 4-bit floats, from rows of codes ``packed`` uint8 [rows, cols/2] (the even
     column in the low nibble) and ``scale`` uint8 [rows, cols/32] (2^(scale - 127); 255: NaN).
 
-    It keeps a copy of its own in the order that the kernels read (``codes`` and ``scales``, tiles of 32
-    rows and 128 columns); :attr:`packed` and :attr:`scale` are the rows again, made at each access."""
+    It keeps a copy of its own in the order that the kernels read (:attr:`codes` and :attr:`scales`, tiles
+    of 32 rows and 128 columns); :attr:`packed` and :attr:`scale` are the rows again, made at each access."""
 
     def __init__(self, packed: torch.Tensor, scale: torch.Tensor):
         if packed.dtype != torch.uint8 or scale.dtype != torch.uint8:
@@ -63,30 +63,40 @@ class MXTensor:
             raise ValueError(f"packed is on {packed.device}, scale on {scale.device}")
         packed, scale = packed.contiguous(), scale.contiguous()
         if not packed.is_cuda:
-            self._setup(_order(packed, 16).transpose(2, 3).reshape(-1), _order(scale, 1).reshape(-1), rows, cols)
+            codes, scales = _order(packed, 16).transpose(2, 3).reshape(-1), _order(scale, 1).reshape(-1)
+            self._setup(torch.cat((codes, scales)), rows, cols)
             return
         if packed.data_ptr() % 4:
             packed = packed.clone()
         self._new(packed, rows, cols)
         call_on(self._index, "q4d_mx_pack", packed.data_ptr(), scale.data_ptr(), self._ref)
 
-    def _setup(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int) -> "MXTensor":
-        self.codes, self.scales, self.shape = codes, scales, (rows, cols)
-        self._desc = Q4dMX(codes.data_ptr(), scales.data_ptr(), rows, cols)
+    def _setup(self, memory: torch.Tensor, rows: int, cols: int) -> "MXTensor":
+        """Over ``memory``: the codes' bytes, then the scales'."""
+        at = memory.data_ptr()
+        self._memory, self.shape = memory, (rows, cols)
+        self._desc = Q4dMX(at, at + memory.numel() // 17 * 16, rows, cols)  # 2048 and 128 bytes a tile
         self._ref = ctypes.byref(self._desc)
-        self._index = codes.get_device()
+        self._index = memory.get_device()
         return self
 
     def _new(self, like: torch.Tensor, rows: int, cols: int) -> "MXTensor":
         """Memory for rows x cols on the device of ``like``."""
-        tiles = -(-rows // TILE_ROWS) * -(-cols // TILE_COLS)
-        return self._setup(like.new_empty(tiles * 2048, dtype=torch.uint8), like.new_empty(tiles * 128, dtype=torch.uint8), rows, cols)
+        return self._setup(like.new_empty(-(-rows // TILE_ROWS) * -(-cols // TILE_COLS) * 2176, dtype=torch.uint8), rows, cols)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._memory[:self._memory.numel() // 17 * 16]
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._memory[self._memory.numel() // 17 * 16:]
 
     def _rows(self) -> tuple[torch.Tensor, torch.Tensor]:
         rows, cols = self.shape
         if self._index >= 0:
-            packed = self.codes.new_empty((rows, cols // 2))
-            scale = self.codes.new_empty((rows, cols // BLOCK))
+            packed = self._memory.new_empty((rows, cols // 2))
+            scale = self._memory.new_empty((rows, cols // BLOCK))
             call_on(self._index, "q4d_mx_unpack", self._ref, packed.data_ptr(), scale.data_ptr())
             return packed, scale
         rt, kt = -(-rows // TILE_ROWS), -(-cols // TILE_COLS)
@@ -104,14 +114,14 @@ class MXTensor:
 
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self._memory.device
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self._memory.numel()
 
     def to(self, device) -> "MXTensor":
-        return MXTensor.__new__(MXTensor)._setup(self.codes.to(device), self.scales.to(device), *self.shape)
+        return MXTensor.__new__(MXTensor)._setup(self._memory.to(device), *self.shape)
 
     def numpy(self) -> tuple[np.ndarray, np.ndarray]:
         packed, scale = self._rows()
@@ -128,7 +138,7 @@ class MXTensor:
         if dtype not in _DTYPES:
             raise ValueError(f"dtype must be fp32, fp16 or bf16, got {dtype}")
         _on_gpu(self)
-        y = self.codes.new_empty(self.shape, dtype=dtype)
+        y = self._memory.new_empty(self.shape, dtype=dtype)
         call_on(self._index, "q4d_mx_dequantize", self._ref, y.data_ptr(), _DTYPES[dtype])
         return y
 
@@ -206,7 +216,7 @@ def mx_linear(x: torch.Tensor | MXTensor, weight: MXTensor, out_dtype: torch.dty
         y_kind = kind if out_dtype is None else out_dtype
         if y_kind not in _DTYPES:
             raise ValueError(f"out_dtype must be fp32, fp16 or bf16, got {y_kind}")
-        out = weight.codes.new_empty((*lead, n), dtype=y_kind)
+        out = weight._memory.new_empty((*lead, n), dtype=y_kind)
     else:
         y_kind = out.dtype
         if (y_kind not in _DTYPES or out_dtype not in (None, y_kind) or out.shape != (*lead, n) or not out.is_contiguous()
