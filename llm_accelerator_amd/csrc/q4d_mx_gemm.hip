@@ -7,7 +7,6 @@
 // with 16-bit x four 32x32x16 products of 8 columns a lane after the codes are made 16-bit floats, with x
 // in 4 bits one 32x32x64 product that takes codes and scales as they are.
 // The weights are the first operand, so that a lane holds outputs of one row of x.
-#include <float.h>
 #include <math.h>
 
 #include <type_traits>
@@ -263,8 +262,7 @@ __global__ __launch_bounds__(256, PER_CU) void mx_gemm_kernel(const MxProduct a)
   } else {
     __syncthreads();  // everybody is done with x's tiles
     float* s_stat = reinterpret_cast<float*>(lds);  // [4 waves][32 MT rows][3]
-    const bool part = n0 + kTileN > a.N;            // outputs past the last have the weight 0
-    const bool none = n0 + 64 * w >= a.N;           // ... and are all that the wave has
+    const bool part = n0 + kTileN > a.N;            // outputs past the last are as -Inf
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       const int m = m0 + 32 * j + r;
@@ -281,30 +279,41 @@ __global__ __launch_bounds__(256, PER_CU) void mx_gemm_kernel(const MxProduct a)
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (nb + 32 * i + 8 * (e >> 2) + (e & 3) >= a.N) acc[i][j][e] = -1e30f;
+            if (nb + 32 * i + 8 * (e >> 2) + (e & 3) >= a.N) acc[i][j][e] = -INFINITY;
       }
-      float top = -FLT_MAX;
+      float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, acc[i][j][e]);
       top = halves<false>(top);
+      const float base = top == -INFINITY ? 0.f : top;
       float l = 0.f, u = 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float d = acc[i][j][e] - top, p = exp_neg(d);
+          const float d = acc[i][j][e] - base, p = exp_neg(d);
           l += p;
           u = fmaf(p, d, u);
         }
+      if (__ballot(u != u && l == l)) {  // 0 x -Inf (seldom: an operation an output otherwise)
+        u = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float d = acc[i][j][e] - base;
+            u = fmaf(exp_neg(d), fmaxf(d, -1000.f), u);
+          }
+      }
       l = halves<true>(l);
       u = halves<true>(u);
       if (h == 0) {
         float* at = s_stat + (w * kTileM + 32 * j + r) * 3;
-        at[0] = none ? -INFINITY : top;
-        at[1] = none ? 0.f : l;
-        at[2] = none ? 0.f : u;
+        at[0] = top;
+        at[1] = l;
+        at[2] = u;
       }
     }
     __syncthreads();

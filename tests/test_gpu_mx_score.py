@@ -112,3 +112,60 @@ def test_no_rows_and_refusals(dev):
                 lambda: mx_score(x[:, :32], w, t), lambda: mx_score(x, w, t.cpu()), lambda: mx_score(x.cpu(), w, t)):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("m,n", [(6, 300), (100, 300), (100, 1025), (6, 49152), (20, 49200)])  # each kernel, ragged tiles
+def test_logits_of_minus_inf_and_far_apart(dev, m, n):
+    """-Inf has the probability 0, nothing but -Inf is NaN, and what is finite counts however large.  Every logit is
+    one product of powers of two and short numbers, so that the bound is the softmax's alone (2^-17: 2^-22 of 1 + |log
+    probability|, which is below 24 here)."""
+    rng = np.random.default_rng(n)
+    codes = np.zeros((n, 64), dtype=np.uint8)
+    codes[37, 0] = 15                        # -6
+    codes[:, 1] = rng.integers(0, 16, n)
+    codes[:, 2] = 10                         # -1
+    codes[:, 3] = 15
+    codes[36, 4], codes[38, 4] = 2, 10       # 1, -1
+    packed = codes[:, 0::2] | codes[:, 1::2] << 4
+    w = MXTensor.from_numpy(packed, np.full((n, 2), 127, dtype=np.uint8), device=dev)
+    x = torch.zeros(m, 64, device=dev, dtype=torch.bfloat16)
+    x[0, 0], x[0, 1] = 2.0 ** 127, 1.0       # token 37: -Inf
+    x[1, 1] = 1.0
+    x[2, 2] = 2.0 ** 120                     # all alike, far below 0
+    x[3, 3] = 2.0 ** 127                     # all -Inf
+    x[4, 4] = 2.0 ** 127                     # one far above, one as far below
+    t = torch.full((m,), 37, device=dev, dtype=torch.int32)
+    got = mx_score(x, w, t)
+    z = torch.from_numpy(mx_ref.values(packed, np.full((n, 2), 127))[:, 1])
+    for row in (0, 1):
+        zr = z.clone()
+        if row == 0:
+            zr[37] = -float("inf")
+        lp = torch.log_softmax(zr, 0)
+        h, best = -(lp.exp() * lp).nansum(), lp.amax()
+        lse = (h + 402) * 2.0 ** -23
+        assert got.logprob[row].item() == -float("inf") if row == 0 else (got.logprob[row].cpu().double() - lp[37]).abs() <= lse + 2.0 ** -17
+        assert (got.best[row].cpu().double() - best).abs() <= lse + 2.0 ** -17
+        assert (got.entropy[row].cpu().double() - h).abs() <= lse + 2 * lse * (h - best + 1) + 2.0 ** -17
+    even = float(np.log(n))
+    lse = (even + 402) * 2.0 ** -23 + 2.0 ** -17
+    assert abs(got.logprob[2].item() + even) <= lse and abs(got.best[2].item() + even) <= lse
+    assert abs(got.entropy[2].item() - even) <= lse + 2 * lse
+    assert all(v[3].isnan() for v in got)
+    assert got.logprob[4].item() == -2.0 ** 127 and got.best[4].item() == 0 and got.entropy[4].item() == 0
+    far = mx_score(x, w, torch.full_like(t, 38))
+    assert far.logprob[4].item() == -float("inf")  # -2^128
+    assert (got.logprob[5:] + even).abs().amax() <= lse  # rows of zeros
+
+
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(1, 49152, 32), (5, 49153, 96), (16, 50001, 4096), (17, 49200, 2080), (32, 49155, 2048), (32, 60004, 160),
+                                   (21, 131001, 1024), (33, 49157, 288), (24, 49151, 128)])
+def test_many_tokens(dev, m, n, k, kind):
+    rng = np.random.default_rng(n)
+    p, s = mx_ref.random_mx(rng, n, k, 121, 125)
+    w = MXTensor.from_numpy(p, s, device=dev)
+    x = torch.from_numpy(rng.standard_normal((m, k)) / np.sqrt(k) * 8).to(dev).to(kind)
+    targets = torch.from_numpy(rng.integers(0, n, m)).to(dev).int()
+    targets[0], targets[-1] = 0, n - 1
+    check(mx_score(x, w, targets), x, w.dequantize().double(), targets)
