@@ -172,3 +172,17 @@ def test_refusals(dev):
             bad()
     with pytest.raises(TypeError):
         mx_linear(x, x)
+
+
+# An output head's rows: x is held in LDS (up to 128 KB: 32 rows of 2048, 16 of 4096), past that and past 32 rows it is not.
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(16, 49152, 32), (17, 49153, 96), (16, 50001, 4096), (17, 49200, 2080), (32, 49155, 2048), (32, 60004, 160),
+                                   (21, 131001, 1024), (33, 49157, 288), (24, 49151, 128), (1, 800001, 64)])
+def test_many_outputs(dev, m, n, k, kind):
+    rng = np.random.default_rng(n)
+    p, s = mx_ref.random_mx(rng, n, k)
+    w = MXTensor.from_numpy(p, s, device=dev)
+    x = torch.from_numpy(rng.standard_normal((m, k))).to(dev).to(kind)
+    wv = w.dequantize().double()
+    for out in (torch.float32, kind):
+        compare(mx_linear(x, w, out_dtype=out), x.double(), wv)
