@@ -178,3 +178,45 @@ def test_order_in_memory_and_back(rows, cols):
             tile = row // 32 * kt + block // 4
             at = tile * 2048 + block % 4 * 512 + row % 32 * 16
             assert not codes[at:at + 16].any() and scales[tile * 128 + row % 32 * 4 + block % 4] == 0
+
+
+def test_sizes_past_the_counts(lib):
+    def linear(stride, m, w=mx()):
+        return lib.q4d_mx_linear(w, FAKE, F16, stride, m, FAKE, F32, None)
+    assert linear(1 << 24, 2) == linear(1 << 40, 2 ** 31 - 1) == SHAPE
+    assert linear(64, 2 ** 31 - 1, mx(rows=2 ** 27, cols=64)) == SHAPE  # more tiles than a launch has
+    assert lib.q4d_mx_score_workspace_bytes(48, 64, 1 << 23) > 0 == lib.q4d_mx_score_workspace_bytes(48, 64, (1 << 23) + 1)
+    assert lib.q4d_mx_score(mx(), FAKE, F16, 64, (1 << 23) + 1, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 60, None) == SHAPE
+    assert lib.q4d_mx_matmul(mx(rows=2 ** 31 - 256, cols=32), mx(rows=9, cols=32), FAKE, F32, None) == SHAPE
+    assert lib.q4d_token_logprobs_workspace_bytes(1 << 23, 16384, 0) > 0 == lib.q4d_token_logprobs_workspace_bytes(1 << 23, 16385, 0)
+    for rows, cols in ((1, 1 << 32), ((1 << 32) + 1, 32)):
+        with pytest.raises(ValueError, match="at most"):
+            MXTensor.__new__(MXTensor)._new(torch.zeros(1), rows, cols)
+
+
+def test_calls_run_on_the_tensors_device(monkeypatch):
+    """On another current device: the tensors' is made current for the call, with its own stream, and the caller's
+    again afterwards, whether the call succeeds, fails or raises."""
+    from llm_accelerator_amd import model
+    now, log = [0], []
+
+    class Lib:
+        def q4d_some_call(self, *args):
+            log.append((now[0], args))
+            if args[0] == "raise":
+                raise TypeError
+            return args[0]
+    monkeypatch.setattr(model, "_device", lambda: now[0])
+    monkeypatch.setattr(model, "_stream", lambda i: 100 + i)
+    monkeypatch.setattr(torch.cuda, "set_device", lambda i: now.__setitem__(0, i))
+    monkeypatch.setattr(_lib, "load", Lib)
+    for here in (0, 3):
+        now[0] = here
+        model.call_on(3, "q4d_some_call", 0, "x")
+        assert log[-1] == (3, (0, "x", 103)) and now[0] == here
+        with pytest.raises(_lib.Q4DecError):
+            model.call_on(3, "q4d_some_call", SHAPE)
+        assert now[0] == here
+        with pytest.raises(TypeError):
+            model.call_on(3, "q4d_some_call", "raise")
+        assert now[0] == here
