@@ -556,10 +556,11 @@ int q4d_mx_quantize(const void* x, int32_t dtype, int64_t ld, int32_t rule, cons
 /* y [rows, cols] = the values, in y_dtype (16-byte aligned): exact in fp32 and bf16 but for what lies past
  * their largest number (Inf), rounded once in fp16. */
 int q4d_mx_dequantize(const q4d_mx_t* t, void* y, int32_t y_dtype, void* stream);
-/* y[m, :] = W x[m, :], m < M: x fp16 or bf16, row m at m * x_stride elements, 16-byte aligned rows;
+/* y[m, :] = W x[m, :], m < M: x fp16 or bf16, row m at m * x_stride (< 2^24) elements, 16-byte aligned rows;
  * y [M, rows] in any of the three types, 16-byte aligned.  The weights enter as numbers of x's type
  * (as q4d_mx_dequantize makes them); fp32 sums, rounded once.  A row's last bits may depend on M,
- * though not on the other rows' values. */
+ * though not on the other rows' values.  M up to 2^29 and M * rows to about 2^37 (more is refused); y
+ * apart from x and w. */
 int q4d_mx_linear(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M, void* y, int32_t y_dtype,
                   void* stream);
 /* The same with x ([M, cols]) in 4 bits too: products and scales are exact, sums fp32. */
@@ -567,7 +568,8 @@ int q4d_mx_matmul(const q4d_mx_t* w, const q4d_mx_t* x, void* y, int32_t y_dtype
 /* How likely token targets[m] is under the output head w ([vocab, hidden]) at hidden row x[m] (as in
  * q4d_mx_linear), with z = W x[m] in fp32 and never in memory: logprob[m] = z[target] - log sum e^z
  * (a target outside the vocabulary, a padded row's: NaN), entropy[m] of the distribution, best[m] =
- * the largest log probability.  A row whose z hold NaN or +Inf gives NaN.  ws: 256-byte aligned,
+ * the largest log probability.  A z of -Inf has the probability 0; a row with nothing else, or with NaN
+ * or +Inf, gives NaN.  M up to 2^23.  ws: 256-byte aligned,
  * q4d_mx_score_workspace_bytes(w->rows, w->cols, M) bytes, holds nothing between calls. */
 size_t q4d_mx_score_workspace_bytes(int32_t rows, int32_t cols, int32_t M);
 int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M, const int32_t* targets,
@@ -578,7 +580,8 @@ int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_st
  * [rows, top], in order.  Tokens are ordered by logit, equal ones by index, the lowest first; NaN comes
  * last.  A target outside the vocabulary: logprob NaN, rank -1.  -Inf (a masked token) has the
  * probability 0; a row with nothing else, or with NaN or +Inf, has NaN for its log probabilities and
- * entropy.  fp32 arithmetic.  ws: 256-byte aligned, holds nothing between calls. */
+ * entropy.  fp32 arithmetic.  rows * ceil(vocab / 16384) up to 2^23 (the workspace is 0 bytes past that).
+ * ws: 256-byte aligned, holds nothing between calls. */
 size_t q4d_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top);
 int q4d_token_logprobs(const void* logits, int32_t dtype, int64_t stride, int32_t rows, int32_t vocab, const int32_t* targets,
                        int32_t top, float* logprob, int32_t* rank, float* entropy, float* top_logprobs, int32_t* top_ids,

@@ -23,6 +23,11 @@ struct MxProduct {
 
 enum MxKind { MX_X4 = 0, MX_F16 = 1, MX_BF16 = 2 };  // x: codes or 16-bit floats
 
+// x's rows lie less than this many elements apart (64 of them within 32 bits), a score has up to so many rows (a
+// launch's threads are counted in 32 bits, the join's are 256 a row).
+constexpr long long kMxStride = 1 << 24;
+constexpr int kMxScored = 1 << 23;
+
 bool mx_shape(int32_t rows, int32_t cols);
 int check_mx(const q4d_mx_t* t);
 

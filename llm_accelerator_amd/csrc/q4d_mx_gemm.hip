@@ -332,7 +332,8 @@ __global__ __launch_bounds__(256, PER_CU) void mx_gemm_kernel(const MxProduct a)
 template <MxKind KIND, bool SCORE, int NT, int MT, int RING, int PER_CU>
 int launch(const MxProduct& p, hipStream_t st) {
   const long long tiles = (p.N + 128LL * NT - 1) / (128 * NT) * ((p.M + 32LL * MT - 1) / (32 * MT));
-  if (tiles > (1 << 23) || (KIND != MX_X4 && 2 * p.x_stride * 32 * MT > 0x7FFFFFFFLL)) return Q4D_ERR_SHAPE;  // a tile's offsets are 32 bits
+  static_assert(KIND == MX_X4 || MT == 2, "");  // x's offsets in a tile, 64 rows of 2 kMxStride bytes, are 32 bits
+  if (tiles > (1 << 23)) return Q4D_ERR_SHAPE;
   hipLaunchKernelGGL((mx_gemm_kernel<KIND, SCORE, NT, MT, RING, PER_CU>), dim3((unsigned)tiles), dim3(256), 0, st, p);
   return check_launch();
 }

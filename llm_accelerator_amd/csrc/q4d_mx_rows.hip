@@ -152,7 +152,7 @@ __global__ __launch_bounds__(64 * NW) void mx_rows_kernel(const MxProduct a) {
 template <MxKind KIND, int MT, int NT, int NW>
 int launch(const MxProduct& p, hipStream_t st) {
   const dim3 grid((unsigned)((p.N + 16LL * NT - 1) / (16 * NT)), (unsigned)((p.M + 16 * MT - 1) / (16 * MT)));
-  if (grid.y > 65535u) return Q4D_ERR_SHAPE;
+  if (grid.y > 65535u || (long long)grid.x * (64 * NW) > 0xFFFFFFFFLL) return Q4D_ERR_SHAPE;
   hipLaunchKernelGGL((mx_rows_kernel<KIND, MT, NT, NW, false>), grid, dim3(64 * NW), 0, st, p);
   return check_launch();
 }
@@ -179,6 +179,7 @@ int launch(const MxProduct& p, hipStream_t st) {
 template <MxKind KIND, int MT, int NT>
 int launch_score(const MxProduct& p, hipStream_t st) {
   const dim3 grid((unsigned)((p.N + 16LL * NT - 1) / (16 * NT)));
+  if ((long long)grid.x * 256 > 0xFFFFFFFFLL) return Q4D_ERR_SHAPE;
   hipLaunchKernelGGL((mx_rows_kernel<KIND, MT, NT, 4, true>), grid, dim3(256), 0, st, p);
   return check_launch();
 }

@@ -48,7 +48,7 @@ int check_x(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride,
   if (const int rc = check_mx(w)) return rc;
   if (!x) return Q4D_ERR_NULL;
   if (x_dtype != Q4D_F16 && x_dtype != Q4D_BF16) return Q4D_ERR_DTYPE;
-  if (M <= 0 || (M > 1 && x_stride < w->cols)) return Q4D_ERR_SHAPE;
+  if (M <= 0 || (M > 1 && (x_stride < w->cols || x_stride >= kMxStride))) return Q4D_ERR_SHAPE;
   return aligned(x, 16) && (M == 1 || x_stride % 8 == 0) ? Q4D_OK : Q4D_ERR_BAD_ADDR;
 }
 int check_y(const void* y, int32_t y_dtype) {
@@ -125,7 +125,7 @@ extern "C" int q4d_mx_matmul(const q4d_mx_t* w, const q4d_mx_t* x, void* y, int3
 }
 
 extern "C" size_t q4d_mx_score_workspace_bytes(int32_t rows, int32_t cols, int32_t M) {
-  if (!mx_shape(rows, cols) || M <= 0) return 0;
+  if (!mx_shape(rows, cols) || M <= 0 || M > kMxScored) return 0;
   return hit_bytes(M) + (size_t)score_parts(M, rows, cols) * M * sizeof(f32x4);
 }
 
@@ -134,6 +134,7 @@ extern "C" int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, i
                             void* stream) {
   int rc = check_x(w, x, x_dtype, x_stride, M);
   if (rc) return rc;
+  if (M > kMxScored) return Q4D_ERR_SHAPE;
   if (!targets || !logprob || !entropy || !best || !ws) return Q4D_ERR_NULL;
   if (!aligned(targets, 4) || !aligned(logprob, 4) || !aligned(entropy, 4) || !aligned(best, 4) || !aligned(ws, 256))
     return Q4D_ERR_BAD_ADDR;

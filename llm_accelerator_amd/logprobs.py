@@ -36,9 +36,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     probability and rank of ``targets`` [...] (int32; ``None``: neither), the entropy, and the ``top``
     most likely tokens (0 .. 32).  Tokens are ordered by logit, equal ones by index, the lowest first.
 
-    A token of -Inf (a masked one) has the probability 0.  A target outside the vocabulary (a padded row's)
-    gives NaN and rank -1.  A row with nothing but -Inf, or with NaN or +Inf, has NaN for log probabilities
-    and entropy; NaN comes last in the order."""
+    Up to 2^23 rows (x ceil(vocab / 16384)).  A token of -Inf (a masked one) has the probability 0.  A target
+    outside the vocabulary (a padded row's) gives NaN and rank -1.  A row with nothing but -Inf, or with NaN or
+    +Inf, has NaN for log probabilities and entropy; NaN comes last in the order."""
     if not logits.is_cuda:
         raise ValueError("logits must be a GPU tensor (libq4dec has no CPU path)")
     if logits.dtype not in _DTYPES:
@@ -53,22 +53,22 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
             raise ValueError(f"targets must be int32 {tuple(lead)} on {logits.device}")
         targets = targets.contiguous()
     x = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
-    if (vocab > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < vocab):
-        x = x.contiguous()
-    rows, have = x.shape[0], targets is not None
+    rows, step, have = x.shape[0], x.stride(0), targets is not None
+    if rows * -(-vocab // 16384) > 1 << 23:
+        raise ValueError(f"rows x ceil(vocab / 16384) must be at most 2^23, got {tuple(logits.shape)}")
+    if (vocab > 1 and x.stride(1) != 1) or (rows > 1 and step < vocab):
+        x, step = x.contiguous(), vocab
     nbytes = _lib.load().q4d_token_logprobs_workspace_bytes(rows, vocab, top) if rows else 0
-    if rows and nbytes == 0:
-        raise _lib.Q4DecError(-11, "q4d_token_logprobs_workspace_bytes")
     # the results lie side by side in one allocation, behind the workspace if that is small
     inside = (nbytes + 3) // 4 if nbytes <= SMALL_WORKSPACE else 0
     got = x.new_empty(inside + rows * (3 + 2 * top), dtype=torch.float32)
     _, logprob, entropy, rank, top_logprobs, top_ids = got.split((inside, rows, rows, rows, rows * top, rows * top))
     if rows:
         ws = got if inside else x.new_empty(nbytes, dtype=torch.uint8)
-        at, step = got.data_ptr() + 4 * inside, 4 * rows
-        call_on(index, "q4d_token_logprobs", x.data_ptr(), _DTYPES[x.dtype], x.stride(0), rows, vocab,
-                targets.data_ptr() if have else None, top, at if have else None, at + 2 * step if have else None, at + step,
-                at + 3 * step if top else None, at + (3 + top) * step if top else None, ws.data_ptr(), nbytes)
+        at, size = got.data_ptr() + 4 * inside, 4 * rows
+        call_on(index, "q4d_token_logprobs", x.data_ptr(), _DTYPES[x.dtype], step, rows, vocab,
+                targets.data_ptr() if have else None, top, at if have else None, at + 2 * size if have else None, at + size,
+                at + 3 * size if top else None, at + (3 + top) * size if top else None, ws.data_ptr(), nbytes)
     if len(lead) != 1:
         logprob, entropy, rank = logprob.view(lead), entropy.view(lead), rank.view(lead)
     wide = (*lead, top)

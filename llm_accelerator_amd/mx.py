@@ -33,6 +33,7 @@ _RULES = {"floor": 0, "ceil": 1}
 
 
 TILE_ROWS, TILE_COLS = 32, 128  # of the order in memory (q4d_mx_t)
+_MOST = 0x7FFFFF00              # rows or columns, counted in 32 bits behind the C interface
 
 
 def _order(rows_bytes: torch.Tensor, width: int) -> torch.Tensor:
@@ -82,6 +83,8 @@ class MXTensor:
 
     def _new(self, like: torch.Tensor, rows: int, cols: int) -> "MXTensor":
         """Memory for rows x cols on the device of ``like``."""
+        if rows > _MOST or cols > _MOST:
+            raise ValueError(f"an MXTensor has at most {_MOST} rows and columns, got {rows} x {cols}")
         return self._setup(like.new_empty(-(-rows // TILE_ROWS) * -(-cols // TILE_COLS) * 2176, dtype=torch.uint8), rows, cols)
 
     @property
@@ -160,7 +163,8 @@ def _rows(x: torch.Tensor, name: str, cols: int | None = None):
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
     step = x.stride(0) if x.shape[0] > 1 else x.shape[1]
-    if x.data_ptr() % 16 or (x.shape[1] > 1 and x.stride(1) != 1) or step < x.shape[1] or step * x.element_size() % 16:
+    if (x.data_ptr() % 16 or (x.shape[1] > 1 and x.stride(1) != 1) or step < x.shape[1] or step >= 1 << 24
+            or step * x.element_size() % 16):
         x = x.clone(memory_format=torch.contiguous_format)
         step = x.shape[1]
     return x, x.shape[0], step
@@ -192,7 +196,7 @@ def mx_linear(x: torch.Tensor | MXTensor, weight: MXTensor, out_dtype: torch.dty
     """``x @ weight.T``: x [..., cols] in fp16 or bf16, where the weights enter as numbers of that type
     (``weight.dequantize(x.dtype)``), or an :class:`MXTensor` [rows, cols], where both enter as they are.
     fp32 sums, rounded once to ``out_dtype`` (fp32, fp16 or bf16; ``None``: x's type, bf16 for an
-    MXTensor).  ``out``: a contiguous result of the caller's."""
+    MXTensor).  ``out``: a contiguous result of the caller's, apart from x."""
     if not isinstance(weight, MXTensor):
         raise TypeError("weight must be an MXTensor")
     _on_gpu(weight)
@@ -224,6 +228,8 @@ def mx_linear(x: torch.Tensor | MXTensor, weight: MXTensor, out_dtype: torch.dty
             raise ValueError(f"out must be contiguous {(*lead, n)} in fp32, fp16 or bf16 (out_dtype) on {weight.device}, 16-byte aligned")
     if m == 0:
         return out
+    if m > _MOST:
+        raise ValueError(f"x has at most {_MOST} rows, got {m}")
     if codes:
         call_on(index, "q4d_mx_matmul", weight._ref, x._ref, out.data_ptr(), _DTYPES[y_kind])
     else:
@@ -240,8 +246,9 @@ class MXScores(NamedTuple):
 def mx_score(hidden: torch.Tensor, weight: MXTensor, targets: torch.Tensor) -> MXScores:
     """How likely ``targets`` [...] (int32) are under the output head ``weight`` [vocab, cols] at the rows
     ``hidden`` [..., cols] (fp16 or bf16): the log softmax of ``mx_linear(hidden, weight)`` in fp32 at the
-    targets, its entropy and its maximum, fp32 [...] each, without the products in memory.  A target
-    outside the vocabulary (a padded row's) gives NaN."""
+    targets, its entropy and its maximum, fp32 [...] each, without the products in memory.  Up to 2^23 rows.
+    A target outside the vocabulary (a padded row's) gives NaN, and so does a row whose products hold NaN, +Inf or
+    nothing but -Inf."""
     if not isinstance(weight, MXTensor):
         raise TypeError("weight must be an MXTensor")
     _on_gpu(weight)
@@ -256,6 +263,8 @@ def mx_score(hidden: torch.Tensor, weight: MXTensor, targets: torch.Tensor) -> M
         raise ValueError(f"targets must be int32 {tuple(lead)} on {x.device}")
     targets = targets.contiguous()
     got = x.new_empty((3, *lead), dtype=torch.float32)
+    if m > 1 << 23:
+        raise ValueError(f"up to 2^23 rows, got {m}")
     if m:
         nbytes = _lib.load().q4d_mx_score_workspace_bytes(*weight.shape, m)
         ws = x.new_empty(nbytes, dtype=torch.uint8)

@@ -195,3 +195,12 @@ def test_no_rows_and_refusals(dev):
                 lambda: token_logprobs(torch.empty(1, MAX_VOCAB + 1, device=dev, dtype=torch.float16))):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_more_rows_than_are_counted(dev):
+    one = torch.zeros(1, 1, device=dev)
+    for rows in ((1 << 23) + 1, 2 ** 32 + 5):
+        with pytest.raises(ValueError, match="2\\^23"):
+            token_logprobs(one.expand(rows, 1))
+    got = token_logprobs(torch.zeros(1 << 23, 1, device=dev, dtype=torch.float16), top=1)
+    assert (got.entropy == 0).all() and (got.top_ids == 0).all() and (got.top_logprobs == 0).all()

@@ -186,3 +186,15 @@ def test_many_outputs(dev, m, n, k, kind):
     wv = w.dequantize().double()
     for out in (torch.float32, kind):
         compare(mx_linear(x, w, out_dtype=out), x.double(), wv)
+
+
+@pytest.mark.parametrize("m,n", [(3, 100), (70, 16500)])
+def test_rows_far_apart(dev, m, n):
+    """Rows 2^24 - 8 elements apart are read in place, those of 2^24 from a copy."""
+    rng = np.random.default_rng(0)
+    w, wv = make(rng, n, 96, dev)
+    rows = torch.from_numpy(rng.standard_normal((m, 96))).to(dev).to(torch.bfloat16)
+    for step in ((1 << 24) - 8, 1 << 24):
+        x = torch.empty(m * step, device=dev, dtype=torch.bfloat16).view(m, step)[:, :96]
+        x.copy_(rows)
+        compare(mx_linear(x, w), rows.double(), wv)
