@@ -184,3 +184,37 @@ def test_two_streams_at_once(dev):
     for i, out in enumerate(outs):
         for a, b in zip(out, jobs[i % 3][3]):
             assert torch.equal(a.nan_to_num(nan=7.0) if a.is_floating_point() else a, b.nan_to_num(nan=7.0) if b.is_floating_point() else b)
+
+
+def test_one_row_without_dims_and_targets_apart(dev):
+    """hidden [cols] and logits [vocab] with a target of no dims; targets and logits that are slices; x of leading dims
+    of which one is empty."""
+    rng = np.random.default_rng(6)
+    head = mx_quantize(torch.from_numpy(rng.standard_normal((900, 96))).to(dev).float())
+    x = torch.from_numpy(rng.standard_normal((6, 96))).to(dev).to(torch.bfloat16)
+    t = torch.from_numpy(rng.integers(0, 900, 12)).to(dev).int()
+    whole = mx_score(x, head, t[::2])
+    assert all(torch.equal(a, b) for a, b in zip(whole, mx_score(x, head, t[::2].contiguous())))
+    one = mx_score(x[2], head, t[4])
+    assert all(v.shape == () for v in one) and all(torch.equal(a, b[2]) for a, b in zip(one, mx_score(x[:3], head, t[:6:2])))
+    logits = mx_linear(x, head, out_dtype=torch.float32)
+    wide = torch.empty(6, 2000, device=dev)
+    wide[:, 101:1001] = logits
+    a, b = token_logprobs(wide[:, 101:1001], t[::2], top=3), token_logprobs(logits, t[::2].contiguous(), top=3)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    c = token_logprobs(wide[2, 101:1001], t[4], top=3)
+    assert c.logprob.shape == c.rank.shape == c.entropy.shape == () and c.top_ids.shape == (3,)
+    assert all(torch.equal(u, v[2]) for u, v in zip(c, b))
+    assert mx_linear(x.view(2, 3, 96)[:, :0], head).shape == (2, 0, 900)
+    assert mx_score(x.view(2, 3, 96)[:, :0], head, t.view(2, 6)[:, :0]).entropy.shape == (2, 0)
+    empty = token_logprobs(logits.view(2, 3, 900)[:, :0], t.view(2, 6)[:, :0], top=2)
+    assert empty.rank.shape == (2, 0) and empty.top_ids.shape == (2, 0, 2)
+
+
+def test_a_tensor_times_itself(dev):
+    rng = np.random.default_rng(7)
+    a = mx_quantize(torch.from_numpy(rng.standard_normal((70, 160))).to(dev).float())
+    v = a.dequantize().double()
+    # 160 products, exact, and as many additions of half a step of sum |a a|; the output's rounding
+    size = v.abs() @ v.abs().T
+    assert ((mx_linear(a, a, out_dtype=torch.float32).double() - v @ v.T).abs() <= 161 * 2.0 ** -23 * size).all()
