@@ -306,6 +306,7 @@ __global__ __launch_bounds__(64 * W) void logprob_part_kernel(const LogprobArgs 
     }
   }
   __syncthreads();
+  if (w && 64 * w >= count) return;  // nothing of the wave's is among the candidates
   s = SoftSum{s_stat[0][0], s_stat[0][1], s_stat[0][2]};
 #pragma unroll
   for (int i = 1; i < W; ++i) s = soft_join(s, SoftSum{s_stat[i][0], s_stat[i][1], s_stat[i][2]});
