@@ -13,7 +13,7 @@
 // Logits are ordered by value, then by index, the lower first; NaN comes last, after -Inf.
 //
 // Bound by the vector units, about twelve operations a logit and an exponential: 1100 bf16 rows of 151669 with one
-// alternative 88-95 us, 3.5-3.8 TB/s (units busy 76 %), 64 fp32 rows of 151936 with 20 16 us, 2.4 TB/s (66 %; all
+// alternative 88-95 us, 3.5-3.8 TB/s (units busy 76 %), 64 fp32 rows of 151936 with 20 15 us, 2.6 TB/s (66 %; all
 // blocks at once, each its load, its sums and its search).  One row: 6.3 us, and 3-5 us for a join, both latency.
 #include <math.h>
 
