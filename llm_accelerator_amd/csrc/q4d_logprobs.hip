@@ -15,6 +15,7 @@
 // Bound by the vector units, about twelve operations a logit and an exponential: 1100 bf16 rows of 151669 with one
 // alternative 88-95 us, 3.5-3.8 TB/s (units busy 76 %), 64 fp32 rows of 151936 with 20 15 us, 2.6 TB/s (66 %; all
 // blocks at once, each its load, its sums and its search).  One row: 6.3 us, and 3-5 us for a join, both latency.
+#include <float.h>
 #include <math.h>
 
 #include "q4d_internal.h"
@@ -249,7 +250,9 @@ __global__ __launch_bounds__(64 * W) void logprob_part_kernel(const LogprobArgs 
     } else {
       __syncthreads();  // (s_count is set)
     }
-    const float least = key_value((uint64_t)bound << 32);
+    float least = key_value((uint64_t)bound << 32);
+    // fewer than K lanes have a number: all numbers, if they fit (13 rows of 233 in bf16, K = 31, 27 -> 13 us)
+    if (W == 1 && !(least > -INFINITY) && a.vocab <= kGather) least = -FLT_MAX;
     if (least > -INFINITY) {
       if (mine >= least) {
 #pragma unroll
@@ -267,7 +270,7 @@ __global__ __launch_bounds__(64 * W) void logprob_part_kernel(const LogprobArgs 
       __syncthreads();
       count = s_count;
     }
-    if (count == 0 || count > kGather) {
+    if (count < a.top || count > kGather) {
       // by keys: of each thread's best the K-th best of the block is reached by K logits, and at most
       // HELD K reach it
       uint64_t best = 0;
@@ -326,14 +329,23 @@ __global__ __launch_bounds__(64 * W) void logprob_part_kernel(const LogprobArgs 
       a.before[slot] = before;
     }
   }
-  for (int c = t; c < count; c += kThreads) {
-    const uint64_t k = s_cand[c];
-    int rank = 0;
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) rank += s_cand[i] > k;
-    if (rank >= a.top) continue;
+  const auto place = [&](uint64_t k, int rank) {
+    if (rank >= a.top) return;
     if (whole) finish_top(a, row, s, ll, rank, k);
     else a.best[slot * a.top + rank] = k;
+  };
+  constexpr int kAt = W == 1 ? 2 : 1;  // of a lane, side by side: 64 lanes have up to 256 (50 rows of 1000, K = 32, 27 -> 19 us)
+  for (int c = t; c < count; c += kAt * kThreads) {
+    const bool second = W == 1 && c + kThreads < count;
+    const uint64_t k = s_cand[c], k2 = second ? s_cand[c + kThreads] : ~0ull;
+    int rank = 0, rank2 = 0;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+      rank += s_cand[i] > k;
+      if (W == 1) rank2 += s_cand[i] > k2;
+    }
+    place(k, rank);
+    if (second) place(k2, rank2);
   }
   if (!whole)
     for (int c = count + t; c < a.top; c += kThreads) a.best[slot * a.top + c] = 0;  // a last part of fewer logits

@@ -204,3 +204,19 @@ def test_more_rows_than_are_counted(dev):
             token_logprobs(one.expand(rows, 1))
     got = token_logprobs(torch.zeros(1 << 23, 1, device=dev, dtype=torch.float16), top=1)
     assert (got.entropy == 0).all() and (got.top_ids == 0).all() and (got.top_logprobs == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab,top", [(33, 32), (233, 31), (256, 32), (257, 32), (500, 32), (1000, 32), (1024, 20)])
+def test_short_rows_with_many_alternatives(dev, vocab, top, dtype):
+    """Rows of which few lanes hold all, whole and masked down to fewer tokens than alternatives."""
+    x = logits(70, vocab, dtype, dev, seed=vocab)
+    g = torch.Generator(device=dev).manual_seed(1)
+    for row, share in enumerate((0.3, 0.7, 0.9, 0.98)):
+        x[10 * row:10 * row + 10][torch.rand(10, vocab, generator=g, device=dev) < share] = -math.inf
+    x[40:50] = x[40:50].round()         # many alike
+    x[50, :] = 0
+    x[51, 1::2] = math.nan              # (NaN comes last, whatever it stands beside)
+    x[52, : vocab - 3] = -math.inf
+    x[53, 5:] = torch.finfo(dtype).min
+    check(x, targets(70, vocab, dev), top)
