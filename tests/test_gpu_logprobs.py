@@ -220,3 +220,25 @@ def test_short_rows_with_many_alternatives(dev, vocab, top, dtype):
     x[52, : vocab - 3] = -math.inf
     x[53, 5:] = torch.finfo(dtype).min
     check(x, targets(70, vocab, dev), top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab,top", [(5000, 20), (40000, 32), (151936, 3), (151936, 20)])
+def test_few_tokens_left(dev, vocab, top, dtype):
+    """Grammars: a handful to a few hundred tokens left, here and there or side by side; NaN among what is masked."""
+    x = logits(12, vocab, dtype, dev, seed=vocab)
+    g = torch.Generator(device=dev).manual_seed(2)
+    left = [1, 2, 5, 19, 20, 21, 33, 70, 300, 1000]
+    for row, n in enumerate(left):
+        keep = torch.randperm(vocab, generator=g, device=dev)[:n]
+        if row % 3 == 2:
+            keep = torch.arange(n, device=dev) + vocab // 2
+        masked = torch.full_like(x[row], -math.inf)
+        masked[keep] = x[row, keep]
+        x[row] = masked
+    x[10, 7:] = -math.inf
+    x[10, 9:100:2] = math.nan             # fewer than 64 of the first are -Inf
+    x[11, :] = -math.inf
+    x[11, :80] = math.nan
+    x[11, vocab - 5:] = 1.0
+    check(x, targets(12, vocab, dev), top)
