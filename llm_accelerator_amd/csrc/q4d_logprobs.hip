@@ -3,14 +3,14 @@
 //
 // A row is cut into parts of 64 W x HELD logits; a block of W waves holds a part in registers, HELD logits a
 // thread, and leaves the part's softmax sums, how many of its logits come before the target, and its K best.  A row
-// of one part is finished there; else a second kernel joins a row's parts, a wave a row.
+// of one part is finished there; else a second kernel joins a row's parts, a block a row.
 //
 // The K best: of the lanes' own maxima in a wave the K-th largest, found bit by bit with ballots, is reached by
-// K logits, and so is the smallest of the waves' K/W-th largest; the larger of such bounds serves.  The
-// few logits that reach it are gathered in LDS and ordered by counting.  Where masks leave fewer than K numbers, -Inf follows by index (64 rows of 151936
-// with 15 tokens left, K = 20, 21 us instead of 75; 1100 bf16 rows with 150 left, K = 5, 116 instead of 287).  Where the
-// logits are too many (equal ones) or NaN matters the bound is found again among keys of value and index, which no two
-// logits share.  The parts' lists are joined the same way.
+// K logits, and so is the smallest of the waves' K/W-th largest; the larger of such bounds serves.  The few logits
+// that reach it are gathered in LDS and ordered by counting.  Where masks leave fewer than K numbers, -Inf follows by
+// index (64 rows of 151936 with 15 tokens left, K = 20, 21 us instead of 75; 1100 bf16 rows with 150 left, K = 5, 116
+// instead of 287).  Where the logits are too many (equal ones) or NaN matters the bound is found again among keys of
+// value and index, which no two logits share.  The parts' lists are joined by such a bound, too.
 //
 // Logits are ordered by value, then by index, the lower first; NaN comes last, after -Inf.
 //
