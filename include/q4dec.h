@@ -569,8 +569,9 @@ int q4d_mx_matmul(const q4d_mx_t* w, const q4d_mx_t* x, void* y, int32_t y_dtype
  * q4d_mx_linear), with z = W x[m] in fp32 and never in memory: logprob[m] = z[target] - log sum e^z
  * (a target outside the vocabulary, a padded row's: NaN), entropy[m] of the distribution, best[m] =
  * the largest log probability.  A z of -Inf has the probability 0; a row with nothing else, or with NaN
- * or +Inf, gives NaN.  M up to 2^23.  ws: 256-byte aligned,
- * q4d_mx_score_workspace_bytes(w->rows, w->cols, M) bytes, holds nothing between calls. */
+ * or +Inf, gives NaN.  M, and ceil(M / 64) * ceil(vocab / 256), up to 2^23 (the workspace is 0 bytes
+ * past that).  ws: 256-byte aligned, q4d_mx_score_workspace_bytes(w->rows, w->cols, M)
+ * bytes, holds nothing between calls. */
 size_t q4d_mx_score_workspace_bytes(int32_t rows, int32_t cols, int32_t M);
 int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M, const int32_t* targets,
                  float* logprob, float* entropy, float* best, void* ws, size_t ws_bytes, void* stream);

@@ -27,6 +27,8 @@ enum MxKind { MX_X4 = 0, MX_F16 = 1, MX_BF16 = 2 };  // x: codes or 16-bit float
 // launch's threads are counted in 32 bits, the join's are 256 a row).
 constexpr long long kMxStride = 1 << 24;
 constexpr int kMxScored = 1 << 23;
+// ... and the tiles' kernel so many blocks.
+constexpr long long kMxTiles = 1 << 23;
 
 bool mx_shape(int32_t rows, int32_t cols);
 int check_mx(const q4d_mx_t* t);
@@ -44,6 +46,7 @@ int launch_mx_head(const MxProduct& p, MxKind kind, hipStream_t st);
 int launch_mx_head_score(const MxProduct& p, MxKind kind, hipStream_t st);
 int launch_mx_gemm(const MxProduct& p, MxKind kind, hipStream_t st);
 __host__ __device__ inline int mx_gemm_parts(int N) { return (int)((N + 255LL) / 256); }
+bool mx_gemm_scores(int M, int N);  // no more tiles than that
 int launch_mx_gemm_score(const MxProduct& p, MxKind kind, hipStream_t st);
 
 }  // namespace q4d

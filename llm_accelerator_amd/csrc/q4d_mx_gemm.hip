@@ -338,11 +338,14 @@ __global__ __launch_bounds__(256, PER_CU) void mx_gemm_kernel(const MxProduct a)
   }
 }
 
+long long tile_count(int M, int N, int nt, int mt) {
+  return (N + 128LL * nt - 1) / (128 * nt) * ((M + 32LL * mt - 1) / (32 * mt));
+}
 template <MxKind KIND, bool SCORE, int NT, int MT, int RING, int PER_CU>
 int launch(const MxProduct& p, hipStream_t st) {
-  const long long tiles = (p.N + 128LL * NT - 1) / (128 * NT) * ((p.M + 32LL * MT - 1) / (32 * MT));
+  const long long tiles = tile_count(p.M, p.N, NT, MT);
   static_assert(KIND == MX_X4 || MT == 2, "");  // x's offsets in a tile, 64 rows of 2 kMxStride bytes, are 32 bits
-  if (tiles > (1 << 23)) return Q4D_ERR_SHAPE;
+  if (tiles > kMxTiles) return Q4D_ERR_SHAPE;
   hipLaunchKernelGGL((mx_gemm_kernel<KIND, SCORE, NT, MT, RING, PER_CU>), dim3((unsigned)tiles), dim3(256), 0, st, p);
   return check_launch();
 }
@@ -368,8 +371,10 @@ int launch_mx_gemm(const MxProduct& p, MxKind kind, hipStream_t st) {
   if (kind == MX_X4) return launch<MX_X4>(p, st);
   return kind == MX_BF16 ? launch<MX_BF16>(p, st) : launch<MX_F16>(p, st);
 }
+constexpr int kScoreNT = 2, kScoreMT = 2;
+bool mx_gemm_scores(int M, int N) { return tile_count(M, N, kScoreNT, kScoreMT) <= kMxTiles; }
 int launch_mx_gemm_score(const MxProduct& p, MxKind kind, hipStream_t st) {
-  return kind == MX_BF16 ? launch<MX_BF16, true, 2, 2, 3, 3>(p, st) : launch<MX_F16, true, 2, 2, 3, 3>(p, st);
+  return kind == MX_BF16 ? launch<MX_BF16, true, kScoreNT, kScoreMT, 3, 3>(p, st) : launch<MX_F16, true, kScoreNT, kScoreMT, 3, 3>(p, st);
 }
 
 }  // namespace q4d

@@ -81,6 +81,10 @@ ScorePath score_path(int M, int N, int K) {
 MxKind kind_of(int32_t x_dtype) { return x_dtype == Q4D_BF16 ? MX_BF16 : MX_F16; }
 
 size_t hit_bytes(int M) { return align_up((size_t)M * 4, 256); }
+// Whether a score has these sizes: what a launch of its path holds.
+bool score_shape(int M, int N, int K) {
+  return mx_shape(N, K) && M > 0 && M <= kMxScored && (score_path(M, N, K) != SCORE_TILES || mx_gemm_scores(M, N));
+}
 int score_parts(int M, int N, int K) {
   const ScorePath path = score_path(M, N, K);
   return path == SCORE_HEAD ? mx_head_parts(N) : path == SCORE_ROWS ? mx_rows_parts(M, N) : mx_gemm_parts(N);
@@ -126,7 +130,7 @@ extern "C" int q4d_mx_matmul(const q4d_mx_t* w, const q4d_mx_t* x, void* y, int3
 }
 
 extern "C" size_t q4d_mx_score_workspace_bytes(int32_t rows, int32_t cols, int32_t M) {
-  if (!mx_shape(rows, cols) || M <= 0 || M > kMxScored) return 0;
+  if (!score_shape(M, rows, cols)) return 0;
   return hit_bytes(M) + (size_t)score_parts(M, rows, cols) * M * sizeof(f32x4);
 }
 
@@ -135,7 +139,7 @@ extern "C" int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, i
                             void* stream) {
   int rc = check_x(w, x, x_dtype, x_stride, M);
   if (rc) return rc;
-  if (M > kMxScored) return Q4D_ERR_SHAPE;
+  if (!score_shape(M, w->rows, w->cols)) return Q4D_ERR_SHAPE;
   if (!targets || !logprob || !entropy || !best || !ws) return Q4D_ERR_NULL;
   if (!aligned(targets, 4) || !aligned(logprob, 4) || !aligned(entropy, 4) || !aligned(best, 4) || !aligned(ws, 256))
     return Q4D_ERR_BAD_ADDR;

@@ -246,7 +246,8 @@ class MXScores(NamedTuple):
 def mx_score(hidden: torch.Tensor, weight: MXTensor, targets: torch.Tensor) -> MXScores:
     """How likely ``targets`` [...] (int32) are under the output head ``weight`` [vocab, cols] at the rows
     ``hidden`` [..., cols] (fp16 or bf16): the log softmax of ``mx_linear(hidden, weight)`` in fp32 at the
-    targets, its entropy and its maximum, fp32 [...] each, without the products in memory.  Up to 2^23 rows.
+    targets, its entropy and its maximum, fp32 [...] each, without the products in memory.  Up to 2^23 rows, and
+    ceil(rows / 64) x ceil(vocab / 256) up to 2^23 (903808 rows of 151936 tokens).
     A target outside the vocabulary (a padded row's) gives NaN, and so does a row whose products hold NaN, +Inf or
     nothing but -Inf."""
     if not isinstance(weight, MXTensor):
@@ -262,11 +263,13 @@ def mx_score(hidden: torch.Tensor, weight: MXTensor, targets: torch.Tensor) -> M
     if targets.dtype != torch.int32 or targets.shape != lead or targets.get_device() != index:
         raise ValueError(f"targets must be int32 {tuple(lead)} on {x.device}")
     targets = targets.contiguous()
-    got = x.new_empty((3, *lead), dtype=torch.float32)
     if m > 1 << 23:
         raise ValueError(f"up to 2^23 rows, got {m}")
+    nbytes = _lib.load().q4d_mx_score_workspace_bytes(*weight.shape, m) if m else 0
+    if m and not nbytes:
+        raise ValueError(f"ceil(rows / 64) x ceil(vocab / 256) up to 2^23, got {m} rows of {weight.shape[0]}")
+    got = x.new_empty((3, *lead), dtype=torch.float32)
     if m:
-        nbytes = _lib.load().q4d_mx_score_workspace_bytes(*weight.shape, m)
         ws = x.new_empty(nbytes, dtype=torch.uint8)
         base, row = got.data_ptr(), 4 * m
         call_on(index, "q4d_mx_score", weight._ref, x.data_ptr(), _DTYPES[x.dtype], step, m, targets.data_ptr(), base,
