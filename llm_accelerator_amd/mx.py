@@ -87,6 +87,14 @@ class MXTensor:
             raise ValueError(f"an MXTensor has at most {_MOST} rows and columns, got {rows} x {cols}")
         return self._setup(like.new_empty(-(-rows // TILE_ROWS) * -(-cols // TILE_COLS) * 2176, dtype=torch.uint8), rows, cols)
 
+    # (copies and pickles: the descriptor holds addresses, and is made anew over the memory that came)
+    def __getstate__(self) -> tuple:
+        return self._memory, self.shape
+
+    def __setstate__(self, state: tuple) -> None:
+        memory, shape = state
+        self._setup(memory, *shape)
+
     @property
     def codes(self) -> torch.Tensor:
         return self._memory[:self._memory.numel() // 17 * 16]
