@@ -138,6 +138,9 @@ __global__ __launch_bounds__(256, PER_CU) void mx_gemm_kernel(const MxProduct a)
           if (group(MT * w + j) < have) v = *reinterpret_cast<const u32x4*>(base + from[j]);
           *reinterpret_cast<u32x4*>(lds + at + kWaveX * w + 1024 * j + 16 * lane) = v;
         }
+        // This stage, the last, has MT DMA loads fewer than the loop counts on: with those of all stages before it
+        // complete here, the loop's waits for them are met whatever they count.
+        wait_loads<0>();
       }
 #pragma unroll
       for (int j = 0; j < NT; ++j)
