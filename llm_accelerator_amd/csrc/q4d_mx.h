@@ -33,17 +33,30 @@ constexpr long long kMxTiles = 1 << 23;
 bool mx_shape(int32_t rows, int32_t cols);
 int check_mx(const q4d_mx_t* t);
 
+// A product's kernel, and its form: the blocks' rows of x and of weights in units of 16 (32 and 128 for tiles).
+enum MxPath { MX_ROWS = 0, MX_HEAD = 1, MX_TILES = 2 };
+struct MxForm {
+  int path, mt, nt, waves;
+};
+MxForm mx_form(int M, int N, int K, MxKind kind);
+MxForm mx_score_form(int M, int N, int K);
+
 // Few rows (q4d_mx_rows.hip; a score: up to kMxFewRows) and tiles of many (q4d_mx_gemm.hip), and the ranges of N
 // that a score's blocks leave.
 constexpr int kMxFewRows = 64;
 int launch_mx_rows(const MxProduct& p, MxKind kind, hipStream_t st);
 int launch_mx_rows_score(const MxProduct& p, MxKind kind, hipStream_t st);
 int mx_rows_parts(int M, int N);
+MxForm mx_rows_form(int M, int N, int K);
+MxForm mx_rows_score_form(int M);
 // Few rows and many weights (q4d_mx_head.hip), where x fits in LDS.
 bool mx_head_fits(int M, int K);
 int mx_head_parts(int N);
+MxForm mx_head_form(int M, int N);
 int launch_mx_head(const MxProduct& p, MxKind kind, hipStream_t st);
 int launch_mx_head_score(const MxProduct& p, MxKind kind, hipStream_t st);
+MxForm mx_gemm_form(int M, int N, MxKind kind);
+MxForm mx_gemm_score_form();
 int launch_mx_gemm(const MxProduct& p, MxKind kind, hipStream_t st);
 __host__ __device__ inline int mx_gemm_parts(int N) { return (int)((N + 255LL) / 256); }
 bool mx_gemm_scores(int M, int N);  // no more tiles than that

@@ -352,29 +352,34 @@ int launch(const MxProduct& p, hipStream_t st) {
   hipLaunchKernelGGL((mx_gemm_kernel<KIND, SCORE, NT, MT, RING, PER_CU>), dim3((unsigned)tiles), dim3(256), 0, st, p);
   return check_launch();
 }
+template <MxKind KIND>
+int launch(const MxProduct& p, hipStream_t st) {
+  const MxForm f = mx_gemm_form(p.M, p.N, KIND);
+  if constexpr (KIND == MX_X4) {
+    if (f.mt == 4) return launch<KIND, false, 2, 4, 3, 2>(p, st);
+  }
+  if (f.nt == 2) return launch<KIND, false, 2, 2, 3, KIND == MX_X4 ? 2 : 3>(p, st);
+  return launch<KIND, false, 1, 2, KIND == MX_X4 ? 5 : 6, 2>(p, st);
+}
+constexpr int kScoreNT = 2, kScoreMT = 2;
+
+}  // namespace
+
 // Tiles of 256 x 64, three blocks a CU (two with x in 4 bits); 128 x 64 where those are no more than one a CU:
 // 1024 x 4096 x 4096 in 16 bits 42 / 39 us, 512 x 16384 x 1024 (two a CU) 20 / 24.  With x in 4 bits, whose
 // products take a quarter of the time their operands are moved for, 256 x 128 where that gives two a CU:
 // 4096 x 8192 x 4096 78 instead of 98 us, 2000 x 4096 x 4096 (one a CU) 31 instead of 28; in 16 bits the
 // larger tile is no faster (8192 x 8192 x 8192 864 instead of 844, 2000 x 16384 x 1024 66 instead of 68).
-template <MxKind KIND>
-int launch(const MxProduct& p, hipStream_t st) {
-  const auto tiles = [&](int n, int m) { return (p.N + (long long)n - 1) / n * ((p.M + (long long)m - 1) / m); };
+MxForm mx_gemm_form(int M, int N, MxKind kind) {
   const int cus = device_cus();
-  if constexpr (KIND == MX_X4) {
-    if (tiles(256, 128) >= 2 * cus) return launch<KIND, false, 2, 4, 3, 2>(p, st);
-  }
-  if (tiles(256, 64) > cus) return launch<KIND, false, 2, 2, 3, KIND == MX_X4 ? 2 : 3>(p, st);
-  return launch<KIND, false, 1, 2, KIND == MX_X4 ? 5 : 6, 2>(p, st);
+  if (kind == MX_X4 && tile_count(M, N, 2, 4) >= 2 * cus) return {MX_TILES, 4, 2, 4};
+  return {MX_TILES, 2, tile_count(M, N, 2, 2) > cus ? 2 : 1, 4};
 }
-
-}  // namespace
-
+MxForm mx_gemm_score_form() { return {MX_TILES, kScoreMT, kScoreNT, 4}; }
 int launch_mx_gemm(const MxProduct& p, MxKind kind, hipStream_t st) {
   if (kind == MX_X4) return launch<MX_X4>(p, st);
   return kind == MX_BF16 ? launch<MX_BF16>(p, st) : launch<MX_F16>(p, st);
 }
-constexpr int kScoreNT = 2, kScoreMT = 2;
 bool mx_gemm_scores(int M, int N) { return tile_count(M, N, kScoreNT, kScoreMT) <= kMxTiles; }
 int launch_mx_gemm_score(const MxProduct& p, MxKind kind, hipStream_t st) {
   return kind == MX_BF16 ? launch<MX_BF16, true, kScoreNT, kScoreMT, 3, 3>(p, st) : launch<MX_F16, true, kScoreNT, kScoreMT, 3, 3>(p, st);

@@ -195,6 +195,7 @@ int launch(const MxProduct& p, hipStream_t st) {
 }  // namespace
 
 bool mx_head_fits(int M, int K) { return M <= 32 && lds_bytes(M, K) <= (size_t)kHeadLds; }
+MxForm mx_head_form(int M, int N) { return {MX_HEAD, M <= 16 ? 1 : 2, kUnit, head_shape(N).waves}; }
 int mx_head_parts(int N) { return head_shape(N).blocks; }
 int launch_mx_head(const MxProduct& p, MxKind kind, hipStream_t st) {
   return kind == MX_BF16 ? launch<true, false>(p, st) : launch<false, false>(p, st);

@@ -160,24 +160,17 @@ int launch(const MxProduct& p, hipStream_t st) {
   hipLaunchKernelGGL((mx_rows_kernel<KIND, MT, NT, NW, false>), grid, dim3(64 * NW), 0, st, p);
   return check_launch();
 }
-// 16 weight rows a block where those are at most one a CU, else 32, which share what is loaded of x: one row of
-// 4096 x 1024 3.2 / 3.4 us, 16 of 8192 x 1024 4.7 / 4.1, 64 of 4096 x 4096 17.8 / 11.3.  64 for very many (16 rows
-// of 24000 x 1024 6.7 / 6.6).  Eight waves where K is long (one row of 8192 x 8192 10.2 instead of 12.5 us).
-template <MxKind KIND, int MT>
-int launch(const MxProduct& p, hipStream_t st) {
-  const long long blocks = (p.N + 15LL) / 16 * ((p.M + 16LL * MT - 1) / (16 * MT));
-  const bool deep = p.K > 1024;
-  if (p.N >= 32768 && !deep) return launch<KIND, MT, MT == 4 ? 2 : 4, 4>(p, st);
-  if (blocks > device_cus()) return deep ? launch<KIND, MT, 2, 8>(p, st) : launch<KIND, MT, 2, 4>(p, st);
-  return deep ? launch<KIND, MT, 1, 8>(p, st) : launch<KIND, MT, 1, 4>(p, st);
-}
 template <MxKind KIND>
 int launch(const MxProduct& p, hipStream_t st) {
-  // the fewest rows a block that leave no more blocks than two a CU
-  const long long tiles = (p.N + 15LL) / 16, most = 2LL * device_cus();
-  if (p.M <= 16 || tiles * ((p.M + 15) / 16) <= most) return launch<KIND, 1>(p, st);
-  if (p.M <= 32 || tiles * ((p.M + 31) / 32) <= most) return launch<KIND, 2>(p, st);
-  return launch<KIND, 4>(p, st);
+  const MxForm f = mx_rows_form(p.M, p.N, p.K);
+  if (f.mt == 4) return f.waves == 8 ? launch<KIND, 4, 2, 8>(p, st) : launch<KIND, 4, 2, 4>(p, st);
+  if (f.mt == 2) {
+    if (f.nt == 4) return launch<KIND, 2, 4, 4>(p, st);
+    return f.waves == 8 ? launch<KIND, 2, 2, 8>(p, st) : launch<KIND, 2, 2, 4>(p, st);
+  }
+  if (f.nt == 4) return launch<KIND, 1, 4, 4>(p, st);
+  if (f.nt == 2) return f.waves == 8 ? launch<KIND, 1, 2, 8>(p, st) : launch<KIND, 1, 2, 4>(p, st);
+  return f.waves == 8 ? launch<KIND, 1, 1, 8>(p, st) : launch<KIND, 1, 1, 4>(p, st);
 }
 
 template <MxKind KIND, int MT, int NT>
@@ -189,12 +182,27 @@ int launch_score(const MxProduct& p, hipStream_t st) {
 }
 template <MxKind KIND>
 int launch_score(const MxProduct& p, hipStream_t st) {
-  if (p.M <= 16) return launch_score<KIND, 1, 4>(p, st);
-  if (p.M <= 32) return launch_score<KIND, 2, 4>(p, st);
-  return launch_score<KIND, 4, 2>(p, st);
+  const MxForm f = mx_rows_score_form(p.M);
+  if (f.mt == 1) return launch_score<KIND, 1, 4>(p, st);
+  return f.mt == 2 ? launch_score<KIND, 2, 4>(p, st) : launch_score<KIND, 4, 2>(p, st);
 }
 
 }  // namespace
+
+// x's rows a block (16 mt): the fewest that leave no more blocks of 16 weight rows than two a CU.
+// Weight rows a block (16 nt): 16 where those are at most one a CU, else 32, which share what is loaded of x: one row of
+// 4096 x 1024 3.2 / 3.4 us, 16 of 8192 x 1024 4.7 / 4.1, 64 of 4096 x 4096 17.8 / 11.3.  64 for very many (16 rows
+// of 24000 x 1024 6.7 / 6.6).  Eight waves where K is long (one row of 8192 x 8192 10.2 instead of 12.5 us).
+MxForm mx_rows_form(int M, int N, int K) {
+  const long long tiles = (N + 15LL) / 16;
+  const int cus = device_cus();
+  const auto blocks = [&](int mt) { return tiles * ((M + 16LL * mt - 1) / (16 * mt)); };
+  const int mt = M <= 16 || blocks(1) <= 2 * cus ? 1 : M <= 32 || blocks(2) <= 2 * cus ? 2 : 4;
+  const bool deep = K > 1024;
+  if (N >= 32768 && !deep) return {MX_ROWS, mt, mt == 4 ? 2 : 4, 4};
+  return {MX_ROWS, mt, blocks(mt) > cus ? 2 : 1, deep ? 8 : 4};  // (mt > 1: more than one a CU)
+}
+MxForm mx_rows_score_form(int M) { return M <= 16 ? MxForm{MX_ROWS, 1, 4, 4} : M <= 32 ? MxForm{MX_ROWS, 2, 4, 4} : MxForm{MX_ROWS, 4, 2, 4}; }
 
 int launch_mx_rows(const MxProduct& p, MxKind kind, hipStream_t st) {
   if (kind == MX_X4) return launch<MX_X4>(p, st);
@@ -203,6 +211,9 @@ int launch_mx_rows(const MxProduct& p, MxKind kind, hipStream_t st) {
 int launch_mx_rows_score(const MxProduct& p, MxKind kind, hipStream_t st) {
   return kind == MX_BF16 ? launch_score<MX_BF16>(p, st) : launch_score<MX_F16>(p, st);
 }
-int mx_rows_parts(int M, int N) { return (int)((N + (M <= 32 ? 63LL : 31LL)) / (M <= 32 ? 64 : 32)); }
+int mx_rows_parts(int M, int N) {
+  const int n = 16 * mx_rows_score_form(M).nt;
+  return (int)((N + n - 1LL) / n);
+}
 
 }  // namespace q4d

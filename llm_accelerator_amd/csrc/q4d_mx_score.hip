@@ -64,33 +64,47 @@ int check_y(const void* y, int32_t y_dtype) {
 // LDS (24 rows of 151936 x 1024 22 us, tiles 29; 48 rows 32 / 31).
 constexpr long long kFewOutputs = 750000, kFewOutputs4 = 1000000;
 constexpr int kHeadRows = 49152;
+MxPath product_path(int M, int N, int K, MxKind kind) {
+  const long long outputs = (long long)M * N;
+  if (kind == MX_X4) return outputs <= kFewOutputs4 || M <= 16 ? MX_ROWS : MX_TILES;
+  if (outputs <= kFewOutputs) return MX_ROWS;
+  return N >= kHeadRows && mx_head_fits(M, K) ? MX_HEAD : MX_TILES;
+}
 int product(const MxProduct& p, MxKind kind, hipStream_t st) {
-  const long long outputs = (long long)p.M * p.N;
-  if (kind == MX_X4) return outputs <= kFewOutputs4 || p.M <= 16 ? launch_mx_rows(p, kind, st) : launch_mx_gemm(p, kind, st);
-  if (outputs <= kFewOutputs) return launch_mx_rows(p, kind, st);
-  return p.N >= kHeadRows && mx_head_fits(p.M, p.K) ? launch_mx_head(p, kind, st) : launch_mx_gemm(p, kind, st);
+  const MxPath path = product_path(p.M, p.N, p.K, kind);
+  if (path == MX_ROWS) return launch_mx_rows(p, kind, st);
+  return path == MX_HEAD ? launch_mx_head(p, kind, st) : launch_mx_gemm(p, kind, st);
 }
 // A score's kernels: the same three, few outputs being up to 1100000 and 64 rows (32 rows of 32000 x 1024 13.8 us,
 // tiles 15.2; 48 rows 22 / 16; 64 of 8000 x 1024 10.9 / 15.6).
 constexpr long long kFewScores = 1100000;
-enum ScorePath { SCORE_ROWS, SCORE_HEAD, SCORE_TILES };
-ScorePath score_path(int M, int N, int K) {
-  if (N >= kHeadRows && mx_head_fits(M, K)) return SCORE_HEAD;
-  return M <= 16 || (M <= kMxFewRows && (long long)M * N <= kFewScores) ? SCORE_ROWS : SCORE_TILES;
+MxPath score_path(int M, int N, int K) {
+  if (N >= kHeadRows && mx_head_fits(M, K)) return MX_HEAD;
+  return M <= 16 || (M <= kMxFewRows && (long long)M * N <= kFewScores) ? MX_ROWS : MX_TILES;
 }
 MxKind kind_of(int32_t x_dtype) { return x_dtype == Q4D_BF16 ? MX_BF16 : MX_F16; }
 
 size_t hit_bytes(int M) { return align_up((size_t)M * 4, 256); }
 // Whether a score has these sizes: what a launch of its path holds.
 bool score_shape(int M, int N, int K) {
-  return mx_shape(N, K) && M > 0 && M <= kMxScored && (score_path(M, N, K) != SCORE_TILES || mx_gemm_scores(M, N));
+  return mx_shape(N, K) && M > 0 && M <= kMxScored && (score_path(M, N, K) != MX_TILES || mx_gemm_scores(M, N));
 }
 int score_parts(int M, int N, int K) {
-  const ScorePath path = score_path(M, N, K);
-  return path == SCORE_HEAD ? mx_head_parts(N) : path == SCORE_ROWS ? mx_rows_parts(M, N) : mx_gemm_parts(N);
+  const MxPath path = score_path(M, N, K);
+  return path == MX_HEAD ? mx_head_parts(N) : path == MX_ROWS ? mx_rows_parts(M, N) : mx_gemm_parts(N);
 }
 
 }  // namespace
+
+MxForm mx_form(int M, int N, int K, MxKind kind) {
+  const MxPath path = product_path(M, N, K, kind);
+  return path == MX_ROWS ? mx_rows_form(M, N, K) : path == MX_HEAD ? mx_head_form(M, N) : mx_gemm_form(M, N, kind);
+}
+MxForm mx_score_form(int M, int N, int K) {
+  const MxPath path = score_path(M, N, K);
+  return path == MX_ROWS ? mx_rows_score_form(M) : path == MX_HEAD ? mx_head_form(M, N) : mx_gemm_score_form();
+}
+
 }  // namespace q4d
 
 using namespace q4d;
@@ -158,9 +172,9 @@ extern "C" int q4d_mx_score(const q4d_mx_t* w, const void* x, int32_t x_dtype, i
   p.stats = ws_ptr<f32x4>(ws, hit_bytes(M));
   const int parts = score_parts(M, p.N, p.K);
   const MxKind kind = kind_of(x_dtype);
-  const ScorePath path = score_path(M, p.N, p.K);
-  if (path == SCORE_HEAD) rc = launch_mx_head_score(p, kind, st);
-  else rc = path == SCORE_ROWS ? launch_mx_rows_score(p, kind, st) : launch_mx_gemm_score(p, kind, st);
+  const MxPath path = score_path(M, p.N, p.K);
+  if (path == MX_HEAD) rc = launch_mx_head_score(p, kind, st);
+  else rc = path == MX_ROWS ? launch_mx_rows_score(p, kind, st) : launch_mx_gemm_score(p, kind, st);
   if (rc) return rc;
   const JoinArgs j = {p.stats, p.hit, targets, parts, M, p.N, logprob, entropy, best};
   hipLaunchKernelGGL(mx_score_join_kernel, dim3((unsigned)M), dim3(256), 0, st, j);
