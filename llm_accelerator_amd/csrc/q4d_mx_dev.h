@@ -47,9 +47,14 @@ __device__ __forceinline__ u32x4 mx_dequant8(uint32_t w, float scale) {
 
 // Sum / maximum of a wave, in every lane: in the 16-lane rows by DPP, then over the rows by lane swaps (shuffles
 // through LDS would be a few hundred clocks of a chain).
+// No addition takes in the product that v may be: fused, it would be rounded for the other lane and not for the own,
+// and the lanes would hold sums a rounding apart.
 template <bool SUM>
 __device__ __forceinline__ float wave_all(float v) {
-  const auto op = [](float a, float b) { return SUM ? a + b : fmaxf(a, b); };
+  const auto op = [](float a, float b) {
+#pragma clang fp contract(off)
+    return SUM ? a + b : fmaxf(a, b);
+  };
   v = op(v, dpp_f<kDppQuadSwap1>(v));
   v = op(v, dpp_f<kDppQuadSwap2>(v));
   v = op(v, dpp_f<kDppRowHalfMirror>(v));
