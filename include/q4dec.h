@@ -558,7 +558,10 @@ int q4d_mx_quantize(const void* x, int32_t dtype, int64_t ld, int32_t rule, cons
 int q4d_mx_dequantize(const q4d_mx_t* t, void* y, int32_t y_dtype, void* stream);
 /* y[m, :] = W x[m, :], m < M: x fp16 or bf16, row m at m * x_stride (< 2^24) elements, 16-byte aligned rows;
  * y [M, rows] in any of the three types, 16-byte aligned.  The weights enter as numbers of x's type
- * (as q4d_mx_dequantize makes them); fp32 sums, rounded once.  A row's last bits may depend on M,
+ * (as q4d_mx_dequantize makes them: blocks whose scale lies outside 2^-23 .. 2^13 rounded or Inf in
+ * fp16, exact in bf16); fp32 sums, rounded once.  In fp16 the matrix units add a product of a number
+ * below 2^-14 as if that were 2^-14: a sum is off by up to cols 2^-23 of the sum of
+ * max(|x|, 2^-14) max(|w|, 2^-14).  A row's last bits may depend on M,
  * though not on the other rows' values.  M up to 2^29 and M * rows to about 2^37 (more is refused); y
  * apart from x and w. */
 int q4d_mx_linear(const q4d_mx_t* w, const void* x, int32_t x_dtype, int64_t x_stride, int32_t M, void* y, int32_t y_dtype,

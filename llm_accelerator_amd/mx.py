@@ -202,8 +202,9 @@ def mx_quantize(x: torch.Tensor, rule: str = "floor") -> MXTensor:
 def mx_linear(x: torch.Tensor | MXTensor, weight: MXTensor, out_dtype: torch.dtype | None = None,
               out: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T``: x [..., cols] in fp16 or bf16, where the weights enter as numbers of that type
-    (``weight.dequantize(x.dtype)``), or an :class:`MXTensor` [rows, cols], where both enter as they are.
-    fp32 sums, rounded once to ``out_dtype`` (fp32, fp16 or bf16; ``None``: x's type, bf16 for an
+    (``weight.dequantize(x.dtype)``: exact in bf16; in fp16 blocks whose scale lies outside 2^-23 .. 2^13 are
+    rounded or Inf, and numbers below 2^-14 are added with the precision of 2^-14), or an :class:`MXTensor`
+    [rows, cols], where both enter as they are.  fp32 sums, rounded once to ``out_dtype`` (fp32, fp16 or bf16; ``None``: x's type, bf16 for an
     MXTensor).  ``out``: a contiguous result of the caller's, apart from x."""
     if not isinstance(weight, MXTensor):
         raise TypeError("weight must be an MXTensor")
@@ -253,7 +254,7 @@ class MXScores(NamedTuple):
 
 def mx_score(hidden: torch.Tensor, weight: MXTensor, targets: torch.Tensor) -> MXScores:
     """How likely ``targets`` [...] (int32) are under the output head ``weight`` [vocab, cols] at the rows
-    ``hidden`` [..., cols] (fp16 or bf16): the log softmax of ``mx_linear(hidden, weight)`` in fp32 at the
+    ``hidden`` [..., cols] (fp16 or bf16, with weights of that type): the log softmax of ``mx_linear(hidden, weight)`` in fp32 at the
     targets, its entropy and its maximum, fp32 [...] each, without the products in memory.  Up to 2^23 rows, and
     ceil(rows / 64) x ceil(vocab / 256) up to 2^23 (903808 rows of 151936 tokens).
     A target outside the vocabulary (a padded row's) gives NaN, and so does a row whose products hold NaN, +Inf or
