@@ -14,9 +14,11 @@
 //
 // Logits are ordered by value, then by index, the lower first; NaN comes last, after -Inf.
 //
-// Bound by the vector units, about twelve operations a logit and an exponential: 1100 bf16 rows of 151669 with one
-// alternative 88-95 us, 3.5-3.8 TB/s (units busy 76 %), 64 fp32 rows of 151936 with 20 15 us, 2.6 TB/s (66 %; all
-// blocks at once, each its load, its sums and its search).  One row: 6.3 us, and 3-5 us for a join, both latency.
+// Bound by the vector units, about twelve operations a logit and an exponential, and by loads that wait for the
+// blocks before: 1100 bf16 rows of 151669 with one alternative 88-95 us, 3.5-3.8 TB/s (units busy 76 %; 102 registers,
+// four waves a SIMD, which wait 55 % of their time), 64 fp32 rows of 151936 with 20 15 us, 2.6 TB/s (66 %; 2432 blocks on
+// 2048 places, each its load, its sums and its search: the second round is a fifth full).  One row: 6.3 us, and 3-5 us
+// for a join, both latency.
 #include <float.h>
 #include <math.h>
 
@@ -421,7 +423,11 @@ __global__ __launch_bounds__(kJoinThreads) void logprob_join_kernel(const Logpro
   }
 }
 
-// How a row is cut: short rows are a wave's, others parts of four waves.
+// How a row is cut: short rows are a wave's, others parts of four waves, of 16 logits a thread up to 4096 such blocks
+// and of 64 past them (16 / 64 a thread, rows of 151936 in fp32 with 20 alternatives: 53 rows, 2014 blocks of 16 a
+// thread, 17.9 / 19.7 us; 107 rows 25.2 / 26.2, 161 31.2 / 31.0, 315 49.9 / 45.7; with one alternative 107 rows 18.4 / 21.0,
+// 315 40.9 / 39.8; in bf16 with 20 107 rows 26.3 / 27.2, 131 29.7 / 29.2).  Rows that 64 a thread hold in one part, up to
+// 16384, want them earlier: 1000 rows of 10000 22.3 / 18.5 with 20, 13.6 / 12.8 with none.
 struct Cut {
   int held, waves, parts;
 };

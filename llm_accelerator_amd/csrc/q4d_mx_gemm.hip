@@ -10,7 +10,9 @@
 //
 // Bound by the matrix units and the clock that they leave (1.5 GHz): 2000 x 6144 x 1024 28 us, 0.90 PFLOP/s (units busy
 // 56 %; one round of blocks), 8192 x 8192 x 8192 844 us, 1.30 PFLOP/s, a score of 1999 rows of 151936 x
-// 1024 560 us, 1.11 PFLOP/s (68 %), 4096 x 8192 x 4096 in 4 bits 76 us, 3.6 PFLOP/s (52 %).
+// 1024 560 us, 1.11 PFLOP/s (68 %).  In 4 bits, where a stage is 16 products a wave, by the stages' start: 4096 x 8192
+// x 4096 76 us, 3.6 PFLOP/s (units busy 52 %), waves wait 28 % of their time for the stage, for each other and for the first
+// operands, which are read after the barrier.
 #include <math.h>
 
 #include <type_traits>

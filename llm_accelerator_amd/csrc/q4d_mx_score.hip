@@ -57,11 +57,15 @@ int check_y(const void* y, int32_t y_dtype) {
   if (y_dtype != Q4D_F16 && y_dtype != Q4D_BF16 && y_dtype != Q4D_F32) return Q4D_ERR_DTYPE;
   return aligned(y, 16) ? Q4D_OK : Q4D_ERR_BAD_ADDR;
 }
-// Few outputs go to the kernel of few rows, which reads x once a weight tile but whose waves share K: with 16-bit
-// x up to 750000 (64 rows of 8192 x 1024 7.6 us, tiles of many rows 9.8; 64 of 16384 11.6 / 10.1; 128 of 4096 x 4096
-// 21 / 28), with x in 4 bits, a quarter of the bytes, up to a million or 16 rows (64 of 16384 x 1024 5.3 / 6.0, 128 of
-// 16384 9.0 / 6.4, 16 of 151936 18.2 / 19.8).  Up to 32 rows of many more weights: the kernel that holds x in
-// LDS (24 rows of 151936 x 1024 22 us, tiles 29; 48 rows 32 / 31).
+// Few outputs go to the kernel of few rows, which reads x once a weight tile but whose waves share K (us, rows' kernel
+// / tiles): with 16-bit x up to 750000 (64 rows of 8192 x 1024 7.6 / 9.5, of 12288 11.4 / 9.5; 128 of 4096 x 4096
+// 19.1 / 27.4, of 8192 x 4096 37.8 / 27.8), with x in 4 bits, a quarter of the bytes, up to a million or 16 rows
+// (64 of 12288 x 1024 5.2 / 5.8, of 17408 7.3 / 5.9; 16 of 151936 18.2 / 19.8).  Beside the lines K and the last round
+// of blocks decide, and outputs alone may miss: 64 of 11718 12.5 / 11.9 with K = 1024 and 38.7 / 30.1 with 4096, in
+// 4 bits 64 of 16384 5.3 / 5.8 and 15.2 / 12.8.
+// Up to 32 rows of many more weights: the kernel that holds x in LDS, from 49152 on (24 rows, rows / tiles / LDS: of
+// 32768 x 1024 8.9 / 9.7 / 10.8, 49152 12.2 / 12.2 / 11.7, 65536 15.1 / 16.1 / 12.6, 151936 31 / 29 / 22; with
+// K = 512 it is the faster one from 65536 on, with 2048 from 40960).
 constexpr long long kFewOutputs = 750000, kFewOutputs4 = 1000000;
 constexpr int kHeadRows = 49152;
 MxPath product_path(int M, int N, int K, MxKind kind) {
@@ -75,8 +79,10 @@ int product(const MxProduct& p, MxKind kind, hipStream_t st) {
   if (path == MX_ROWS) return launch_mx_rows(p, kind, st);
   return path == MX_HEAD ? launch_mx_head(p, kind, st) : launch_mx_gemm(p, kind, st);
 }
-// A score's kernels: the same three, few outputs being up to 1100000 and 64 rows (32 rows of 32000 x 1024 13.8 us,
-// tiles 15.2; 48 rows 22 / 16; 64 of 8000 x 1024 10.9 / 15.6).
+// A score's kernels: the same three, few outputs being up to 1100000 and 64 rows (rows' kernel / tiles: 32 rows of
+// 32768 x 1024 13.9 / 15.1 us, 40960 18.2 / 15.6; 48 of 16384 13.4 / 15.6, 24576 18.3 / 15.7; 64 of 12288 15.1 / 15.6,
+// just below the line 64 of 17187 20.0 / 15.6), the one with x in LDS from 49152 tokens on (24 rows 17.4 / 15.6 / 14.7; 16
+// rows 13.1 on the rows' kernel / 13.2, of 65536 15.0 / 14.3; one row 11.5 / 12.2, of 98304 17.0 / 15.9).
 constexpr long long kFewScores = 1100000;
 MxPath score_path(int M, int N, int K) {
   if (N >= kHeadRows && mx_head_fits(M, K)) return MX_HEAD;
